@@ -44,6 +44,13 @@ extern "C" {
 #define GPIC_DTYPE_BF16 0
 #define GPIC_DTYPE_F32 1
 
+/* Activations of the row-scaled linears: silu(z) = z sigmoid(z); gelu_tanh(z) = z (1 + tanh(sqrt(2 / pi) (z + 0.044715 z^3))) / 2;
+ * SwiGLU: silu of 4 columns times the next 4, in runs of 8 (half as many columns come out). */
+#define GPIC_ACT_NONE 0
+#define GPIC_ACT_SILU 1
+#define GPIC_ACT_GELU_TANH 2
+#define GPIC_ACT_SWIGLU 3
+
 /* Library version string and a message for a status code (host memory, static). */
 const char *gpic_fp8_version(void);
 const char *gpic_fp8_status_string(int status);
@@ -326,6 +333,77 @@ int gpic_fp8_gemm_mn_f32(const uint8_t *A, int64_t lda, const float *sa, const u
  */
 int gpic_fp8_bf16_gemm_mn(const uint16_t *A, int64_t lda, const uint16_t *B, int64_t ldb, void *C, int c_dtype,
                           int64_t ldc, int64_t M, int64_t N, int64_t K, void *ws, size_t ws_bytes, void *stream);
+
+/*
+ * The row-scaled operators. No counterpart in the reference, whose casts have one scale per tensor (fp8_native.py:33-49): here
+ * each row of an e4m3 matrix (a token, or an output channel of a weight) has its own, so a cast needs no maximum over the
+ * chip, a token's bytes do not depend on the others, and one token is one short launch. The rule for a row h (fp32):
+ *   a = max(max|h|, 1e-12);  s = RN(a / 448);  q = e4m3(min(max(RN(h * RN(448 / a)), -448), 448))
+ * A NaN in a row makes its scale NaN (and so the row of a product that reads it), an infinity infinite. None of them needs the
+ * cast workspace or keeps anything from call to call. Every matrix's rows are 16-byte aligned (leading dimensions are
+ * multiples of 8 bf16, 16 e4m3) and its columns a multiple of 8 (GEMM operands: of 16); outputs without a leading dimension
+ * are contiguous. rows == 0 is allowed.
+ */
+
+/* The row cast of x [rows, cols] (bf16 or fp32, row stride ldx) -> q [rows, cols] e4m3, s [rows]. cols <= 32768. */
+int gpic_fp8_tcast_rows(const void *x, int dtype, int64_t ldx, int64_t rows, int64_t cols, uint8_t *q, float *s,
+                        void *stream);
+
+/* qt [cols, ldt] = q [rows, cols] transposed (bytes; cols, ldt % 16 == 0, ldt >= rows, columns rows..ldt-1 zero): a weight's
+ * bytes as the K-major operand of its dgrad. */
+int gpic_fp8_transpose_bytes(const uint8_t *q, int64_t rows, int64_t cols, uint8_t *qt, int64_t ldt, void *stream);
+
+/*
+ * RMSNorm with the residual's addition and a row-scaled e4m3 output:
+ *   x_new = bf16(x + gate * a) -> xn (a != NULL; gate NULL: x + a), else x_new = x
+ *   rstd = 1 / sqrt(mean(x_new^2) + eps) -> rstd [rows]
+ *   h = (w * (x_new * rstd)) * (1 + scale) + shift (shift, scale NULL: without them), fp32 -> q, s by row, and as bf16 to
+ *       h when h != NULL
+ *   x, a [rows, C] bf16 (row strides ldx, lda); xn, h [rows, C] bf16; q [rows, C]; s [rows]; w [C] of w_dtype
+ *   gate, shift, scale: bf16 rows (strides sg, ssh, ssc); row r uses row r / ntok of them (rows % ntok == 0)
+ *   C % 8 == 0, C <= 16384, rows < 2^31.
+ */
+int gpic_fp8_rmsnorm_rows(const uint16_t *x, int64_t ldx, const uint16_t *a, int64_t lda, const uint16_t *gate, int64_t sg,
+                          const void *w, int w_dtype, const uint16_t *shift, int64_t ssh, const uint16_t *scale,
+                          int64_t ssc, int64_t rows, int64_t ntok, int64_t C, float eps, uint16_t *xn, uint16_t *h,
+                          float *rstd, uint8_t *q, float *s, void *stream);
+
+/*
+ * Its backward without gate, shift and scale (with them: gpic_fp8_res_mod_rmsnorm_bwd), dh the gradient of h:
+ *   t = xs * rstd, dt = dh * w;  dx = bf16(rstd (dt - t sum_row(dt t) / C) + dxn);  dw = sum over the rows of dh t
+ *   dh, dxn (or NULL), xs (x_new, or x), dx [rows, C] bf16 contiguous; w [C] of w_dtype; dw [C] of dw_dtype (one rounding).
+ *   dx is the gradient of x and of a. C % 8 == 0, C <= 16384. The sums are taken in a fixed order.
+ *   ws: gpic_fp8_rmsnorm_rows_bwd_workspace_bytes(rows, C) bytes, scratch of this call.
+ */
+size_t gpic_fp8_rmsnorm_rows_bwd_workspace_bytes(int64_t rows, int64_t C);
+int gpic_fp8_rmsnorm_rows_bwd(const uint16_t *dh, const uint16_t *dxn, const uint16_t *xs, const void *w, int w_dtype,
+                              const float *rstd, int64_t rows, int64_t C, uint16_t *dx, void *dw, int dw_dtype, void *ws,
+                              size_t ws_bytes, void *stream);
+
+/*
+ * The GEMM of row-scaled operands with bias, activation and residual in its epilogue (fp32, one rounding):
+ *   z[m, n] = sa[m] * sb[n] * sum_k A[m, k] * B[n, k] + bias[n];  C = bf16(res + gate * act(z))
+ *   A [M, K], B [N, K] e4m3 (row strides lda, ldb); sa [M], sb [N] fp32, or NULL (ones); bias [N] of bias_dtype, or NULL
+ *   act: GPIC_ACT_*; SWIGLU (N % 32 == 0) makes N / 2 columns, column 4 i + j of z columns 8 i + j and 8 i + 4 + j
+ *   res: bf16, C's shape (row stride ldr), or NULL; gate: bf16 rows of C's width (stride sg), row m uses row m / ntok
+ *       (M % ntok == 0), or NULL
+ *   C bf16 (row stride ldc); z: where to keep z as bf16 [M, N] (row stride ldz; for the activation's backward), or NULL
+ *   K > 0; sizes and strides otherwise as gpic_fp8_gemm's, ldr, ldz < 2^22; any M; res may not overlap C.
+ *   ws: gpic_fp8_gemm_workspace_bytes(M, N, K) bytes. Deterministic.
+ */
+int gpic_fp8_gemm_rows(const uint8_t *A, int64_t lda, const float *sa, const uint8_t *B, int64_t ldb, const float *sb,
+                       const void *bias, int bias_dtype, int act, const uint16_t *res, int64_t ldr, const uint16_t *gate,
+                       int64_t sg, int64_t ntok, uint16_t *C, int64_t ldc, uint16_t *z, int64_t ldz, int64_t M, int64_t N,
+                       int64_t K, void *ws, size_t ws_bytes, void *stream);
+
+/*
+ * The epilogue's backward: d = dy * act'(z) (act NONE, SILU or GELU_TANH; z and dz unused with NONE)
+ *   dz = bf16(d): the operand of the weight's gradient;  q, s = the row cast of d * sw, sw [N] the weight's row scales, which
+ *   lie on the dgrad's reduction: with them in the gradient, the dgrad reads the forward's weight bytes, transposed.
+ *   dy, z [rows, N] bf16 (row strides lddy, ldz); dz [rows, N] bf16; q [rows, N]; s [rows]. N % 8 == 0, N <= 32768.
+ */
+int gpic_fp8_act_bwd_rows(const uint16_t *dy, int64_t lddy, const uint16_t *z, int64_t ldz, int act, const float *sw,
+                          int64_t rows, int64_t N, uint16_t *dz, uint8_t *q, float *s, void *stream);
 
 #ifdef __cplusplus
 }

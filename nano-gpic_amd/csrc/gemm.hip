@@ -38,7 +38,7 @@
 #include <atomic>
 #include <type_traits>
 
-#include "gpic_device.h"
+#include "gpic_act.h"
 #include "gpic_launch.h"
 
 namespace gpic {
@@ -155,6 +155,91 @@ __device__ __forceinline__ u32x4 bias8(const void *bias, bool f32, int n) {
   return u32x4{x.x, x.y, y.x, y.y};
 }
 
+// The epilogue of the row-scaled GEMM (gpic_fp8_gemm_rows): the instances with RowsEpi apply it in fp32 to the accumulators
+// and round once, to bf16; those with NoEpi are the tensorwise GEMM's.
+struct NoEpi {};
+struct RowsEpi {
+  const float *sa, *sb;   // dequantization scales of A's and B's rows, or null (1)
+  const void *bias;       // [N] bf16, or fp32 (bias32), or null
+  const uint16_t *res;    // [M, N] bf16 (SwiGLU: [M, N / 2], as C), row stride ldr, or null
+  const uint16_t *gate;   // one row per ntok rows of C, row stride sg, or null
+  uint16_t *z;            // [M, N] bf16, row stride ldz: the values before the activation, or null
+  int64_t sg;
+  uint32_t ntok;
+  int ldr, ldz, bias32, act;
+};
+
+__device__ __forceinline__ void unpack8(u32x4 v, float (&f)[8]) {
+#pragma unroll
+  for (int e = 0; e < 4; e++) f[2 * e] = bf16_lo(v[e]), f[2 * e + 1] = bf16_hi(v[e]);
+}
+__device__ __forceinline__ u32x4 pack8(const float (&f)[8]) {
+  return u32x4{pack_bf16(f[0], f[1]), pack_bf16(f[2], f[3]), pack_bf16(f[4], f[5]), pack_bf16(f[6], f[7])};
+}
+// Eight fp32 of a vector at n, or eight of its bf16, or ones / zeros (`none`) where there is no vector.
+__device__ __forceinline__ void vec8(const void *p, bool f32, int n, float none, float (&f)[8]) {
+  if (!p) {
+#pragma unroll
+    for (int e = 0; e < 8; e++) f[e] = none;
+  } else if (f32) {
+    const v4f x = reinterpret_cast<const v4f *>(static_cast<const float *>(p) + n)[0];
+    const v4f y = reinterpret_cast<const v4f *>(static_cast<const float *>(p) + n)[1];
+#pragma unroll
+    for (int e = 0; e < 4; e++) f[e] = x[e], f[4 + e] = y[e];
+  } else {
+    unpack8(*reinterpret_cast<const u32x4 *>(static_cast<const uint16_t *>(p) + n), f);
+  }
+}
+// Eight columns of one row: v = z = v sa sb + bias; y = bf16(res + gate act(z)) packed (SwiGLU: the run holds 4 gate columns
+// and their 4 partners, y is 4 values in .x and .y, and so are res and gate).
+__device__ __forceinline__ u32x4 epi8(const RowsEpi &ep, float (&v)[8], float sa, const float (&sb)[8],
+                                      const float (&b)[8], u32x4 res, u32x4 gate) {
+#pragma unroll
+  for (int e = 0; e < 8; e++) v[e] = __builtin_fmaf(v[e] * sa, sb[e], b[e]);
+  float y[8], r[8], g[8];
+  if (ep.act == GPIC_ACT_SWIGLU) {
+#pragma unroll
+    for (int e = 0; e < 4; e++) y[e] = v[e] * fast_sigmoid(v[e]) * v[4 + e], y[4 + e] = 0.0f;
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; e++) y[e] = act_fwd(v[e], ep.act);
+  }
+  if (ep.res) {
+    unpack8(res, r);
+    if (ep.gate) {
+      unpack8(gate, g);
+#pragma unroll
+      for (int e = 0; e < 8; e++) y[e] = __builtin_fmaf(g[e], y[e], r[e]);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; e++) y[e] += r[e];
+    }
+  } else if (ep.gate) {
+    unpack8(gate, g);
+#pragma unroll
+    for (int e = 0; e < 8; e++) y[e] *= g[e];
+  }
+  return pack8(y);
+}
+// epi8 of row m (< M), columns n .. n + 7, with its loads and stores (16 bytes, SwiGLU: 8).
+__device__ __forceinline__ void epi8_row(const RowsEpi &ep, float (&v)[8], const float (&sb)[8], const float (&b)[8],
+                                         uint16_t *C, int64_t ldc, int64_t m, int n) {
+  const bool half = ep.act == GPIC_ACT_SWIGLU;
+  const int no = half ? n >> 1 : n;
+  u32x4 r{0u, 0u, 0u, 0u}, g{0u, 0u, 0u, 0u};
+  auto load = [&](const uint16_t *p) {
+    if (!half) return *reinterpret_cast<const u32x4 *>(p);
+    const u32x2 h = *reinterpret_cast<const u32x2 *>(p);
+    return u32x4{h.x, h.y, 0u, 0u};
+  };
+  if (ep.res) r = load(ep.res + m * ep.ldr + no);
+  if (ep.gate) g = load(ep.gate + (int64_t)((uint32_t)m / ep.ntok) * ep.sg + no);
+  const u32x4 y = epi8(ep, v, ep.sa ? ep.sa[m] : 1.0f, sb, b, r, g);
+  if (ep.z) *reinterpret_cast<u32x4 *>(ep.z + m * ep.ldz + n) = pack8(v);
+  if (half) *reinterpret_cast<u32x2 *>(C + m * ldc + no) = u32x2{y.x, y.y};
+  else *reinterpret_cast<u32x4 *>(C + m * ldc + no) = y;
+}
+
 // Half h of a 32-byte fragment as a bf16 MFMA operand.
 __device__ __forceinline__ v8bf frag16(const v8i &f, int h) {
   return __builtin_bit_cast(v8bf, v4i{f[4 * h], f[4 * h + 1], f[4 * h + 2], f[4 * h + 3]});
@@ -182,13 +267,15 @@ __device__ __forceinline__ int xcd_remap(int bid, int G) {
 // the caller leaves few tokens with a small gradient to the library ([2048, 1024 x 1024] 25.2 us against 17.4). (A bf16 dgrad
 // with this kernel, its B read MN-major, was not kept: 6-20% faster on some shapes, 14-25% slower on others, with no rule on sizes between them.)
 // kC32: C is fp32 and holds the bf16-rounded results: the gradient of an fp32 weight, without a separate conversion.
-template <bool kTail, bool kMN, int kBNt, int kEl = 1, bool kC32 = false, typename CT = std::conditional_t<kC32, float, uint16_t>>
+template <bool kTail, bool kMN, int kBNt, int kEl = 1, bool kC32 = false, typename EPI = NoEpi,
+          typename CT = std::conditional_t<kC32, float, uint16_t>>
 __global__ __launch_bounds__(kThreads) void gemm_tn_kernel(const uint8_t *__restrict__ A, int lda,
                                                             const uint8_t *__restrict__ B, int ldb,
                                                             const float *__restrict__ sa, const float *__restrict__ sb,
                                                             const void *__restrict__ bias, int bias32, CT *__restrict__ C,
                                                             int64_t ldc, float *__restrict__ P, int M, int N, int K,
-                                                            int ksplit, int tiles_m, int tiles_n, int splits) {
+                                                            int ksplit, int tiles_m, int tiles_n, int splits, EPI ep) {
+  constexpr bool kRows = std::is_same_v<EPI, RowsEpi>;
   static_assert(kBNt == 256 || kBNt == 128, "tile widths: 256 or 128");
   static_assert(kMN || (kEl == 1 && !kC32), "bf16 operands and fp32 outputs: MN-major only");
   static_assert(!(kMN && kTail) || kBNt == 256, "MN-major rows masked lane by lane: the wide tile only");
@@ -239,7 +326,7 @@ __global__ __launch_bounds__(kThreads) void gemm_tn_kernel(const uint8_t *__rest
   // MN-major: the same loads for K rows with bit 5 set, whose chunks are swizzled with one more bit
   const int baseA1 = mrow * lda + 16 * (mchunk ^ kMFlip);
   const int baseB1 = mrowB * ldb + 16 * (mchunkB ^ kMFlip);
-  const float s = kEl == 1 ? sa[0] * sb[0] : 1.0f;
+  const float s = kEl == 1 && !kRows ? sa[0] * sb[0] : 1.0f;
 
   // ---- persistent: work item `it` (a tile and a K split) goes to workgroup it % gridDim.x. The grid is a multiple
   // of 8 (or covers every item in one pass), so it & 7 is the XCD the workgroup runs on and xcd_remap gives each
@@ -547,6 +634,92 @@ __global__ __launch_bounds__(kThreads) void gemm_tn_kernel(const uint8_t *__rest
                                                  r < rows_c && n < N ? (r * N + n) * 4 : kOOB, 0, 0);
         }
       pend = kStoresF32;
+    } else if constexpr (kRows) {
+      // The row-scaled epilogue. The accumulators go through LDS as fp32, one 16-row block of the wave at a time (8 KiB, the
+      // narrow tile 4: the same regions as below), so that each lane holds 8 consecutive columns of a row and the same
+      // columns in every row: its scales and biases are loaded once a tile, residual and C move as whole row segments.
+      // 16-byte chunk c (4 columns) of row r sits in slot c ^ r: the 16 lanes of a write (one chunk of 16 rows) hit
+      // 16 different slots. Those of a read take 16 runs of two chunks (wide: of one row; narrow: of two); where they
+      // are of one row, the upper 8 lanes read their second chunk first, so that both reads hit 16 different slots mod 16.
+      GPIC_LDS uint8_t *cst =
+          (GPIC_LDS uint8_t *)smem + (group == 0 ? a_half(2) : b_half(1)) + (wave & 3) * kCStage;
+      constexpr int kRow = kWTNt * 4, kLPR = kWTNt / 8, kRPI = 64 / kLPR, kNI = 16 / kRPI;
+      static_assert(16 * kRow == kCStage && kTM * kNI == kStoresBF16, "the same LDS and the same stores as the bf16 epilogue");
+      const bool half = ep.act == GPIC_ACT_SWIGLU;
+      const int rr = (unsigned)el / kLPR, rc = (unsigned)el % kLPR, flip = kBNt == 256 ? rc >> 3 : 0;
+      const int n = cur.n0 + wn * kWTNt + 8 * rc, no = half ? n >> 1 : n;
+      const bool in = n < N;
+      const __amdgpu_buffer_rsrc_t rC = __builtin_amdgcn_make_buffer_rsrc((void *)(C + (int64_t)cur.m0 * ldc), 0,
+                                                                          rows_c * (int)ldc * 2, kBufferFlags);
+      const __amdgpu_buffer_rsrc_t rR = __builtin_amdgcn_make_buffer_rsrc(
+          (void *)(ep.res + (int64_t)cur.m0 * ep.ldr), 0, ep.res ? rows_c * ep.ldr * 2 : 0, kBufferFlags);
+      const __amdgpu_buffer_rsrc_t rZ = __builtin_amdgcn_make_buffer_rsrc(
+          (void *)(ep.z + (int64_t)cur.m0 * ep.ldz), 0, ep.z ? rows_c * ep.ldz * 2 : 0, kBufferFlags);
+      float sb8[8], b8[8];
+      vec8(in ? ep.sb : nullptr, true, n, 1.0f, sb8);
+      vec8(in ? ep.bias : nullptr, ep.bias32, n, 0.0f, b8);
+      // lane l: the scale and the gate's row of the wave's row l (rows past M: the last one's)
+      const int mrow_l = min(cur.m0 + wm * kWTM + el, M - 1);
+      const float sa_l = ep.sa ? ep.sa[mrow_l] : 1.0f;
+      const int gb_l = ep.gate ? (int)((uint32_t)mrow_l / ep.ntok) : 0;
+#pragma unroll
+      for (int mi = 0; mi < kTM; mi++) {
+        const int rl0 = wm * kWTM + mi * 16 + rr;   // row within the tile of j = 0; row j is rl0 + kRPI j
+        u32x4 R[kNI], G[kNI];
+#pragma unroll
+        for (int j = 0; j < kNI; j++) {
+          const int rl = rl0 + kRPI * j;
+          R[j] = G[j] = u32x4{0u, 0u, 0u, 0u};
+          if (ep.res) {
+            const int off = in && rl < rows_c ? (rl * ep.ldr + no) * 2 : kOOB;
+            if (half) {
+              const u32x2 h = __builtin_bit_cast(u32x2, __builtin_amdgcn_raw_buffer_load_b64(rR, off, 0, 0));
+              R[j] = u32x4{h.x, h.y, 0u, 0u};
+            } else {
+              R[j] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(rR, off, 0, 0));
+            }
+          }
+          if (ep.gate) {   // (the shuffle with every lane active; columns past N read the row's first)
+            const uint16_t *g = ep.gate + (int64_t)__shfl(gb_l, mi * 16 + kRPI * j + rr, 64) * ep.sg + (in ? no : 0);
+            if (half) {
+              const u32x2 h = *reinterpret_cast<const u32x2 *>(g);
+              G[j] = u32x4{h.x, h.y, 0u, 0u};
+            } else {
+              G[j] = *reinterpret_cast<const u32x4 *>(g);
+            }
+          }
+        }
+#pragma unroll
+        for (int ni = 0; ni < kTNt; ni++)
+          *(GPIC_LDS f4a_t *)(cst + wr * kRow + 16 * ((8 * (ni >> 1) + 2 * wg + (ni & 1)) ^ wr)) = acc[ni][mi];
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // the block is complete before any lane reads it back
+        f4a_t X[kNI], Y[kNI];
+#pragma unroll
+        for (int j = 0; j < kNI; j++) {
+          const int r = kRPI * j + rr;
+          X[j] = *(const GPIC_LDS f4a_t *)(cst + r * kRow + 16 * ((2 * rc + flip) ^ r));
+          Y[j] = *(const GPIC_LDS f4a_t *)(cst + r * kRow + 16 * ((2 * rc + 1 - flip) ^ r));
+        }
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // read back before the next block overwrites it
+#pragma unroll
+        for (int j = 0; j < kNI; j++) {
+          const int rl = rl0 + kRPI * j;
+          float v[8];
+#pragma unroll
+          for (int e = 0; e < 4; e++) {
+            v[e] = flip ? Y[j][e] : X[j][e];
+            v[4 + e] = flip ? X[j][e] : Y[j][e];
+          }
+          const u32x4 y = epi8(ep, v, __shfl(sa_l, mi * 16 + kRPI * j + rr, 64), sb8, b8, R[j], G[j]);
+          const bool on = in && rl < rows_c;
+          if (ep.z)
+            __builtin_amdgcn_raw_buffer_store_b128(pack8(v), rZ, on ? (rl * ep.ldz + n) * 2 : kOOB, 0, kStoreNT);
+          const int off = on ? (rl * (int)ldc + no) * 2 : kOOB;
+          if (half) __builtin_amdgcn_raw_buffer_store_b64(u32x2{y.x, y.y}, rC, off, 0, kStoreNT);
+          else __builtin_amdgcn_raw_buffer_store_b128(y, rC, off, 0, kStoreNT);
+        }
+      }
+      pend = ep.z ? 2 * kStoresBF16 : kStoresBF16;
     } else {
       // bf16 output through LDS: each lane rounds its runs of 8 columns (scaled) to bf16 and writes them to LDS as
       // 16 bytes (MN-major: its runs of 4 as 8 bytes), one 32 x 128 block (two 16-row tile rows) of the wave at a
@@ -646,13 +819,13 @@ __global__ __launch_bounds__(kThreads) void gemm_tn_kernel(const uint8_t *__rest
 // summed in the same order with the same instruction, so the results have the same bits as the other classes': where
 // their plan splits K, the accumulators are folded into a sum after every `per` K tiles (kSplit), as the reduce adds the
 // splits' partials.
-template <int kSM, int kSN, int kSS, bool kTail, bool kSplit>
+template <int kSM, int kSN, int kSS, bool kTail, bool kSplit, typename EPI = NoEpi>
 __global__ __launch_bounds__(256) void gemm_small_kernel(const uint8_t *__restrict__ A, int lda,
                                                          const uint8_t *__restrict__ B, int ldb,
                                                          const float *__restrict__ sa, const float *__restrict__ sb,
                                                          const void *__restrict__ bias, int bias32,
                                                          uint16_t *__restrict__ C, int64_t ldc, int M, int N, int K,
-                                                         int tiles_n, int per) {
+                                                         int tiles_n, int per, EPI ep) {
   constexpr int kA = kSM * kBK, kStage = (kSM + kSN) * kBK;   // bytes of a stage's A part, of a stage
   constexpr int kLA = kSM / 32, kLB = kSN / 32, kL = kLA + kLB;   // loads per wave and K tile: 8 rows each
   constexpr int kFM = kSM / 32, kFN = kSN / 32;               // 16 x 16 tiles per wave
@@ -748,6 +921,24 @@ __global__ __launch_bounds__(256) void gemm_small_kernel(const uint8_t *__restri
 #pragma unroll
       for (int j = 0; j < kFM; j++) acc[i][j] = sum[i][j];
   }
+  if constexpr (std::is_same_v<EPI, RowsEpi>) {
+#pragma unroll
+    for (int p = 0; p < kFN / 2; p++) {
+      const int n = n0 + wn * (kSN / 2) + 32 * p + 8 * (lane >> 4);
+      if (n >= N) continue;
+      float sb8[8], b8[8];
+      vec8(ep.sb, true, n, 1.0f, sb8);
+      vec8(ep.bias, ep.bias32, n, 0.0f, b8);
+#pragma unroll
+      for (int mi = 0; mi < kFM; mi++) {
+        const int m = m0 + wm * (kSM / 2) + 16 * mi + frow;
+        const v4f &x = acc[2 * p][mi], &y = acc[2 * p + 1][mi];
+        float v[8] = {x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]};
+        if (m < M) epi8_row(ep, v, sb8, b8, C, ldc, m, n);
+      }
+    }
+    return;
+  }
   const float s = sa[0] * sb[0];
 #pragma unroll
   for (int p = 0; p < kFN / 2; p++) {
@@ -799,6 +990,89 @@ __global__ __launch_bounds__(256) void splitk_reduce_kernel(const float *__restr
       *reinterpret_cast<u32x4 *>(C + m * ldc + n) = u32x4{w.x << 16, w.x & 0xffff0000u, w.y << 16, w.y & 0xffff0000u};
     else *reinterpret_cast<u32x2 *>(C + m * ldc + n) = w;
   }
+}
+
+// The same sum of the partials with the row-scaled epilogue, 8 columns a thread.
+__global__ __launch_bounds__(256) void splitk_rows_kernel(const float *__restrict__ P, int splits, int M, int N,
+                                                          uint16_t *__restrict__ C, int64_t ldc, RowsEpi ep) {
+  const int64_t runs = (int64_t)M * (N / 8);
+  for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < runs; i += (int64_t)gridDim.x * blockDim.x) {
+    const int64_t m = i / (N / 8);
+    const int n = (int)(i % (N / 8)) * 8;
+    v4f x{0.0f, 0.0f, 0.0f, 0.0f}, y = x;
+    for (int z = 0; z < splits; z++) {
+      const v4f *q = reinterpret_cast<const v4f *>(P + ((int64_t)z * M + m) * N + n);
+      x += q[0];
+      y += q[1];
+    }
+    float v[8] = {x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]}, sb8[8], b8[8];
+    vec8(ep.sb, true, n, 1.0f, sb8);
+    vec8(ep.bias, ep.bias32, n, 0.0f, b8);
+    epi8_row(ep, v, sb8, b8, C, ldc, m, n);
+  }
+}
+
+// Few rows (kF blocks of 16): the weight's bytes bound it, each read once. A workgroup takes 16 columns, its kW waves every
+// kW-th K tile, straight from memory into the MFMA's operand registers (lane l: row l & 15, 32 bytes at K 32 (l / 16): whole
+// 128-byte lines), and the waves' sums are added in their order through LDS. Rows past M read the last row.
+template <int kF, int kW>
+__global__ __launch_bounds__(64 * kW) void gemm_few_kernel(const uint8_t *__restrict__ A, int64_t lda,
+                                                           const uint8_t *__restrict__ B, int64_t ldb,
+                                                           uint16_t *__restrict__ C, int64_t ldc, int M, int K, RowsEpi ep) {
+  __shared__ __attribute__((aligned(16))) f4a_t red[kW][kF][64];
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int n0 = blockIdx.x * 16, row = lane & 15, kl = 32 * (lane >> 4);
+  const uint8_t *b = B + (n0 + row) * ldb + kl;
+  const uint8_t *a[kF];
+#pragma unroll
+  for (int f = 0; f < kF; f++) a[f] = A + (int64_t)min(16 * f + row, M - 1) * lda + kl;
+  v4f acc[kF];
+#pragma unroll
+  for (int f = 0; f < kF; f++) acc[f] = v4f{};
+  auto frag = [&](const uint8_t *p, int k0) {   // (K % 16 == 0: a 16-byte half lies in K or past it)
+    u32x4 x{0u, 0u, 0u, 0u}, y{0u, 0u, 0u, 0u};
+    if (k0 + kl < K) x = *reinterpret_cast<const u32x4 *>(p + k0);
+    if (k0 + kl + 16 < K) y = *reinterpret_cast<const u32x4 *>(p + k0 + 16);
+    return v8i{(int)x.x, (int)x.y, (int)x.z, (int)x.w, (int)y.x, (int)y.y, (int)y.z, (int)y.w};
+  };
+  const int nk = (K + kBK - 1) / kBK;
+  constexpr int kU = kF == 1 ? 4 : 2;   // K tiles in flight
+  for (int kt = wave; kt < nk; kt += kU * kW) {
+    v8i fb[kU], fa[kU][kF];
+#pragma unroll
+    for (int u = 0; u < kU; u++) {   // (tiles past K: zeros)
+      const int k0 = (kt + u * kW) * kBK;
+      fb[u] = frag(b, k0);
+#pragma unroll
+      for (int f = 0; f < kF; f++) fa[u][f] = frag(a[f], k0);
+    }
+#pragma unroll
+    for (int u = 0; u < kU; u++)
+#pragma unroll
+      for (int f = 0; f < kF; f++)
+        acc[f] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(fb[u], fa[u][f], acc[f], 0, 0, 0, 0, 0, 0);
+  }
+#pragma unroll
+  for (int f = 0; f < kF; f++) red[wave][f][lane] = acc[f];
+  __syncthreads();
+  if (wave >= kF) return;
+  // wave f: lane l holds C[16 f + (l & 15)][n0 + 4 (l / 16) + [0, 4)]; with lane l ^ 16, runs of 8
+  f4a_t s = red[0][wave][lane];
+#pragma unroll
+  for (int w = 1; w < kW; w++) s += red[w][wave][lane];
+  float v[8];
+#pragma unroll
+  for (int e = 0; e < 4; e++) {
+    v[e] = s[e];
+    v[4 + e] = __shfl_xor(s[e], 16, 64);
+  }
+  const int m = 16 * wave + row, n = n0 + 4 * (lane >> 4);
+  if ((lane & 16) || m >= M) return;
+  float sb8[8], b8[8];
+  vec8(ep.sb, true, n, 1.0f, sb8);
+  vec8(ep.bias, ep.bias32, n, 0.0f, b8);
+  epi8_row(ep, v, sb8, b8, C, ldc, m, n);
 }
 
 // ------------------------------------------------------------------------------------------- host side
@@ -894,16 +1168,16 @@ static Plan plan_of(int64_t M, int64_t N, int64_t K) {
   return p;
 }
 
-template <int kSM, int kSN, int kSS>
+template <int kSM, int kSN, int kSS, typename EPI>
 static void launch_small(const void *A, int64_t lda, const float *sa, const void *B, int64_t ldb, const float *sb,
                          const void *bias, int bias32, uint16_t *C, int64_t ldc, int64_t M, int64_t N, int64_t K,
-                         const Plan &p, hipStream_t st) {
+                         const Plan &p, hipStream_t st, const EPI &ep) {
   const int tiles_n = (int)((N + kSN - 1) / kSN), tiles = (int)((M + kSM - 1) / kSM) * tiles_n;
-  auto *kernel = K % kBK ? gemm_small_kernel<kSM, kSN, kSS, true, false> : gemm_small_kernel<kSM, kSN, kSS, false, false>;
-  if constexpr (kSM < 128)   // (the largest tile takes no split plan)
+  auto *kernel = K % kBK ? gemm_small_kernel<kSM, kSN, kSS, true, false, EPI> : gemm_small_kernel<kSM, kSN, kSS, false, false, EPI>;
+  if constexpr (kSM < 128 && std::is_same_v<EPI, NoEpi>)   // (the largest tile takes no split plan)
     if (p.splits > 1) kernel = K % kBK ? gemm_small_kernel<kSM, kSN, kSS, true, true> : gemm_small_kernel<kSM, kSN, kSS, false, true>;
   kernel<<<tiles, 256, 0, st>>>(static_cast<const uint8_t *>(A), (int)lda, static_cast<const uint8_t *>(B), (int)ldb, sa,
-                                sb, bias, bias32, C, ldc, (int)M, (int)N, (int)K, tiles_n, p.ksplit / kBK);
+                                sb, bias, bias32, C, ldc, (int)M, (int)N, (int)K, tiles_n, p.ksplit / kBK, ep);
 }
 
 // Millions of bytes that the eight XCDs read for t small-class tiles of sm x 64 in xcd_remap's order: each, through its own
@@ -942,20 +1216,21 @@ static bool small_beats_split(const Plan &p, int64_t sm, int64_t t, int64_t M, i
 //   110 MB ([512 x 6144 x 2560] 22.2 us against 20.2, [512 x 6144 x 4608] 35.6 / 32.2; [800 x 3072 x 4096], 107 MB, 24.7 / 28.9).
 // Plans that split K take the 32 x 64 or 64 x 64 tile where small_beats_split says so (their partials and the reduce's
 // launch fall away).
+template <typename EPI = NoEpi>
 static bool launch_small_class(const void *A, int64_t lda, const float *sa, const void *B, int64_t ldb, const float *sb,
                                const void *bias, int bias32, uint16_t *C, int64_t ldc, int64_t M, int64_t N, int64_t K,
-                               const Plan &p, hipStream_t st) {
+                               const Plan &p, hipStream_t st, const EPI &ep = EPI()) {
   const int64_t cus = num_cus(), n64 = (N + 63) / 64, t32 = (M + 31) / 32 * n64, t64 = (M + 63) / 64 * n64,
                 t128 = (M + 127) / 128 * n64;
   const bool split = p.splits > 1;
   if (t32 <= 2 * cus) {
     if (split && !small_beats_split(p, 32, t32, M, N, K)) return false;
-    launch_small<32, 64, 4>(A, lda, sa, B, ldb, sb, bias, bias32, C, ldc, M, N, K, p, st);
+    launch_small<32, 64, 4>(A, lda, sa, B, ldb, sb, bias, bias32, C, ldc, M, N, K, p, st, ep);
   } else if (t64 <= 3 * cus && (split || t64 <= 2 * cus || small_traffic(64, t64, M, N, K) <= 110.0)) {
     if (split && !small_beats_split(p, 64, t64, M, N, K)) return false;
-    launch_small<64, 64, 3>(A, lda, sa, B, ldb, sb, bias, bias32, C, ldc, M, N, K, p, st);
+    launch_small<64, 64, 3>(A, lda, sa, B, ldb, sb, bias, bias32, C, ldc, M, N, K, p, st, ep);
   } else if (t128 <= 2 * cus && !split) {
-    launch_small<128, 64, 3>(A, lda, sa, B, ldb, sb, bias, bias32, C, ldc, M, N, K, p, st);
+    launch_small<128, 64, 3>(A, lda, sa, B, ldb, sb, bias, bias32, C, ldc, M, N, K, p, st, ep);
   } else {
     return false;
   }
@@ -1001,12 +1276,47 @@ static int launch_gemm(const void *A, int64_t lda, const float *sa, const void *
   }
   kernel<<<grid, kThreads, 0, st>>>(
       static_cast<const uint8_t *>(A), (int)lda * kEl, static_cast<const uint8_t *>(B), (int)ldb * kEl, sa, sb, bias, bias32, C,
-      ldc, P, (int)M, (int)N, (int)K, p.ksplit, p.tiles_m, p.tiles_n, p.splits);
+      ldc, P, (int)M, (int)N, (int)K, p.ksplit, p.tiles_m, p.tiles_n, p.splits, NoEpi());
   if (P) {
     const int64_t quads = M * (N / 4);
     int64_t g = (quads + 255) / 256;
     if (g > 8192) g = 8192;
     splitk_reduce_kernel<CT><<<(int)g, 256, 0, st>>>(P, p.splits, (int)M, (int)N, sa, sb, bias, bias32, C, ldc);
+  }
+  return (int)hipGetLastError();
+}
+
+// The row-scaled GEMM (arguments checked by the entry point; M, N, K > 0): the same plans and tile classes.
+static int launch_gemm_rows(const uint8_t *A, int64_t lda, const uint8_t *B, int64_t ldb, uint16_t *C, int64_t ldc, int64_t M,
+                            int64_t N, int64_t K, const RowsEpi &ep, void *ws, size_t ws_bytes, hipStream_t st) {
+  Plan p = plan_of(M, N, K);
+  float *P = nullptr;
+  if (p.splits > 1) {
+    if (!ws || ws_bytes < (size_t)p.splits * M * N * sizeof(float)) return GPIC_EWORKSPACE;
+    if (!aligned16(ws)) return GPIC_EALIGN;
+    P = static_cast<float *>(ws);
+  }
+  if (M <= 32) {
+    auto *few = M <= 16 ? (K <= 512 ? gemm_few_kernel<1, 4> : K <= 2048 ? gemm_few_kernel<1, 8> : gemm_few_kernel<1, 16>)
+                        : (K <= 512 ? gemm_few_kernel<2, 4> : K <= 2048 ? gemm_few_kernel<2, 8> : gemm_few_kernel<2, 16>);
+    const int threads = K <= 512 ? 256 : K <= 2048 ? 512 : 1024;
+    few<<<(unsigned)(N / 16), threads, 0, st>>>(A, lda, B, ldb, C, ldc, (int)M, (int)K, ep);
+    return (int)hipGetLastError();
+  }
+  if (launch_small_class<RowsEpi>(A, lda, nullptr, B, ldb, nullptr, nullptr, 0, C, ldc, M, N, K, p, st, ep))
+    return (int)hipGetLastError();
+  const int work = p.tiles_m * p.tiles_n * p.splits;
+  const int slots = num_cus() & ~7;
+  const int grid = work <= slots || slots < 8 ? work : slots;
+  auto *kernel = p.bn == 128 ? (K % kBK ? gemm_tn_kernel<true, false, 128, 1, false, RowsEpi>
+                                        : gemm_tn_kernel<false, false, 128, 1, false, RowsEpi>)
+                             : (K % kBK ? gemm_tn_kernel<true, false, 256, 1, false, RowsEpi>
+                                        : gemm_tn_kernel<false, false, 256, 1, false, RowsEpi>);
+  kernel<<<grid, kThreads, 0, st>>>(A, (int)lda, B, (int)ldb, nullptr, nullptr, nullptr, 0, C, ldc, P, (int)M, (int)N, (int)K,
+                                    p.ksplit, p.tiles_m, p.tiles_n, p.splits, ep);
+  if (P) {
+    const int64_t g = (M * (N / 8) + 255) / 256;
+    splitk_rows_kernel<<<(int)std::min<int64_t>(g, 8192), 256, 0, st>>>(P, p.splits, (int)M, (int)N, C, ldc, ep);
   }
   return (int)hipGetLastError();
 }
@@ -1046,6 +1356,29 @@ int gpic_fp8_gemm_bias32(const uint8_t *A, int64_t lda, const float *sa, const u
   if (M < 0 || N < 0 || K < 0 || !sa || !sb || !bias || (M > 0 && N > 0 && !C)) return GPIC_EINVAL;
   if (!tn_shape_ok(lda, ldb, ldc, M, N, K)) return GPIC_ESHAPE;
   return launch_gemm<false>(A, lda, sa, B, ldb, sb, bias, C, ldc, M, N, K, ws, ws_bytes, (hipStream_t)stream, 1);
+}
+
+int gpic_fp8_gemm_rows(const uint8_t *A, int64_t lda, const float *sa, const uint8_t *B, int64_t ldb, const float *sb,
+                       const void *bias, int bias_dtype, int act, const uint16_t *res, int64_t ldr, const uint16_t *gate,
+                       int64_t sg, int64_t ntok, uint16_t *C, int64_t ldc, uint16_t *z, int64_t ldz, int64_t M, int64_t N,
+                       int64_t K, void *ws, size_t ws_bytes, void *stream) {
+  status_scope();
+  if (M < 0 || N < 0 || K <= 0 || act < GPIC_ACT_NONE || act > GPIC_ACT_SWIGLU || (gate && ntok <= 0)) return GPIC_EINVAL;
+  if (M > 0 && N > 0 && (!A || !B || !C)) return GPIC_EINVAL;
+  if (bias && bias_dtype != GPIC_DTYPE_BF16 && bias_dtype != GPIC_DTYPE_F32) return GPIC_EDTYPE;
+  const int64_t No = act == GPIC_ACT_SWIGLU ? N / 2 : N;
+  if (!tn_shape_ok(lda, ldb, std::max(ldc, N), M, N, K) || ldc < No || ldc % 8) return GPIC_ESHAPE;
+  if (act == GPIC_ACT_SWIGLU && N % 32) return GPIC_ESHAPE;
+  if ((res && (ldr % 8 || ldr < No || ldr >= (1 << 22))) || (z && (ldz % 8 || ldz < N || ldz >= (1 << 22))) ||
+      (gate && (sg % 8 || sg < No || M % ntok)))
+    return GPIC_ESHAPE;
+  if (!aligned16(A) || !aligned16(B) || !aligned16(C) || !aligned16(sb) || !aligned16(bias) || !aligned16(res) ||
+      !aligned16(gate) || !aligned16(z))
+    return GPIC_EALIGN;
+  if (M == 0 || N == 0) return GPIC_OK;
+  const RowsEpi ep{sa, sb, bias, res, gate, z, sg, (uint32_t)(gate ? ntok : 1), (int)ldr, (int)ldz,
+                   bias && bias_dtype == GPIC_DTYPE_F32, act};
+  return launch_gemm_rows(A, lda, B, ldb, C, ldc, M, N, K, ep, ws, ws_bytes, (hipStream_t)stream);
 }
 
 int gpic_fp8_gemm_mn(const uint8_t *A, int64_t lda, const float *sa, const uint8_t *B, int64_t ldb, const float *sb,

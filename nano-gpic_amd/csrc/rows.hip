@@ -1,0 +1,573 @@
+// The row-scaled producers: operators whose e4m3 output carries one scale per row (token, or output channel of a weight)
+// instead of one per tensor. A row's maximum is known to the threads that hold the row, so there is no fold over the chip
+// and no second pass: each kernel reads its inputs once and writes its outputs once, and one row alone is one short launch.
+//
+//   row cast      a = max(max|h|, 1e-12), s = RN(a / 448), q = e4m3(min(max(RN(h RN(448 / a)), -448), 448))
+//   norm          x_new = bf16(x + gate a); rstd = 1 / sqrt(mean(x_new^2) + eps);
+//                 h = (w (x_new rstd)) (1 + scale) + shift, cast by row
+//   its backward  t = x_new rstd, dt = dh w, dx = bf16(rstd (dt - t mean(dt t)) + dx_new), dw = sum over rows of dh t
+//   activation's backward  dz = dy act'(z) as bf16, and (dz sw) cast by row
+//
+// h and dz sw are fp32 until the one rounding to e4m3: the tensorwise norm sites (norm.hip) round n and h to bf16 because the
+// reference's ops hand them on in bf16; here nothing between the row's statistics and its bytes is held in memory.
+// A NaN anywhere in a row makes the row's maximum, and so its scale, NaN (the maximum of the magnitudes' bit patterns: a
+// NaN's is above infinity's): a product of the row is then NaN. The tensorwise casts ignore NaN, as the reference's.
+// An infinity makes the scale infinite.
+//
+// A team of T threads holds a row, 8 elements (16 bytes of bf16) a thread and step: a wave for rows of up to 2048, four waves
+// up to 8192, sixteen above. What bounds them is memory; each vector of a row is requested before any is used.
+#include <algorithm>
+#include <type_traits>
+
+#include "gpic_act.h"
+#include "gpic_launch.h"
+
+namespace gpic {
+
+constexpr int kMaxNormC = 16384;    // the norm's widest row (16 elements a thread: the backward also holds w and dw of them)
+constexpr int kMaxRowC = 32768;     // the casts' widest row
+constexpr int kMaxRowBlocks = 16384;
+
+__device__ __forceinline__ void unpack8(u32x4 v, float (&f)[8]) {
+  f[0] = bf16_lo(v.x), f[1] = bf16_hi(v.x), f[2] = bf16_lo(v.y), f[3] = bf16_hi(v.y);
+  f[4] = bf16_lo(v.z), f[5] = bf16_hi(v.z), f[6] = bf16_lo(v.w), f[7] = bf16_hi(v.w);
+}
+__device__ __forceinline__ u32x4 pack8(const float (&f)[8]) {
+  return u32x4{pack_bf16(f[0], f[1]), pack_bf16(f[2], f[3]), pack_bf16(f[4], f[5]), pack_bf16(f[6], f[7])};
+}
+__device__ __forceinline__ u32x4 ld16(const void *p) { return *reinterpret_cast<const u32x4 *>(p); }
+
+// Eight elements of a bf16 or (f32) fp32 vector at element c.
+__device__ __forceinline__ void load8(const void *p, bool f32, int64_t c, float (&f)[8]) {
+  if (f32) {
+    const float4 x = *reinterpret_cast<const float4 *>(static_cast<const float *>(p) + c);
+    const float4 y = *reinterpret_cast<const float4 *>(static_cast<const float *>(p) + c + 4);
+    f[0] = x.x, f[1] = x.y, f[2] = x.z, f[3] = x.w, f[4] = y.x, f[5] = y.y, f[6] = y.z, f[7] = y.w;
+  } else {
+    unpack8(ld16(static_cast<const uint16_t *>(p) + c), f);
+  }
+}
+
+__device__ __forceinline__ u32x2 cast8(const float (&h)[8], float s) {
+  return u32x2{e4m3x4(sat(h[0] * s), sat(h[1] * s), sat(h[2] * s), sat(h[3] * s)),
+               e4m3x4(sat(h[4] * s), sat(h[5] * s), sat(h[6] * s), sat(h[7] * s))};
+}
+
+__device__ __forceinline__ uint32_t absmax8(const float (&h)[8], uint32_t m) {
+#pragma unroll
+  for (int e = 0; e < 8; e++) m = max(m, __float_as_uint(h[e]) & 0x7fffffffu);
+  return m;
+}
+
+// Sum, or maximum, over a team of T threads (T == 64: one wave; else the whole workgroup, through LDS, the waves' values in
+// their order), the result in every thread. red: T / 64 words for this use alone; two uses alternate over a row, so the
+// barrier of one protects the words of the other from the next row's writes.
+template <int T>
+__device__ __forceinline__ float team_sum(float v, float *red) {
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
+  if constexpr (T > 64) {
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+    lds_barrier();
+    v = red[0];
+#pragma unroll
+    for (int i = 1; i < T / 64; i++) v += red[i];
+  }
+  return v;
+}
+template <int T>
+__device__ __forceinline__ uint32_t team_max(uint32_t v, uint32_t *red) {
+  v = wave_max_u32(v);
+  if constexpr (T > 64) {
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+    lds_barrier();
+    v = red[0];
+#pragma unroll
+    for (int i = 1; i < T / 64; i++) v = max(v, red[i]);
+  }
+  return v;
+}
+
+template <int T>
+constexpr int kWG = T > 256 ? T : 256;   // threads of a workgroup: 256 / T teams, or one
+
+// The team's first row and the rows between two of its rows.
+template <int T>
+__device__ __forceinline__ int64_t team_row() {
+  constexpr int R = kWG<T> / T;
+  if constexpr (R == 1) return blockIdx.x;
+  return (int64_t)blockIdx.x * R + __builtin_amdgcn_readfirstlane(threadIdx.x / T);
+}
+template <int T>
+__device__ __forceinline__ int64_t team_step() {
+  return (int64_t)gridDim.x * (kWG<T> / T);
+}
+
+struct NormRowsArgs {
+  const uint16_t *x, *a, *gate, *shift, *scale;
+  const void *w;
+  uint16_t *xn, *h;
+  float *rstd, *s;
+  uint8_t *q;
+  int64_t rows, ntok, ldx, lda, sg, ssh, ssc;
+  int C, w32;
+  float eps;
+};
+
+template <int T, int kV, bool kRes, bool kMod>
+__global__ __launch_bounds__(kWG<T>) void rmsnorm_rows_kernel(NormRowsArgs p) {
+  __shared__ float red_s[T > 64 ? T / 64 : 1];
+  __shared__ uint32_t red_m[T > 64 ? T / 64 : 1];
+  const int t = threadIdx.x % T, nv = p.C / 8;
+  for (int64_t row = team_row<T>(); row < p.rows; row += team_step<T>()) {
+    const int64_t b = kMod || (kRes && p.gate) ? (int64_t)((uint32_t)row / (uint32_t)p.ntok) : 0;
+    const uint16_t *xr = p.x + row * p.ldx;
+    const uint16_t *ar = kRes ? p.a + row * p.lda : nullptr;
+    u32x4 X[kV], A[kV];
+#pragma unroll
+    for (int j = 0; j < kV; j++) {
+      const int v = t + T * j;
+      X[j] = A[j] = u32x4{0u, 0u, 0u, 0u};
+      if (v < nv) {
+        X[j] = ld16(xr + 8 * v);
+        if (kRes) A[j] = ld16(ar + 8 * v);
+      }
+    }
+    float ss = 0.0f;
+#pragma unroll
+    for (int j = 0; j < kV; j++) {
+      const int v = t + T * j;
+      float x[8];
+      unpack8(X[j], x);
+      if (kRes && v < nv) {
+        float av[8];
+        unpack8(A[j], av);
+        if (p.gate) {
+          float g[8];
+          unpack8(ld16(p.gate + b * p.sg + 8 * v), g);
+#pragma unroll
+          for (int e = 0; e < 8; e++) x[e] = __builtin_fmaf(g[e], av[e], x[e]);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 8; e++) x[e] += av[e];
+        }
+        X[j] = pack8(x);
+        *reinterpret_cast<u32x4 *>(p.xn + row * p.C + 8 * v) = X[j];
+        unpack8(X[j], x);
+      }
+#pragma unroll
+      for (int e = 0; e < 8; e++) ss = __builtin_fmaf(x[e], x[e], ss);
+    }
+    ss = team_sum<T>(ss, red_s);
+    const float rstd = __fdiv_rn(1.0f, __builtin_sqrtf(__fdiv_rn(ss, (float)p.C) + p.eps));
+    float H[kV][8];
+    uint32_t m = 0;
+#pragma unroll
+    for (int j = 0; j < kV; j++) {
+      const int v = t + T * j;
+      if (v < nv) {
+        float x[8], w[8];
+        unpack8(X[j], x);
+        load8(p.w, p.w32, 8 * v, w);
+#pragma unroll
+        for (int e = 0; e < 8; e++) H[j][e] = w[e] * (x[e] * rstd);
+        if (kMod) {
+          float sh[8], sc[8];
+          unpack8(ld16(p.shift + b * p.ssh + 8 * v), sh);
+          unpack8(ld16(p.scale + b * p.ssc + 8 * v), sc);
+#pragma unroll
+          for (int e = 0; e < 8; e++) H[j][e] = __builtin_fmaf(H[j][e], 1.0f + sc[e], sh[e]);
+        }
+        m = absmax8(H[j], m);
+        if (p.h) *reinterpret_cast<u32x4 *>(p.h + row * p.C + 8 * v) = pack8(H[j]);
+      }
+    }
+    float scale, dequant;
+    scales_from_amax(team_max<T>(m, red_m), scale, dequant);
+#pragma unroll
+    for (int j = 0; j < kV; j++) {
+      const int v = t + T * j;
+      if (v < nv) *reinterpret_cast<u32x2 *>(p.q + row * p.C + 8 * v) = cast8(H[j], scale);
+    }
+    if (t == 0) {
+      p.s[row] = dequant;
+      p.rstd[row] = rstd;
+    }
+  }
+}
+
+template <int T, int kV, bool kF32>
+__global__ __launch_bounds__(kWG<T>) void tcast_rows_kernel(const void *__restrict__ x, int64_t ldx, int64_t rows, int C,
+                                                            uint8_t *__restrict__ q, float *__restrict__ s) {
+  __shared__ uint32_t red_m[2][T > 64 ? T / 64 : 1];
+  const int t = threadIdx.x % T, nv = C / 8;
+  int turn = 0;
+  for (int64_t row = team_row<T>(); row < rows; row += team_step<T>(), turn ^= 1) {
+    float H[kV][8];
+    uint32_t m = 0;
+#pragma unroll
+    for (int j = 0; j < kV; j++) {
+      const int v = t + T * j;
+      if (v < nv) load8(x, kF32, row * ldx + 8 * v, H[j]);
+    }
+#pragma unroll
+    for (int j = 0; j < kV; j++)
+      if (t + T * j < nv) m = absmax8(H[j], m);
+    float scale, dequant;
+    scales_from_amax(team_max<T>(m, red_m[turn]), scale, dequant);
+#pragma unroll
+    for (int j = 0; j < kV; j++) {
+      const int v = t + T * j;
+      if (v < nv) *reinterpret_cast<u32x2 *>(q + row * C + 8 * v) = cast8(H[j], scale);
+    }
+    if (t == 0) s[row] = dequant;
+  }
+}
+
+struct ActBwdArgs {
+  const uint16_t *dy, *z;
+  const float *sw;
+  uint16_t *dz;
+  uint8_t *q;
+  float *s;
+  int64_t rows, lddy, ldz;
+  int N, act;
+};
+
+template <int T, int kV>
+__global__ __launch_bounds__(kWG<T>) void act_bwd_rows_kernel(ActBwdArgs p) {
+  __shared__ uint32_t red_m[2][T > 64 ? T / 64 : 1];
+  const int t = threadIdx.x % T, nv = p.N / 8;
+  int turn = 0;
+  for (int64_t row = team_row<T>(); row < p.rows; row += team_step<T>(), turn ^= 1) {
+    u32x4 Y[kV], Z[kV];
+#pragma unroll
+    for (int j = 0; j < kV; j++) {
+      const int v = t + T * j;
+      Y[j] = Z[j] = u32x4{0u, 0u, 0u, 0u};
+      if (v < nv) {
+        Y[j] = ld16(p.dy + row * p.lddy + 8 * v);
+        if (p.act) Z[j] = ld16(p.z + row * p.ldz + 8 * v);
+      }
+    }
+    float H[kV][8];
+    uint32_t m = 0;
+#pragma unroll
+    for (int j = 0; j < kV; j++) {
+      const int v = t + T * j;
+      if (v < nv) {
+        float d[8], z[8];
+        unpack8(Y[j], d);
+        if (p.act) {
+          unpack8(Z[j], z);
+#pragma unroll
+          for (int e = 0; e < 8; e++) d[e] *= act_bwd(z[e], p.act);
+          *reinterpret_cast<u32x4 *>(p.dz + row * p.N + 8 * v) = pack8(d);
+        }
+        float w[8];
+        load8(p.sw, true, 8 * v, w);
+#pragma unroll
+        for (int e = 0; e < 8; e++) H[j][e] = d[e] * w[e];
+        m = absmax8(H[j], m);
+      }
+    }
+    float scale, dequant;
+    scales_from_amax(team_max<T>(m, red_m[turn]), scale, dequant);
+#pragma unroll
+    for (int j = 0; j < kV; j++) {
+      const int v = t + T * j;
+      if (v < nv) *reinterpret_cast<u32x2 *>(p.q + row * p.N + 8 * v) = cast8(H[j], scale);
+    }
+    if (t == 0) p.s[row] = dequant;
+  }
+}
+
+struct NormBwdRowsArgs {
+  const uint16_t *dh, *dxn, *xs;
+  const void *w;
+  const float *rstd;
+  uint16_t *dx;
+  float *P;   // [gridDim.x, C] partial sums of dw
+  int64_t rows;
+  int C, w32;
+};
+
+// The rows of a workgroup in their order, each thread's columns' dw in registers; a workgroup's teams are added in their
+// order, then the workgroups in theirs (rmsnorm_rows_dw_kernel): the same sums in every run.
+template <int T, int kV>
+__global__ __launch_bounds__(kWG<T>) void rmsnorm_rows_bwd_kernel(NormBwdRowsArgs p) {
+  constexpr int R = kWG<T> / T;
+  __shared__ float red_s[2][T > 64 ? T / 64 : 1];
+  __shared__ __attribute__((aligned(16))) float part[R > 1 ? T * kV * 8 : 4];
+  const int t = threadIdx.x % T, team = threadIdx.x / T, nv = p.C / 8;
+  float W[kV][8], D[kV][8];
+#pragma unroll
+  for (int j = 0; j < kV; j++) {
+    const int v = t + T * j;
+#pragma unroll
+    for (int e = 0; e < 8; e++) W[j][e] = D[j][e] = 0.0f;
+    if (v < nv) load8(p.w, p.w32, 8 * v, W[j]);
+  }
+  const float rC = 1.0f / (float)p.C;
+  int turn = 0;
+  for (int64_t row = team_row<T>(); row < p.rows; row += team_step<T>(), turn ^= 1) {
+    u32x4 Y[kV], X[kV], N[kV];
+#pragma unroll
+    for (int j = 0; j < kV; j++) {
+      const int v = t + T * j;
+      Y[j] = X[j] = N[j] = u32x4{0u, 0u, 0u, 0u};
+      if (v < nv) {
+        Y[j] = ld16(p.dh + row * p.C + 8 * v);
+        X[j] = ld16(p.xs + row * p.C + 8 * v);
+        if (p.dxn) N[j] = ld16(p.dxn + row * p.C + 8 * v);
+      }
+    }
+    const float rs = p.rstd[row];
+    float sum = 0.0f;
+#pragma unroll
+    for (int j = 0; j < kV; j++) {
+      float d[8], x[8];
+      unpack8(Y[j], d);
+      unpack8(X[j], x);
+#pragma unroll
+      for (int e = 0; e < 8; e++) {
+        const float tt = x[e] * rs;
+        sum = __builtin_fmaf(d[e] * W[j][e], tt, sum);
+        D[j][e] = __builtin_fmaf(d[e], tt, D[j][e]);
+      }
+    }
+    const float mean = team_sum<T>(sum, red_s[turn]) * rC;
+#pragma unroll
+    for (int j = 0; j < kV; j++) {
+      const int v = t + T * j;
+      if (v < nv) {
+        float d[8], x[8], n[8];
+        unpack8(Y[j], d);
+        unpack8(X[j], x);
+        unpack8(N[j], n);
+#pragma unroll
+        for (int e = 0; e < 8; e++)
+          n[e] = __builtin_fmaf(rs, __builtin_fmaf(-(x[e] * rs), mean, d[e] * W[j][e]), n[e]);
+        *reinterpret_cast<u32x4 *>(p.dx + row * p.C + 8 * v) = pack8(n);
+      }
+    }
+  }
+  if constexpr (R > 1) {   // the teams' sums, added in their order by the first
+    for (int i = 1; i < R; i++) {
+      __syncthreads();
+      if (team == i) {
+#pragma unroll
+        for (int j = 0; j < kV; j++)
+#pragma unroll
+          for (int e = 0; e < 8; e++) part[(j * 8 + e) * T + t] = D[j][e];
+      }
+      __syncthreads();
+      if (team == 0) {
+#pragma unroll
+        for (int j = 0; j < kV; j++)
+#pragma unroll
+          for (int e = 0; e < 8; e++) D[j][e] += part[(j * 8 + e) * T + t];
+      }
+    }
+    if (team != 0) return;
+  }
+#pragma unroll
+  for (int j = 0; j < kV; j++) {
+    const int v = t + T * j;
+    if (v < nv) {
+      float *o = p.P + (int64_t)blockIdx.x * p.C + 8 * v;
+      *reinterpret_cast<float4 *>(o) = float4{D[j][0], D[j][1], D[j][2], D[j][3]};
+      *reinterpret_cast<float4 *>(o + 4) = float4{D[j][4], D[j][5], D[j][6], D[j][7]};
+    }
+  }
+}
+
+// dw[c] = sum over g of P[g, c]: 16 threads of a workgroup take 64 columns, its 16 groups every 16th row each.
+__global__ __launch_bounds__(256) void rmsnorm_rows_dw_kernel(const float *__restrict__ P, int G, int C,
+                                                              void *__restrict__ dw, int dw32) {
+  __shared__ float4 red[16][16];
+  const int c4 = threadIdx.x & 15, g0 = threadIdx.x >> 4;
+  const int c = blockIdx.x * 64 + 4 * c4;
+  float4 a{0.0f, 0.0f, 0.0f, 0.0f};
+  if (c < C)
+    for (int g = g0; g < G; g += 16) {
+      const float4 v = *reinterpret_cast<const float4 *>(P + (int64_t)g * C + c);
+      a.x += v.x, a.y += v.y, a.z += v.z, a.w += v.w;
+    }
+  red[g0][c4] = a;
+  __syncthreads();
+  if (g0 != 0 || c >= C) return;
+  for (int i = 1; i < 16; i++) {
+    const float4 v = red[i][c4];
+    a.x += v.x, a.y += v.y, a.z += v.z, a.w += v.w;
+  }
+  if (dw32) *reinterpret_cast<float4 *>(static_cast<float *>(dw) + c) = a;
+  else
+    *reinterpret_cast<u32x2 *>(static_cast<uint16_t *>(dw) + c) = u32x2{pack_bf16(a.x, a.y), pack_bf16(a.z, a.w)};
+}
+
+// qt[c, r] = q[r, c]: tiles of 64 x 64 bytes through LDS, 16 bytes a thread in and out; columns rows .. ldt - 1 of qt zero.
+__global__ __launch_bounds__(256) void transpose_bytes_kernel(const uint8_t *__restrict__ q, int64_t rows, int64_t cols,
+                                                              uint8_t *__restrict__ qt, int64_t ldt, int64_t tiles_c) {
+  __shared__ uint8_t tile[64][80];   // (80: 16-byte rows on different banks)
+  const int64_t r0 = (int64_t)blockIdx.x / tiles_c * 64, c0 = (int64_t)blockIdx.x % tiles_c * 64;
+  const int i = threadIdx.x >> 2, k = 16 * (threadIdx.x & 3);
+  u32x4 v{0u, 0u, 0u, 0u};
+  if (r0 + i < rows && c0 + k < cols) v = ld16(q + (r0 + i) * cols + c0 + k);
+  *reinterpret_cast<u32x4 *>(&tile[i][k]) = v;
+  __syncthreads();
+  if (c0 + i < cols && r0 + k < ldt) {
+    uint32_t o[4];
+#pragma unroll
+    for (int w = 0; w < 4; w++)
+      o[w] = (uint32_t)tile[k + 4 * w][i] | (uint32_t)tile[k + 4 * w + 1][i] << 8 |
+             (uint32_t)tile[k + 4 * w + 2][i] << 16 | (uint32_t)tile[k + 4 * w + 3][i] << 24;
+    *reinterpret_cast<u32x4 *>(qt + (c0 + i) * ldt + r0 + k) = u32x4{o[0], o[1], o[2], o[3]};
+  }
+}
+
+// ------------------------------------------------------------------------------------------- host side
+
+// Calls f(T, kV) with the team and the steps for rows of C elements (C <= 8 T kV).
+template <class F>
+static void with_team(int64_t C, F f) {
+  typedef std::integral_constant<int, 64> W;
+  typedef std::integral_constant<int, 256> Q;
+  typedef std::integral_constant<int, 1024> S;
+  typedef std::integral_constant<int, 1> V1;
+  typedef std::integral_constant<int, 2> V2;
+  typedef std::integral_constant<int, 4> V4;
+  if (C <= 512) f(W(), V1());
+  else if (C <= 1024) f(W(), V2());
+  else if (C <= 2048) f(W(), V4());
+  else if (C <= 4096) f(Q(), V2());
+  else if (C <= 8192) f(Q(), V4());
+  else if (C <= 16384) f(S(), V2());
+  else f(S(), V4());
+}
+
+static unsigned row_blocks(int64_t rows, int teams) {
+  return (unsigned)std::min<int64_t>((rows + teams - 1) / teams, kMaxRowBlocks);
+}
+
+static bool dtype_ok(int d) { return d == GPIC_DTYPE_BF16 || d == GPIC_DTYPE_F32; }
+
+// Workgroups of the norm's backward: each leaves a partial row of dw.
+static int norm_bwd_blocks(int64_t rows, int64_t C) {
+  const int teams = C <= 2048 ? 4 : 1;
+  return (int)std::min<int64_t>((rows + teams - 1) / teams, 512);
+}
+
+}  // namespace gpic
+
+using namespace gpic;
+
+extern "C" {
+
+int gpic_fp8_tcast_rows(const void *x, int dtype, int64_t ldx, int64_t rows, int64_t cols, uint8_t *q, float *s,
+                        void *stream) {
+  status_scope();
+  if (rows < 0 || cols <= 0 || (rows > 0 && (!x || !q || !s))) return GPIC_EINVAL;
+  if (!dtype_ok(dtype)) return GPIC_EDTYPE;
+  if (cols % 8 || cols > kMaxRowC || ldx % 8 || ldx < cols) return GPIC_ESHAPE;
+  if (!aligned16(x) || !aligned16(q)) return GPIC_EALIGN;
+  if (rows == 0) return GPIC_OK;
+  const hipStream_t st = (hipStream_t)stream;
+  with_team(cols, [&](auto T, auto V) {
+    constexpr int t = decltype(T)::value, v = decltype(V)::value;
+    const unsigned g = row_blocks(rows, kWG<t> / t);
+    if (dtype == GPIC_DTYPE_F32) tcast_rows_kernel<t, v, true><<<g, kWG<t>, 0, st>>>(x, ldx, rows, (int)cols, q, s);
+    else tcast_rows_kernel<t, v, false><<<g, kWG<t>, 0, st>>>(x, ldx, rows, (int)cols, q, s);
+  });
+  return (int)hipGetLastError();
+}
+
+int gpic_fp8_transpose_bytes(const uint8_t *q, int64_t rows, int64_t cols, uint8_t *qt, int64_t ldt, void *stream) {
+  status_scope();
+  if (rows < 0 || cols < 0) return GPIC_EINVAL;
+  if (cols % 16 || ldt % 16 || ldt < rows) return GPIC_ESHAPE;
+  if (rows == 0 || cols == 0) return GPIC_OK;
+  if (!q || !qt) return GPIC_EINVAL;
+  if (!aligned16(q) || !aligned16(qt)) return GPIC_EALIGN;
+  const int64_t tc = (cols + 63) / 64, tiles = (ldt + 63) / 64 * tc;
+  if (tiles >= (int64_t(1) << 24)) return GPIC_ESHAPE;   // (a launch's threads are counted in 32 bits)
+  transpose_bytes_kernel<<<(unsigned)tiles, 256, 0, (hipStream_t)stream>>>(q, rows, cols, qt, ldt, tc);
+  return (int)hipGetLastError();
+}
+
+int gpic_fp8_rmsnorm_rows(const uint16_t *x, int64_t ldx, const uint16_t *a, int64_t lda, const uint16_t *gate, int64_t sg,
+                          const void *w, int w_dtype, const uint16_t *shift, int64_t ssh, const uint16_t *scale,
+                          int64_t ssc, int64_t rows, int64_t ntok, int64_t C, float eps, uint16_t *xn, uint16_t *h,
+                          float *rstd, uint8_t *q, float *s, void *stream) {
+  status_scope();
+  if (rows < 0 || C <= 0 || ntok <= 0 || (gate && !a) || !shift != !scale) return GPIC_EINVAL;
+  if (rows > 0 && (!x || !w || !rstd || !q || !s || (a && !xn))) return GPIC_EINVAL;
+  if (!dtype_ok(w_dtype)) return GPIC_EDTYPE;
+  if (C % 8 || C > kMaxNormC || rows >= (int64_t(1) << 31) || rows % ntok || ldx % 8 || ldx < C || (a && (lda % 8 || lda < C)) ||
+      (gate && (sg % 8 || sg < C)) || (shift && (ssh % 8 || ssh < C || ssc % 8 || ssc < C)))
+    return GPIC_ESHAPE;
+  if (!aligned16(x) || !aligned16(a) || !aligned16(gate) || !aligned16(w) || !aligned16(shift) || !aligned16(scale) ||
+      !aligned16(xn) || !aligned16(h) || !aligned16(q))
+    return GPIC_EALIGN;
+  if (rows == 0) return GPIC_OK;
+  const NormRowsArgs p{x, a, gate, shift, scale, w, xn, h, rstd, s, q, rows, ntok, ldx, lda, sg, ssh, ssc,
+                       (int)C, w_dtype == GPIC_DTYPE_F32, eps};
+  const hipStream_t st = (hipStream_t)stream;
+  with_team(C, [&](auto T, auto V) {
+    constexpr int t = decltype(T)::value, v = decltype(V)::value;
+    if constexpr (t * v * 8 <= kMaxNormC) {
+      const unsigned g = row_blocks(rows, kWG<t> / t);
+      auto *k = a ? (shift ? rmsnorm_rows_kernel<t, v, true, true> : rmsnorm_rows_kernel<t, v, true, false>)
+                  : (shift ? rmsnorm_rows_kernel<t, v, false, true> : rmsnorm_rows_kernel<t, v, false, false>);
+      k<<<g, kWG<t>, 0, st>>>(p);
+    }
+  });
+  return (int)hipGetLastError();
+}
+
+size_t gpic_fp8_rmsnorm_rows_bwd_workspace_bytes(int64_t rows, int64_t C) {
+  if (rows <= 0 || C <= 0) return 0;
+  return (size_t)norm_bwd_blocks(rows, C) * C * sizeof(float);
+}
+
+int gpic_fp8_rmsnorm_rows_bwd(const uint16_t *dh, const uint16_t *dxn, const uint16_t *xs, const void *w, int w_dtype,
+                              const float *rstd, int64_t rows, int64_t C, uint16_t *dx, void *dw, int dw_dtype, void *ws,
+                              size_t ws_bytes, void *stream) {
+  status_scope();
+  if (rows < 0 || C <= 0 || !dw || !w || (rows > 0 && (!dh || !xs || !rstd || !dx))) return GPIC_EINVAL;
+  if (!dtype_ok(w_dtype) || !dtype_ok(dw_dtype)) return GPIC_EDTYPE;
+  if (C % 8 || C > kMaxNormC) return GPIC_ESHAPE;
+  if (!aligned16(dh) || !aligned16(dxn) || !aligned16(xs) || !aligned16(w) || !aligned16(dx) || !aligned16(dw) ||
+      !aligned16(ws))
+    return GPIC_EALIGN;
+  if (ws_bytes < gpic_fp8_rmsnorm_rows_bwd_workspace_bytes(rows, C) || (rows > 0 && !ws)) return GPIC_EWORKSPACE;
+  const hipStream_t st = (hipStream_t)stream;
+  const int g = rows ? norm_bwd_blocks(rows, C) : 0;
+  const NormBwdRowsArgs p{dh, dxn, xs, w, rstd, dx, static_cast<float *>(ws), rows, (int)C, w_dtype == GPIC_DTYPE_F32};
+  if (g > 0)
+    with_team(C, [&](auto T, auto V) {
+      constexpr int t = decltype(T)::value, v = decltype(V)::value;
+      if constexpr (t * v * 8 <= kMaxNormC) rmsnorm_rows_bwd_kernel<t, v><<<g, kWG<t>, 0, st>>>(p);
+    });
+  rmsnorm_rows_dw_kernel<<<(unsigned)((C + 63) / 64), 256, 0, st>>>(static_cast<const float *>(ws), g, (int)C, dw,
+                                                                    dw_dtype == GPIC_DTYPE_F32);
+  return (int)hipGetLastError();
+}
+
+int gpic_fp8_act_bwd_rows(const uint16_t *dy, int64_t lddy, const uint16_t *z, int64_t ldz, int act, const float *sw,
+                          int64_t rows, int64_t N, uint16_t *dz, uint8_t *q, float *s, void *stream) {
+  status_scope();
+  if (rows < 0 || N <= 0 || act < GPIC_ACT_NONE || act > GPIC_ACT_GELU_TANH) return GPIC_EINVAL;
+  if (rows > 0 && (!dy || !sw || !q || !s || (act && (!z || !dz)))) return GPIC_EINVAL;
+  if (N % 8 || N > kMaxRowC || lddy % 8 || lddy < N || (act && (ldz % 8 || ldz < N))) return GPIC_ESHAPE;
+  if (!aligned16(dy) || !aligned16(sw) || !aligned16(q) || (act && (!aligned16(z) || !aligned16(dz)))) return GPIC_EALIGN;
+  if (rows == 0) return GPIC_OK;
+  const ActBwdArgs p{dy, z, sw, dz, q, s, rows, lddy, ldz, (int)N, act};
+  with_team(N, [&](auto T, auto V) {
+    constexpr int t = decltype(T)::value, v = decltype(V)::value;
+    act_bwd_rows_kernel<t, v><<<row_blocks(rows, kWG<t> / t), kWG<t>, 0, (hipStream_t)stream>>>(p);
+  });
+  return (int)hipGetLastError();
+}
+
+}  // extern "C"

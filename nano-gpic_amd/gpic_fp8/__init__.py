@@ -12,6 +12,8 @@ from .heads import Fp8HeadsLinearF8, convert_fused_heads
 from .norm import (Fp8NormLinearF8, convert_fused_norm, fp8_mod_rmsnorm_linear, fp8_res_mod_rmsnorm_mlp,
                    mod_rmsnorm, res_mod_rmsnorm, res_mod_rmsnorm_bwd, res_mod_rmsnorm_fwd, res_mod_rmsnorm_q)
 from .norm import reference as norm_reference
+from .rows import (RowsWeight, act_bwd_rows, fp8_gemm_rows, fp8_linear_rows, fp8_rmsnorm_linear_rows, rmsnorm_rows,
+                   rmsnorm_rows_bwd, rows_weight, swiglu_layout, tcast_rows)
 
 __all__ = ["E4", "FMAX", "TINY", "Fp8Linear", "Fp8LinearF8", "convert_native", "convert_fp8", "fp8_filter", "KEEP",
            "fp8_gemm", "fp8_gemm_mn", "fp8_linear", "fp8_linear_f8", "fp8_mlp", "fp8_mlp_f8", "fp8_swiglu_w3", "reference",
@@ -19,4 +21,6 @@ __all__ = ["E4", "FMAX", "TINY", "Fp8Linear", "Fp8LinearF8", "convert_native", "
            "weight_casts", "_mm",
            "mod_rmsnorm", "res_mod_rmsnorm", "res_mod_rmsnorm_q", "norm_reference", "fp8_mod_rmsnorm_linear",
            "fp8_res_mod_rmsnorm_mlp", "Fp8NormLinearF8", "convert_fused_norm", "tcast_heads", "fp8_heads_linear_f8",
-           "Fp8HeadsLinearF8", "convert_fused_heads", "res_mod_rmsnorm_fwd", "res_mod_rmsnorm_bwd"]
+           "Fp8HeadsLinearF8", "convert_fused_heads", "res_mod_rmsnorm_fwd", "res_mod_rmsnorm_bwd",
+           "RowsWeight", "act_bwd_rows", "fp8_gemm_rows", "fp8_linear_rows", "fp8_rmsnorm_linear_rows", "rmsnorm_rows",
+           "rmsnorm_rows_bwd", "rows_weight", "swiglu_layout", "tcast_rows"]

@@ -10,7 +10,7 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(os.path.dirname(HERE), "csrc")
 INCLUDE = os.path.join(os.path.dirname(os.path.dirname(HERE)), "include")
 LIB = os.path.join(HERE, "libgpic_fp8.so")
-SOURCES = ["api.hip", "cast.hip", "gemm.hip", "norm.hip"]
+SOURCES = ["api.hip", "cast.hip", "gemm.hip", "norm.hip", "rows.hip"]
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 
 FLAGS = [
