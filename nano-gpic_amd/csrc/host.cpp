@@ -1,6 +1,6 @@
 // The host side of the path's calls in one native module (_gpic_host): output allocation and the C-ABI calls of a cast
-// group, a GEMM, a weight gradient, and the whole forward or backward of a phase-3 linear, without a Python frame, a
-// ctypes conversion and a tensor constructor for each piece. A linear of a few hundred rows is bound by that host time,
+// group, a GEMM, a weight gradient, the whole forward or backward of a phase-3 linear, and the row-scaled operators with the
+// forward and backward of their linears, without a Python frame, a ctypes conversion and a tensor constructor for each piece. A linear of a few hundred rows is bound by that host time,
 // not by its kernels (~40 us of Python for 25 us of kernels in a sampler's proj).
 //
 // Every function takes tensors of the usual form only (on the current device, contiguous, 16-byte aligned, the types
@@ -235,6 +235,297 @@ py::object linear_bwd(const at::Tensor &dy, const at::Tensor &xq, const at::Tens
   return py::make_tuple(dx, dw, db);
 }
 
+// ------------------------------------------------------------------------------------------- row-scaled operators
+
+constexpr int64_t kRowsMaxNorm = 16384, kRowsMaxCast = 32768;   // the C ABI's widest rows
+typedef std::optional<at::Tensor> opt;
+
+bool bf16(const at::Tensor &t, int dev) { return t.scalar_type() == at::kBFloat16 && plain(t, dev); }
+// A vector of n bf16 or fp32, or none
+bool vector_ok(const at::Tensor &t, int64_t n, int dev) { return castable(t, dev) && t.dim() == 1 && t.size(0) == n; }
+bool scales_ok(const opt &s, int64_t n, int dev) {
+  return !s || (s->scalar_type() == at::kFloat && plain(*s, dev) && s->numel() == n);
+}
+uint16_t *u16(const opt &t) { return t ? ptr<uint16_t>(*t) : nullptr; }
+at::Tensor none_of(const at::Tensor &like, at::ScalarType ty) { return make(like, {0}, ty); }
+
+// Modulation rows [B, 1, C], [B, C] or [C] bf16: base, row stride and B; false for a form that the general path copies. batch:
+// x's first extent where x has a batch (B is then that or 1), else 0 (B divides the rows).
+struct Mod {
+  const uint16_t *p = nullptr;
+  int64_t ld = 0, B = 0;
+};
+bool mod_ok(const opt &t, int64_t C, int64_t batch, int64_t rows, int dev, Mod &m) {
+  if (!t) return true;
+  const int64_t d = t->dim();
+  if (d < 1 || d > 3 || t->scalar_type() != at::kBFloat16 || !t->is_cuda() || t->get_device() != dev ||
+      t->layout() != at::kStrided || t->size(d - 1) != C || t->stride(d - 1) != 1 || (d == 3 && t->size(1) != 1))
+    return false;
+  m.B = d == 1 ? 1 : t->size(0);
+  m.ld = m.B > 1 ? t->stride(0) : C;
+  m.p = ptr<uint16_t>(*t);
+  if (m.B < 1 || (m.B != 1 && (batch ? m.B != batch : rows % m.B)) || m.ld % 8 || m.ld < C) return false;
+  return (reinterpret_cast<uintptr_t>(m.p) & 15u) == 0;
+}
+
+struct RowCast {
+  at::Tensor q, s;
+};
+bool row_castable(const at::Tensor &x, int dev) {
+  return castable(x, dev) && x.dim() >= 1 && x.size(-1) > 0 && x.size(-1) % 8 == 0 && x.size(-1) <= kRowsMaxCast;
+}
+RowCast row_cast(const at::Tensor &x, void *stream) {
+  const int64_t C = x.size(-1), M = x.numel() / C;
+  RowCast o{make(x, x.sizes(), kE4), make(x, {M}, at::kFloat)};
+  check(gpic_fp8_tcast_rows(x.data_ptr(), dtype_code(x), C, M, C, ptr<uint8_t>(o.q), ptr<float>(o.s), stream),
+        "gpic_fp8_tcast_rows");
+  return o;
+}
+
+struct NormOut {
+  at::Tensor xn, h, q, s, rstd;
+};
+struct NormIn {
+  Mod gate, shift, scale;
+  int64_t ntok = 1;
+};
+bool norm_ok(const at::Tensor &x, const at::Tensor &w, const opt &a, const opt &gate, const opt &shift, const opt &scale,
+             int dev, NormIn &in) {
+  if (x.dim() < 2 || !bf16(x, dev)) return false;
+  const int64_t C = x.size(-1);
+  if (C <= 0 || C % 8 || C > kRowsMaxNorm) return false;
+  const int64_t M = x.numel() / C, batch = x.dim() > 2 ? x.size(0) : 0;
+  if (M < 1 || !vector_ok(w, C, dev) || (a && (!bf16(*a, dev) || a->sizes() != x.sizes())) || (gate && !a) ||
+      shift.has_value() != scale.has_value() || !mod_ok(gate, C, batch, M, dev, in.gate) ||
+      !mod_ok(shift, C, batch, M, dev, in.shift) || !mod_ok(scale, C, batch, M, dev, in.scale))
+    return false;
+  int64_t B = 0;
+  for (const Mod *m : {&in.gate, &in.shift, &in.scale})
+    if (m->B) {
+      if (B && B != m->B) return false;
+      B = m->B;
+    }
+  in.ntok = B ? M / B : 1;
+  return true;
+}
+NormOut norm_rows_run(const at::Tensor &x, const at::Tensor &w, double eps, const opt &a, const NormIn &in, bool want_h,
+                      void *stream) {
+  const int64_t C = x.size(-1), M = x.numel() / C;
+  NormOut o;
+  o.xn = a ? make(x, x.sizes(), at::kBFloat16) : none_of(x, at::kBFloat16);
+  o.h = want_h ? make(x, x.sizes(), at::kBFloat16) : none_of(x, at::kBFloat16);
+  o.q = make(x, x.sizes(), kE4);
+  o.s = make(x, {M}, at::kFloat);
+  o.rstd = make(x, {M}, at::kFloat);
+  check(gpic_fp8_rmsnorm_rows(ptr<uint16_t>(x), C, u16(a), C, in.gate.p, in.gate.ld, w.data_ptr(), dtype_code(w), in.shift.p,
+                              in.shift.ld, in.scale.p, in.scale.ld, M, in.ntok, C, (float)eps,
+                              a ? ptr<uint16_t>(o.xn) : nullptr, want_h ? ptr<uint16_t>(o.h) : nullptr, ptr<float>(o.rstd),
+                              ptr<uint8_t>(o.q), ptr<float>(o.s), stream),
+        "gpic_fp8_rmsnorm_rows");
+  return o;
+}
+
+struct GemmOut {
+  at::Tensor y, z;
+};
+bool operand_rows(const at::Tensor &t, int dev) {
+  return t.scalar_type() == kE4 && t.dim() == 2 && t.size(1) > 0 && t.size(1) % 16 == 0 && plain(t, dev);
+}
+// (shapes of a and b, and bias, checked by the callers)
+GemmOut gemm_rows_run(const at::Tensor &a, const opt &sa, const at::Tensor &b, const opt &sb, const opt &bias, int act,
+                      const opt &res, const Mod &gate, bool want_z, void *stream) {
+  const int64_t M = a.size(0), K = a.size(1), N = b.size(0), No = act == GPIC_ACT_SWIGLU ? N / 2 : N;
+  GemmOut o;
+  o.y = make(a, {M, No}, at::kBFloat16);
+  o.z = want_z ? make(a, {M, N}, at::kBFloat16) : none_of(a, at::kBFloat16);
+  const Scratch w(a, M, N, K);
+  check(gpic_fp8_gemm_rows(ptr<uint8_t>(a), K, sa ? ptr<float>(*sa) : nullptr, ptr<uint8_t>(b), K,
+                           sb ? ptr<float>(*sb) : nullptr, bias ? bias->data_ptr() : nullptr, bias ? dtype_code(*bias) : 0,
+                           act, u16(res), No, gate.p, gate.ld, gate.B ? M / gate.B : 1, ptr<uint16_t>(o.y), No,
+                           want_z ? ptr<uint16_t>(o.z) : nullptr, N, M, N, K, w.p(), w.bytes, stream),
+        "gpic_fp8_gemm_rows");
+  return o;
+}
+
+py::object cast_rows(const at::Tensor &x, int dev, handle, handle stream) {
+  if (!row_castable(x, dev)) return py::none();
+  RowCast o;
+  {
+    NoGil no_gil;
+    o = row_cast(x, vp(stream));
+  }
+  return py::make_tuple(o.q, o.s);
+}
+
+py::object norm_rows(const at::Tensor &x, const at::Tensor &w, double eps, const opt &a, const opt &gate, const opt &shift,
+                     const opt &scale, bool want_h, int dev, handle, handle stream) {
+  NormIn in;
+  if (!norm_ok(x, w, a, gate, shift, scale, dev, in)) return py::none();
+  NormOut o;
+  {
+    NoGil no_gil;
+    o = norm_rows_run(x, w, eps, a, in, want_h, vp(stream));
+  }
+  return py::make_tuple(o.xn, o.h, o.q, o.s, o.rstd);
+}
+
+py::object gemm_rows(const at::Tensor &a, const opt &sa, const at::Tensor &b, const opt &sb, const opt &bias, int act,
+                     const opt &res, const opt &gate, bool want_z, int dev, handle, handle stream) {
+  if (!operand_rows(a, dev) || !operand_rows(b, dev) || a.size(1) != b.size(1)) return py::none();
+  const int64_t M = a.size(0), N = b.size(0), No = act == GPIC_ACT_SWIGLU ? N / 2 : N;
+  Mod g;
+  if (M < 1 || N < 16 || N % (act == GPIC_ACT_SWIGLU ? 32 : 16) || !scales_ok(sa, M, dev) || !scales_ok(sb, N, dev) ||
+      !bias_ok(bias, N, dev) || (res && (!bf16(*res, dev) || res->dim() != 2 || res->size(0) != M || res->size(1) != No)) ||
+      !mod_ok(gate, No, 0, M, dev, g))
+    return py::none();
+  GemmOut o;
+  {
+    NoGil no_gil;
+    o = gemm_rows_run(a, sa, b, sb, bias, act, res, g, want_z, vp(stream));
+  }
+  return py::make_tuple(o.y, o.z);
+}
+
+bool norm_bwd_ok(const at::Tensor &dh, const opt &dxn, const at::Tensor &xs, const at::Tensor &w, const at::Tensor &rstd,
+                 int dev) {
+  if (xs.dim() < 1 || !bf16(xs, dev)) return false;
+  const int64_t C = xs.size(-1);
+  return C > 0 && C % 8 == 0 && C <= kRowsMaxNorm && vector_ok(w, C, dev) && bf16(dh, dev) && dh.numel() == xs.numel() &&
+         (!dxn || (bf16(*dxn, dev) && dxn->sizes() == xs.sizes())) && scales_ok(rstd, xs.numel() / C, dev);
+}
+std::pair<at::Tensor, at::Tensor> norm_bwd_run(const at::Tensor &dh, const opt &dxn, const at::Tensor &xs,
+                                               const at::Tensor &w, const at::Tensor &rstd, void *stream) {
+  const int64_t C = xs.size(-1), M = xs.numel() / C;
+  at::Tensor dx = make(xs, xs.sizes(), at::kBFloat16), dw = make(xs, {C}, w.scalar_type());
+  const size_t bytes = gpic_fp8_rmsnorm_rows_bwd_workspace_bytes(M, C);
+  at::Tensor ws = make(xs, {std::max<int64_t>((int64_t)bytes, 16)}, at::kByte);
+  check(gpic_fp8_rmsnorm_rows_bwd(ptr<uint16_t>(dh), u16(dxn), ptr<uint16_t>(xs), w.data_ptr(), dtype_code(w),
+                                  ptr<float>(rstd), M, C, ptr<uint16_t>(dx), dw.data_ptr(), dtype_code(dw), ws.data_ptr(),
+                                  bytes, stream),
+        "gpic_fp8_rmsnorm_rows_bwd");
+  return {dx, dw};
+}
+py::object norm_rows_bwd(const at::Tensor &dh, const opt &dxn, const at::Tensor &xs, const at::Tensor &w,
+                         const at::Tensor &rstd, int dev, handle, handle stream) {
+  if (!norm_bwd_ok(dh, dxn, xs, w, rstd, dev) || dh.sizes() != xs.sizes()) return py::none();
+  std::pair<at::Tensor, at::Tensor> o;
+  {
+    NoGil no_gil;
+    o = norm_bwd_run(dh, dxn, xs, w, rstd, vp(stream));
+  }
+  return py::make_tuple(o.first, o.second);
+}
+
+bool rows_weight_ok(const at::Tensor &w, int64_t K, int dev) {
+  return w.dim() == 2 && w.size(1) == K && w.size(0) >= 16 && w.size(0) % 16 == 0 && K % 16 == 0 && row_castable(w, dev);
+}
+
+// x [M, K] bf16, w [N, K], bias [N] or None, residual [M, N] bf16 or None -> (y [M, N], z [M, N] or empty, w's bytes and scales)
+py::object linear_rows_fwd(const at::Tensor &x, const at::Tensor &w, const opt &bias, int act, const opt &res, bool want_z,
+                           int dev, handle, handle stream) {
+  if (x.dim() != 2 || x.size(0) < 1 || !bf16(x, dev) || !row_castable(x, dev) || !rows_weight_ok(w, x.size(1), dev) ||
+      !bias_ok(bias, w.size(0), dev) ||
+      (res && (!bf16(*res, dev) || res->dim() != 2 || res->size(0) != x.size(0) || res->size(1) != w.size(0))))
+    return py::none();
+  RowCast wc;
+  GemmOut o;
+  {
+    NoGil no_gil;
+    wc = row_cast(w, vp(stream));
+    const RowCast xc = row_cast(x, vp(stream));
+    o = gemm_rows_run(xc.q, xc.s, wc.q, wc.s, bias, act, res, Mod(), want_z, vp(stream));
+  }
+  return py::make_tuple(o.y, o.z, wc.q, wc.s);
+}
+
+// The norm and the linear that reads its bytes -> (x_new or empty, h as bf16 or empty, rstd, y, z or empty, w's bytes, scales)
+py::object norm_linear_rows_fwd(const at::Tensor &x, const at::Tensor &wn, double eps, const opt &a, const opt &gate,
+                                const opt &shift, const opt &scale, const at::Tensor &w, const opt &bias, int act, bool want_h,
+                                bool want_z, int dev, handle, handle stream) {
+  NormIn in;
+  if (!norm_ok(x, wn, a, gate, shift, scale, dev, in) || !rows_weight_ok(w, x.size(-1), dev) || !bias_ok(bias, w.size(0), dev))
+    return py::none();
+  RowCast wc;
+  NormOut n;
+  GemmOut o;
+  {
+    NoGil no_gil;
+    wc = row_cast(w, vp(stream));
+    n = norm_rows_run(x, wn, eps, a, in, want_h, vp(stream));
+    o = gemm_rows_run(n.q.view({-1, x.size(-1)}), n.s, wc.q, wc.s, bias, act, std::nullopt, Mod(), want_z, vp(stream));
+  }
+  return py::make_tuple(n.xn, n.h, n.rstd, o.y, o.z, wc.q, wc.s);
+}
+
+struct LinearGrads {
+  at::Tensor dx, dw, db;
+};
+bool linear_bwd_ok(const at::Tensor &dy, const at::Tensor &z, int act, const at::Tensor &wq, const at::Tensor &sw,
+                   const at::Tensor &x, int dev) {
+  if (dy.dim() != 2 || !bf16(dy, dev) || !operand_rows(wq, dev)) return false;
+  const int64_t M = dy.size(0), N = dy.size(1), K = wq.size(1);
+  return M >= 1 && N >= 16 && N % 16 == 0 && N <= kRowsMaxCast && wq.size(0) == N && scales_ok(sw, N, dev) &&
+         (act == GPIC_ACT_NONE || (bf16(z, dev) && z.sizes() == dy.sizes())) && bf16(x, dev) && x.numel() == M * K &&
+         2 * M * std::max(N, K) < (int64_t(1) << 31) && K < (1 << 21);
+}
+// (f32: an fp32 weight's, bias's gradient)
+LinearGrads linear_bwd_run(const at::Tensor &dy, const at::Tensor &z, int act, const at::Tensor &wq, const at::Tensor &sw,
+                           const at::Tensor &x, bool need_dx, bool need_dw, bool need_db, bool w32, bool b32, void *stream) {
+  const int64_t M = dy.size(0), N = dy.size(1), K = wq.size(1);
+  LinearGrads o;
+  const at::Tensor dz = act == GPIC_ACT_NONE ? dy : make(dy, {M, N}, at::kBFloat16);
+  const at::Tensor q = make(dy, {M, N}, kE4), s = make(dy, {M}, at::kFloat);
+  check(gpic_fp8_act_bwd_rows(ptr<uint16_t>(dy), N, act == GPIC_ACT_NONE ? nullptr : ptr<uint16_t>(z), N, act, ptr<float>(sw),
+                              M, N, act == GPIC_ACT_NONE ? nullptr : ptr<uint16_t>(dz), ptr<uint8_t>(q), ptr<float>(s), stream),
+        "gpic_fp8_act_bwd_rows");
+  if (need_dx) {
+    const at::Tensor qt = make(dy, {K, N}, kE4);
+    check(gpic_fp8_transpose_bytes(ptr<uint8_t>(wq), N, K, ptr<uint8_t>(qt), N, stream), "gpic_fp8_transpose_bytes");
+    o.dx = gemm_rows_run(q, s, qt, std::nullopt, std::nullopt, GPIC_ACT_NONE, std::nullopt, Mod(), false, stream).y;
+  }
+  if (need_dw) {
+    o.dw = make(dy, {N, K}, w32 ? at::kFloat : at::kBFloat16);
+    const Scratch w(dy, N, K, 2 * M);   // (planned as an e4m3 GEMM of as many K bytes)
+    check(gpic_fp8_bf16_gemm_mn(ptr<uint16_t>(dz), N, ptr<uint16_t>(x), K, o.dw.data_ptr(),
+                                w32 ? GPIC_DTYPE_F32 : GPIC_DTYPE_BF16, K, N, K, M, w.p(), w.bytes, stream),
+          "gpic_fp8_bf16_gemm_mn");
+  }
+  if (need_db) o.db = bias_grad(dz, b32, stream);
+  return o;
+}
+py::object or_none(const at::Tensor &t) { return t.defined() ? py::cast(t) : py::none(); }
+
+// dy [M, N] bf16, the forward's z, w's bytes and scales and x [M, K] bf16 -> (dx [M, K], dw [N, K], db [N]), None where not needed
+py::object linear_rows_bwd(const at::Tensor &dy, const at::Tensor &z, int act, const at::Tensor &wq, const at::Tensor &sw,
+                           const at::Tensor &x, bool need_dx, bool need_dw, bool need_db, bool w32, bool b32, int dev, handle,
+                           handle stream) {
+  if (!linear_bwd_ok(dy, z, act, wq, sw, x, dev)) return py::none();
+  LinearGrads o;
+  {
+    NoGil no_gil;
+    o = linear_bwd_run(dy, z, act, wq, sw, x, need_dx, need_dw, need_db, w32, b32, vp(stream));
+  }
+  return py::make_tuple(or_none(o.dx), or_none(o.dw), or_none(o.db));
+}
+
+// The same and the norm's backward (without gate, shift and scale): (dx like xs, dwn, dw, db)
+py::object norm_linear_rows_bwd(const at::Tensor &dy, const opt &dxn, const at::Tensor &z, int act, const at::Tensor &wq,
+                                const at::Tensor &sw, const at::Tensor &h, const at::Tensor &xs, const at::Tensor &wn,
+                                const at::Tensor &rstd, bool need_dw, bool need_db, bool w32, bool b32, int dev, handle,
+                                handle stream) {
+  if (!linear_bwd_ok(dy, z, act, wq, sw, h, dev) || xs.numel() != h.numel() || xs.size(-1) != wq.size(1) ||
+      !norm_bwd_ok(h, dxn, xs, wn, rstd, dev))
+    return py::none();
+  LinearGrads o;
+  std::pair<at::Tensor, at::Tensor> n;
+  {
+    NoGil no_gil;
+    o = linear_bwd_run(dy, z, act, wq, sw, h, true, need_dw, need_db, w32, b32, vp(stream));
+    n = norm_bwd_run(o.dx, dxn, xs, wn, rstd, vp(stream));
+  }
+  return py::make_tuple(n.first, n.second, or_none(o.dw), or_none(o.db));
+}
+
 }  // namespace
 
 PYBIND11_MODULE(_gpic_host, m) {   // (wrapped: torch's own errors, out of memory among them, stay what they are)
@@ -243,4 +534,12 @@ PYBIND11_MODULE(_gpic_host, m) {   // (wrapped: torch's own errors, out of memor
   m.def("wgrad", torch::wrap_pybind_function(&wgrad));
   m.def("linear_fwd", torch::wrap_pybind_function(&linear_fwd));
   m.def("linear_bwd", torch::wrap_pybind_function(&linear_bwd));
+  m.def("cast_rows", torch::wrap_pybind_function(&cast_rows));
+  m.def("norm_rows", torch::wrap_pybind_function(&norm_rows));
+  m.def("norm_rows_bwd", torch::wrap_pybind_function(&norm_rows_bwd));
+  m.def("gemm_rows", torch::wrap_pybind_function(&gemm_rows));
+  m.def("linear_rows_fwd", torch::wrap_pybind_function(&linear_rows_fwd));
+  m.def("linear_rows_bwd", torch::wrap_pybind_function(&linear_rows_bwd));
+  m.def("norm_linear_rows_fwd", torch::wrap_pybind_function(&norm_linear_rows_fwd));
+  m.def("norm_linear_rows_bwd", torch::wrap_pybind_function(&norm_linear_rows_bwd));
 }

@@ -80,6 +80,9 @@ def _weight_vec(w, C, name):
 @L.step_op("gpic::fp8_tcast_rows")
 def tcast_rows_op(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     """x [..., C] (any float dtype, C % 8 == 0, C <= 32768) -> (q e4m3, x's shape; s [rows] fp32): each row's own amax."""
+    o = L.native("cast_rows", x, x)
+    if o is not None:
+        return o
     L.require_gpu(x)
     if x.dim() < 1 or x.shape[-1] % 8 or not 0 < x.shape[-1] <= CAST_MAX_C or not x.is_floating_point():
         raise ValueError(f"tcast_rows needs float x [..., C] with C % 8 == 0 and 0 < C <= {CAST_MAX_C}, got {x.dtype} "
@@ -158,6 +161,9 @@ def rmsnorm_rows_op(x: torch.Tensor, w: torch.Tensor, eps: float, a: Optional[to
                     scale: Optional[torch.Tensor] = None, want_h: bool = False
                     ) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
     """rmsnorm_rows, as an op."""
+    o = L.native("norm_rows", x, x, w, eps, a, gate, shift, scale, want_h)
+    if o is not None:
+        return o
     L.require_gpu(x, w, a, gate, shift, scale)
     if x.dim() < 2 or x.dtype != BF or x.shape[-1] % 8 or not 0 < x.shape[-1] <= NORM_MAX_C:
         raise ValueError(f"rmsnorm_rows takes bf16 x [..., C] with C % 8 == 0 and 0 < C <= {NORM_MAX_C}, got {x.dtype} "
@@ -218,6 +224,9 @@ def rmsnorm_rows(x, w, eps, a=None, gate=None, shift=None, scale=None, want_h=Fa
 def rmsnorm_rows_bwd_op(dh: torch.Tensor, dxn: Optional[torch.Tensor], xs: torch.Tensor, w: torch.Tensor,
                         rstd: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     """rmsnorm_rows_bwd, as an op."""
+    o = L.native("norm_rows_bwd", xs, dh, dxn, xs, w, rstd)
+    if o is not None:
+        return o
     L.require_gpu(dh, dxn, xs, w, rstd)
     if xs.dim() < 1 or xs.dtype != BF or xs.shape[-1] % 8 or not 0 < xs.shape[-1] <= NORM_MAX_C:
         raise ValueError(f"rmsnorm_rows_bwd takes bf16 xs [..., C] with C % 8 == 0 and 0 < C <= {NORM_MAX_C}, got {xs.dtype} "
@@ -271,8 +280,11 @@ def gemm_rows_op(a: torch.Tensor, sa: Optional[torch.Tensor], b: torch.Tensor, s
                  bias: Optional[torch.Tensor] = None, act: str = "none", residual: Optional[torch.Tensor] = None,
                  gate: Optional[torch.Tensor] = None, want_z: bool = False) -> tuple[torch.Tensor, torch.Tensor]:
     """fp8_gemm_rows, as an op: (y, z as bf16 when want_z, else an empty tensor)."""
-    L.require_gpu(a, sa, b, sb, bias, residual, gate)
     code = _act(act)
+    o = L.native("gemm_rows", a, a, sa, b, sb, bias, code, residual, gate, want_z)
+    if o is not None:
+        return o
+    L.require_gpu(a, sa, b, sb, bias, residual, gate)
     _same_device(a.device, sa=sa, b=b, sb=sb, bias=bias, residual=residual, gate=gate)
     a, b = _gemm_operand(a, "a"), _gemm_operand(b, "b")
     (M, K), N = a.shape, b.shape[0]
@@ -370,6 +382,11 @@ def act_bwd_rows(dy, z, act, sw):
 
 def _linear_bwd(ctx, dy2, z, wq, sw, x2, need_dx, need_dw, need_db):
     """(dx [M, K] bf16, dw, db) of y = act(x w^T + b), each None unless needed."""
+    r = L.native("linear_rows_bwd", dy2, dy2, z, ACTS[ctx.act], wq, sw, x2, need_dx, need_dw, need_db,
+                 ctx.wdt == torch.float32, ctx.bdt == torch.float32)
+    if r is not None:
+        dx, dw, db = r
+        return dx, dw if dw is None else dw.to(ctx.wdt), db if db is None else db.to(ctx.bdt)
     dz, dq, sd = L.call(act_bwd_rows_op, dy2, z, ctx.act, sw)
     if ctx.act == "none":
         dz = dy2
@@ -383,9 +400,15 @@ class _LinearRows(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, w, b, act, residual):
         x2 = x.reshape(-1, x.shape[-1])
-        xq, sx = L.call(tcast_rows_op, x2)
-        wq, sw = L.call(tcast_rows_op, w)
-        y, z = L.call(gemm_rows_op, xq, sx, wq, sw, b, act, residual, None, act != "none" and any(ctx.needs_input_grad))
+        want_z = act != "none" and any(ctx.needs_input_grad)
+        r2 = None if residual is None else residual.reshape(-1, w.shape[0])
+        r = L.native("linear_rows_fwd", x2, x2, w, b, ACTS[act], r2, want_z)
+        if r is not None:
+            y, z, wq, sw = r
+        else:
+            xq, sx = L.call(tcast_rows_op, x2)
+            wq, sw = L.call(tcast_rows_op, w)
+            y, z = L.call(gemm_rows_op, xq, sx, wq, sw, b, act, r2, None, want_z)
         ctx.save_for_backward(x2, z, wq, sw)
         ctx.act, ctx.wdt, ctx.bdt, ctx.shape = act, w.dtype, None if b is None else b.dtype, x.shape
         return y.view(*x.shape[:-1], w.shape[0])
@@ -406,12 +429,17 @@ class _NormLinearRows(torch.autograd.Function):
     def forward(ctx, x, a, gate, wn, shift, scale, eps, w, b, act):
         C = x.shape[-1]
         train = any(ctx.needs_input_grad)
-        xn, h, hq, sh, rstd = L.call(rmsnorm_rows_op, x, wn, eps, a, gate, shift, scale, train)
-        wq, sw = L.call(tcast_rows_op, w)
-        y, z = L.call(gemm_rows_op, hq.view(-1, C), sh, wq, sw, b, act, None, None, train and act != "none")
+        want_z = train and act != "none"
+        r = L.native("norm_linear_rows_fwd", x, x, wn, eps, a, gate, shift, scale, w, b, ACTS[act], train, want_z)
+        if r is not None:
+            xn, h, rstd, y, z, wq, sw = r
+        else:
+            xn, h, hq, sh, rstd = L.call(rmsnorm_rows_op, x, wn, eps, a, gate, shift, scale, train)
+            wq, sw = L.call(tcast_rows_op, w)
+            y, z = L.call(gemm_rows_op, hq.view(-1, C), sh, wq, sw, b, act, None, None, want_z)
         xs = x if a is None else xn
-        ctx.save_for_backward(xs, a if gate is not None else None, gate, wn, shift, scale, rstd, h.view(-1, C) if train else None, z,
-                              wq, sw)
+        ctx.save_for_backward(xs, a if gate is not None else None, gate, wn, shift, scale, rstd,
+                              h.view(-1, C) if train else None, z, wq, sw)
         ctx.act, ctx.wdt, ctx.bdt = act, w.dtype, None if b is None else b.dtype
         y = y.view(*x.shape[:-1], w.shape[0])
         return y if a is None else (xn, y)
@@ -423,15 +451,26 @@ class _NormLinearRows(torch.autograd.Function):
         dxn, dy = grads if len(grads) == 2 else (None, grads[0])
         need = ctx.needs_input_grad
         below = any(need[:6])   # a gradient through the norm
-        dh, dw, db = _linear_bwd(ctx, dy.reshape(-1, dy.shape[-1]).to(BF), z, wq, sw, h, below, need[7], need[8])
+        dy2 = dy.reshape(-1, dy.shape[-1]).to(BF)
         dx = da = dgate = dwn = dshift = dscale = None
+        r = None
         if below and shift is None:
-            dx, dwn = L.call(rmsnorm_rows_bwd_op, dh.view(xs.shape), dxn, xs, wn, rstd)
+            r = L.native("norm_linear_rows_bwd", dy2, dy2, dxn, z, ACTS[ctx.act], wq, sw, h, xs, wn, rstd, need[7], need[8],
+                         ctx.wdt == torch.float32, ctx.bdt == torch.float32)
+        if r is not None:
+            dx, dwn, dw, db = r
             dwn, da = dwn.to(wn.dtype), dx
-        elif below:
-            dx, da, dg, dwn, dsh, dsc = L.call(res_mod_rmsnorm_bwd_k, dh.view(xs.shape), dxn, xs, a, gate, wn, scale, rstd)
-            dwn, dshift, dscale = dwn.to(wn.dtype), dsh.view(shift.shape).to(shift.dtype), dsc.view(scale.shape).to(scale.dtype)
-            dgate = dg.view(gate.shape).to(gate.dtype) if gate is not None else None
+            dw, db = dw if dw is None else dw.to(ctx.wdt), db if db is None else db.to(ctx.bdt)
+        else:
+            dh, dw, db = _linear_bwd(ctx, dy2, z, wq, sw, h, below, need[7], need[8])
+            if below and shift is None:
+                dx, dwn = L.call(rmsnorm_rows_bwd_op, dh.view(xs.shape), dxn, xs, wn, rstd)
+                dwn, da = dwn.to(wn.dtype), dx
+            elif below:
+                dx, da, dg, dwn, dsh, dsc = L.call(res_mod_rmsnorm_bwd_k, dh.view(xs.shape), dxn, xs, a, gate, wn, scale, rstd)
+                dwn = dwn.to(wn.dtype)
+                dshift, dscale = dsh.view(shift.shape).to(shift.dtype), dsc.view(scale.shape).to(scale.dtype)
+                dgate = dg.view(gate.shape).to(gate.dtype) if gate is not None else None
         out = [dx, da, dgate, dwn, dshift, dscale, None, dw, db, None]
         return tuple(g if n else None for g, n in zip(out, need))
 

@@ -547,3 +547,33 @@ def test_the_raw_calls_have_no_gradient(dev):
     xn = G.rmsnorm_rows(x, torch.ones(64, device=dev), 1e-6, x)[0]
     with pytest.raises(RuntimeError):
         xn.float().sum().backward()
+
+
+@pytest.mark.parametrize("act", ["none", "silu"])
+def test_host_module_and_general_form(dev, monkeypatch, act):
+    """The native host module's calls and the general Python form give the same bits."""
+    g = gen(dev)
+    x, a, w, b = randn(g, 3, 50, 256), randn(g, 3, 50, 256), randn(g, 128, 256, dtype=F32), randn(g, 128, dtype=F32)
+    w2, mod = randn(g, 256, 128), randn(g, 3, 1, 6 * 256, std=0.3).chunk(6, dim=-1)
+    wn = 1 + 0.1 * torch.randn(256, generator=g, device=dev)
+    dy, dxn = randn(g, 3, 50, 256), randn(g, 3, 50, 256)
+
+    def passes():
+        out = []
+        for m in (False, True):
+            leaves = [t.detach().requires_grad_() for t in (x, a, wn, w, b, w2)]
+            X, A, WN, W, B, W2 = leaves
+            kw = dict(gate=mod[2], shift=mod[3], scale=mod[4]) if m else {}
+            xn, h = G.fp8_rmsnorm_linear_rows(X, WN, 1e-6, W, B, act, A, **kw)
+            y = G.fp8_linear_rows(h, W2, None, "none", xn)
+            out += [y.detach(), *torch.autograd.grad((xn, y), leaves, (dxn, dy))]
+        with torch.no_grad():
+            s = dict(x=x, a=a, wn=wn, mod=mod)
+            out += serve(s, G.rows_weight(randn(gen(dev, 5), 256, 256), "swiglu"), G.rows_weight(w2))
+            dh = dy.reshape(-1, 256)
+            out += G.rmsnorm_rows_bwd(dh, None, dxn.reshape(-1, 256), wn, torch.rand(150, generator=gen(dev), device=dev))
+        return out
+    want = passes()
+    monkeypatch.setattr(L, "native", lambda *a: None)
+    got = passes()
+    assert len(want) == len(got) and all(torch.equal(p, q) for p, q in zip(want, got))

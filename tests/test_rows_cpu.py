@@ -208,3 +208,18 @@ def test_fake_kernels():
         assert y.shape == (3, 16) and z.shape == (3, 32) and y.dtype == z.dtype == BF
         dz, q, s = GR.act_bwd_rows_op(e(3, 64), e(3, 64), "silu", e(64, dt=F32))
         assert dz.shape == q.shape == (3, 64) and s.shape == (3,) and q.dtype == E4
+
+
+def test_host_module_takes_no_cpu_tensors():
+    h = L.host()
+    x, w, v = torch.zeros(16, 16, dtype=BF), torch.zeros(16, 16), torch.ones(16)
+    q = torch.zeros(16, 16).to(E4)
+    n = None
+    assert h.cast_rows(x, 0, 0, 0) is None
+    assert h.norm_rows(x, v, 1e-6, n, n, n, n, False, 0, 0, 0) is None
+    assert h.norm_rows_bwd(x, n, x, v, v, 0, 0, 0) is None
+    assert h.gemm_rows(q, n, q, n, n, 0, n, n, False, 0, 0, 0) is None
+    assert h.linear_rows_fwd(x, w, n, 0, n, False, 0, 0, 0) is None
+    assert h.linear_rows_bwd(x, x, 0, q, v, x, True, True, True, True, True, 0, 0, 0) is None
+    assert h.norm_linear_rows_fwd(x, v, 1e-6, n, n, n, n, w, n, 0, True, True, 0, 0, 0) is None
+    assert h.norm_linear_rows_bwd(x, n, x, 0, q, v, x, x, v, v, True, True, True, True, 0, 0, 0) is None
