@@ -110,53 +110,89 @@ struct NormRowsArgs {
   float *rstd, *s;
   uint8_t *q;
   int64_t rows, ntok, ldx, lda, sg, ssh, ssc;
-  int C, w32;
+  int C, w32, chunk;   // chunk: rows of a team
   float eps;
 };
 
+// A team takes `chunk` rows one after another: the row after the current one is requested before the current one's sums, and
+// w, and gate, shift and scale while the batch entry stays the same, are kept in registers.
 template <int T, int kV, bool kRes, bool kMod>
 __global__ __launch_bounds__(kWG<T>) void rmsnorm_rows_kernel(NormRowsArgs p) {
   __shared__ float red_s[T > 64 ? T / 64 : 1];
   __shared__ uint32_t red_m[T > 64 ? T / 64 : 1];
   const int t = threadIdx.x % T, nv = p.C / 8;
-  for (int64_t row = team_row<T>(); row < p.rows; row += team_step<T>()) {
-    const int64_t b = kMod || (kRes && p.gate) ? (int64_t)((uint32_t)row / (uint32_t)p.ntok) : 0;
-    const uint16_t *xr = p.x + row * p.ldx;
-    const uint16_t *ar = kRes ? p.a + row * p.lda : nullptr;
-    u32x4 X[kV], A[kV];
+  int64_t row = team_row<T>() * p.chunk;
+  const int64_t end = min(row + p.chunk, p.rows);
+  if (row >= end) return;
+  u32x4 X[kV], A[kV], G[kV], SH[kV], SC[kV];
+  float W[kV][8];
+  auto fetch = [&](int64_t r) {
 #pragma unroll
     for (int j = 0; j < kV; j++) {
       const int v = t + T * j;
       X[j] = A[j] = u32x4{0u, 0u, 0u, 0u};
       if (v < nv) {
-        X[j] = ld16(xr + 8 * v);
-        if (kRes) A[j] = ld16(ar + 8 * v);
+        X[j] = ld16(p.x + r * p.ldx + 8 * v);
+        if (kRes) A[j] = ld16(p.a + r * p.lda + 8 * v);
       }
     }
+  };
+  fetch(row);
+#pragma unroll
+  for (int j = 0; j < kV; j++)
+    if (t + T * j < nv) load8(p.w, p.w32, 8 * (t + T * j), W[j]);
+  const bool gated = kRes && p.gate;
+  int64_t batch_end = row;   // the first row of the next batch entry
+  for (; row < end; row++) {
+    if ((kMod || gated) && row == batch_end) {
+      const uint32_t b = (uint32_t)row / (uint32_t)p.ntok;
+      batch_end = (int64_t)(b + 1) * p.ntok;
+#pragma unroll
+      for (int j = 0; j < kV; j++) {
+        const int v = t + T * j;
+        if (v < nv) {
+          if (gated) G[j] = ld16(p.gate + b * p.sg + 8 * v);
+          if (kMod) {
+            SH[j] = ld16(p.shift + b * p.ssh + 8 * v);
+            SC[j] = ld16(p.scale + b * p.ssc + 8 * v);
+          }
+        }
+      }
+    }
+    u32x4 V[kV];   // x_new
     float ss = 0.0f;
 #pragma unroll
     for (int j = 0; j < kV; j++) {
-      const int v = t + T * j;
       float x[8];
       unpack8(X[j], x);
-      if (kRes && v < nv) {
+      V[j] = X[j];
+      if (kRes) {
         float av[8];
         unpack8(A[j], av);
-        if (p.gate) {
+        if (gated) {
           float g[8];
-          unpack8(ld16(p.gate + b * p.sg + 8 * v), g);
+          unpack8(G[j], g);
 #pragma unroll
           for (int e = 0; e < 8; e++) x[e] = __builtin_fmaf(g[e], av[e], x[e]);
         } else {
 #pragma unroll
           for (int e = 0; e < 8; e++) x[e] += av[e];
         }
-        X[j] = pack8(x);
-        *reinterpret_cast<u32x4 *>(p.xn + row * p.C + 8 * v) = X[j];
-        unpack8(X[j], x);
+        V[j] = pack8(x);
+        unpack8(V[j], x);
       }
+      if (t + T * j < nv) {   // (past the row's end: zeros times whatever G holds there)
 #pragma unroll
-      for (int e = 0; e < 8; e++) ss = __builtin_fmaf(x[e], x[e], ss);
+        for (int e = 0; e < 8; e++) ss = __builtin_fmaf(x[e], x[e], ss);
+      }
+    }
+    if (row + 1 < end) fetch(row + 1);
+    if (kRes) {
+#pragma unroll
+      for (int j = 0; j < kV; j++) {
+        const int v = t + T * j;
+        if (v < nv) *reinterpret_cast<u32x4 *>(p.xn + row * p.C + 8 * v) = V[j];
+      }
     }
     ss = team_sum<T>(ss, red_s);
     const float rstd = __fdiv_rn(1.0f, __builtin_sqrtf(__fdiv_rn(ss, (float)p.C) + p.eps));
@@ -166,15 +202,14 @@ __global__ __launch_bounds__(kWG<T>) void rmsnorm_rows_kernel(NormRowsArgs p) {
     for (int j = 0; j < kV; j++) {
       const int v = t + T * j;
       if (v < nv) {
-        float x[8], w[8];
-        unpack8(X[j], x);
-        load8(p.w, p.w32, 8 * v, w);
+        float x[8];
+        unpack8(V[j], x);
 #pragma unroll
-        for (int e = 0; e < 8; e++) H[j][e] = w[e] * (x[e] * rstd);
+        for (int e = 0; e < 8; e++) H[j][e] = W[j][e] * (x[e] * rstd);
         if (kMod) {
           float sh[8], sc[8];
-          unpack8(ld16(p.shift + b * p.ssh + 8 * v), sh);
-          unpack8(ld16(p.scale + b * p.ssc + 8 * v), sc);
+          unpack8(SH[j], sh);
+          unpack8(SC[j], sc);
 #pragma unroll
           for (int e = 0; e < 8; e++) H[j][e] = __builtin_fmaf(H[j][e], 1.0f + sc[e], sh[e]);
         }
@@ -293,7 +328,7 @@ struct NormBwdRowsArgs {
 };
 
 // The rows of a workgroup in their order, each thread's columns' dw in registers; a workgroup's teams are added in their
-// order, then the workgroups in theirs (rmsnorm_rows_dw_kernel): the same sums in every run.
+// order, then the workgroups in theirs (column_sum_kernel): the same sums in every run.
 template <int T, int kV>
 __global__ __launch_bounds__(kWG<T>) void rmsnorm_rows_bwd_kernel(NormBwdRowsArgs p) {
   constexpr int R = kWG<T> / T;
@@ -382,28 +417,38 @@ __global__ __launch_bounds__(kWG<T>) void rmsnorm_rows_bwd_kernel(NormBwdRowsArg
   }
 }
 
-// dw[c] = sum over g of P[g, c]: 16 threads of a workgroup take 64 columns, its 16 groups every 16th row each.
-__global__ __launch_bounds__(256) void rmsnorm_rows_dw_kernel(const float *__restrict__ P, int G, int C,
-                                                              void *__restrict__ dw, int dw32) {
-  __shared__ float4 red[16][16];
-  const int c4 = threadIdx.x & 15, g0 = threadIdx.x >> 4;
-  const int c = blockIdx.x * 64 + 4 * c4;
+// out[c] = sum over g of P[g, c], in fp32 in a fixed order: 4 threads of a workgroup take 16 columns, its 64 groups every 64th
+// row each, four requested at a time, and the groups are added in pairs.
+__global__ __launch_bounds__(256) void column_sum_kernel(const float *__restrict__ P, int G, int C, void *__restrict__ out,
+                                                         int out32) {
+  __shared__ float4 red[64][4];
+  const int c4 = threadIdx.x & 3, g0 = threadIdx.x >> 2;
+  const int c = blockIdx.x * 16 + 4 * c4;
   float4 a{0.0f, 0.0f, 0.0f, 0.0f};
+  auto add = [](float4 &x, const float4 &y) { x.x += y.x, x.y += y.y, x.z += y.z, x.w += y.w; };
   if (c < C)
-    for (int g = g0; g < G; g += 16) {
-      const float4 v = *reinterpret_cast<const float4 *>(P + (int64_t)g * C + c);
-      a.x += v.x, a.y += v.y, a.z += v.z, a.w += v.w;
+    for (int g = g0; g < G; g += 256) {
+      float4 v[4];
+#pragma unroll
+      for (int i = 0; i < 4; i++) {
+        v[i] = float4{0.0f, 0.0f, 0.0f, 0.0f};
+        if (g + 64 * i < G) v[i] = *reinterpret_cast<const float4 *>(P + (int64_t)(g + 64 * i) * C + c);
+      }
+#pragma unroll
+      for (int i = 0; i < 4; i++) add(a, v[i]);
     }
   red[g0][c4] = a;
-  __syncthreads();
-  if (g0 != 0 || c >= C) return;
-  for (int i = 1; i < 16; i++) {
-    const float4 v = red[i][c4];
-    a.x += v.x, a.y += v.y, a.z += v.z, a.w += v.w;
+  for (int n = 32; n > 0; n >>= 1) {
+    __syncthreads();
+    if (g0 < n) {
+      add(a, red[g0 + n][c4]);
+      red[g0][c4] = a;
+    }
   }
-  if (dw32) *reinterpret_cast<float4 *>(static_cast<float *>(dw) + c) = a;
+  if (g0 != 0 || c >= C) return;
+  if (out32) *reinterpret_cast<float4 *>(static_cast<float *>(out) + c) = a;
   else
-    *reinterpret_cast<u32x2 *>(static_cast<uint16_t *>(dw) + c) = u32x2{pack_bf16(a.x, a.y), pack_bf16(a.z, a.w)};
+    *reinterpret_cast<u32x2 *>(static_cast<uint16_t *>(out) + c) = u32x2{pack_bf16(a.x, a.y), pack_bf16(a.z, a.w)};
 }
 
 // qt[c, r] = q[r, c]: tiles of 64 x 64 bytes through LDS, 16 bytes a thread in and out; columns rows .. ldt - 1 of qt zero.
@@ -451,6 +496,12 @@ static unsigned row_blocks(int64_t rows, int teams) {
 }
 
 static bool dtype_ok(int d) { return d == GPIC_DTYPE_BF16 || d == GPIC_DTYPE_F32; }
+
+// Rows a team of the norm takes: one while the workgroups do not fill the device twice over, then up to 8.
+static int norm_chunk(int64_t rows, int teams) {
+  const int64_t c = std::min<int64_t>(rows / (2048 * teams), 8);
+  return (int)std::max<int64_t>(std::max<int64_t>(c, 1), rows / ((int64_t)teams << 21) + 1);
+}
 
 // Workgroups of the norm's backward: each leaves a partial row of dw.
 static int norm_bwd_blocks(int64_t rows, int64_t C) {
@@ -511,15 +562,17 @@ int gpic_fp8_rmsnorm_rows(const uint16_t *x, int64_t ldx, const uint16_t *a, int
     return GPIC_EALIGN;
   if (rows == 0) return GPIC_OK;
   const NormRowsArgs p{x, a, gate, shift, scale, w, xn, h, rstd, s, q, rows, ntok, ldx, lda, sg, ssh, ssc,
-                       (int)C, w_dtype == GPIC_DTYPE_F32, eps};
+                       (int)C, w_dtype == GPIC_DTYPE_F32, 1, eps};
   const hipStream_t st = (hipStream_t)stream;
   with_team(C, [&](auto T, auto V) {
     constexpr int t = decltype(T)::value, v = decltype(V)::value;
     if constexpr (t * v * 8 <= kMaxNormC) {
-      const unsigned g = row_blocks(rows, kWG<t> / t);
+      NormRowsArgs q = p;
+      q.chunk = norm_chunk(rows, kWG<t> / t);
+      const unsigned g = (unsigned)((rows + (int64_t)q.chunk * (kWG<t> / t) - 1) / ((int64_t)q.chunk * (kWG<t> / t)));
       auto *k = a ? (shift ? rmsnorm_rows_kernel<t, v, true, true> : rmsnorm_rows_kernel<t, v, true, false>)
                   : (shift ? rmsnorm_rows_kernel<t, v, false, true> : rmsnorm_rows_kernel<t, v, false, false>);
-      k<<<g, kWG<t>, 0, st>>>(p);
+      k<<<g, kWG<t>, 0, st>>>(q);
     }
   });
   return (int)hipGetLastError();
@@ -549,8 +602,8 @@ int gpic_fp8_rmsnorm_rows_bwd(const uint16_t *dh, const uint16_t *dxn, const uin
       constexpr int t = decltype(T)::value, v = decltype(V)::value;
       if constexpr (t * v * 8 <= kMaxNormC) rmsnorm_rows_bwd_kernel<t, v><<<g, kWG<t>, 0, st>>>(p);
     });
-  rmsnorm_rows_dw_kernel<<<(unsigned)((C + 63) / 64), 256, 0, st>>>(static_cast<const float *>(ws), g, (int)C, dw,
-                                                                    dw_dtype == GPIC_DTYPE_F32);
+  column_sum_kernel<<<(unsigned)((C + 15) / 16), 256, 0, st>>>(static_cast<const float *>(ws), g, (int)C, dw,
+                                                               dw_dtype == GPIC_DTYPE_F32);
   return (int)hipGetLastError();
 }
 
