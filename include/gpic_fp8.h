@@ -349,10 +349,6 @@ int gpic_fp8_bf16_gemm_mn(const uint16_t *A, int64_t lda, const uint16_t *B, int
 int gpic_fp8_tcast_rows(const void *x, int dtype, int64_t ldx, int64_t rows, int64_t cols, uint8_t *q, float *s,
                         void *stream);
 
-/* qt [cols, ldt] = q [rows, cols] transposed (bytes; cols, ldt % 16 == 0, ldt >= rows, columns rows..ldt-1 zero): a weight's
- * bytes as the K-major operand of its dgrad. */
-int gpic_fp8_transpose_bytes(const uint8_t *q, int64_t rows, int64_t cols, uint8_t *qt, int64_t ldt, void *stream);
-
 /*
  * RMSNorm with the residual's addition and a row-scaled e4m3 output:
  *   x_new = bf16(x + gate * a) -> xn (a != NULL; gate NULL: x + a), else x_new = x
@@ -401,9 +397,15 @@ int gpic_fp8_gemm_rows(const uint8_t *A, int64_t lda, const float *sa, const uin
  *   dz = bf16(d): the operand of the weight's gradient;  q, s = the row cast of d * sw, sw [N] the weight's row scales, which
  *   lie on the dgrad's reduction: with them in the gradient, the dgrad reads the forward's weight bytes, transposed.
  *   dy, z [rows, N] bf16 (row strides lddy, ldz); dz [rows, N] bf16; q [rows, N]; s [rows]. N % 8 == 0, N <= 32768.
+ *   wq [N, K] e4m3 (or NULL): wqt [K, ldt] gets its bytes transposed (K, ldt % 16 == 0, ldt >= N, columns N..ldt-1 zero), in
+ *   the same launch: the dgrad is gpic_fp8_gemm_rows(q, s, wqt, NULL).
+ *   db (or NULL) [N] of db_dtype: the sum of dz (NONE: of dy) over the rows, fp32 in a fixed order, rounded once. ws (with db):
+ *   gpic_fp8_act_bwd_rows_workspace_bytes(rows, N) bytes, scratch of this call.
  */
+size_t gpic_fp8_act_bwd_rows_workspace_bytes(int64_t rows, int64_t N);
 int gpic_fp8_act_bwd_rows(const uint16_t *dy, int64_t lddy, const uint16_t *z, int64_t ldz, int act, const float *sw,
-                          int64_t rows, int64_t N, uint16_t *dz, uint8_t *q, float *s, void *stream);
+                          int64_t rows, int64_t N, uint16_t *dz, uint8_t *q, float *s, const uint8_t *wq, int64_t K,
+                          uint8_t *wqt, int64_t ldt, void *db, int db_dtype, void *ws, size_t ws_bytes, void *stream);
 
 #ifdef __cplusplus
 }

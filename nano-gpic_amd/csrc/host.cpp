@@ -473,16 +473,24 @@ LinearGrads linear_bwd_run(const at::Tensor &dy, const at::Tensor &z, int act, c
                            const at::Tensor &x, bool need_dx, bool need_dw, bool need_db, bool w32, bool b32, void *stream) {
   const int64_t M = dy.size(0), N = dy.size(1), K = wq.size(1);
   LinearGrads o;
-  const at::Tensor dz = act == GPIC_ACT_NONE ? dy : make(dy, {M, N}, at::kBFloat16);
+  const bool on = act != GPIC_ACT_NONE;
+  const at::Tensor dz = on ? make(dy, {M, N}, at::kBFloat16) : dy;
   const at::Tensor q = make(dy, {M, N}, kE4), s = make(dy, {M}, at::kFloat);
-  check(gpic_fp8_act_bwd_rows(ptr<uint16_t>(dy), N, act == GPIC_ACT_NONE ? nullptr : ptr<uint16_t>(z), N, act, ptr<float>(sw),
-                              M, N, act == GPIC_ACT_NONE ? nullptr : ptr<uint16_t>(dz), ptr<uint8_t>(q), ptr<float>(s), stream),
-        "gpic_fp8_act_bwd_rows");
-  if (need_dx) {
-    const at::Tensor qt = make(dy, {K, N}, kE4);
-    check(gpic_fp8_transpose_bytes(ptr<uint8_t>(wq), N, K, ptr<uint8_t>(qt), N, stream), "gpic_fp8_transpose_bytes");
-    o.dx = gemm_rows_run(q, s, qt, std::nullopt, std::nullopt, GPIC_ACT_NONE, std::nullopt, Mod(), false, stream).y;
+  at::Tensor qt, ws;
+  size_t bytes = 0;
+  if (need_dx) qt = make(dy, {K, N}, kE4);
+  if (need_db) {
+    o.db = make(dy, {N}, b32 ? at::kFloat : at::kBFloat16);
+    bytes = gpic_fp8_act_bwd_rows_workspace_bytes(M, N);
+    ws = make(dy, {(int64_t)bytes}, at::kByte);
   }
+  check(gpic_fp8_act_bwd_rows(ptr<uint16_t>(dy), N, on ? ptr<uint16_t>(z) : nullptr, N, act, ptr<float>(sw), M, N,
+                              on ? ptr<uint16_t>(dz) : nullptr, ptr<uint8_t>(q), ptr<float>(s),
+                              need_dx ? ptr<uint8_t>(wq) : nullptr, K, need_dx ? ptr<uint8_t>(qt) : nullptr, N,
+                              need_db ? o.db.data_ptr() : nullptr, b32 ? GPIC_DTYPE_F32 : GPIC_DTYPE_BF16,
+                              need_db ? ws.data_ptr() : nullptr, bytes, stream),
+        "gpic_fp8_act_bwd_rows");
+  if (need_dx) o.dx = gemm_rows_run(q, s, qt, std::nullopt, std::nullopt, GPIC_ACT_NONE, std::nullopt, Mod(), false, stream).y;
   if (need_dw) {
     o.dw = make(dy, {N, K}, w32 ? at::kFloat : at::kBFloat16);
     const Scratch w(dy, N, K, 2 * M);   // (planned as an e4m3 GEMM of as many K bytes)
@@ -490,7 +498,6 @@ LinearGrads linear_bwd_run(const at::Tensor &dy, const at::Tensor &z, int act, c
                                 w32 ? GPIC_DTYPE_F32 : GPIC_DTYPE_BF16, K, N, K, M, w.p(), w.bytes, stream),
           "gpic_fp8_bf16_gemm_mn");
   }
-  if (need_db) o.db = bias_grad(dz, b32, stream);
   return o;
 }
 py::object or_none(const at::Tensor &t) { return t.defined() ? py::cast(t) : py::none(); }

@@ -259,32 +259,113 @@ __global__ __launch_bounds__(kWG<T>) void tcast_rows_kernel(const void *__restri
   }
 }
 
+// A 64 x 64 tile of qt[c, r] = q[r, c] by 256 threads, 16 bytes each in and out; columns rows .. ldt - 1 of qt zero. on: whether
+// there is a tile (uniform over the 256 threads; all of a workgroup's meet at the barrier).
+struct TransposeTile {
+  uint8_t b[64][80];   // (80: 16-byte rows on different banks)
+};
+__device__ __forceinline__ void transpose_tile(const uint8_t *q, int64_t rows, int64_t cols, uint8_t *qt, int64_t ldt,
+                                               int64_t tile_r, int64_t tile_c, bool on, TransposeTile &tile) {
+  const int64_t r0 = tile_r * 64, c0 = tile_c * 64;
+  const int i = (threadIdx.x & 255) >> 2, k = 16 * (threadIdx.x & 3);
+  u32x4 v{0u, 0u, 0u, 0u};
+  if (on && r0 + i < rows && c0 + k < cols) v = ld16(q + (r0 + i) * cols + c0 + k);
+  *reinterpret_cast<u32x4 *>(&tile.b[i][k]) = v;
+  __syncthreads();
+  if (on && c0 + i < cols && r0 + k < ldt) {
+    uint32_t o[4];
+#pragma unroll
+    for (int w = 0; w < 4; w++)
+      o[w] = (uint32_t)tile.b[k + 4 * w][i] | (uint32_t)tile.b[k + 4 * w + 1][i] << 8 |
+             (uint32_t)tile.b[k + 4 * w + 2][i] << 16 | (uint32_t)tile.b[k + 4 * w + 3][i] << 24;
+    *reinterpret_cast<u32x4 *>(qt + (c0 + i) * ldt + r0 + k) = u32x4{o[0], o[1], o[2], o[3]};
+  }
+}
+
+// The teams' column sums D of a workgroup, added in their order by the first, to row blockIdx.x of P [.., C]. part: T kV 8 words
+// where a workgroup has several teams.
+template <int T, int kV>
+__device__ __forceinline__ void store_column_partials(float (&D)[kV][8], float *part, float *P, int C) {
+  constexpr int R = kWG<T> / T;
+  const int t = threadIdx.x % T, team = threadIdx.x / T;
+  if constexpr (R > 1) {
+    for (int i = 1; i < R; i++) {
+      __syncthreads();
+      if (team == i) {
+#pragma unroll
+        for (int j = 0; j < kV; j++)
+#pragma unroll
+          for (int e = 0; e < 8; e++) part[(j * 8 + e) * T + t] = D[j][e];
+      }
+      __syncthreads();
+      if (team == 0) {
+#pragma unroll
+        for (int j = 0; j < kV; j++)
+#pragma unroll
+          for (int e = 0; e < 8; e++) D[j][e] += part[(j * 8 + e) * T + t];
+      }
+    }
+    if (team != 0) return;
+  }
+#pragma unroll
+  for (int j = 0; j < kV; j++) {
+    const int v = t + T * j;
+    if (v < C / 8) {
+      float *o = P + (int64_t)blockIdx.x * C + 8 * v;
+      *reinterpret_cast<float4 *>(o) = float4{D[j][0], D[j][1], D[j][2], D[j][3]};
+      *reinterpret_cast<float4 *>(o + 4) = float4{D[j][4], D[j][5], D[j][6], D[j][7]};
+    }
+  }
+}
+
+// The epilogue's backward, and beside it, in workgroups of their own, the transposed bytes of the weight that the dgrad reads
+// (independent work: a launch less in the chain). kDb: each thread also sums its columns' dz, as rounded, over its rows, for
+// column_sum_kernel: the same order in every run.
 struct ActBwdArgs {
   const uint16_t *dy, *z;
   const float *sw;
+  const uint8_t *wq;   // [N, K]: transposed by the workgroups past row_blocks
+  uint8_t *wqt;        // [K, ldt]
   uint16_t *dz;
   uint8_t *q;
-  float *s;
-  int64_t rows, lddy, ldz;
-  int N, act;
+  float *s, *P;        // P: [row_blocks, N] partial sums (kDb)
+  int64_t rows, lddy, ldz, K, ldt, tiles_c, tiles;
+  int N, act, row_blocks;
 };
 
-template <int T, int kV>
+template <int T, int kV, bool kDb>
 __global__ __launch_bounds__(kWG<T>) void act_bwd_rows_kernel(ActBwdArgs p) {
+  constexpr int R = kWG<T> / T;
   __shared__ uint32_t red_m[2][T > 64 ? T / 64 : 1];
+  __shared__ TransposeTile tile[kWG<T> / 256];
+  __shared__ __attribute__((aligned(16))) float part[kDb && R > 1 ? T * kV * 8 : 4];
+  if ((int)blockIdx.x >= p.row_blocks) {
+    const int sub = threadIdx.x >> 8;
+    const int64_t i = (int64_t)((int)blockIdx.x - p.row_blocks) * (kWG<T> / 256) + sub;
+    transpose_tile(p.wq, p.N, p.K, p.wqt, p.ldt, i / p.tiles_c, i % p.tiles_c, i < p.tiles, tile[sub]);
+    return;
+  }
   const int t = threadIdx.x % T, nv = p.N / 8;
-  int turn = 0;
-  for (int64_t row = team_row<T>(); row < p.rows; row += team_step<T>(), turn ^= 1) {
-    u32x4 Y[kV], Z[kV];
+  float D[kV][8];
+#pragma unroll
+  for (int j = 0; j < kV; j++)
+#pragma unroll
+    for (int e = 0; e < 8; e++) D[j][e] = 0.0f;
+  u32x4 Y[kV], Z[kV];
+  auto fetch = [&](int64_t r) {
 #pragma unroll
     for (int j = 0; j < kV; j++) {
       const int v = t + T * j;
-      Y[j] = Z[j] = u32x4{0u, 0u, 0u, 0u};
       if (v < nv) {
-        Y[j] = ld16(p.dy + row * p.lddy + 8 * v);
-        if (p.act) Z[j] = ld16(p.z + row * p.ldz + 8 * v);
+        Y[j] = ld16(p.dy + r * p.lddy + 8 * v);
+        if (p.act) Z[j] = ld16(p.z + r * p.ldz + 8 * v);
       }
     }
+  };
+  int64_t row = team_row<T>();
+  const int64_t step = (int64_t)p.row_blocks * R;
+  if (row < p.rows) fetch(row);
+  for (int turn = 0; row < p.rows; row += step, turn ^= 1) {
     float H[kV][8];
     uint32_t m = 0;
 #pragma unroll
@@ -297,7 +378,14 @@ __global__ __launch_bounds__(kWG<T>) void act_bwd_rows_kernel(ActBwdArgs p) {
           unpack8(Z[j], z);
 #pragma unroll
           for (int e = 0; e < 8; e++) d[e] *= act_bwd(z[e], p.act);
-          *reinterpret_cast<u32x4 *>(p.dz + row * p.N + 8 * v) = pack8(d);
+          Y[j] = pack8(d);
+          *reinterpret_cast<u32x4 *>(p.dz + row * p.N + 8 * v) = Y[j];
+        }
+        if (kDb) {
+          float r[8];
+          unpack8(Y[j], r);
+#pragma unroll
+          for (int e = 0; e < 8; e++) D[j][e] += r[e];
         }
         float w[8];
         load8(p.sw, true, 8 * v, w);
@@ -306,6 +394,7 @@ __global__ __launch_bounds__(kWG<T>) void act_bwd_rows_kernel(ActBwdArgs p) {
         m = absmax8(H[j], m);
       }
     }
+    if (row + step < p.rows) fetch(row + step);   // (the next row is under way during this one's maximum and stores)
     float scale, dequant;
     scales_from_amax(team_max<T>(m, red_m[turn]), scale, dequant);
 #pragma unroll
@@ -315,6 +404,7 @@ __global__ __launch_bounds__(kWG<T>) void act_bwd_rows_kernel(ActBwdArgs p) {
     }
     if (t == 0) p.s[row] = dequant;
   }
+  if constexpr (kDb) store_column_partials<T, kV>(D, part, p.P, p.N);
 }
 
 struct NormBwdRowsArgs {
@@ -334,7 +424,7 @@ __global__ __launch_bounds__(kWG<T>) void rmsnorm_rows_bwd_kernel(NormBwdRowsArg
   constexpr int R = kWG<T> / T;
   __shared__ float red_s[2][T > 64 ? T / 64 : 1];
   __shared__ __attribute__((aligned(16))) float part[R > 1 ? T * kV * 8 : 4];
-  const int t = threadIdx.x % T, team = threadIdx.x / T, nv = p.C / 8;
+  const int t = threadIdx.x % T, nv = p.C / 8;
   float W[kV][8], D[kV][8];
 #pragma unroll
   for (int j = 0; j < kV; j++) {
@@ -387,34 +477,7 @@ __global__ __launch_bounds__(kWG<T>) void rmsnorm_rows_bwd_kernel(NormBwdRowsArg
       }
     }
   }
-  if constexpr (R > 1) {   // the teams' sums, added in their order by the first
-    for (int i = 1; i < R; i++) {
-      __syncthreads();
-      if (team == i) {
-#pragma unroll
-        for (int j = 0; j < kV; j++)
-#pragma unroll
-          for (int e = 0; e < 8; e++) part[(j * 8 + e) * T + t] = D[j][e];
-      }
-      __syncthreads();
-      if (team == 0) {
-#pragma unroll
-        for (int j = 0; j < kV; j++)
-#pragma unroll
-          for (int e = 0; e < 8; e++) D[j][e] += part[(j * 8 + e) * T + t];
-      }
-    }
-    if (team != 0) return;
-  }
-#pragma unroll
-  for (int j = 0; j < kV; j++) {
-    const int v = t + T * j;
-    if (v < nv) {
-      float *o = p.P + (int64_t)blockIdx.x * p.C + 8 * v;
-      *reinterpret_cast<float4 *>(o) = float4{D[j][0], D[j][1], D[j][2], D[j][3]};
-      *reinterpret_cast<float4 *>(o + 4) = float4{D[j][4], D[j][5], D[j][6], D[j][7]};
-    }
-  }
+  store_column_partials<T, kV>(D, part, p.P, p.C);
 }
 
 // out[c] = sum over g of P[g, c], in fp32 in a fixed order: 4 threads of a workgroup take 16 columns, its 64 groups every 64th
@@ -451,26 +514,6 @@ __global__ __launch_bounds__(256) void column_sum_kernel(const float *__restrict
     *reinterpret_cast<u32x2 *>(static_cast<uint16_t *>(out) + c) = u32x2{pack_bf16(a.x, a.y), pack_bf16(a.z, a.w)};
 }
 
-// qt[c, r] = q[r, c]: tiles of 64 x 64 bytes through LDS, 16 bytes a thread in and out; columns rows .. ldt - 1 of qt zero.
-__global__ __launch_bounds__(256) void transpose_bytes_kernel(const uint8_t *__restrict__ q, int64_t rows, int64_t cols,
-                                                              uint8_t *__restrict__ qt, int64_t ldt, int64_t tiles_c) {
-  __shared__ uint8_t tile[64][80];   // (80: 16-byte rows on different banks)
-  const int64_t r0 = (int64_t)blockIdx.x / tiles_c * 64, c0 = (int64_t)blockIdx.x % tiles_c * 64;
-  const int i = threadIdx.x >> 2, k = 16 * (threadIdx.x & 3);
-  u32x4 v{0u, 0u, 0u, 0u};
-  if (r0 + i < rows && c0 + k < cols) v = ld16(q + (r0 + i) * cols + c0 + k);
-  *reinterpret_cast<u32x4 *>(&tile[i][k]) = v;
-  __syncthreads();
-  if (c0 + i < cols && r0 + k < ldt) {
-    uint32_t o[4];
-#pragma unroll
-    for (int w = 0; w < 4; w++)
-      o[w] = (uint32_t)tile[k + 4 * w][i] | (uint32_t)tile[k + 4 * w + 1][i] << 8 |
-             (uint32_t)tile[k + 4 * w + 2][i] << 16 | (uint32_t)tile[k + 4 * w + 3][i] << 24;
-    *reinterpret_cast<u32x4 *>(qt + (c0 + i) * ldt + r0 + k) = u32x4{o[0], o[1], o[2], o[3]};
-  }
-}
-
 // ------------------------------------------------------------------------------------------- host side
 
 // Calls f(T, kV) with the team and the steps for rows of C elements (C <= 8 T kV).
@@ -491,6 +534,21 @@ static void with_team(int64_t C, F f) {
   else f(S(), V4());
 }
 
+// The same for the epilogue's backward, which holds dy, z, db and two rows' loads: at most two steps a thread up to 16384.
+template <class F>
+static void with_short_team(int64_t C, F f) {
+  typedef std::integral_constant<int, 1> V1;
+  typedef std::integral_constant<int, 2> V2;
+  typedef std::integral_constant<int, 256> Q;
+  if (C <= 512) f(std::integral_constant<int, 64>(), V1());
+  else if (C <= 1024) f(std::integral_constant<int, 64>(), V2());
+  else if (C <= 2048) f(Q(), V1());
+  else if (C <= 4096) f(Q(), V2());
+  else if (C <= 8192) f(std::integral_constant<int, 512>(), V2());
+  else if (C <= 16384) f(std::integral_constant<int, 1024>(), V2());
+  else f(std::integral_constant<int, 1024>(), std::integral_constant<int, 4>());
+}
+
 static unsigned row_blocks(int64_t rows, int teams) {
   return (unsigned)std::min<int64_t>((rows + teams - 1) / teams, kMaxRowBlocks);
 }
@@ -501,6 +559,12 @@ static bool dtype_ok(int d) { return d == GPIC_DTYPE_BF16 || d == GPIC_DTYPE_F32
 static int norm_chunk(int64_t rows, int teams) {
   const int64_t c = std::min<int64_t>(rows / (2048 * teams), 8);
   return (int)std::max<int64_t>(std::max<int64_t>(c, 1), rows / ((int64_t)teams << 21) + 1);
+}
+
+// Workgroups of the epilogue's backward: with db each leaves a partial row of it.
+static int act_bwd_blocks(int64_t rows, int64_t N, bool db) {
+  const int teams = N <= 1024 ? 4 : 1;
+  return (int)std::min<int64_t>((rows + teams - 1) / teams, db ? N <= 4096 ? 768 : 512 : kMaxRowBlocks);
 }
 
 // Workgroups of the norm's backward: each leaves a partial row of dw.
@@ -530,19 +594,6 @@ int gpic_fp8_tcast_rows(const void *x, int dtype, int64_t ldx, int64_t rows, int
     if (dtype == GPIC_DTYPE_F32) tcast_rows_kernel<t, v, true><<<g, kWG<t>, 0, st>>>(x, ldx, rows, (int)cols, q, s);
     else tcast_rows_kernel<t, v, false><<<g, kWG<t>, 0, st>>>(x, ldx, rows, (int)cols, q, s);
   });
-  return (int)hipGetLastError();
-}
-
-int gpic_fp8_transpose_bytes(const uint8_t *q, int64_t rows, int64_t cols, uint8_t *qt, int64_t ldt, void *stream) {
-  status_scope();
-  if (rows < 0 || cols < 0) return GPIC_EINVAL;
-  if (cols % 16 || ldt % 16 || ldt < rows) return GPIC_ESHAPE;
-  if (rows == 0 || cols == 0) return GPIC_OK;
-  if (!q || !qt) return GPIC_EINVAL;
-  if (!aligned16(q) || !aligned16(qt)) return GPIC_EALIGN;
-  const int64_t tc = (cols + 63) / 64, tiles = (ldt + 63) / 64 * tc;
-  if (tiles >= (int64_t(1) << 24)) return GPIC_ESHAPE;   // (a launch's threads are counted in 32 bits)
-  transpose_bytes_kernel<<<(unsigned)tiles, 256, 0, (hipStream_t)stream>>>(q, rows, cols, qt, ldt, tc);
   return (int)hipGetLastError();
 }
 
@@ -607,19 +658,40 @@ int gpic_fp8_rmsnorm_rows_bwd(const uint16_t *dh, const uint16_t *dxn, const uin
   return (int)hipGetLastError();
 }
 
+size_t gpic_fp8_act_bwd_rows_workspace_bytes(int64_t rows, int64_t N) {
+  if (rows <= 0 || N <= 0) return 0;
+  return (size_t)act_bwd_blocks(rows, N, true) * N * sizeof(float);
+}
+
 int gpic_fp8_act_bwd_rows(const uint16_t *dy, int64_t lddy, const uint16_t *z, int64_t ldz, int act, const float *sw,
-                          int64_t rows, int64_t N, uint16_t *dz, uint8_t *q, float *s, void *stream) {
+                          int64_t rows, int64_t N, uint16_t *dz, uint8_t *q, float *s, const uint8_t *wq, int64_t K,
+                          uint8_t *wqt, int64_t ldt, void *db, int db_dtype, void *ws, size_t ws_bytes, void *stream) {
   status_scope();
-  if (rows < 0 || N <= 0 || act < GPIC_ACT_NONE || act > GPIC_ACT_GELU_TANH) return GPIC_EINVAL;
+  if (rows < 0 || N <= 0 || act < GPIC_ACT_NONE || act > GPIC_ACT_GELU_TANH || !wq != !wqt || (wq && K < 0)) return GPIC_EINVAL;
   if (rows > 0 && (!dy || !sw || !q || !s || (act && (!z || !dz)))) return GPIC_EINVAL;
+  if (db && !dtype_ok(db_dtype)) return GPIC_EDTYPE;
   if (N % 8 || N > kMaxRowC || lddy % 8 || lddy < N || (act && (ldz % 8 || ldz < N))) return GPIC_ESHAPE;
-  if (!aligned16(dy) || !aligned16(sw) || !aligned16(q) || (act && (!aligned16(z) || !aligned16(dz)))) return GPIC_EALIGN;
-  if (rows == 0) return GPIC_OK;
-  const ActBwdArgs p{dy, z, sw, dz, q, s, rows, lddy, ldz, (int)N, act};
-  with_team(N, [&](auto T, auto V) {
-    constexpr int t = decltype(T)::value, v = decltype(V)::value;
-    act_bwd_rows_kernel<t, v><<<row_blocks(rows, kWG<t> / t), kWG<t>, 0, (hipStream_t)stream>>>(p);
-  });
+  if (wq && (K % 16 || ldt % 16 || ldt < N)) return GPIC_ESHAPE;
+  if (!aligned16(dy) || !aligned16(sw) || !aligned16(q) || (act && (!aligned16(z) || !aligned16(dz))) || !aligned16(wq) ||
+      !aligned16(wqt) || !aligned16(db) || !aligned16(ws))
+    return GPIC_EALIGN;
+  if (db && (ws_bytes < gpic_fp8_act_bwd_rows_workspace_bytes(rows, N) || (rows > 0 && !ws))) return GPIC_EWORKSPACE;
+  const hipStream_t st = (hipStream_t)stream;
+  const int64_t tc = wq ? (K + 63) / 64 : 1, tiles = wq ? (ldt + 63) / 64 * tc : 0;
+  if (tiles >= (int64_t(1) << 23)) return GPIC_ESHAPE;   // (a launch's threads are counted in 32 bits)
+  const int g = rows ? act_bwd_blocks(rows, N, db != nullptr) : 0;
+  if (g == 0 && tiles == 0 && !db) return GPIC_OK;
+  const ActBwdArgs p{dy, z, sw, wq, wqt, dz, q, s, static_cast<float *>(ws), rows, lddy, ldz, K, ldt, tc, tiles,
+                     (int)N, act, g};
+  if (g > 0 || tiles > 0)
+    with_short_team(N, [&](auto T, auto V) {
+      constexpr int t = decltype(T)::value, v = decltype(V)::value, sub = kWG<t> / 256;
+      auto *k = db ? act_bwd_rows_kernel<t, v, true> : act_bwd_rows_kernel<t, v, false>;
+      k<<<(unsigned)(g + (tiles + sub - 1) / sub), kWG<t>, 0, st>>>(p);
+    });
+  if (db)
+    column_sum_kernel<<<(unsigned)((N + 15) / 16), 256, 0, st>>>(static_cast<const float *>(ws), g, (int)N, db,
+                                                                 db_dtype == GPIC_DTYPE_F32);
   return (int)hipGetLastError();
 }
 

@@ -22,7 +22,7 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from . import _lib as L
-from .fp8_native import E4, _bias_grad, _gemm_operand, _no_autocast, _r16, _rows, bf16_wgrad
+from .fp8_native import E4, _gemm_operand, _no_autocast, _r16, _rows, bf16_wgrad
 from .norm import BWD_MAX_C, res_mod_rmsnorm_bwd_k
 
 ACTS = {"none": 0, "silu": 1, "gelu_tanh": 2, "swiglu": 3}
@@ -109,24 +109,6 @@ def tcast_rows(x):
     """x [..., C] (any float dtype, C % 8 == 0, C <= 32768) -> (q e4m3, x's shape; s [rows] fp32): tcast with one amax, and
     one scale, a row. A NaN in a row makes its scale NaN."""
     return _run(tcast_rows_op, x)
-
-
-@L.step_op("gpic::fp8_transpose_bytes")
-def transpose_bytes(q: torch.Tensor) -> torch.Tensor:
-    """q [R, C] e4m3 (C % 16 == 0) -> [C, R16], its bytes transposed, zero past R."""
-    L.require_gpu(q)
-    q = L.aligned(q.contiguous())
-    R, C = q.shape
-    qt = torch.empty(C, _r16(R), dtype=E4, device=q.device)
-    with L.on_device(q.device):
-        L.check(L.lib().gpic_fp8_transpose_bytes(q.data_ptr(), R, C, qt.data_ptr(), qt.shape[1], L.stream_ptr(q.device)),
-                "gpic_fp8_transpose_bytes")
-    return qt
-
-
-@transpose_bytes.register_fake
-def _(q):
-    return q.new_empty(q.shape[1], _r16(q.shape[0]))
 
 
 class RowsWeight(NamedTuple):
@@ -338,43 +320,58 @@ def fp8_gemm_rows(a, sa, b, sb, bias=None, act="none", residual=None, gate=None)
 
 
 @L.step_op("gpic::fp8_act_bwd_rows")
-def act_bwd_rows_op(dy: torch.Tensor, z: Optional[torch.Tensor], act: str, sw: torch.Tensor
-                    ) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
-    """act_bwd_rows, as an op (dz empty for act="none")."""
-    L.require_gpu(dy, z, sw)
+def act_bwd_rows_op(dy: torch.Tensor, z: Optional[torch.Tensor], act: str, sw: torch.Tensor,
+                    wq: Optional[torch.Tensor] = None, want_db: bool = False, db32: bool = False
+                    ) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
+    """act_bwd_rows, as an op: (dz, empty for act="none"; q; s; wq [N, K]'s bytes transposed [K, N16]; the sum of dz over the
+    rows, bf16 or db32), the last two empty unless asked for."""
+    L.require_gpu(dy, z, sw, wq)
     code = _act(act, train=True)
     if dy.dim() != 2 or dy.dtype != BF or dy.shape[1] % 8 or not 0 < dy.shape[1] <= CAST_MAX_C:
         raise ValueError(f"act_bwd_rows takes bf16 dy [M, N] with N % 8 == 0 and 0 < N <= {CAST_MAX_C}, got {dy.dtype} "
                          f"{tuple(dy.shape)}")
     M, N = dy.shape
     dev = dy.device
-    _same_device(dev, z=z, sw=sw)
+    _same_device(dev, z=z, sw=sw, wq=wq)
     if code and (z is None or z.shape != dy.shape or z.dtype != BF):
         raise ValueError("act_bwd_rows needs the forward's bf16 z, of dy's shape")
+    if wq is not None and (wq.dtype != E4 or wq.dim() != 2 or wq.shape[0] != N or wq.shape[1] % 16):
+        raise ValueError(f"wq must be e4m3 [{N}, K] with K % 16 == 0, got {wq.dtype} {tuple(wq.shape)}")
     sw = _scales(sw, N, "sw")
     dy, ldy = _rows(dy)
     z, ldz = _rows(z) if code else (None, 0)
     dz = torch.empty((M, N) if code else (0,), dtype=BF, device=dev)
     q = torch.empty(M, N, dtype=E4, device=dev)
     s = torch.empty(M, dtype=torch.float32, device=dev)
+    K = 0 if wq is None else wq.shape[1]
+    wq = None if wq is None else L.aligned(wq.contiguous())
+    wqt = torch.empty((0,) if wq is None else (K, _r16(N)), dtype=E4, device=dev)
+    db = torch.empty(N if want_db else 0, dtype=torch.float32 if db32 else BF, device=dev)
     with L.on_device(dev):
-        L.check(L.lib().gpic_fp8_act_bwd_rows(dy.data_ptr(), ldy, L.ptr(z), ldz, code, sw.data_ptr(), M, N,
-                                              dz.data_ptr() if code else None, q.data_ptr(), s.data_ptr(),
-                                              L.stream_ptr(dev)), "gpic_fp8_act_bwd_rows")
-    return dz, q, s
+        nws = L.lib().gpic_fp8_act_bwd_rows_workspace_bytes(M, N) if want_db else 0
+        ws = torch.empty(max(nws, 16), dtype=torch.uint8, device=dev) if want_db else None
+        L.check(L.lib().gpic_fp8_act_bwd_rows(
+            dy.data_ptr(), ldy, L.ptr(z), ldz, code, sw.data_ptr(), M, N, dz.data_ptr() if code else None, q.data_ptr(),
+            s.data_ptr(), L.ptr(wq), K, wqt.data_ptr() if wq is not None else None, _r16(N),
+            db.data_ptr() if want_db else None, L.DTYPE_CODE[db.dtype], L.ptr(ws), nws, L.stream_ptr(dev)),
+            "gpic_fp8_act_bwd_rows")
+    return dz, q, s, wqt, db
 
 
 @act_bwd_rows_op.register_fake
-def _(dy, z, act, sw):
+def _(dy, z, act, sw, wq=None, want_db=False, db32=False):
+    N = dy.shape[1]
     return (dy.new_empty(dy.shape if act != "none" else (0,)), dy.new_empty(dy.shape, dtype=E4),
-            dy.new_empty(dy.shape[0], dtype=torch.float32))
+            dy.new_empty(dy.shape[0], dtype=torch.float32),
+            dy.new_empty((0,) if wq is None else (wq.shape[1], _r16(N)), dtype=E4),
+            dy.new_empty(N if want_db else 0, dtype=torch.float32 if db32 else BF))
 
 
 def act_bwd_rows(dy, z, act, sw):
     """dy [M, N] bf16 and the forward's z [M, N] bf16 (unused for act="none") -> (dz = dy act'(z) as bf16, dy itself for
     "none"; dz sw as e4m3; its scales [M]): the operands of the weight's gradient and, against the weight's bytes
     transposed, of the dgrad (sw [N]: the weight's scales, which lie on its reduction)."""
-    dz, q, s = _run(act_bwd_rows_op, dy, z, act, sw)
+    dz, q, s, _, _ = _run(act_bwd_rows_op, dy, z, act, sw)
     return (dy if act == "none" else dz), q, s
 
 
@@ -387,13 +384,13 @@ def _linear_bwd(ctx, dy2, z, wq, sw, x2, need_dx, need_dw, need_db):
     if r is not None:
         dx, dw, db = r
         return dx, dw if dw is None else dw.to(ctx.wdt), db if db is None else db.to(ctx.bdt)
-    dz, dq, sd = L.call(act_bwd_rows_op, dy2, z, ctx.act, sw)
+    dz, dq, sd, wqt, db = L.call(act_bwd_rows_op, dy2, z, ctx.act, sw, wq if need_dx else None, need_db,
+                                 ctx.bdt == torch.float32)
     if ctx.act == "none":
         dz = dy2
-    dx = L.call(gemm_rows_op, dq, sd, L.call(transpose_bytes, wq), None)[0] if need_dx else None
+    dx = L.call(gemm_rows_op, dq, sd, wqt, None)[0] if need_dx else None
     dw = L.call(bf16_wgrad, dz, x2, ctx.wdt == torch.float32).to(ctx.wdt) if need_dw else None
-    db = _bias_grad(dz, ctx.bdt) if need_db else None
-    return dx, dw, db
+    return dx, dw, db.to(ctx.bdt) if need_db else None
 
 
 class _LinearRows(torch.autograd.Function):

@@ -84,14 +84,6 @@ def test_tcast_rows_past_32_bits(dev):
     assert not q[:1000].view(torch.uint8).any()
 
 
-@pytest.mark.parametrize("rows,C", [(1, 16), (16, 64), (17, 48), (100, 80), (200, 1040), (64, 64), (1000, 176)])
-def test_transpose_bytes(dev, rows, C):
-    q = torch.randint(0, 256, (rows, C), generator=gen(dev), device=dev, dtype=torch.uint8).view(E4)
-    t = GR.transpose_bytes(q)
-    assert t.shape == (C, (rows + 15) // 16 * 16)
-    assert torch.equal(u8(t)[:, :rows], u8(q).t()) and not u8(t)[:, rows:].any()
-
-
 # ------------------------------------------------------------------------------------------------ norm
 
 def eps_of(C, mag):
@@ -328,6 +320,29 @@ def test_act_bwd_rows(dev, M, N, act):
     else:
         R.within(dz, ref, ref.abs() * R.UBF + 2 * eps, "dz")
     R.check_rowq(q, s, ref * sw.double(), (eps + ref.abs() * U) * sw.double())
+
+
+@pytest.mark.parametrize("act", ["none", "gelu_tanh"])
+@pytest.mark.parametrize("M,N,K", [(1, 16, 16), (0, 64, 32), (5, 72, 48), (3, 1040, 200 // 16 * 16), (1000, 2048, 64),
+                                   (7, 4104, 80), (900, 2056, 16), (2, 16392, 176), (4000, 64, 1024)])
+def test_act_bwd_rows_transpose_and_sum(dev, M, N, K, act):
+    """The weight's bytes transposed in the same launch, and the column sums of the dz that it wrote."""
+    g = gen(dev, N)
+    dy, z, sw = randn(g, M, N), randn(g, M, N), torch.rand(N, generator=g, device=dev) + 0.5
+    wq = torch.randint(0, 256, (N, K), generator=g, device=dev, dtype=torch.uint8).view(E4)
+    for b32 in (False, True):
+        dz, q, s, wqt, db = GR.act_bwd_rows_op(dy, z, act, sw, wq, True, b32)
+        assert wqt.shape == (K, (N + 15) // 16 * 16)
+        assert torch.equal(u8(wqt)[:, :N], u8(wq).t()) and not u8(wqt)[:, N:].any()
+        d = (dy if act == "none" else dz).double()
+        # a chain of rows per team (M over 768 x 4, 768, or all in one), 3 teams, 16 partial rows, 6 pairs
+        chain = -(-M // 3072) if N <= 2048 else -(-M // 768)
+        bound = d.abs().sum(0) * (chain + 28) * U + (0 if b32 else d.sum(0).abs() * R.UBF)
+        assert db.dtype == (F32 if b32 else BF)
+        R.within(db, d.sum(0), bound + 1e-38, "db")
+        plain = GR.act_bwd_rows_op(dy, z, act, sw)
+        assert torch.equal(u8(plain[1]), u8(q)) and torch.equal(plain[0], dz) and torch.equal(plain[2], s)
+        assert torch.equal(db, GR.act_bwd_rows_op(dy, z, act, sw, None, True, b32)[4])
 
 
 def test_act_bwd_differences(dev):

@@ -28,15 +28,6 @@ def test_tcast_rows_codes(p):
     assert f(x=p + 8) == EALIGN and f(q=p + 8) == EALIGN
 
 
-def test_transpose_bytes_codes(p):
-    f = lambda q=p, r=20, c=32, qt=p, ld=32: L.lib().gpic_fp8_transpose_bytes(q, r, c, qt, ld, None)  # noqa: E731
-    assert f(r=0) == 0 and f(c=0) == 0
-    assert f(r=-1) == EINVAL and f(q=None) == EINVAL and f(qt=None) == EINVAL
-    assert f(c=24) == ESHAPE and f(ld=16) == ESHAPE and f(ld=24) == ESHAPE
-    assert f(r=1 << 40, ld=1 << 40) == ESHAPE
-    assert f(q=p + 4) == EALIGN and f(qt=p + 4) == EALIGN
-
-
 def test_rmsnorm_rows_codes(p):
     def f(x=p, ldx=64, a=p, lda=64, gate=p, sg=64, w=p, wd=1, sh=p, ssh=64, sc=p, ssc=64, rows=4, ntok=2, C=64, xn=p, h=None,
           rstd=p, q=p, s=p):
@@ -91,16 +82,22 @@ def test_gemm_rows_codes(p):
 
 
 def test_act_bwd_rows_codes(p):
-    def f(dy=p, ldy=64, z=p, ldz=64, act=1, sw=p, rows=4, N=64, dz=p, q=p, s=p):
-        return L.lib().gpic_fp8_act_bwd_rows(dy, ldy, z, ldz, act, sw, rows, N, dz, q, s, None)
-    assert f(rows=0) == 0
+    def f(dy=p, ldy=64, z=p, ldz=64, act=1, sw=p, rows=4, N=64, dz=p, q=p, s=p, wq=p, K=32, wqt=p, ldt=64, db=p, dd=0, ws=p,
+          nws=1 << 20):
+        return L.lib().gpic_fp8_act_bwd_rows(dy, ldy, z, ldz, act, sw, rows, N, dz, q, s, wq, K, wqt, ldt, db, dd, ws, nws, None)
+    need = L.lib().gpic_fp8_act_bwd_rows_workspace_bytes
+    assert need(0, 64) == 0 and need(4, 64) >= 64 * 4 and need(1 << 20, 1024) % (1024 * 4) == 0
+    assert f(rows=0, wq=None, wqt=None, db=None) == 0
     for bad in (dict(rows=-1), dict(N=0), dict(act=3), dict(act=-1), dict(dy=None), dict(z=None), dict(sw=None), dict(dz=None),
-                dict(q=None), dict(s=None)):
+                dict(q=None), dict(s=None), dict(wq=None), dict(wqt=None), dict(K=-16)):
         assert f(**bad) == EINVAL, bad
-    for bad in (dict(N=60), dict(N=32776, ldy=32776, ldz=32776), dict(ldy=60), dict(ldy=56), dict(ldz=60), dict(ldz=56)):
+    assert f(dd=4) == EDTYPE
+    for bad in (dict(N=60), dict(N=32776, ldy=32776, ldz=32776), dict(ldy=60), dict(ldy=56), dict(ldz=60), dict(ldz=56),
+                dict(K=24), dict(ldt=48), dict(ldt=72), dict(K=1 << 40)):
         assert f(**bad) == ESHAPE, bad
-    for name in ("dy", "z", "sw", "dz", "q"):
+    for name in ("dy", "z", "sw", "dz", "q", "wq", "wqt", "db", "ws"):
         assert f(**{name: p + 8}) == EALIGN, name
+    assert f(nws=need(4, 64) - 1) == EWORKSPACE and f(ws=None) == EWORKSPACE
 
 
 def test_cpu_tensors_are_refused():
@@ -152,6 +149,7 @@ def test_refusals(no_gpu_check):
         lambda: G.fp8_gemm_rows(z(4, 64), None, z(16, 64, dt=F32).to(E4), None),
         lambda: G.fp8_gemm_rows(q[:, :0], None, q[:, :0], None),
         lambda: G.act_bwd_rows(z(4, 64), None, "silu", w), lambda: G.act_bwd_rows(z(4, 64), z(4, 64), "swiglu", w),
+        lambda: GR.act_bwd_rows_op(z(4, 64), None, "none", w, q), lambda: GR.act_bwd_rows_op(z(4, 64), None, "none", w, z(64, 32)),
         lambda: G.act_bwd_rows(z(4, 64, dt=F32), None, "none", w), lambda: G.act_bwd_rows(z(4, 64), None, "none", w[:32]),
         lambda: G.rows_weight(z(24, 64)), lambda: G.rows_weight(z(32, 24)), lambda: G.rows_weight(z(32, 64), "relu6"),
         lambda: G.rows_weight(z(16, 64), "swiglu"), lambda: G.swiglu_layout(z(16)),
@@ -198,7 +196,6 @@ def test_fake_kernels():
         e = lambda *s, dt=BF: torch.empty(*s, dtype=dt, device="cuda")  # noqa: E731
         q, s = GR.tcast_rows_op(e(2, 3, 64))
         assert q.shape == (2, 3, 64) and q.dtype == E4 and s.shape == (6,) and s.dtype == F32
-        assert GR.transpose_bytes(e(20, 32, dt=E4)).shape == (32, 32)
         xn, h, q, s, r = GR.rmsnorm_rows_op(e(2, 3, 64), e(64, dt=F32), 1e-6, e(2, 3, 64), None, None, None, True)
         assert xn.shape == h.shape == q.shape == (2, 3, 64) and s.shape == r.shape == (6,) and xn.dtype == h.dtype == BF
         assert GR.rmsnorm_rows_op(e(3, 64), e(64), 1e-6)[0].numel() == 0
@@ -206,8 +203,9 @@ def test_fake_kernels():
         assert dx.shape == (3, 64) and dw.shape == (64,) and dw.dtype == BF
         y, z = GR.gemm_rows_op(e(3, 64, dt=E4), None, e(32, 64, dt=E4), None, None, "swiglu", None, None, True)
         assert y.shape == (3, 16) and z.shape == (3, 32) and y.dtype == z.dtype == BF
-        dz, q, s = GR.act_bwd_rows_op(e(3, 64), e(3, 64), "silu", e(64, dt=F32))
+        dz, q, s, t, b = GR.act_bwd_rows_op(e(3, 64), e(3, 64), "silu", e(64, dt=F32), e(64, 32, dt=E4), True, True)
         assert dz.shape == q.shape == (3, 64) and s.shape == (3,) and q.dtype == E4
+        assert t.shape == (32, 64) and b.shape == (64,) and b.dtype == F32
 
 
 def test_host_module_takes_no_cpu_tensors():
