@@ -157,7 +157,6 @@ __device__ __forceinline__ u32x4 bias8(const void *bias, bool f32, int n) {
 
 // The epilogue of the row-scaled GEMM (gpic_fp8_gemm_rows): the instances with RowsEpi apply it in fp32 to the accumulators
 // and round once, to bf16; those with NoEpi are the tensorwise GEMM's.
-struct NoEpi {};
 struct RowsEpi {
   const float *sa, *sb;   // dequantization scales of A's and B's rows, or null (1)
   const void *bias;       // [N] bf16, or fp32 (bias32), or null
@@ -168,6 +167,22 @@ struct RowsEpi {
   uint32_t ntok;
   int ldr, ldz, bias32, act;
 };
+// The large tiles' instances: with residual or gate (kAdd), with z (kZ); what an instance lacks costs it no registers.
+template <bool kAddP, bool kZP>
+struct RowsEpiT : RowsEpi {
+  static constexpr bool kAdd = kAddP, kZ = kZP;
+};
+struct NoEpi {
+  static constexpr bool kAdd = false, kZ = false;
+};
+
+// The same values, out of the compiler's sight: what is derived from them is derived where it is used, per tile, instead of
+// being kept across the K loop (null tests, addresses: 60 scalar registers' worth, spilled).
+__device__ __forceinline__ RowsEpi opaque_epi(const RowsEpi &p) {
+  RowsEpi e = p;
+  asm volatile("" : "+s"(e.sa), "+s"(e.sb), "+s"(e.bias), "+s"(e.res), "+s"(e.gate), "+s"(e.z), "+s"(e.act), "+s"(e.bias32));
+  return e;
+}
 
 __device__ __forceinline__ void unpack8(u32x4 v, float (&f)[8]) {
 #pragma unroll
@@ -190,54 +205,70 @@ __device__ __forceinline__ void vec8(const void *p, bool f32, int n, float none,
     unpack8(*reinterpret_cast<const u32x4 *>(static_cast<const uint16_t *>(p) + n), f);
   }
 }
-// Eight columns of one row: v = z = v sa sb + bias; y = bf16(res + gate act(z)) packed (SwiGLU: the run holds 4 gate columns
-// and their 4 partners, y is 4 values in .x and .y, and so are res and gate).
-__device__ __forceinline__ u32x4 epi8(const RowsEpi &ep, float (&v)[8], float sa, const float (&sb)[8],
-                                      const float (&b)[8], u32x4 res, u32x4 gate) {
+__device__ __forceinline__ void load8f(__amdgpu_buffer_rsrc_t r, int off, float (&f)[8]) {
+  const v4f x = __builtin_bit_cast(v4f, __builtin_amdgcn_raw_buffer_load_b128(r, off, 0, 0));
+  const v4f y = __builtin_bit_cast(v4f, __builtin_amdgcn_raw_buffer_load_b128(r, off + 16, 0, 0));
 #pragma unroll
-  for (int e = 0; e < 8; e++) v[e] = __builtin_fmaf(v[e] * sa, sb[e], b[e]);
-  float y[8], r[8], g[8];
-  if (ep.act == GPIC_ACT_SWIGLU) {
+  for (int e = 0; e < 4; e++) f[e] = x[e], f[4 + e] = y[e];
+}
+// act of 8 columns of z, in place; SwiGLU: 4 values in f[0..3] from 4 gate columns and their 4 partners.
+template <int kAct>
+__device__ __forceinline__ void act8(float (&f)[8]) {
+  if constexpr (kAct == GPIC_ACT_SWIGLU) {
 #pragma unroll
-    for (int e = 0; e < 4; e++) y[e] = v[e] * fast_sigmoid(v[e]) * v[4 + e], y[4 + e] = 0.0f;
+    for (int e = 0; e < 4; e++) f[e] = f[e] * fast_sigmoid(f[e]) * f[4 + e];
   } else {
 #pragma unroll
-    for (int e = 0; e < 8; e++) y[e] = act_fwd(v[e], ep.act);
+    for (int e = 0; e < 8; e++) f[e] = act_fwd(f[e], kAct);
+  }
+}
+// Calls f with the activation as a constant: one (uniform) branch around code that has none.
+template <class F>
+__device__ __forceinline__ void with_act(int act, F f) {
+  if (act == GPIC_ACT_NONE) f(std::integral_constant<int, GPIC_ACT_NONE>());
+  else if (act == GPIC_ACT_SILU) f(std::integral_constant<int, GPIC_ACT_SILU>());
+  else if (act == GPIC_ACT_GELU_TANH) f(std::integral_constant<int, GPIC_ACT_GELU_TANH>());
+  else f(std::integral_constant<int, GPIC_ACT_SWIGLU>());
+}
+// y = res + gate y of 8 columns; res and gate packed bf16, where the epilogue has them.
+__device__ __forceinline__ void add8(const RowsEpi &ep, float (&y)[8], u32x4 res, u32x4 gate) {
+  float r[8], g[8];
+  if (ep.gate) {
+    unpack8(gate, g);
+#pragma unroll
+    for (int e = 0; e < 8; e++) y[e] *= g[e];   // (with -ffp-contract=off: two roundings in fp32)
   }
   if (ep.res) {
     unpack8(res, r);
-    if (ep.gate) {
-      unpack8(gate, g);
 #pragma unroll
-      for (int e = 0; e < 8; e++) y[e] = __builtin_fmaf(g[e], y[e], r[e]);
-    } else {
-#pragma unroll
-      for (int e = 0; e < 8; e++) y[e] += r[e];
-    }
-  } else if (ep.gate) {
-    unpack8(gate, g);
-#pragma unroll
-    for (int e = 0; e < 8; e++) y[e] *= g[e];
+    for (int e = 0; e < 8; e++) y[e] += r[e];
   }
-  return pack8(y);
 }
-// epi8 of row m (< M), columns n .. n + 7, with its loads and stores (16 bytes, SwiGLU: 8).
-__device__ __forceinline__ void epi8_row(const RowsEpi &ep, float (&v)[8], const float (&sb)[8], const float (&b)[8],
-                                         uint16_t *C, int64_t ldc, int64_t m, int n) {
+// 16 bytes of a bf16 row, or (half, SwiGLU's 4 columns) 8 and zeros.
+__device__ __forceinline__ u32x4 row8(const uint16_t *p, bool half) {
+  if (!half) return *reinterpret_cast<const u32x4 *>(p);
+  const u32x2 h = *reinterpret_cast<const u32x2 *>(p);
+  return u32x4{h.x, h.y, 0u, 0u};
+}
+// The epilogue of 8 columns n .. n + 7 of row m (< M): v the accumulators, sa, sb, b the scales and biases, r the residual.
+__device__ __forceinline__ void epi8_row(const RowsEpi &ep, float (&v)[8], float sa, const float (&sb)[8],
+                                         const float (&b)[8], u32x4 r, uint16_t *C, int64_t ldc, int64_t m, int n) {
   const bool half = ep.act == GPIC_ACT_SWIGLU;
   const int no = half ? n >> 1 : n;
-  u32x4 r{0u, 0u, 0u, 0u}, g{0u, 0u, 0u, 0u};
-  auto load = [&](const uint16_t *p) {
-    if (!half) return *reinterpret_cast<const u32x4 *>(p);
-    const u32x2 h = *reinterpret_cast<const u32x2 *>(p);
-    return u32x4{h.x, h.y, 0u, 0u};
-  };
-  if (ep.res) r = load(ep.res + m * ep.ldr + no);
-  if (ep.gate) g = load(ep.gate + (int64_t)((uint32_t)m / ep.ntok) * ep.sg + no);
-  const u32x4 y = epi8(ep, v, ep.sa ? ep.sa[m] : 1.0f, sb, b, r, g);
+#pragma unroll
+  for (int e = 0; e < 8; e++) v[e] = __builtin_fmaf(v[e] * sa, sb[e], b[e]);
   if (ep.z) *reinterpret_cast<u32x4 *>(ep.z + m * ep.ldz + n) = pack8(v);
-  if (half) *reinterpret_cast<u32x2 *>(C + m * ldc + no) = u32x2{y.x, y.y};
-  else *reinterpret_cast<u32x4 *>(C + m * ldc + no) = y;
+  u32x4 g{0u, 0u, 0u, 0u};
+  if (ep.gate) g = row8(ep.gate + (int64_t)((uint32_t)m / ep.ntok) * ep.sg + no, half);
+  with_act(ep.act, [&](auto act) { act8<decltype(act)::value>(v); });
+  add8(ep, v, r, g);
+  if (half) *reinterpret_cast<u32x2 *>(C + m * ldc + no) = u32x2{pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3])};
+  else *reinterpret_cast<u32x4 *>(C + m * ldc + no) = pack8(v);
+}
+// Its residual, zeros without one.
+__device__ __forceinline__ u32x4 epi8_res(const RowsEpi &ep, int64_t m, int n) {
+  const bool half = ep.act == GPIC_ACT_SWIGLU;
+  return ep.res ? row8(ep.res + m * ep.ldr + (half ? n >> 1 : n), half) : u32x4{0u, 0u, 0u, 0u};
 }
 
 // Half h of a 32-byte fragment as a bf16 MFMA operand.
@@ -274,8 +305,8 @@ __global__ __launch_bounds__(kThreads) void gemm_tn_kernel(const uint8_t *__rest
                                                             const float *__restrict__ sa, const float *__restrict__ sb,
                                                             const void *__restrict__ bias, int bias32, CT *__restrict__ C,
                                                             int64_t ldc, float *__restrict__ P, int M, int N, int K,
-                                                            int ksplit, int tiles_m, int tiles_n, int splits, EPI ep) {
-  constexpr bool kRows = std::is_same_v<EPI, RowsEpi>;
+                                                            int ksplit, int tiles_m, int tiles_n, int splits, EPI epi) {
+  constexpr bool kRows = std::is_base_of_v<RowsEpi, EPI>, kAdd = EPI::kAdd, kKeepZ = EPI::kZ;
   static_assert(kBNt == 256 || kBNt == 128, "tile widths: 256 or 128");
   static_assert(kMN || (kEl == 1 && !kC32), "bf16 operands and fp32 outputs: MN-major only");
   static_assert(!(kMN && kTail) || kBNt == 256, "MN-major rows masked lane by lane: the wide tile only");
@@ -611,6 +642,101 @@ __global__ __launch_bounds__(kThreads) void gemm_tn_kernel(const uint8_t *__rest
     // so their latency passes during this item's epilogue
     const int nit = it + gridDim.x;
     const bool more = nit < work;
+    // the row-scaled epilogue's operands of block h: a lane's rows row_of(h, i) (of the tile) and runs of 8 columns from
+    // col_of_run(h, q); the first block's are waited for here, before the prologue's loads queue behind them
+    constexpr bool kLdsRes = kAdd && kBNt == 256;
+    constexpr int kRM = 2, kBlocks = kTNt / 2;   // 16-row tiles of a block; blocks: rows 32 (h & 1), columns 64 (h / 2)
+    float e_sa[kTM], e_sb[2][8], e_b[2][8];
+    u32x4 e_res[2][kRM], e_gate[2][kRM];
+    std::conditional_t<kRows, RowsEpi, NoEpi> ep;
+    if constexpr (kRows) ep = opaque_epi(epi);
+    auto row_of = [&](int l, int h, int i) { return wm * kWTM + 32 * (h & 1) + 16 * i + (l & 15); };
+    auto col_of_run = [&](int l, int h, int q) { return cur.n0 + wn * kWTNt + 64 * (h >> 1) + 32 * q + 8 * (l >> 4); };
+    auto e_load = [&](int h) {
+      if constexpr (kRows) {
+        const int l = opaque_v(lane);
+        // (buffer loads: columns past N, and a vector that is not there, read zeros without a branch around the load, whose
+        // other arm's constants the compiler would keep in registers across the K loop)
+        if (!(h & 1)) {
+          const __amdgpu_buffer_rsrc_t rS = __builtin_amdgcn_make_buffer_rsrc((void *)ep.sb, 0, ep.sb ? N * 4 : 0, kBufferFlags);
+          const __amdgpu_buffer_rsrc_t rB = __builtin_amdgcn_make_buffer_rsrc(
+              (void *)ep.bias, 0, ep.bias ? N * (ep.bias32 ? 4 : 2) : 0, kBufferFlags);
+          const float one = ep.sb ? 0.0f : 1.0f;
+#pragma unroll
+          for (int q = 0; q < 2; q++) {
+            const int n = col_of_run(l, h, q);
+            load8f(rS, n * 4, e_sb[q]);
+#pragma unroll
+            for (int e = 0; e < 8; e++) e_sb[q][e] += one;
+            if (ep.bias32) load8f(rB, n * 4, e_b[q]);
+            else unpack8(__builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(rB, n * 2, 0, 0)), e_b[q]);
+          }
+        }
+        if constexpr (kAdd) {
+          const bool half = ep.act == GPIC_ACT_SWIGLU;
+          // (a SwiGLU's 8 bytes: the 16 that hold them)
+          auto col = [&](int n) { return half ? (n >> 1) & ~7 : n; };
+          // the gate's row of a row of the tile, counted from the tile's first (its descriptor's base)
+          const uint32_t b0 = ep.gate ? (uint32_t)cur.m0 / ep.ntok : 0;
+          const __amdgpu_buffer_rsrc_t rG = __builtin_amdgcn_make_buffer_rsrc(
+              (void *)(ep.gate + (int64_t)b0 * ep.sg), 0,
+              ep.gate ? (int)(((uint32_t)(min(cur.m0 + kBM, M) - 1) / ep.ntok - b0) * (uint32_t)ep.sg + (half ? N >> 1 : N)) * 2 : 0,
+              kBufferFlags);
+#pragma unroll
+          for (int i = 0; i < kRM; i++) {
+            const int m = cur.m0 + row_of(l, h, i);
+            const int b = ep.gate && m < M ? (int)((uint32_t)m / ep.ntok - b0) : 0;
+#pragma unroll
+            for (int q = 0; q < 2; q++)
+              e_gate[q][i] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(
+                                                           rG, (b * (int)ep.sg + col(col_of_run(l, h, q))) * 2, 0, 0));
+          }
+          if constexpr (!kLdsRes) {
+            const int rows = min(M - cur.m0, kBM);
+            const __amdgpu_buffer_rsrc_t rR = __builtin_amdgcn_make_buffer_rsrc(
+                (void *)(ep.res + (int64_t)cur.m0 * ep.ldr), 0, ep.res ? rows * ep.ldr * 2 : 0, kBufferFlags);   // (none: zeros)
+#pragma unroll
+            for (int q = 0; q < 2; q++)
+#pragma unroll
+              for (int i = 0; i < kRM; i++) {
+                const int n = col_of_run(l, h, q), r = row_of(l, h, i);
+                const int off = n < N && r < rows ? (r * ep.ldr + col(n)) * 2 : kOOB;
+                e_res[q][i] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(rR, off, 0, 0));
+              }
+          }
+        }
+      }
+    };
+    // The wide tile's residual of block h by LDS DMA, in the layout in which y is staged, to the 4 KiB after the staged block: no
+    // registers, and whole 128-byte lines (as 64-byte runs into registers, some spilled, [32768 x 1024 x 4096] took 125 us).
+    auto res_send = [&](int h) {
+      if constexpr (kLdsRes) {
+        if (!ep.res) return;
+        const bool half = ep.act == GPIC_ACT_SWIGLU;
+        const int l = opaque_v(lane), rows = min(M - cur.m0, kBM);
+        const v4i rR = buffer_rsrc(ep.res + (int64_t)cur.m0 * ep.ldr, rows * ep.ldr * 2);
+        const uint32_t to = lds_addr(smem) + (group == 0 ? a_half(2) : b_half(1)) + (wave & 3) * kCStage + 4096;
+        const int n = cur.n0 + wn * kWTNt + 64 * (h >> 1), row0 = wm * kWTM + 32 * (h & 1);
+        const int lr = half ? l >> 2 : l >> 3;   // (columns past N: the next row's, or zeros; never stored)
+        for (int i = 0; i < (half ? 2 : 4); i++) {
+          const int r = (half ? 16 : 8) * i + lr;
+          const int c = half ? (l & 3) ^ ((r >> 2) & 3) : (l & 7) ^ ((r >> 1) & 7);
+          lds_dma16(rR, ((row0 + r) * ep.ldr + (half ? n >> 1 : n) + 8 * c) * 2, 0, to + 1024 * i);
+        }
+      }
+    };
+    if constexpr (kRows) {   // (split-K partials do not use them; under a condition they would be carried across the K loop)
+      const __amdgpu_buffer_rsrc_t rA = __builtin_amdgcn_make_buffer_rsrc(
+          (void *)(ep.sa + cur.m0), 0, ep.sa ? min(M - cur.m0, kBM) * 4 : 0, kBufferFlags);
+      const float one = ep.sa ? 0.0f : 1.0f;
+#pragma unroll
+      for (int i = 0; i < kTM; i++)
+        e_sa[i] = one + __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(
+                                                      rA, (wm * kWTM + 16 * i + (lane & 15)) * 4, 0, 0));
+      res_send(0);
+      e_load(0);
+      __builtin_amdgcn_s_waitcnt(0x0f70);   // vmcnt(0)
+    }
     if (more && group == 0) send_prologue(item(nit));
 
     // ---- epilogue: acc[ni][mi] lane l holds C[m][n + v], v = 0..3, for m = mi * 16 + (l & 15) and, through col_of,
@@ -635,91 +761,106 @@ __global__ __launch_bounds__(kThreads) void gemm_tn_kernel(const uint8_t *__rest
         }
       pend = kStoresF32;
     } else if constexpr (kRows) {
-      // The row-scaled epilogue. The accumulators go through LDS as fp32, one 16-row block of the wave at a time (8 KiB, the
-      // narrow tile 4: the same regions as below), so that each lane holds 8 consecutive columns of a row and the same
-      // columns in every row: its scales and biases are loaded once a tile, residual and C move as whole row segments.
-      // 16-byte chunk c (4 columns) of row r sits in slot c ^ r: the 16 lanes of a write (one chunk of 16 rows) hit
-      // 16 different slots. Those of a read take 16 runs of two chunks (wide: of one row; narrow: of two); where they
-      // are of one row, the upper 8 lanes read their second chunk first, so that both reads hit 16 different slots mod 16.
+      // The row-scaled epilogue, in blocks of 32 rows x 64 columns (four, the narrow tile two). Scales, bias,
+      // activation, gate and residual are applied to a lane's runs of 8 columns where the accumulators are; the rounded
+      // runs go through LDS (chunk c of a 128-byte block row r in slot c ^ ((r / 2) & 7); a SwiGLU's rows are 64 bytes, its
+      // runs 8, chunk c in slot c ^ ((r / 4) & 3): the 16 lanes of a write or a read hit 16 different 16-byte slots) and
+      // leave as whole row segments. fp32 through LDS and the rest of the epilogue at the store took half as long again:
+      // [6592 x 4096 x 1024] 46 us. A wait for a load also waits for everything this wave sent before it, so the first
+      // block's operands have landed before the next item's prologue is sent (above), and a later block's are requested
+      // before the stores of the one ahead of it.
       GPIC_LDS uint8_t *cst =
           (GPIC_LDS uint8_t *)smem + (group == 0 ? a_half(2) : b_half(1)) + (wave & 3) * kCStage;
-      constexpr int kRow = kWTNt * 4, kLPR = kWTNt / 8, kRPI = 64 / kLPR, kNI = 16 / kRPI;
-      static_assert(16 * kRow == kCStage && kTM * kNI == kStoresBF16, "the same LDS and the same stores as the bf16 epilogue");
       const bool half = ep.act == GPIC_ACT_SWIGLU;
-      const int rr = (unsigned)el / kLPR, rc = (unsigned)el % kLPR, flip = kBNt == 256 ? rc >> 3 : 0;
-      const int n = cur.n0 + wn * kWTNt + 8 * rc, no = half ? n >> 1 : n;
-      const bool in = n < N;
-      const __amdgpu_buffer_rsrc_t rC = __builtin_amdgcn_make_buffer_rsrc((void *)(C + (int64_t)cur.m0 * ldc), 0,
+      const int64_t c0row = (int64_t)cur.m0;
+      const __amdgpu_buffer_rsrc_t rC = __builtin_amdgcn_make_buffer_rsrc((void *)(C + c0row * ldc), 0,
                                                                           rows_c * (int)ldc * 2, kBufferFlags);
-      const __amdgpu_buffer_rsrc_t rR = __builtin_amdgcn_make_buffer_rsrc(
-          (void *)(ep.res + (int64_t)cur.m0 * ep.ldr), 0, ep.res ? rows_c * ep.ldr * 2 : 0, kBufferFlags);
       const __amdgpu_buffer_rsrc_t rZ = __builtin_amdgcn_make_buffer_rsrc(
-          (void *)(ep.z + (int64_t)cur.m0 * ep.ldz), 0, ep.z ? rows_c * ep.ldz * 2 : 0, kBufferFlags);
-      float sb8[8], b8[8];
-      vec8(in ? ep.sb : nullptr, true, n, 1.0f, sb8);
-      vec8(in ? ep.bias : nullptr, ep.bias32, n, 0.0f, b8);
-      // lane l: the scale and the gate's row of the wave's row l (rows past M: the last one's)
-      const int mrow_l = min(cur.m0 + wm * kWTM + el, M - 1);
-      const float sa_l = ep.sa ? ep.sa[mrow_l] : 1.0f;
-      const int gb_l = ep.gate ? (int)((uint32_t)mrow_l / ep.ntok) : 0;
+          (void *)(ep.z + c0row * ep.ldz), 0, ep.z ? rows_c * ep.ldz * 2 : 0, kBufferFlags);
+      // block h of z (kZ) or of y; `before`: called ahead of the stores
+      auto block = [&](auto act_c, auto z_c, auto h_c, auto before) {
+        constexpr int kAct = decltype(act_c)::value, h = decltype(h_c)::value;
+        constexpr bool kZ = decltype(z_c)::value, kHalf = !kZ && kAct == GPIC_ACT_SWIGLU;
+        constexpr int kRowOut = kHalf ? 64 : 128, kLPR = kRowOut / 16, kRPI = 64 / kLPR, kNI = 16 * kRM / kRPI;
+        // (an opaque lane per block: the blocks' addresses are computed in them, not shared by all and held throughout)
+        const int bl = opaque_v(el), wr = bl & 15, wg = bl >> 4;
+        // the residual's loads, sent before the stores of the block ahead (and this one's z), have landed
+        if constexpr (kLdsRes && !kZ && h > 0)
+          asm volatile("s_waitcnt vmcnt(%0)" ::"n"(kNI + (kKeepZ ? 4 : 0)) : "memory");
 #pragma unroll
-      for (int mi = 0; mi < kTM; mi++) {
-        const int rl0 = wm * kWTM + mi * 16 + rr;   // row within the tile of j = 0; row j is rl0 + kRPI j
-        u32x4 R[kNI], G[kNI];
+        for (int q = 0; q < 2; q++)
 #pragma unroll
-        for (int j = 0; j < kNI; j++) {
-          const int rl = rl0 + kRPI * j;
-          R[j] = G[j] = u32x4{0u, 0u, 0u, 0u};
-          if (ep.res) {
-            const int off = in && rl < rows_c ? (rl * ep.ldr + no) * 2 : kOOB;
-            if (half) {
-              const u32x2 h = __builtin_bit_cast(u32x2, __builtin_amdgcn_raw_buffer_load_b64(rR, off, 0, 0));
-              R[j] = u32x4{h.x, h.y, 0u, 0u};
-            } else {
-              R[j] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(rR, off, 0, 0));
+          for (int i = 0; i < kRM; i++) {
+            const int pp = 2 * (h >> 1) + q, mi = 2 * (h & 1) + i, r = 16 * i + wr;
+            const int at = kHalf ? r * 64 + 16 * ((2 * q + (wg >> 1)) ^ ((r >> 2) & 3)) + 8 * (wg & 1)
+                                 : r * 128 + 16 * ((4 * q + wg) ^ ((r >> 1) & 7));
+            const v4f &x = acc[2 * pp][mi], &y = acc[2 * pp + 1][mi];
+            float v[8] = {x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]};
+            float sa_m = e_sa[mi];
+            asm volatile("" : "+v"(sa_m));   // (the pass that stores z does not keep its values for the one that stores y)
+#pragma unroll
+            for (int e = 0; e < 8; e++) v[e] = __builtin_fmaf(v[e] * sa_m, e_sb[q][e], e_b[q][e]);
+            if (!kZ) {
+              act8<kAct>(v);
+              if constexpr (kAdd) {
+                u32x4 g = e_gate[q][i], rs{0u, 0u, 0u, 0u};
+                const bool up = kHalf && (col_of_run(bl, h, q) & 8);   // (which 8 of the 16 bytes)
+                if constexpr (!kLdsRes) rs = e_res[q][i];
+                else if (kHalf) {
+                  const st8_t w = *(const GPIC_LDS st8_t *)(cst + 4096 + at);
+                  rs = u32x4{w.x, w.y, 0u, 0u};
+                } else {
+                  rs = __builtin_bit_cast(u32x4, *(const GPIC_LDS st16_t *)(cst + 4096 + at));
+                }
+                if (up && !kLdsRes) rs.x = rs.z, rs.y = rs.w;
+                if (up) g.x = g.z, g.y = g.w;
+                add8(ep, v, rs, g);
+              }
             }
+            if constexpr (kHalf)
+              *(GPIC_LDS st8_t *)(cst + at) = st8_t{pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3])};
+            else
+              *(GPIC_LDS st16_t *)(cst + at) = st16_t{pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3]), pack_bf16(v[4], v[5]), pack_bf16(v[6], v[7])};
           }
-          if (ep.gate) {   // (the shuffle with every lane active; columns past N read the row's first)
-            const uint16_t *g = ep.gate + (int64_t)__shfl(gb_l, mi * 16 + kRPI * j + rr, 64) * ep.sg + (in ? no : 0);
-            if (half) {
-              const u32x2 h = *reinterpret_cast<const u32x2 *>(g);
-              G[j] = u32x4{h.x, h.y, 0u, 0u};
-            } else {
-              G[j] = *reinterpret_cast<const u32x4 *>(g);
-            }
-          }
-        }
-#pragma unroll
-        for (int ni = 0; ni < kTNt; ni++)
-          *(GPIC_LDS f4a_t *)(cst + wr * kRow + 16 * ((8 * (ni >> 1) + 2 * wg + (ni & 1)) ^ wr)) = acc[ni][mi];
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // the block is complete before any lane reads it back
-        f4a_t X[kNI], Y[kNI];
+        const int rr = (unsigned)bl / kLPR, rc = (unsigned)bl % kLPR;
+        st16_t wv[kNI];
 #pragma unroll
         for (int j = 0; j < kNI; j++) {
           const int r = kRPI * j + rr;
-          X[j] = *(const GPIC_LDS f4a_t *)(cst + r * kRow + 16 * ((2 * rc + flip) ^ r));
-          Y[j] = *(const GPIC_LDS f4a_t *)(cst + r * kRow + 16 * ((2 * rc + 1 - flip) ^ r));
+          wv[j] = *(const GPIC_LDS st16_t *)(cst + r * kRowOut + 16 * (rc ^ (kHalf ? (r >> 2) & 3 : (r >> 1) & 7)));
         }
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // read back before the next block overwrites it
+        before();
+        const int n = cur.n0 + wn * kWTNt + 64 * (h >> 1);
+        const int no = (kHalf ? n >> 1 : n) + 8 * rc, ld = kZ ? ep.ldz : (int)ldc;
+        const int rl = wm * kWTM + 32 * (h & 1) + rr;
 #pragma unroll
-        for (int j = 0; j < kNI; j++) {
-          const int rl = rl0 + kRPI * j;
-          float v[8];
-#pragma unroll
-          for (int e = 0; e < 4; e++) {
-            v[e] = flip ? Y[j][e] : X[j][e];
-            v[4 + e] = flip ? X[j][e] : Y[j][e];
-          }
-          const u32x4 y = epi8(ep, v, __shfl(sa_l, mi * 16 + kRPI * j + rr, 64), sb8, b8, R[j], G[j]);
-          const bool on = in && rl < rows_c;
-          if (ep.z)
-            __builtin_amdgcn_raw_buffer_store_b128(pack8(v), rZ, on ? (rl * ep.ldz + n) * 2 : kOOB, 0, kStoreNT);
-          const int off = on ? (rl * (int)ldc + no) * 2 : kOOB;
-          if (half) __builtin_amdgcn_raw_buffer_store_b64(u32x2{y.x, y.y}, rC, off, 0, kStoreNT);
-          else __builtin_amdgcn_raw_buffer_store_b128(y, rC, off, 0, kStoreNT);
+        for (int j = 0; j < kNI; j++)
+          __builtin_amdgcn_raw_buffer_store_b128(
+              __builtin_bit_cast(u32x4, wv[j]), kZ ? rZ : rC,
+              rl + kRPI * j < rows_c && no < (kHalf ? N >> 1 : N) ? ((rl + kRPI * j) * ld + no) * 2 : kOOB, 0, kStoreNT);
+      };
+      with_act(ep.act, [&](auto act) {
+        auto both = [&](auto h) {
+          constexpr int next = decltype(h)::value + 1;
+          if constexpr (kKeepZ) block(act, std::true_type(), h, []() {});
+          block(act, std::false_type(), h, [&]() {
+            if constexpr (next < kBlocks) {
+              res_send(next);
+              e_load(next);
+            }
+          });
+        };
+        both(std::integral_constant<int, 0>());
+        both(std::integral_constant<int, 1>());
+        if constexpr (kBlocks > 2) {
+          both(std::integral_constant<int, 2>());
+          both(std::integral_constant<int, 3>());
         }
-      }
-      pend = ep.z ? 2 * kStoresBF16 : kStoresBF16;
+      });
+      // (stores: a SwiGLU's half as many; counting fewer than there are only waits longer)
+      pend = kKeepZ ? (half ? kStoresBF16 : 2 * kStoresBF16) : half ? 0 : kStoresBF16;
     } else {
       // bf16 output through LDS: each lane rounds its runs of 8 columns (scaled) to bf16 and writes them to LDS as
       // 16 bytes (MN-major: its runs of 4 as 8 bytes), one 32 x 128 block (two 16-row tile rows) of the wave at a
@@ -860,6 +1001,27 @@ __global__ __launch_bounds__(256) void gemm_small_kernel(const uint8_t *__restri
       else lds_dma16(rB, vo, k0, to + kA + 32 * i * kBK);
     }
   };
+  // the row-scaled epilogue's operands, requested before the K tiles: a lane's 8 columns (one pair of 16-column tiles) and its
+  // kFM rows ([512 x 8192 x 1024]: 12.6 us with the loads after the last K tile)
+  constexpr bool kRows = std::is_same_v<EPI, RowsEpi>;
+  static_assert(!kRows || kFN == 2, "one run of 8 columns a lane");
+  struct Operands {
+    int n;
+    float sa[kFM], sb[8], b[8];
+    u32x4 res[kFM];
+  };
+  std::conditional_t<kRows, Operands, NoEpi> eo;
+  if constexpr (kRows) {
+    eo.n = n0 + wn * (kSN / 2) + 8 * (lane >> 4);
+    vec8(eo.n < N ? ep.sb : nullptr, true, eo.n, 1.0f, eo.sb);
+    vec8(eo.n < N ? ep.bias : nullptr, ep.bias32, eo.n, 0.0f, eo.b);
+#pragma unroll
+    for (int mi = 0; mi < kFM; mi++) {
+      const int m = m0 + wm * (kSM / 2) + 16 * mi + (lane & 15);
+      eo.sa[mi] = ep.sa && m < M ? ep.sa[m] : 1.0f;
+      eo.res[mi] = m < M && eo.n < N ? epi8_res(ep, m, eo.n) : u32x4{0u, 0u, 0u, 0u};
+    }
+  }
 #pragma unroll
   for (int kt = 0; kt < kSS - 1; kt++)
     if (kt < nk) send(kt);
@@ -921,21 +1083,13 @@ __global__ __launch_bounds__(256) void gemm_small_kernel(const uint8_t *__restri
 #pragma unroll
       for (int j = 0; j < kFM; j++) acc[i][j] = sum[i][j];
   }
-  if constexpr (std::is_same_v<EPI, RowsEpi>) {
+  if constexpr (kRows) {
 #pragma unroll
-    for (int p = 0; p < kFN / 2; p++) {
-      const int n = n0 + wn * (kSN / 2) + 32 * p + 8 * (lane >> 4);
-      if (n >= N) continue;
-      float sb8[8], b8[8];
-      vec8(ep.sb, true, n, 1.0f, sb8);
-      vec8(ep.bias, ep.bias32, n, 0.0f, b8);
-#pragma unroll
-      for (int mi = 0; mi < kFM; mi++) {
-        const int m = m0 + wm * (kSM / 2) + 16 * mi + frow;
-        const v4f &x = acc[2 * p][mi], &y = acc[2 * p + 1][mi];
-        float v[8] = {x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]};
-        if (m < M) epi8_row(ep, v, sb8, b8, C, ldc, m, n);
-      }
+    for (int mi = 0; mi < kFM; mi++) {
+      const int m = m0 + wm * (kSM / 2) + 16 * mi + frow;
+      const v4f &x = acc[0][mi], &y = acc[1][mi];
+      float v[8] = {x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]};
+      if (m < M && eo.n < N) epi8_row(ep, v, eo.sa[mi], eo.sb, eo.b, eo.res[mi], C, ldc, m, eo.n);
     }
     return;
   }
@@ -1008,7 +1162,7 @@ __global__ __launch_bounds__(256) void splitk_rows_kernel(const float *__restric
     float v[8] = {x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]}, sb8[8], b8[8];
     vec8(ep.sb, true, n, 1.0f, sb8);
     vec8(ep.bias, ep.bias32, n, 0.0f, b8);
-    epi8_row(ep, v, sb8, b8, C, ldc, m, n);
+    epi8_row(ep, v, ep.sa ? ep.sa[m] : 1.0f, sb8, b8, epi8_res(ep, m, n), C, ldc, m, n);
   }
 }
 
@@ -1027,6 +1181,17 @@ __global__ __launch_bounds__(64 * kW) void gemm_few_kernel(const uint8_t *__rest
   const uint8_t *a[kF];
 #pragma unroll
   for (int f = 0; f < kF; f++) a[f] = A + (int64_t)min(16 * f + row, M - 1) * lda + kl;
+  // the epilogue's operands (wave f < kF, the lanes that will store), requested before the weight's bytes
+  const int em = 16 * wave + row, en = n0 + 4 * (lane >> 4);
+  const bool stores = wave < kF && !(lane & 16) && em < M;
+  float sb8[8], b8[8], sa_m = 1.0f;
+  u32x4 res{0u, 0u, 0u, 0u};
+  if (stores) {
+    vec8(ep.sb, true, en, 1.0f, sb8);
+    vec8(ep.bias, ep.bias32, en, 0.0f, b8);
+    if (ep.sa) sa_m = ep.sa[em];
+    res = epi8_res(ep, em, en);
+  }
   v4f acc[kF];
 #pragma unroll
   for (int f = 0; f < kF; f++) acc[f] = v4f{};
@@ -1067,12 +1232,7 @@ __global__ __launch_bounds__(64 * kW) void gemm_few_kernel(const uint8_t *__rest
     v[e] = s[e];
     v[4 + e] = __shfl_xor(s[e], 16, 64);
   }
-  const int m = 16 * wave + row, n = n0 + 4 * (lane >> 4);
-  if ((lane & 16) || m >= M) return;
-  float sb8[8], b8[8];
-  vec8(ep.sb, true, n, 1.0f, sb8);
-  vec8(ep.bias, ep.bias32, n, 0.0f, b8);
-  epi8_row(ep, v, sb8, b8, C, ldc, m, n);
+  if (stores) epi8_row(ep, v, sa_m, sb8, b8, res, C, ldc, em, en);
 }
 
 // ------------------------------------------------------------------------------------------- host side
@@ -1308,12 +1468,18 @@ static int launch_gemm_rows(const uint8_t *A, int64_t lda, const uint8_t *B, int
   const int work = p.tiles_m * p.tiles_n * p.splits;
   const int slots = num_cus() & ~7;
   const int grid = work <= slots || slots < 8 ? work : slots;
-  auto *kernel = p.bn == 128 ? (K % kBK ? gemm_tn_kernel<true, false, 128, 1, false, RowsEpi>
-                                        : gemm_tn_kernel<false, false, 128, 1, false, RowsEpi>)
-                             : (K % kBK ? gemm_tn_kernel<true, false, 256, 1, false, RowsEpi>
-                                        : gemm_tn_kernel<false, false, 256, 1, false, RowsEpi>);
-  kernel<<<grid, kThreads, 0, st>>>(A, (int)lda, B, (int)ldb, nullptr, nullptr, nullptr, 0, C, ldc, P, (int)M, (int)N, (int)K,
-                                    p.ksplit, p.tiles_m, p.tiles_n, p.splits, ep);
+  auto launch = [&](auto e) {
+    typedef decltype(e) E;
+    auto *kernel = p.bn == 128 ? (K % kBK ? gemm_tn_kernel<true, false, 128, 1, false, E> : gemm_tn_kernel<false, false, 128, 1, false, E>)
+                               : (K % kBK ? gemm_tn_kernel<true, false, 256, 1, false, E> : gemm_tn_kernel<false, false, 256, 1, false, E>);
+    kernel<<<grid, kThreads, 0, st>>>(A, (int)lda, B, (int)ldb, nullptr, nullptr, nullptr, 0, C, ldc, P, (int)M, (int)N, (int)K,
+                                      p.ksplit, p.tiles_m, p.tiles_n, p.splits, e);
+  };
+  const bool add = ep.res || ep.gate;
+  if (P || (!add && !ep.z)) launch(RowsEpiT<false, false>{ep});   // (partials carry no epilogue)
+  else if (!add) launch(RowsEpiT<false, true>{ep});
+  else if (!ep.z) launch(RowsEpiT<true, false>{ep});
+  else launch(RowsEpiT<true, true>{ep});
   if (P) {
     const int64_t g = (M * (N / 8) + 255) / 256;
     splitk_rows_kernel<<<(int)std::min<int64_t>(g, 8192), 256, 0, st>>>(P, p.splits, (int)M, (int)N, C, ldc, ep);
@@ -1370,7 +1536,7 @@ int gpic_fp8_gemm_rows(const uint8_t *A, int64_t lda, const float *sa, const uin
   if (!tn_shape_ok(lda, ldb, std::max(ldc, N), M, N, K) || ldc < No || ldc % 8) return GPIC_ESHAPE;
   if (act == GPIC_ACT_SWIGLU && N % 32) return GPIC_ESHAPE;
   if ((res && (ldr % 8 || ldr < No || ldr >= (1 << 22))) || (z && (ldz % 8 || ldz < N || ldz >= (1 << 22))) ||
-      (gate && (sg % 8 || sg < No || M % ntok)))
+      (gate && (sg % 8 || sg < No || sg >= (1 << 22) || M % ntok)))
     return GPIC_ESHAPE;
   if (!aligned16(A) || !aligned16(B) || !aligned16(C) || !aligned16(sb) || !aligned16(bias) || !aligned16(res) ||
       !aligned16(gate) || !aligned16(z))
