@@ -167,7 +167,8 @@ struct RowsEpi {
   uint32_t ntok;
   int ldr, ldz, bias32, act;
 };
-// The large tiles' instances: with residual or gate (kAdd), with z (kZ); what an instance lacks costs it no registers.
+// The large tiles' instances: with residual or gate (kAdd), with z (kZ); what an instance lacks costs it no registers. Both: the
+// general one, for z or a gate whose rows change within a wave's 64 as well.
 template <bool kAddP, bool kZP>
 struct RowsEpiT : RowsEpi {
   static constexpr bool kAdd = kAddP, kZ = kZP;
@@ -642,80 +643,59 @@ __global__ __launch_bounds__(kThreads) void gemm_tn_kernel(const uint8_t *__rest
     // so their latency passes during this item's epilogue
     const int nit = it + gridDim.x;
     const bool more = nit < work;
-    // the row-scaled epilogue's operands of block h: a lane's rows row_of(h, i) (of the tile) and runs of 8 columns from
-    // col_of_run(h, q); the first block's are waited for here, before the prologue's loads queue behind them
-    constexpr bool kLdsRes = kAdd && kBNt == 256;
-    constexpr int kRM = 2, kBlocks = kTNt / 2;   // 16-row tiles of a block; blocks: rows 32 (h & 1), columns 64 (h / 2)
-    float e_sa[kTM], e_sb[2][8], e_b[2][8];
-    u32x4 e_res[2][kRM], e_gate[2][kRM];
+    // the row-scaled epilogue's operands, of blocks h of 32 rows (32 (h & 1)) x 64 columns (64 (h / 2)): a lane's rows
+    // row_of(h, i) of the tile and runs of 8 columns from col_of_run(h, q). A block's are requested at least a block ahead: with
+    // HBM and L2 busy a load takes longer than a block does.
+    constexpr bool kLdsRes = kAdd && !kKeepZ && kBNt == 256;
+    constexpr int kRM = 2, kBlocks = kTNt / 2, kPairs = kBlocks / 2;   // 16-row tiles of a block; blocks; column groups
+    float e_sa[kTM], e_sb[kPairs][2][8], e_b[kPairs][2][8];
+    u32x4 e_res[2][kRM], e_gate[kPairs][2];
     std::conditional_t<kRows, RowsEpi, NoEpi> ep;
     if constexpr (kRows) ep = opaque_epi(epi);
     auto row_of = [&](int l, int h, int i) { return wm * kWTM + 32 * (h & 1) + 16 * i + (l & 15); };
     auto col_of_run = [&](int l, int h, int q) { return cur.n0 + wn * kWTNt + 64 * (h >> 1) + 32 * q + 8 * (l >> 4); };
-    auto e_load = [&](int h) {
+    // scales, bias and gate of column group p (buffer loads: columns past N, and a vector that is not there, read zeros without a
+    // branch around the load, whose other arm's constants the compiler would keep in registers across the K loop)
+    auto e_load = [&](int p) {
       if constexpr (kRows) {
         const int l = opaque_v(lane);
-        // (buffer loads: columns past N, and a vector that is not there, read zeros without a branch around the load, whose
-        // other arm's constants the compiler would keep in registers across the K loop)
-        if (!(h & 1)) {
-          const __amdgpu_buffer_rsrc_t rS = __builtin_amdgcn_make_buffer_rsrc((void *)ep.sb, 0, ep.sb ? N * 4 : 0, kBufferFlags);
-          const __amdgpu_buffer_rsrc_t rB = __builtin_amdgcn_make_buffer_rsrc(
-              (void *)ep.bias, 0, ep.bias ? N * (ep.bias32 ? 4 : 2) : 0, kBufferFlags);
-          const float one = ep.sb ? 0.0f : 1.0f;
+        const __amdgpu_buffer_rsrc_t rS = __builtin_amdgcn_make_buffer_rsrc((void *)ep.sb, 0, ep.sb ? N * 4 : 0, kBufferFlags);
+        const __amdgpu_buffer_rsrc_t rB = __builtin_amdgcn_make_buffer_rsrc(
+            (void *)ep.bias, 0, ep.bias ? N * (ep.bias32 ? 4 : 2) : 0, kBufferFlags);
+        const float one = ep.sb ? 0.0f : 1.0f;
 #pragma unroll
-          for (int q = 0; q < 2; q++) {
-            const int n = col_of_run(l, h, q);
-            load8f(rS, n * 4, e_sb[q]);
+        for (int q = 0; q < 2; q++) {
+          const int n = col_of_run(l, 2 * p, q);
+          load8f(rS, n * 4, e_sb[p][q]);
 #pragma unroll
-            for (int e = 0; e < 8; e++) e_sb[q][e] += one;
-            if (ep.bias32) load8f(rB, n * 4, e_b[q]);
-            else unpack8(__builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(rB, n * 2, 0, 0)), e_b[q]);
-          }
+          for (int e = 0; e < 8; e++) e_sb[p][q][e] += one;
+          if (ep.bias32) load8f(rB, n * 4, e_b[p][q]);
+          else unpack8(__builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(rB, n * 2, 0, 0)), e_b[p][q]);
         }
-        if constexpr (kAdd) {
+        if constexpr (kAdd && !kKeepZ) {   // (the gate's one row for the wave's 64)
           const bool half = ep.act == GPIC_ACT_SWIGLU;
-          // (a SwiGLU's 8 bytes: the 16 that hold them)
-          auto col = [&](int n) { return half ? (n >> 1) & ~7 : n; };
-          // the gate's row of a row of the tile, counted from the tile's first (its descriptor's base)
-          const uint32_t b0 = ep.gate ? (uint32_t)cur.m0 / ep.ntok : 0;
+          const uint32_t b = ep.gate ? (uint32_t)min(cur.m0 + wm * kWTM, M - 1) / ep.ntok : 0;
           const __amdgpu_buffer_rsrc_t rG = __builtin_amdgcn_make_buffer_rsrc(
-              (void *)(ep.gate + (int64_t)b0 * ep.sg), 0,
-              ep.gate ? (int)(((uint32_t)(min(cur.m0 + kBM, M) - 1) / ep.ntok - b0) * (uint32_t)ep.sg + (half ? N >> 1 : N)) * 2 : 0,
-              kBufferFlags);
+              (void *)(ep.gate + (int64_t)b * ep.sg), 0, ep.gate ? (half ? N >> 1 : N) * 2 : 0, kBufferFlags);
 #pragma unroll
-          for (int i = 0; i < kRM; i++) {
-            const int m = cur.m0 + row_of(l, h, i);
-            const int b = ep.gate && m < M ? (int)((uint32_t)m / ep.ntok - b0) : 0;
-#pragma unroll
-            for (int q = 0; q < 2; q++)
-              e_gate[q][i] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(
-                                                           rG, (b * (int)ep.sg + col(col_of_run(l, h, q))) * 2, 0, 0));
-          }
-          if constexpr (!kLdsRes) {
-            const int rows = min(M - cur.m0, kBM);
-            const __amdgpu_buffer_rsrc_t rR = __builtin_amdgcn_make_buffer_rsrc(
-                (void *)(ep.res + (int64_t)cur.m0 * ep.ldr), 0, ep.res ? rows * ep.ldr * 2 : 0, kBufferFlags);   // (none: zeros)
-#pragma unroll
-            for (int q = 0; q < 2; q++)
-#pragma unroll
-              for (int i = 0; i < kRM; i++) {
-                const int n = col_of_run(l, h, q), r = row_of(l, h, i);
-                const int off = n < N && r < rows ? (r * ep.ldr + col(n)) * 2 : kOOB;
-                e_res[q][i] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(rR, off, 0, 0));
-              }
+          for (int q = 0; q < 2; q++) {   // (a SwiGLU's 8 bytes: the 16 that hold them)
+            const int n = col_of_run(l, 2 * p, q);
+            e_gate[p][q] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(
+                                                         rG, (half ? (n >> 1) & ~7 : n) * 2, 0, 0));
           }
         }
       }
     };
-    // The wide tile's residual of block h by LDS DMA, in the layout in which y is staged, to the 4 KiB after the staged block: no
-    // registers, and whole 128-byte lines (as 64-byte runs into registers, some spilled, [32768 x 1024 x 4096] took 125 us).
-    auto res_send = [&](int h) {
+    // The residual of block h. The wide tile's by LDS DMA, in the layout in which y is staged, to where y will replace it (4 KiB,
+    // turn about): no registers, and whole 128-byte lines. Else 8 columns a run to registers.
+    auto res_load = [&](int h) {
       if constexpr (kLdsRes) {
         if (!ep.res) return;
         const bool half = ep.act == GPIC_ACT_SWIGLU;
         const int l = opaque_v(lane), rows = min(M - cur.m0, kBM);
         const v4i rR = buffer_rsrc(ep.res + (int64_t)cur.m0 * ep.ldr, rows * ep.ldr * 2);
-        const uint32_t to = lds_addr(smem) + (group == 0 ? a_half(2) : b_half(1)) + (wave & 3) * kCStage + 4096;
+        const uint32_t to =
+            lds_addr(smem) + (group == 0 ? a_half(2) : b_half(1)) + (wave & 3) * kCStage + 4096 * (h & 1);
         const int n = cur.n0 + wn * kWTNt + 64 * (h >> 1), row0 = wm * kWTM + 32 * (h & 1);
         const int lr = half ? l >> 2 : l >> 3;   // (columns past N: the next row's, or zeros; never stored)
         for (int i = 0; i < (half ? 2 : 4); i++) {
@@ -723,6 +703,19 @@ __global__ __launch_bounds__(kThreads) void gemm_tn_kernel(const uint8_t *__rest
           const int c = half ? (l & 3) ^ ((r >> 2) & 3) : (l & 7) ^ ((r >> 1) & 7);
           lds_dma16(rR, ((row0 + r) * ep.ldr + (half ? n >> 1 : n) + 8 * c) * 2, 0, to + 1024 * i);
         }
+      } else if constexpr (kAdd) {
+        const bool half = ep.act == GPIC_ACT_SWIGLU;
+        const int l = opaque_v(lane), rows = min(M - cur.m0, kBM);
+        const __amdgpu_buffer_rsrc_t rR = __builtin_amdgcn_make_buffer_rsrc(
+            (void *)(ep.res + (int64_t)cur.m0 * ep.ldr), 0, ep.res ? rows * ep.ldr * 2 : 0, kBufferFlags);   // (none: zeros)
+#pragma unroll
+        for (int q = 0; q < 2; q++)
+#pragma unroll
+          for (int i = 0; i < kRM; i++) {
+            const int n = col_of_run(l, h, q), r = row_of(l, h, i);
+            const int off = n < N && r < rows ? (r * ep.ldr + (half ? (n >> 1) & ~7 : n)) * 2 : kOOB;
+            e_res[q][i] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(rR, off, 0, 0));
+          }
       }
     };
     if constexpr (kRows) {   // (split-K partials do not use them; under a condition they would be carried across the K loop)
@@ -733,9 +726,10 @@ __global__ __launch_bounds__(kThreads) void gemm_tn_kernel(const uint8_t *__rest
       for (int i = 0; i < kTM; i++)
         e_sa[i] = one + __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(
                                                       rA, (wm * kWTM + 16 * i + (lane & 15)) * 4, 0, 0));
-      res_send(0);
+      res_load(0);
       e_load(0);
-      __builtin_amdgcn_s_waitcnt(0x0f70);   // vmcnt(0)
+      __builtin_amdgcn_s_waitcnt(0x0f70);   // vmcnt(0): before the prologue's loads queue behind them
+      if constexpr (kLdsRes) res_load(1);
     }
     if (more && group == 0) send_prologue(item(nit));
 
@@ -769,7 +763,7 @@ __global__ __launch_bounds__(kThreads) void gemm_tn_kernel(const uint8_t *__rest
       // [6592 x 4096 x 1024] 46 us. A wait for a load also waits for everything this wave sent before it, so the first
       // block's operands have landed before the next item's prologue is sent (above), and a later block's are requested
       // before the stores of the one ahead of it.
-      GPIC_LDS uint8_t *cst =
+      GPIC_LDS uint8_t *cst0 =
           (GPIC_LDS uint8_t *)smem + (group == 0 ? a_half(2) : b_half(1)) + (wave & 3) * kCStage;
       const bool half = ep.act == GPIC_ACT_SWIGLU;
       const int64_t c0row = (int64_t)cur.m0;
@@ -784,9 +778,12 @@ __global__ __launch_bounds__(kThreads) void gemm_tn_kernel(const uint8_t *__rest
         constexpr int kRowOut = kHalf ? 64 : 128, kLPR = kRowOut / 16, kRPI = 64 / kLPR, kNI = 16 * kRM / kRPI;
         // (an opaque lane per block: the blocks' addresses are computed in them, not shared by all and held throughout)
         const int bl = opaque_v(el), wr = bl & 15, wg = bl >> 4;
-        // the residual's loads, sent before the stores of the block ahead (and this one's z), have landed
-        if constexpr (kLdsRes && !kZ && h > 0)
-          asm volatile("s_waitcnt vmcnt(%0)" ::"n"(kNI + (kKeepZ ? 4 : 0)) : "memory");
+        GPIC_LDS uint8_t *cst = cst0 + (kLdsRes ? 4096 * (h & 1) : 0);
+        // the residual's loads have landed (block 0's: above). At least so many operations follow them: block 1's, block 2's
+        // loads (as many as a block has store instructions) and block 0's stores; block 2's, the stores of blocks 0 and 1 and
+        // block 3's loads; block 3's, the stores of blocks 1 and 2
+        constexpr int after = h == 2 ? 3 * kNI : 2 * kNI;
+        if constexpr (kLdsRes && h > 0) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(after) : "memory");
 #pragma unroll
         for (int q = 0; q < 2; q++)
 #pragma unroll
@@ -799,21 +796,29 @@ __global__ __launch_bounds__(kThreads) void gemm_tn_kernel(const uint8_t *__rest
             float sa_m = e_sa[mi];
             asm volatile("" : "+v"(sa_m));   // (the pass that stores z does not keep its values for the one that stores y)
 #pragma unroll
-            for (int e = 0; e < 8; e++) v[e] = __builtin_fmaf(v[e] * sa_m, e_sb[q][e], e_b[q][e]);
+            for (int e = 0; e < 8; e++) v[e] = __builtin_fmaf(v[e] * sa_m, e_sb[h >> 1][q][e], e_b[h >> 1][q][e]);
             if (!kZ) {
               act8<kAct>(v);
               if constexpr (kAdd) {
-                u32x4 g = e_gate[q][i], rs{0u, 0u, 0u, 0u};
-                const bool up = kHalf && (col_of_run(bl, h, q) & 8);   // (which 8 of the 16 bytes)
-                if constexpr (!kLdsRes) rs = e_res[q][i];
-                else if (kHalf) {
-                  const st8_t w = *(const GPIC_LDS st8_t *)(cst + 4096 + at);
+                u32x4 g{0u, 0u, 0u, 0u}, rs{0u, 0u, 0u, 0u};
+                const int n = col_of_run(bl, h, q);
+                const bool up = kHalf && (n & 8);   // (which 8 of the 16 bytes)
+                if constexpr (!kKeepZ) {
+                  g = e_gate[h >> 1][q];
+                  if (up) g.x = g.z, g.y = g.w;
+                } else if (ep.gate) {   // (rows past M, columns past N: any that exist)
+                  const int m = min(cur.m0 + row_of(bl, h, i), M - 1);
+                  g = row8(ep.gate + (int64_t)((uint32_t)m / ep.ntok) * ep.sg + (n < N ? kHalf ? n >> 1 : n : 0), kHalf);
+                }
+                if constexpr (!kLdsRes) {
+                  rs = e_res[q][i];
+                  if (up) rs.x = rs.z, rs.y = rs.w;
+                } else if (kHalf) {
+                  const st8_t w = *(const GPIC_LDS st8_t *)(cst + at);
                   rs = u32x4{w.x, w.y, 0u, 0u};
                 } else {
-                  rs = __builtin_bit_cast(u32x4, *(const GPIC_LDS st16_t *)(cst + 4096 + at));
+                  rs = __builtin_bit_cast(u32x4, *(const GPIC_LDS st16_t *)(cst + at));
                 }
-                if (up && !kLdsRes) rs.x = rs.z, rs.y = rs.w;
-                if (up) g.x = g.z, g.y = g.w;
                 add8(ep, v, rs, g);
               }
             }
@@ -844,12 +849,11 @@ __global__ __launch_bounds__(kThreads) void gemm_tn_kernel(const uint8_t *__rest
       with_act(ep.act, [&](auto act) {
         auto both = [&](auto h) {
           constexpr int next = decltype(h)::value + 1;
-          if constexpr (kKeepZ) block(act, std::true_type(), h, []() {});
+          if (kKeepZ && (!kAdd || ep.z)) block(act, std::bool_constant<kKeepZ>(), h, []() {});
           block(act, std::false_type(), h, [&]() {
-            if constexpr (next < kBlocks) {
-              res_send(next);
-              e_load(next);
-            }
+            if constexpr (kLdsRes && next + 1 < kBlocks) res_load(next + 1);
+            if constexpr (!kLdsRes && next < kBlocks) res_load(next);
+            if constexpr (next == 1 && kPairs > 1) e_load(1);   // (the first block's accumulators have left their registers)
           });
         };
         both(std::integral_constant<int, 0>());
@@ -860,7 +864,7 @@ __global__ __launch_bounds__(kThreads) void gemm_tn_kernel(const uint8_t *__rest
         }
       });
       // (stores: a SwiGLU's half as many; counting fewer than there are only waits longer)
-      pend = kKeepZ ? (half ? kStoresBF16 : 2 * kStoresBF16) : half ? 0 : kStoresBF16;
+      pend = kKeepZ && (!kAdd || ep.z) ? (half ? kStoresBF16 : 2 * kStoresBF16) : half ? 0 : kStoresBF16;
     } else {
       // bf16 output through LDS: each lane rounds its runs of 8 columns (scaled) to bf16 and writes them to LDS as
       // 16 bytes (MN-major: its runs of 4 as 8 bytes), one 32 x 128 block (two 16-row tile rows) of the wave at a
@@ -1478,7 +1482,7 @@ static int launch_gemm_rows(const uint8_t *A, int64_t lda, const uint8_t *B, int
   const bool add = ep.res || ep.gate;
   if (P || (!add && !ep.z)) launch(RowsEpiT<false, false>{ep});   // (partials carry no epilogue)
   else if (!add) launch(RowsEpiT<false, true>{ep});
-  else if (!ep.z) launch(RowsEpiT<true, false>{ep});
+  else if (!ep.z && (!ep.gate || ep.ntok % kWTM == 0)) launch(RowsEpiT<true, false>{ep});
   else launch(RowsEpiT<true, true>{ep});
   if (P) {
     const int64_t g = (M * (N / 8) + 255) / 256;

@@ -15,9 +15,10 @@ __device__ __forceinline__ float fast_sigmoid(float x) {
 constexpr float kGelu2C = 1.59576912f;            // 2 sqrt(2 / pi)
 constexpr float kGelu2C3 = 0.0713548163f;         // 2 sqrt(2 / pi) 0.044715
 
-// gelu_tanh(z) = z (1 + tanh u) / 2 = z sigmoid(2 u), u = sqrt(2 / pi) (z + 0.044715 z^3)
+// gelu_tanh(z) = z (1 + tanh u) / 2 = z sigmoid(2 u), u = sqrt(2 / pi) (z + 0.044715 z^3); e^-2u as 2^t, log2 e in the constants
 __device__ __forceinline__ float gelu_sig(float z) {
-  return fast_sigmoid(z * __builtin_fmaf(kGelu2C3, z * z, kGelu2C));
+  const float t = z * __builtin_fmaf(-1.44269504f * kGelu2C3, z * z, -1.44269504f * kGelu2C);
+  return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(t));
 }
 
 // act(z); act: GPIC_ACT_NONE / SILU / GELU_TANH (uniform over the wave)
