@@ -345,9 +345,10 @@ int gpic_fp8_bf16_gemm_mn(const uint16_t *A, int64_t lda, const uint16_t *B, int
  * are contiguous. rows == 0 is allowed.
  */
 
-/* The row cast of x [rows, cols] (bf16 or fp32, row stride ldx) -> q [rows, cols] e4m3, s [rows]. cols <= 32768. */
+/* The row cast of x [rows, cols] (bf16 or fp32, row stride ldx) -> q [rows, cols] e4m3, s [rows]; and, in the same launch, of
+ * x2 [rows2, cols] (NULL: none) -> q2, s2: a linear's input and weight. cols <= 32768. */
 int gpic_fp8_tcast_rows(const void *x, int dtype, int64_t ldx, int64_t rows, int64_t cols, uint8_t *q, float *s,
-                        void *stream);
+                        const void *x2, int dtype2, int64_t ldx2, int64_t rows2, uint8_t *q2, float *s2, void *stream);
 
 /*
  * RMSNorm with the residual's addition and a row-scaled e4m3 output:
@@ -358,11 +359,14 @@ int gpic_fp8_tcast_rows(const void *x, int dtype, int64_t ldx, int64_t rows, int
  *   x, a [rows, C] bf16 (row strides ldx, lda); xn, h [rows, C] bf16; q [rows, C]; s [rows]; w [C] of w_dtype
  *   gate, shift, scale: bf16 rows (strides sg, ssh, ssc); row r uses row r / ntok of them (rows % ntok == 0)
  *   C % 8 == 0, C <= 16384, rows < 2^31.
+ *   wt [N, C] of wt_dtype, contiguous (NULL: none) -> wq [N, C], sw [N]: in the same launch, the row cast of the weight of the
+ *       linear that reads q.
  */
 int gpic_fp8_rmsnorm_rows(const uint16_t *x, int64_t ldx, const uint16_t *a, int64_t lda, const uint16_t *gate, int64_t sg,
                           const void *w, int w_dtype, const uint16_t *shift, int64_t ssh, const uint16_t *scale,
                           int64_t ssc, int64_t rows, int64_t ntok, int64_t C, float eps, uint16_t *xn, uint16_t *h,
-                          float *rstd, uint8_t *q, float *s, void *stream);
+                          float *rstd, uint8_t *q, float *s, const void *wt, int wt_dtype, int64_t N, uint8_t *wq, float *sw,
+                          void *stream);
 
 /*
  * Its backward without gate, shift and scale (with them: gpic_fp8_res_mod_rmsnorm_bwd), dh the gradient of h:
@@ -384,7 +388,7 @@ int gpic_fp8_rmsnorm_rows_bwd(const uint16_t *dh, const uint16_t *dxn, const uin
  *   res: bf16, C's shape (row stride ldr), or NULL; gate: bf16 rows of C's width (stride sg), row m uses row m / ntok
  *       (M % ntok == 0), or NULL
  *   C bf16 (row stride ldc); z: where to keep z as bf16 [M, N] (row stride ldz; for the activation's backward), or NULL
- *   K > 0; sizes and strides otherwise as gpic_fp8_gemm's, ldr, ldz < 2^22; any M; res may not overlap C.
+ *   K > 0; sizes and strides otherwise as gpic_fp8_gemm's, ldr, ldz, sg < 2^22; any M; res may not overlap C.
  *   ws: gpic_fp8_gemm_workspace_bytes(M, N, K) bytes. Deterministic.
  */
 int gpic_fp8_gemm_rows(const uint8_t *A, int64_t lda, const float *sa, const uint8_t *B, int64_t ldb, const float *sb,

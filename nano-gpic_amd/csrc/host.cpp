@@ -9,6 +9,7 @@
 // current stream's cast workspace (0 for the calls that cast nothing) and that stream. The GIL is released while a call
 // allocates and launches, as ctypes and torch's own operations release it: a launch waits where the queue is full.
 #include <ATen/ATen.h>
+#include <c10/core/GradMode.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/utils/pybind.h>
 
@@ -241,13 +242,36 @@ constexpr int64_t kRowsMaxNorm = 16384, kRowsMaxCast = 32768;   // the C ABI's w
 typedef std::optional<at::Tensor> opt;
 
 bool bf16(const at::Tensor &t, int dev) { return t.scalar_type() == at::kBFloat16 && plain(t, dev); }
-// A vector of n bf16 or fp32, or none
+// A vector of n bf16 or fp32
 bool vector_ok(const at::Tensor &t, int64_t n, int dev) { return castable(t, dev) && t.dim() == 1 && t.size(0) == n; }
 bool scales_ok(const opt &s, int64_t n, int dev) {
   return !s || (s->scalar_type() == at::kFloat && plain(*s, dev) && s->numel() == n);
 }
 uint16_t *u16(const opt &t) { return t ? ptr<uint16_t>(*t) : nullptr; }
 at::Tensor none_of(const at::Tensor &like, at::ScalarType ty) { return make(like, {0}, ty); }
+// Whether a call on these records a gradient: the operators themselves have none, and the general form says so.
+bool records(std::initializer_list<const opt *> ts) {
+  if (!c10::GradMode::is_enabled()) return false;
+  for (const opt *t : ts)
+    if (*t && (*t)->requires_grad()) return true;
+  return false;
+}
+
+// The temporary tensors of one call as parts of one allocation.
+struct Arena {
+  size_t n = 0;
+  at::Tensor t;
+  size_t add(size_t bytes) {
+    const size_t at = n;
+    n += (bytes + 255) & ~size_t(255);
+    return at;
+  }
+  void make_like(const at::Tensor &like) { t = make(like, {(int64_t)std::max<size_t>(n, 16)}, at::kByte); }
+  template <class T>
+  T *at(size_t offset) const {
+    return reinterpret_cast<T *>(static_cast<uint8_t *>(t.data_ptr()) + offset);
+  }
+};
 
 // Modulation rows [B, 1, C], [B, C] or [C] bf16: base, row stride and B; false for a form that the general path copies. batch:
 // x's first extent where x has a batch (B is then that or 1), else 0 (B divides the rows).
@@ -268,23 +292,13 @@ bool mod_ok(const opt &t, int64_t C, int64_t batch, int64_t rows, int dev, Mod &
   return (reinterpret_cast<uintptr_t>(m.p) & 15u) == 0;
 }
 
-struct RowCast {
-  at::Tensor q, s;
-};
 bool row_castable(const at::Tensor &x, int dev) {
   return castable(x, dev) && x.dim() >= 1 && x.size(-1) > 0 && x.size(-1) % 8 == 0 && x.size(-1) <= kRowsMaxCast;
 }
-RowCast row_cast(const at::Tensor &x, void *stream) {
-  const int64_t C = x.size(-1), M = x.numel() / C;
-  RowCast o{make(x, x.sizes(), kE4), make(x, {M}, at::kFloat)};
-  check(gpic_fp8_tcast_rows(x.data_ptr(), dtype_code(x), C, M, C, ptr<uint8_t>(o.q), ptr<float>(o.s), stream),
-        "gpic_fp8_tcast_rows");
-  return o;
+bool operand_rows(const at::Tensor &t, int dev) {
+  return t.scalar_type() == kE4 && t.dim() == 2 && t.size(1) > 0 && t.size(1) % 16 == 0 && plain(t, dev);
 }
 
-struct NormOut {
-  at::Tensor xn, h, q, s, rstd;
-};
 struct NormIn {
   Mod gate, shift, scale;
   int64_t ntok = 1;
@@ -308,112 +322,124 @@ bool norm_ok(const at::Tensor &x, const at::Tensor &w, const opt &a, const opt &
   in.ntok = B ? M / B : 1;
   return true;
 }
-NormOut norm_rows_run(const at::Tensor &x, const at::Tensor &w, double eps, const opt &a, const NormIn &in, bool want_h,
-                      void *stream) {
+struct NormOut {
+  at::Tensor xn, h, rstd;
+};
+// q, s: where the bytes and scales go; weight (or none) -> wq, sw in the same launch
+NormOut norm_run(const at::Tensor &x, const at::Tensor &w, double eps, const opt &a, const NormIn &in, bool want_h, uint8_t *q,
+                 float *s, const at::Tensor *weight, uint8_t *wq, float *sw, void *stream) {
   const int64_t C = x.size(-1), M = x.numel() / C;
   NormOut o;
   o.xn = a ? make(x, x.sizes(), at::kBFloat16) : none_of(x, at::kBFloat16);
   o.h = want_h ? make(x, x.sizes(), at::kBFloat16) : none_of(x, at::kBFloat16);
-  o.q = make(x, x.sizes(), kE4);
-  o.s = make(x, {M}, at::kFloat);
   o.rstd = make(x, {M}, at::kFloat);
   check(gpic_fp8_rmsnorm_rows(ptr<uint16_t>(x), C, u16(a), C, in.gate.p, in.gate.ld, w.data_ptr(), dtype_code(w), in.shift.p,
                               in.shift.ld, in.scale.p, in.scale.ld, M, in.ntok, C, (float)eps,
-                              a ? ptr<uint16_t>(o.xn) : nullptr, want_h ? ptr<uint16_t>(o.h) : nullptr, ptr<float>(o.rstd),
-                              ptr<uint8_t>(o.q), ptr<float>(o.s), stream),
+                              a ? ptr<uint16_t>(o.xn) : nullptr, want_h ? ptr<uint16_t>(o.h) : nullptr, ptr<float>(o.rstd), q,
+                              s, weight ? weight->data_ptr() : nullptr, weight ? dtype_code(*weight) : 0,
+                              weight ? weight->size(0) : 0, wq, sw, stream),
         "gpic_fp8_rmsnorm_rows");
   return o;
 }
 
-struct GemmOut {
-  at::Tensor y, z;
+struct GemmIn {
+  const uint8_t *a, *b;
+  const float *sa, *sb;
+  int64_t M, N, K;
+  const opt *bias = nullptr;
+  int act = GPIC_ACT_NONE;
+  const uint16_t *res = nullptr;
+  Mod gate;
 };
-bool operand_rows(const at::Tensor &t, int dev) {
-  return t.scalar_type() == kE4 && t.dim() == 2 && t.size(1) > 0 && t.size(1) % 16 == 0 && plain(t, dev);
-}
-// (shapes of a and b, and bias, checked by the callers)
-GemmOut gemm_rows_run(const at::Tensor &a, const opt &sa, const at::Tensor &b, const opt &sb, const opt &bias, int act,
-                      const opt &res, const Mod &gate, bool want_z, void *stream) {
-  const int64_t M = a.size(0), K = a.size(1), N = b.size(0), No = act == GPIC_ACT_SWIGLU ? N / 2 : N;
-  GemmOut o;
-  o.y = make(a, {M, No}, at::kBFloat16);
-  o.z = want_z ? make(a, {M, N}, at::kBFloat16) : none_of(a, at::kBFloat16);
-  const Scratch w(a, M, N, K);
-  check(gpic_fp8_gemm_rows(ptr<uint8_t>(a), K, sa ? ptr<float>(*sa) : nullptr, ptr<uint8_t>(b), K,
-                           sb ? ptr<float>(*sb) : nullptr, bias ? bias->data_ptr() : nullptr, bias ? dtype_code(*bias) : 0,
-                           act, u16(res), No, gate.p, gate.ld, gate.B ? M / gate.B : 1, ptr<uint16_t>(o.y), No,
-                           want_z ? ptr<uint16_t>(o.z) : nullptr, N, M, N, K, w.p(), w.bytes, stream),
+// y [M, N] (SwiGLU: N / 2), z [M, N] or null; ws: gpic_fp8_gemm_workspace_bytes(M, N, K)
+void gemm_rows_call(const GemmIn &g, uint16_t *y, uint16_t *z, void *ws, size_t bytes, void *stream) {
+  const int64_t No = g.act == GPIC_ACT_SWIGLU ? g.N / 2 : g.N;
+  const bool b = g.bias && *g.bias;
+  check(gpic_fp8_gemm_rows(g.a, g.K, g.sa, g.b, g.K, g.sb, b ? (*g.bias)->data_ptr() : nullptr, b ? dtype_code(**g.bias) : 0,
+                           g.act, g.res, No, g.gate.p, g.gate.ld, g.gate.B ? g.M / g.gate.B : 1, y, No, z, g.N, g.M, g.N, g.K,
+                           bytes ? ws : nullptr, bytes, stream),
         "gpic_fp8_gemm_rows");
-  return o;
 }
 
 py::object cast_rows(const at::Tensor &x, int dev, handle, handle stream) {
-  if (!row_castable(x, dev)) return py::none();
-  RowCast o;
+  const opt ox = x;
+  if (!row_castable(x, dev) || records({&ox})) return py::none();
+  const int64_t C = x.size(-1), M = x.numel() / C;
+  at::Tensor q, s;
   {
     NoGil no_gil;
-    o = row_cast(x, vp(stream));
+    q = make(x, x.sizes(), kE4);
+    s = make(x, {M}, at::kFloat);
+    check(gpic_fp8_tcast_rows(x.data_ptr(), dtype_code(x), C, M, C, ptr<uint8_t>(q), ptr<float>(s), nullptr, 0, 0, 0, nullptr,
+                              nullptr, vp(stream)),
+          "gpic_fp8_tcast_rows");
   }
-  return py::make_tuple(o.q, o.s);
+  return py::make_tuple(q, s);
 }
 
 py::object norm_rows(const at::Tensor &x, const at::Tensor &w, double eps, const opt &a, const opt &gate, const opt &shift,
                      const opt &scale, bool want_h, int dev, handle, handle stream) {
   NormIn in;
-  if (!norm_ok(x, w, a, gate, shift, scale, dev, in)) return py::none();
+  const opt ox = x, ow = w;
+  if (!norm_ok(x, w, a, gate, shift, scale, dev, in) || records({&ox, &ow, &a, &gate, &shift, &scale})) return py::none();
   NormOut o;
+  at::Tensor q, s;
   {
     NoGil no_gil;
-    o = norm_rows_run(x, w, eps, a, in, want_h, vp(stream));
+    q = make(x, x.sizes(), kE4);
+    s = make(x, {x.numel() / x.size(-1)}, at::kFloat);
+    o = norm_run(x, w, eps, a, in, want_h, ptr<uint8_t>(q), ptr<float>(s), nullptr, nullptr, nullptr, vp(stream));
   }
-  return py::make_tuple(o.xn, o.h, o.q, o.s, o.rstd);
+  return py::make_tuple(o.xn, o.h, q, s, o.rstd);
 }
 
 py::object gemm_rows(const at::Tensor &a, const opt &sa, const at::Tensor &b, const opt &sb, const opt &bias, int act,
                      const opt &res, const opt &gate, bool want_z, int dev, handle, handle stream) {
   if (!operand_rows(a, dev) || !operand_rows(b, dev) || a.size(1) != b.size(1)) return py::none();
-  const int64_t M = a.size(0), N = b.size(0), No = act == GPIC_ACT_SWIGLU ? N / 2 : N;
-  Mod g;
+  const int64_t M = a.size(0), K = a.size(1), N = b.size(0), No = act == GPIC_ACT_SWIGLU ? N / 2 : N;
+  GemmIn g{ptr<uint8_t>(a), ptr<uint8_t>(b), sa ? ptr<float>(*sa) : nullptr, sb ? ptr<float>(*sb) : nullptr, M, N, K,
+           &bias, act, u16(res)};
   if (M < 1 || N < 16 || N % (act == GPIC_ACT_SWIGLU ? 32 : 16) || !scales_ok(sa, M, dev) || !scales_ok(sb, N, dev) ||
       !bias_ok(bias, N, dev) || (res && (!bf16(*res, dev) || res->dim() != 2 || res->size(0) != M || res->size(1) != No)) ||
-      !mod_ok(gate, No, 0, M, dev, g))
+      !mod_ok(gate, No, 0, M, dev, g.gate) || records({&sa, &sb, &bias, &res, &gate}))
     return py::none();
-  GemmOut o;
+  at::Tensor y, z;
   {
     NoGil no_gil;
-    o = gemm_rows_run(a, sa, b, sb, bias, act, res, g, want_z, vp(stream));
+    y = make(a, {M, No}, at::kBFloat16);
+    z = want_z ? make(a, {M, N}, at::kBFloat16) : none_of(a, at::kBFloat16);
+    const Scratch w(a, M, N, K);
+    gemm_rows_call(g, ptr<uint16_t>(y), want_z ? ptr<uint16_t>(z) : nullptr, w.p(), w.bytes, vp(stream));
   }
-  return py::make_tuple(o.y, o.z);
+  return py::make_tuple(y, z);
 }
 
-bool norm_bwd_ok(const at::Tensor &dh, const opt &dxn, const at::Tensor &xs, const at::Tensor &w, const at::Tensor &rstd,
-                 int dev) {
+bool norm_bwd_ok(int64_t M, const opt &dxn, const at::Tensor &xs, const at::Tensor &w, const at::Tensor &rstd, int dev) {
   if (xs.dim() < 1 || !bf16(xs, dev)) return false;
   const int64_t C = xs.size(-1);
-  return C > 0 && C % 8 == 0 && C <= kRowsMaxNorm && vector_ok(w, C, dev) && bf16(dh, dev) && dh.numel() == xs.numel() &&
-         (!dxn || (bf16(*dxn, dev) && dxn->sizes() == xs.sizes())) && scales_ok(rstd, xs.numel() / C, dev);
-}
-std::pair<at::Tensor, at::Tensor> norm_bwd_run(const at::Tensor &dh, const opt &dxn, const at::Tensor &xs,
-                                               const at::Tensor &w, const at::Tensor &rstd, void *stream) {
-  const int64_t C = xs.size(-1), M = xs.numel() / C;
-  at::Tensor dx = make(xs, xs.sizes(), at::kBFloat16), dw = make(xs, {C}, w.scalar_type());
-  const size_t bytes = gpic_fp8_rmsnorm_rows_bwd_workspace_bytes(M, C);
-  at::Tensor ws = make(xs, {std::max<int64_t>((int64_t)bytes, 16)}, at::kByte);
-  check(gpic_fp8_rmsnorm_rows_bwd(ptr<uint16_t>(dh), u16(dxn), ptr<uint16_t>(xs), w.data_ptr(), dtype_code(w),
-                                  ptr<float>(rstd), M, C, ptr<uint16_t>(dx), dw.data_ptr(), dtype_code(dw), ws.data_ptr(),
-                                  bytes, stream),
-        "gpic_fp8_rmsnorm_rows_bwd");
-  return {dx, dw};
+  return C > 0 && C % 8 == 0 && C <= kRowsMaxNorm && xs.numel() == M * C && vector_ok(w, C, dev) &&
+         (!dxn || (bf16(*dxn, dev) && dxn->sizes() == xs.sizes())) && scales_ok(rstd, M, dev);
 }
 py::object norm_rows_bwd(const at::Tensor &dh, const opt &dxn, const at::Tensor &xs, const at::Tensor &w,
                          const at::Tensor &rstd, int dev, handle, handle stream) {
-  if (!norm_bwd_ok(dh, dxn, xs, w, rstd, dev) || dh.sizes() != xs.sizes()) return py::none();
-  std::pair<at::Tensor, at::Tensor> o;
+  const opt odh = dh, oxs = xs, ow = w, ors = rstd;
+  if (xs.dim() < 1 || xs.size(-1) <= 0 || !bf16(dh, dev) || dh.sizes() != xs.sizes() ||
+      !norm_bwd_ok(xs.numel() / xs.size(-1), dxn, xs, w, rstd, dev) || records({&odh, &dxn, &oxs, &ow, &ors}))
+    return py::none();
+  const int64_t C = xs.size(-1), M = xs.numel() / C;
+  at::Tensor dx, dw;
   {
     NoGil no_gil;
-    o = norm_bwd_run(dh, dxn, xs, w, rstd, vp(stream));
+    dx = make(xs, xs.sizes(), at::kBFloat16);
+    dw = make(xs, {C}, w.scalar_type());
+    const size_t bytes = gpic_fp8_rmsnorm_rows_bwd_workspace_bytes(M, C);
+    const at::Tensor ws = make(xs, {std::max<int64_t>((int64_t)bytes, 16)}, at::kByte);
+    check(gpic_fp8_rmsnorm_rows_bwd(ptr<uint16_t>(dh), u16(dxn), ptr<uint16_t>(xs), w.data_ptr(), dtype_code(w),
+                                    ptr<float>(rstd), M, C, ptr<uint16_t>(dx), dw.data_ptr(), dtype_code(dw), ws.data_ptr(),
+                                    bytes, vp(stream)),
+          "gpic_fp8_rmsnorm_rows_bwd");
   }
-  return py::make_tuple(o.first, o.second);
+  return py::make_tuple(dx, dw);
 }
 
 bool rows_weight_ok(const at::Tensor &w, int64_t K, int dev) {
@@ -427,15 +453,24 @@ py::object linear_rows_fwd(const at::Tensor &x, const at::Tensor &w, const opt &
       !bias_ok(bias, w.size(0), dev) ||
       (res && (!bf16(*res, dev) || res->dim() != 2 || res->size(0) != x.size(0) || res->size(1) != w.size(0))))
     return py::none();
-  RowCast wc;
-  GemmOut o;
+  const int64_t M = x.size(0), K = x.size(1), N = w.size(0);
+  at::Tensor wq, sw, y, z;
   {
     NoGil no_gil;
-    wc = row_cast(w, vp(stream));
-    const RowCast xc = row_cast(x, vp(stream));
-    o = gemm_rows_run(xc.q, xc.s, wc.q, wc.s, bias, act, res, Mod(), want_z, vp(stream));
+    wq = make(w, w.sizes(), kE4);
+    sw = make(w, {N}, at::kFloat);
+    y = make(x, {M, N}, at::kBFloat16);
+    z = want_z ? make(x, {M, N}, at::kBFloat16) : none_of(x, at::kBFloat16);
+    Arena m;
+    const size_t bytes = gpic_fp8_gemm_workspace_bytes(M, N, K), q = m.add(M * K), s = m.add(4 * M), ws = m.add(bytes);
+    m.make_like(x);
+    check(gpic_fp8_tcast_rows(x.data_ptr(), GPIC_DTYPE_BF16, K, M, K, m.at<uint8_t>(q), m.at<float>(s), w.data_ptr(),
+                              dtype_code(w), K, N, ptr<uint8_t>(wq), ptr<float>(sw), vp(stream)),
+          "gpic_fp8_tcast_rows");
+    const GemmIn g{m.at<uint8_t>(q), ptr<uint8_t>(wq), m.at<float>(s), ptr<float>(sw), M, N, K, &bias, act, u16(res)};
+    gemm_rows_call(g, ptr<uint16_t>(y), want_z ? ptr<uint16_t>(z) : nullptr, m.at<uint8_t>(ws), bytes, vp(stream));
   }
-  return py::make_tuple(o.y, o.z, wc.q, wc.s);
+  return py::make_tuple(y, z, wq, sw);
 }
 
 // The norm and the linear that reads its bytes -> (x_new or empty, h as bf16 or empty, rstd, y, z or empty, w's bytes, scales)
@@ -445,57 +480,83 @@ py::object norm_linear_rows_fwd(const at::Tensor &x, const at::Tensor &wn, doubl
   NormIn in;
   if (!norm_ok(x, wn, a, gate, shift, scale, dev, in) || !rows_weight_ok(w, x.size(-1), dev) || !bias_ok(bias, w.size(0), dev))
     return py::none();
-  RowCast wc;
+  const int64_t K = x.size(-1), M = x.numel() / K, N = w.size(0);
+  at::Tensor wq, sw, y, z;
   NormOut n;
-  GemmOut o;
   {
     NoGil no_gil;
-    wc = row_cast(w, vp(stream));
-    n = norm_rows_run(x, wn, eps, a, in, want_h, vp(stream));
-    o = gemm_rows_run(n.q.view({-1, x.size(-1)}), n.s, wc.q, wc.s, bias, act, std::nullopt, Mod(), want_z, vp(stream));
+    wq = make(w, w.sizes(), kE4);
+    sw = make(w, {N}, at::kFloat);
+    y = make(x, {M, N}, at::kBFloat16);
+    z = want_z ? make(x, {M, N}, at::kBFloat16) : none_of(x, at::kBFloat16);
+    Arena m;
+    const size_t bytes = gpic_fp8_gemm_workspace_bytes(M, N, K), q = m.add(M * K), s = m.add(4 * M), ws = m.add(bytes);
+    m.make_like(x);
+    n = norm_run(x, wn, eps, a, in, want_h, m.at<uint8_t>(q), m.at<float>(s), &w, ptr<uint8_t>(wq), ptr<float>(sw), vp(stream));
+    const GemmIn g{m.at<uint8_t>(q), ptr<uint8_t>(wq), m.at<float>(s), ptr<float>(sw), M, N, K, &bias, act};
+    gemm_rows_call(g, ptr<uint16_t>(y), want_z ? ptr<uint16_t>(z) : nullptr, m.at<uint8_t>(ws), bytes, vp(stream));
   }
-  return py::make_tuple(n.xn, n.h, n.rstd, o.y, o.z, wc.q, wc.s);
+  return py::make_tuple(n.xn, n.h, n.rstd, y, z, wq, sw);
 }
 
 struct LinearGrads {
   at::Tensor dx, dw, db;
 };
-bool linear_bwd_ok(const at::Tensor &dy, const at::Tensor &z, int act, const at::Tensor &wq, const at::Tensor &sw,
-                   const at::Tensor &x, int dev) {
-  if (dy.dim() != 2 || !bf16(dy, dev) || !operand_rows(wq, dev)) return false;
-  const int64_t M = dy.size(0), N = dy.size(1), K = wq.size(1);
-  return M >= 1 && N >= 16 && N % 16 == 0 && N <= kRowsMaxCast && wq.size(0) == N && scales_ok(sw, N, dev) &&
-         (act == GPIC_ACT_NONE || (bf16(z, dev) && z.sizes() == dy.sizes())) && bf16(x, dev) && x.numel() == M * K &&
-         2 * M * std::max(N, K) < (int64_t(1) << 31) && K < (1 << 21);
+struct BwdIn {
+  const at::Tensor &dy, &z, &wq, &sw, &x;
+  int act;
+  bool need_dx, need_dw, need_db, w32, b32;   // (w32, b32: an fp32 weight's, bias's gradient)
+};
+bool linear_bwd_ok(const BwdIn &in, int dev) {
+  if (in.dy.dim() != 2 || !bf16(in.dy, dev) || !operand_rows(in.wq, dev)) return false;
+  const int64_t M = in.dy.size(0), N = in.dy.size(1), K = in.wq.size(1);
+  return M >= 1 && N >= 16 && N % 16 == 0 && N <= kRowsMaxCast && in.wq.size(0) == N && scales_ok(in.sw, N, dev) &&
+         (in.act == GPIC_ACT_NONE || (bf16(in.z, dev) && in.z.sizes() == in.dy.sizes())) && bf16(in.x, dev) &&
+         in.x.numel() == M * K && 2 * M * std::max(N, K) < (int64_t(1) << 31) && K < (1 << 21);
 }
-// (f32: an fp32 weight's, bias's gradient)
-LinearGrads linear_bwd_run(const at::Tensor &dy, const at::Tensor &z, int act, const at::Tensor &wq, const at::Tensor &sw,
-                           const at::Tensor &x, bool need_dx, bool need_dw, bool need_db, bool w32, bool b32, void *stream) {
-  const int64_t M = dy.size(0), N = dy.size(1), K = wq.size(1);
+// The parts of a linear's backward in its call's arena, and the bytes of its workspaces.
+struct BwdParts {
+  size_t q, s, dz, qt, ws, b_db, b_dx, b_dw;
+};
+BwdParts linear_bwd_parts(const BwdIn &in, Arena &m) {
+  const int64_t M = in.dy.size(0), N = in.dy.size(1), K = in.wq.size(1);
+  BwdParts p;
+  p.q = m.add(M * N);
+  p.s = m.add(4 * M);
+  p.dz = in.act == GPIC_ACT_NONE ? 0 : m.add(2 * M * N);
+  p.qt = in.need_dx ? m.add(K * N) : 0;
+  p.b_db = in.need_db ? gpic_fp8_act_bwd_rows_workspace_bytes(M, N) : 0;
+  p.b_dx = in.need_dx ? gpic_fp8_gemm_workspace_bytes(M, K, N) : 0;
+  p.b_dw = in.need_dw ? gpic_fp8_gemm_workspace_bytes(N, K, 2 * M) : 0;   // (planned as an e4m3 GEMM of as many K bytes)
+  p.ws = m.add(std::max(p.b_db, std::max(p.b_dx, p.b_dw)));               // (one after the other on one stream)
+  return p;
+}
+// dx: where the input's gradient goes (need_dx), or null: to a tensor of its own
+LinearGrads linear_bwd_run(const BwdIn &in, const BwdParts &p, const Arena &m, uint16_t *dx, void *stream) {
+  const int64_t M = in.dy.size(0), N = in.dy.size(1), K = in.wq.size(1);
   LinearGrads o;
-  const bool on = act != GPIC_ACT_NONE;
-  const at::Tensor dz = on ? make(dy, {M, N}, at::kBFloat16) : dy;
-  const at::Tensor q = make(dy, {M, N}, kE4), s = make(dy, {M}, at::kFloat);
-  at::Tensor qt, ws;
-  size_t bytes = 0;
-  if (need_dx) qt = make(dy, {K, N}, kE4);
-  if (need_db) {
-    o.db = make(dy, {N}, b32 ? at::kFloat : at::kBFloat16);
-    bytes = gpic_fp8_act_bwd_rows_workspace_bytes(M, N);
-    ws = make(dy, {(int64_t)bytes}, at::kByte);
-  }
-  check(gpic_fp8_act_bwd_rows(ptr<uint16_t>(dy), N, on ? ptr<uint16_t>(z) : nullptr, N, act, ptr<float>(sw), M, N,
-                              on ? ptr<uint16_t>(dz) : nullptr, ptr<uint8_t>(q), ptr<float>(s),
-                              need_dx ? ptr<uint8_t>(wq) : nullptr, K, need_dx ? ptr<uint8_t>(qt) : nullptr, N,
-                              need_db ? o.db.data_ptr() : nullptr, b32 ? GPIC_DTYPE_F32 : GPIC_DTYPE_BF16,
-                              need_db ? ws.data_ptr() : nullptr, bytes, stream),
+  const bool on = in.act != GPIC_ACT_NONE;
+  uint16_t *dz = on ? m.at<uint16_t>(p.dz) : ptr<uint16_t>(in.dy);
+  void *ws = m.at<uint8_t>(p.ws);
+  if (in.need_db) o.db = make(in.dy, {N}, in.b32 ? at::kFloat : at::kBFloat16);
+  check(gpic_fp8_act_bwd_rows(ptr<uint16_t>(in.dy), N, on ? ptr<uint16_t>(in.z) : nullptr, N, in.act, ptr<float>(in.sw), M, N,
+                              on ? dz : nullptr, m.at<uint8_t>(p.q), m.at<float>(p.s),
+                              in.need_dx ? ptr<uint8_t>(in.wq) : nullptr, K, in.need_dx ? m.at<uint8_t>(p.qt) : nullptr, N,
+                              in.need_db ? o.db.data_ptr() : nullptr, in.b32 ? GPIC_DTYPE_F32 : GPIC_DTYPE_BF16,
+                              in.need_db ? ws : nullptr, p.b_db, stream),
         "gpic_fp8_act_bwd_rows");
-  if (need_dx) o.dx = gemm_rows_run(q, s, qt, std::nullopt, std::nullopt, GPIC_ACT_NONE, std::nullopt, Mod(), false, stream).y;
-  if (need_dw) {
-    o.dw = make(dy, {N, K}, w32 ? at::kFloat : at::kBFloat16);
-    const Scratch w(dy, N, K, 2 * M);   // (planned as an e4m3 GEMM of as many K bytes)
-    check(gpic_fp8_bf16_gemm_mn(ptr<uint16_t>(dz), N, ptr<uint16_t>(x), K, o.dw.data_ptr(),
-                                w32 ? GPIC_DTYPE_F32 : GPIC_DTYPE_BF16, K, N, K, M, w.p(), w.bytes, stream),
+  if (in.need_dx) {
+    if (!dx) {
+      o.dx = make(in.dy, {M, K}, at::kBFloat16);
+      dx = ptr<uint16_t>(o.dx);
+    }
+    const GemmIn g{m.at<uint8_t>(p.q), m.at<uint8_t>(p.qt), m.at<float>(p.s), nullptr, M, K, N};
+    gemm_rows_call(g, dx, nullptr, ws, p.b_dx, stream);
+  }
+  if (in.need_dw) {
+    o.dw = make(in.dy, {N, K}, in.w32 ? at::kFloat : at::kBFloat16);
+    check(gpic_fp8_bf16_gemm_mn(dz, N, ptr<uint16_t>(in.x), K, o.dw.data_ptr(), in.w32 ? GPIC_DTYPE_F32 : GPIC_DTYPE_BF16, K, N,
+                                K, M, p.b_dw ? ws : nullptr, p.b_dw, stream),
           "gpic_fp8_bf16_gemm_mn");
   }
   return o;
@@ -506,11 +567,15 @@ py::object or_none(const at::Tensor &t) { return t.defined() ? py::cast(t) : py:
 py::object linear_rows_bwd(const at::Tensor &dy, const at::Tensor &z, int act, const at::Tensor &wq, const at::Tensor &sw,
                            const at::Tensor &x, bool need_dx, bool need_dw, bool need_db, bool w32, bool b32, int dev, handle,
                            handle stream) {
-  if (!linear_bwd_ok(dy, z, act, wq, sw, x, dev)) return py::none();
+  const BwdIn in{dy, z, wq, sw, x, act, need_dx, need_dw, need_db, w32, b32};
+  if (!linear_bwd_ok(in, dev)) return py::none();
   LinearGrads o;
   {
     NoGil no_gil;
-    o = linear_bwd_run(dy, z, act, wq, sw, x, need_dx, need_dw, need_db, w32, b32, vp(stream));
+    Arena m;
+    const BwdParts p = linear_bwd_parts(in, m);
+    m.make_like(dy);
+    o = linear_bwd_run(in, p, m, nullptr, vp(stream));
   }
   return py::make_tuple(or_none(o.dx), or_none(o.dw), or_none(o.db));
 }
@@ -520,17 +585,28 @@ py::object norm_linear_rows_bwd(const at::Tensor &dy, const opt &dxn, const at::
                                 const at::Tensor &sw, const at::Tensor &h, const at::Tensor &xs, const at::Tensor &wn,
                                 const at::Tensor &rstd, bool need_dw, bool need_db, bool w32, bool b32, int dev, handle,
                                 handle stream) {
-  if (!linear_bwd_ok(dy, z, act, wq, sw, h, dev) || xs.numel() != h.numel() || xs.size(-1) != wq.size(1) ||
-      !norm_bwd_ok(h, dxn, xs, wn, rstd, dev))
+  const BwdIn in{dy, z, wq, sw, h, act, true, need_dw, need_db, w32, b32};
+  if (!linear_bwd_ok(in, dev) || xs.dim() < 1 || xs.size(-1) != wq.size(1) ||
+      !norm_bwd_ok(dy.size(0), dxn, xs, wn, rstd, dev))
     return py::none();
+  const int64_t M = dy.size(0), K = wq.size(1);
   LinearGrads o;
-  std::pair<at::Tensor, at::Tensor> n;
+  at::Tensor dx, dwn;
   {
     NoGil no_gil;
-    o = linear_bwd_run(dy, z, act, wq, sw, h, true, need_dw, need_db, w32, b32, vp(stream));
-    n = norm_bwd_run(o.dx, dxn, xs, wn, rstd, vp(stream));
+    Arena m;
+    const BwdParts p = linear_bwd_parts(in, m);
+    const size_t bytes = gpic_fp8_rmsnorm_rows_bwd_workspace_bytes(M, K), dh = m.add(2 * M * K), ws = m.add(bytes);
+    m.make_like(dy);
+    o = linear_bwd_run(in, p, m, m.at<uint16_t>(dh), vp(stream));
+    dx = make(xs, xs.sizes(), at::kBFloat16);
+    dwn = make(xs, {K}, wn.scalar_type());
+    check(gpic_fp8_rmsnorm_rows_bwd(m.at<uint16_t>(dh), u16(dxn), ptr<uint16_t>(xs), wn.data_ptr(), dtype_code(wn),
+                                    ptr<float>(rstd), M, K, ptr<uint16_t>(dx), dwn.data_ptr(), dtype_code(dwn),
+                                    m.at<uint8_t>(ws), bytes, vp(stream)),
+          "gpic_fp8_rmsnorm_rows_bwd");
   }
-  return py::make_tuple(n.first, n.second, or_none(o.dw), or_none(o.db));
+  return py::make_tuple(dx, dwn, or_none(o.dw), or_none(o.db));
 }
 
 }  // namespace

@@ -103,6 +103,60 @@ __device__ __forceinline__ int64_t team_step() {
   return (int64_t)gridDim.x * (kWG<T> / T);
 }
 
+struct CastArgs {
+  const void *x;   // [rows, C] bf16, or fp32 (f32)
+  uint8_t *q;
+  float *s;
+  int64_t rows, ld;
+  int f32;
+};
+
+// The row cast of p's rows first, first + step, ... by one team. red: two sets of T / 64 words, in turn.
+template <int T, int kV>
+__device__ __forceinline__ void cast_team(const CastArgs &p, int C, int64_t first, int64_t step,
+                                          uint32_t (&red)[2][T > 64 ? T / 64 : 1]) {
+  const int t = threadIdx.x % T, nv = C / 8;
+  int turn = 0;
+  for (int64_t row = first; row < p.rows; row += step, turn ^= 1) {
+    float H[kV][8];
+    uint32_t m = 0;
+#pragma unroll
+    for (int j = 0; j < kV; j++) {
+      const int v = t + T * j;
+      if (v < nv) load8(p.x, p.f32, row * p.ld + 8 * v, H[j]);
+    }
+#pragma unroll
+    for (int j = 0; j < kV; j++)
+      if (t + T * j < nv) m = absmax8(H[j], m);
+    float scale, dequant;
+    scales_from_amax(team_max<T>(m, red[turn]), scale, dequant);
+#pragma unroll
+    for (int j = 0; j < kV; j++) {
+      const int v = t + T * j;
+      if (v < nv) *reinterpret_cast<u32x2 *>(p.q + row * C + 8 * v) = cast8(H[j], scale);
+    }
+    if (t == 0) p.s[row] = dequant;
+  }
+}
+
+// The workgroup's index among `blocks` from blockIdx.x - first, as a team's first row and the rows between two of its rows.
+template <int T>
+__device__ __forceinline__ int64_t team_row_in(int first) {
+  constexpr int R = kWG<T> / T;
+  return ((int64_t)blockIdx.x - first) * R + (R == 1 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x / T));
+}
+
+// One matrix by the first `blocks` workgroups, another (a linear's input and its weight: rows of one length) by the rest.
+template <int T, int kV>
+__global__ __launch_bounds__(kWG<T>) void tcast_rows_kernel(CastArgs a, CastArgs b, int C, int blocks) {
+  __shared__ uint32_t red[2][T > 64 ? T / 64 : 1];
+  constexpr int R = kWG<T> / T;
+  const bool first = (int)blockIdx.x < blocks;
+  const CastArgs p = first ? a : b;
+  cast_team<T, kV>(p, C, team_row_in<T>(first ? 0 : blocks),
+                   (int64_t)(first ? blocks : (int)gridDim.x - blocks) * R, red);
+}
+
 struct NormRowsArgs {
   const uint16_t *x, *a, *gate, *shift, *scale;
   const void *w;
@@ -117,9 +171,14 @@ struct NormRowsArgs {
 // A team takes `chunk` rows one after another: the row after the current one is requested before the current one's sums, and
 // w, and gate, shift and scale while the batch entry stays the same, are kept in registers.
 template <int T, int kV, bool kRes, bool kMod>
-__global__ __launch_bounds__(kWG<T>) void rmsnorm_rows_kernel(NormRowsArgs p) {
+__global__ __launch_bounds__(kWG<T>) void rmsnorm_rows_kernel(NormRowsArgs p, CastArgs weight, int blocks) {
   __shared__ float red_s[T > 64 ? T / 64 : 1];
-  __shared__ uint32_t red_m[T > 64 ? T / 64 : 1];
+  __shared__ uint32_t red_w[2][T > 64 ? T / 64 : 1];
+  uint32_t (&red_m)[T > 64 ? T / 64 : 1] = red_w[0];
+  if ((int)blockIdx.x >= blocks) {   // (the weight of the linear that reads the norm: its cast, beside it)
+    cast_team<T, kV>(weight, p.C, team_row_in<T>(blocks), (int64_t)((int)gridDim.x - blocks) * (kWG<T> / T), red_w);
+    return;
+  }
   const int t = threadIdx.x % T, nv = p.C / 8;
   int64_t row = team_row<T>() * p.chunk;
   const int64_t end = min(row + p.chunk, p.rows);
@@ -228,34 +287,6 @@ __global__ __launch_bounds__(kWG<T>) void rmsnorm_rows_kernel(NormRowsArgs p) {
       p.s[row] = dequant;
       p.rstd[row] = rstd;
     }
-  }
-}
-
-template <int T, int kV, bool kF32>
-__global__ __launch_bounds__(kWG<T>) void tcast_rows_kernel(const void *__restrict__ x, int64_t ldx, int64_t rows, int C,
-                                                            uint8_t *__restrict__ q, float *__restrict__ s) {
-  __shared__ uint32_t red_m[2][T > 64 ? T / 64 : 1];
-  const int t = threadIdx.x % T, nv = C / 8;
-  int turn = 0;
-  for (int64_t row = team_row<T>(); row < rows; row += team_step<T>(), turn ^= 1) {
-    float H[kV][8];
-    uint32_t m = 0;
-#pragma unroll
-    for (int j = 0; j < kV; j++) {
-      const int v = t + T * j;
-      if (v < nv) load8(x, kF32, row * ldx + 8 * v, H[j]);
-    }
-#pragma unroll
-    for (int j = 0; j < kV; j++)
-      if (t + T * j < nv) m = absmax8(H[j], m);
-    float scale, dequant;
-    scales_from_amax(team_max<T>(m, red_m[turn]), scale, dequant);
-#pragma unroll
-    for (int j = 0; j < kV; j++) {
-      const int v = t + T * j;
-      if (v < nv) *reinterpret_cast<u32x2 *>(q + row * C + 8 * v) = cast8(H[j], scale);
-    }
-    if (t == 0) s[row] = dequant;
   }
 }
 
@@ -579,20 +610,29 @@ using namespace gpic;
 
 extern "C" {
 
-int gpic_fp8_tcast_rows(const void *x, int dtype, int64_t ldx, int64_t rows, int64_t cols, uint8_t *q, float *s,
-                        void *stream) {
-  status_scope();
+// A matrix to cast by rows: its status, and whether there is anything to do.
+static int cast_ok(const void *x, int dtype, int64_t ldx, int64_t rows, int64_t cols, int64_t most, const uint8_t *q,
+                   const float *s) {
   if (rows < 0 || cols <= 0 || (rows > 0 && (!x || !q || !s))) return GPIC_EINVAL;
   if (!dtype_ok(dtype)) return GPIC_EDTYPE;
-  if (cols % 8 || cols > kMaxRowC || ldx % 8 || ldx < cols) return GPIC_ESHAPE;
+  if (cols % 8 || cols > most || ldx % 8 || ldx < cols) return GPIC_ESHAPE;
   if (!aligned16(x) || !aligned16(q)) return GPIC_EALIGN;
-  if (rows == 0) return GPIC_OK;
-  const hipStream_t st = (hipStream_t)stream;
+  return GPIC_OK;
+}
+
+int gpic_fp8_tcast_rows(const void *x, int dtype, int64_t ldx, int64_t rows, int64_t cols, uint8_t *q, float *s,
+                        const void *x2, int dtype2, int64_t ldx2, int64_t rows2, uint8_t *q2, float *s2, void *stream) {
+  status_scope();
+  int e = cast_ok(x, dtype, ldx, rows, cols, kMaxRowC, q, s);
+  if (e == GPIC_OK && x2) e = cast_ok(x2, dtype2, ldx2, rows2, cols, kMaxRowC, q2, s2);
+  if (e != GPIC_OK) return e;
+  if (!x2) rows2 = 0;
+  if (rows + rows2 == 0) return GPIC_OK;
+  const CastArgs a{x, q, s, rows, ldx, dtype == GPIC_DTYPE_F32}, b{x2, q2, s2, rows2, ldx2, dtype2 == GPIC_DTYPE_F32};
   with_team(cols, [&](auto T, auto V) {
     constexpr int t = decltype(T)::value, v = decltype(V)::value;
-    const unsigned g = row_blocks(rows, kWG<t> / t);
-    if (dtype == GPIC_DTYPE_F32) tcast_rows_kernel<t, v, true><<<g, kWG<t>, 0, st>>>(x, ldx, rows, (int)cols, q, s);
-    else tcast_rows_kernel<t, v, false><<<g, kWG<t>, 0, st>>>(x, ldx, rows, (int)cols, q, s);
+    const unsigned ga = row_blocks(rows, kWG<t> / t), gb = row_blocks(rows2, kWG<t> / t);
+    tcast_rows_kernel<t, v><<<ga + gb, kWG<t>, 0, (hipStream_t)stream>>>(a, b, (int)cols, (int)ga);
   });
   return (int)hipGetLastError();
 }
@@ -600,7 +640,8 @@ int gpic_fp8_tcast_rows(const void *x, int dtype, int64_t ldx, int64_t rows, int
 int gpic_fp8_rmsnorm_rows(const uint16_t *x, int64_t ldx, const uint16_t *a, int64_t lda, const uint16_t *gate, int64_t sg,
                           const void *w, int w_dtype, const uint16_t *shift, int64_t ssh, const uint16_t *scale,
                           int64_t ssc, int64_t rows, int64_t ntok, int64_t C, float eps, uint16_t *xn, uint16_t *h,
-                          float *rstd, uint8_t *q, float *s, void *stream) {
+                          float *rstd, uint8_t *q, float *s, const void *wt, int wt_dtype, int64_t N, uint8_t *wq, float *sw,
+                          void *stream) {
   status_scope();
   if (rows < 0 || C <= 0 || ntok <= 0 || (gate && !a) || !shift != !scale) return GPIC_EINVAL;
   if (rows > 0 && (!x || !w || !rstd || !q || !s || (a && !xn))) return GPIC_EINVAL;
@@ -611,7 +652,14 @@ int gpic_fp8_rmsnorm_rows(const uint16_t *x, int64_t ldx, const uint16_t *a, int
   if (!aligned16(x) || !aligned16(a) || !aligned16(gate) || !aligned16(w) || !aligned16(shift) || !aligned16(scale) ||
       !aligned16(xn) || !aligned16(h) || !aligned16(q))
     return GPIC_EALIGN;
-  if (rows == 0) return GPIC_OK;
+  if (wt) {
+    const int e = cast_ok(wt, wt_dtype, C, N, C, kMaxNormC, wq, sw);
+    if (e != GPIC_OK) return e;
+  } else {
+    N = 0;
+  }
+  if (rows + N == 0) return GPIC_OK;
+  const CastArgs weight{wt, wq, sw, N, C, wt_dtype == GPIC_DTYPE_F32};
   const NormRowsArgs p{x, a, gate, shift, scale, w, xn, h, rstd, s, q, rows, ntok, ldx, lda, sg, ssh, ssc,
                        (int)C, w_dtype == GPIC_DTYPE_F32, 1, eps};
   const hipStream_t st = (hipStream_t)stream;
@@ -623,7 +671,7 @@ int gpic_fp8_rmsnorm_rows(const uint16_t *x, int64_t ldx, const uint16_t *a, int
       const unsigned g = (unsigned)((rows + (int64_t)q.chunk * (kWG<t> / t) - 1) / ((int64_t)q.chunk * (kWG<t> / t)));
       auto *k = a ? (shift ? rmsnorm_rows_kernel<t, v, true, true> : rmsnorm_rows_kernel<t, v, true, false>)
                   : (shift ? rmsnorm_rows_kernel<t, v, false, true> : rmsnorm_rows_kernel<t, v, false, false>);
-      k<<<g, kWG<t>, 0, st>>>(q);
+      k<<<g + row_blocks(N, kWG<t> / t), kWG<t>, 0, st>>>(q, weight, (int)g);
     }
   });
   return (int)hipGetLastError();

@@ -53,9 +53,9 @@ SIGNATURES = {
     "gpic_fp8_gemm_bias32": (_int, [_vp, _i64, _vp, _vp, _i64, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _vp, _sz, _vp]),
     "gpic_fp8_gemm_mn": (_int, [_vp, _i64, _vp, _vp, _i64, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _vp, _sz, _vp]),
     "gpic_fp8_gemm_mn_f32": (_int, [_vp, _i64, _vp, _vp, _i64, _vp, _vp, _i64, _i64, _i64, _i64, _vp, _sz, _vp]),
-    "gpic_fp8_tcast_rows": (_int, [_vp, _int, _i64, _i64, _i64, _vp, _vp, _vp]),
+    "gpic_fp8_tcast_rows": (_int, [_vp, _int, _i64, _i64, _i64, _vp, _vp, _vp, _int, _i64, _i64, _vp, _vp, _vp]),
     "gpic_fp8_rmsnorm_rows": (_int, [_vp, _i64, _vp, _i64, _vp, _i64, _vp, _int, _vp, _i64, _vp, _i64, _i64, _i64, _i64,
-                                      ctypes.c_float, _vp, _vp, _vp, _vp, _vp, _vp]),
+                                      ctypes.c_float, _vp, _vp, _vp, _vp, _vp, _vp, _int, _i64, _vp, _vp, _vp]),
     "gpic_fp8_rmsnorm_rows_bwd_workspace_bytes": (_sz, [_i64, _i64]),
     "gpic_fp8_rmsnorm_rows_bwd": (_int, [_vp, _vp, _vp, _vp, _int, _vp, _i64, _i64, _vp, _vp, _int, _vp, _sz, _vp]),
     "gpic_fp8_gemm_rows": (_int, [_vp, _i64, _vp, _vp, _i64, _vp, _vp, _int, _int, _vp, _i64, _vp, _i64, _i64, _vp, _i64,

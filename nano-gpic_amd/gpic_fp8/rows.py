@@ -96,7 +96,8 @@ def tcast_rows_op(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     s = torch.empty(x2.shape[0], dtype=torch.float32, device=x.device)
     with L.on_device(x.device):
         L.check(L.lib().gpic_fp8_tcast_rows(x2.data_ptr(), L.DTYPE_CODE[x2.dtype], ld, x2.shape[0], C, q.data_ptr(),
-                                            s.data_ptr(), L.stream_ptr(x.device)), "gpic_fp8_tcast_rows")
+                                            s.data_ptr(), None, 0, 0, 0, None, None, L.stream_ptr(x.device)),
+                "gpic_fp8_tcast_rows")
     return q, s
 
 
@@ -108,7 +109,8 @@ def _(x):
 def tcast_rows(x):
     """x [..., C] (any float dtype, C % 8 == 0, C <= 32768) -> (q e4m3, x's shape; s [rows] fp32): tcast with one amax, and
     one scale, a row. A NaN in a row makes its scale NaN."""
-    return _run(tcast_rows_op, x)
+    o = L.native("cast_rows", x, x)
+    return o if o is not None else _run(tcast_rows_op, x)
 
 
 class RowsWeight(NamedTuple):
@@ -182,8 +184,8 @@ def rmsnorm_rows_op(x: torch.Tensor, w: torch.Tensor, eps: float, a: Optional[to
         L.check(L.lib().gpic_fp8_rmsnorm_rows(
             x2.data_ptr(), ldx, L.ptr(a2), lda, L.ptr(g), sg, wc.data_ptr(), L.DTYPE_CODE[wc.dtype], L.ptr(sh), ssh,
             L.ptr(sc), ssc, M, ntok, C, float(eps), xn.data_ptr() if a is not None else None,
-            h.data_ptr() if want_h else None, rstd.data_ptr(), q.data_ptr(), s.data_ptr(), L.stream_ptr(dev)),
-            "gpic_fp8_rmsnorm_rows")
+            h.data_ptr() if want_h else None, rstd.data_ptr(), q.data_ptr(), s.data_ptr(), None, 0, 0, None, None,
+            L.stream_ptr(dev)), "gpic_fp8_rmsnorm_rows")
     return xn, h, q, s, rstd
 
 
@@ -199,7 +201,8 @@ def rmsnorm_rows(x, w, eps, a=None, gate=None, shift=None, scale=None, want_h=Fa
     (x_new bf16, empty without a; h bf16, empty unless want_h; h's e4m3 bytes; their scales [rows]; rstd [rows]).
     x, a [..., C] bf16, C % 8 == 0, C <= 16384; w [C]; gate, shift, scale [B, 1, C] for x [B, N, C] (or one row for all;
     for x [M, C] any number of rows that divides M). h is rounded once, to e4m3 (and once, to bf16, for want_h)."""
-    return _run(rmsnorm_rows_op, x, w, eps, a, gate, shift, scale, want_h)
+    o = L.native("norm_rows", x, x, w, eps, a, gate, shift, scale, want_h)
+    return o if o is not None else _run(rmsnorm_rows_op, x, w, eps, a, gate, shift, scale, want_h)
 
 
 @L.step_op("gpic::fp8_rmsnorm_rows_bwd")
@@ -244,7 +247,8 @@ def rmsnorm_rows_bwd(dh, dxn, xs, w, rstd):
     """The backward of rmsnorm_rows without gate, shift and scale: dh (of h) and dxn (of x_new, or None) like xs (x_new, or
     x without a) [..., C] bf16, rstd [rows] -> (dx, which is a's gradient too, bf16; dw [C] of w's dtype, summed in fp32 in a
     fixed order)."""
-    return _run(rmsnorm_rows_bwd_op, dh, dxn, xs, w, rstd)
+    o = L.native("norm_rows_bwd", xs, dh, dxn, xs, w, rstd)
+    return o if o is not None else _run(rmsnorm_rows_bwd_op, dh, dxn, xs, w, rstd)
 
 
 # ------------------------------------------------------------------------------------------------ GEMM
@@ -316,7 +320,8 @@ def fp8_gemm_rows(a, sa, b, sb, bias=None, act="none", residual=None, gate=None)
     y [M, N] bf16 = residual + gate act(sa sb a b^T + bias), in fp32 and rounded once. act: "none", "silu", "gelu_tanh", or
     "swiglu" (b's rows as rows_weight(w12, "swiglu") lays them out; y [M, N / 2]). bias [N] bf16 or fp32; residual [M, N]
     bf16; gate [B, 1, N] bf16, B dividing M: a block's gate, one row for M / B rows of y."""
-    return _run(gemm_rows_op, a, sa, b, sb, bias, act, residual, gate)[0]
+    o = L.native("gemm_rows", a, a, sa, b, sb, bias, _act(act), residual, gate, False)
+    return (o if o is not None else _run(gemm_rows_op, a, sa, b, sb, bias, act, residual, gate))[0]
 
 
 @L.step_op("gpic::fp8_act_bwd_rows")

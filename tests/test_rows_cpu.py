@@ -20,8 +20,11 @@ def p():
 
 
 def test_tcast_rows_codes(p):
-    f = lambda x=p, dt=0, ld=64, rows=4, cols=64, q=p, s=p: L.lib().gpic_fp8_tcast_rows(x, dt, ld, rows, cols, q, s, None)  # noqa: E731
-    assert f(rows=0) == 0 and f(rows=0, x=None, q=None, s=None) == 0
+    def f(x=p, dt=0, ld=64, rows=4, cols=64, q=p, s=p, x2=p, dt2=1, ld2=64, rows2=4, q2=p, s2=p):
+        return L.lib().gpic_fp8_tcast_rows(x, dt, ld, rows, cols, q, s, x2, dt2, ld2, rows2, q2, s2, None)
+    assert f(rows=0, rows2=0) == 0 and f(rows=0, x=None, q=None, s=None, x2=None, q2=None, s2=None) == 0
+    assert f(rows2=-1) == EINVAL and f(q2=None) == EINVAL and f(s2=None) == EINVAL and f(dt2=9) == EDTYPE
+    assert f(ld2=68) == ESHAPE and f(ld2=56) == ESHAPE and f(x2=p + 8) == EALIGN and f(q2=p + 8) == EALIGN
     assert f(rows=-1) == EINVAL and f(cols=0) == EINVAL and f(x=None) == EINVAL and f(q=None) == EINVAL and f(s=None) == EINVAL
     assert f(dt=7) == EDTYPE
     assert f(cols=60) == ESHAPE and f(ld=68) == ESHAPE and f(ld=56) == ESHAPE and f(cols=32776, ld=32776) == ESHAPE
@@ -30,10 +33,12 @@ def test_tcast_rows_codes(p):
 
 def test_rmsnorm_rows_codes(p):
     def f(x=p, ldx=64, a=p, lda=64, gate=p, sg=64, w=p, wd=1, sh=p, ssh=64, sc=p, ssc=64, rows=4, ntok=2, C=64, xn=p, h=None,
-          rstd=p, q=p, s=p):
+          rstd=p, q=p, s=p, wt=None, td=0, N=16, wq=p, sw=p):
         return L.lib().gpic_fp8_rmsnorm_rows(x, ldx, a, lda, gate, sg, w, wd, sh, ssh, sc, ssc, rows, ntok, C, 1e-6, xn, h,
-                                             rstd, q, s, None)
+                                             rstd, q, s, wt, td, N, wq, sw, None)
     assert f(rows=0) == 0
+    assert f(wt=p, N=-1) == EINVAL and f(wt=p, wq=None) == EINVAL and f(wt=p, sw=None) == EINVAL and f(wt=p, td=3) == EDTYPE
+    assert f(wt=p + 8) == EALIGN and f(wt=p, wq=p + 8) == EALIGN
     for bad in (dict(rows=-1), dict(C=0), dict(ntok=0), dict(a=None), dict(sh=None), dict(sc=None), dict(x=None), dict(w=None),
                 dict(rstd=None), dict(q=None), dict(s=None), dict(xn=None)):
         assert f(**bad) == EINVAL, bad
@@ -71,7 +76,7 @@ def test_gemm_rows_codes(p):
         assert f(**bad) == EINVAL, bad
     assert f(bd=3) == EDTYPE
     for bad in (dict(K=72), dict(N=24), dict(lda=48), dict(ldb=48), dict(lda=72), dict(ldc=24), dict(ldc=36), dict(ldr=24),
-                dict(ldr=36), dict(ldz=24), dict(sg=24), dict(M=5), dict(ldr=1 << 22), dict(ldz=1 << 22), dict(ldc=1 << 22),
+                dict(ldr=36), dict(ldz=24), dict(sg=24), dict(M=5), dict(ldr=1 << 22), dict(ldz=1 << 22), dict(ldc=1 << 22), dict(sg=1 << 22),
                 dict(act=3, N=48, ldz=48), dict(act=3, ldc=8), dict(act=3, ldr=8)):
         assert f(**bad) == ESHAPE, bad
     for name in ("A", "B", "C", "sb", "bias", "res", "gate", "z"):
