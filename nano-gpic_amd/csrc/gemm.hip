@@ -775,6 +775,7 @@ __global__ __launch_bounds__(kThreads) void gemm_tn_kernel(const uint8_t *__rest
       auto block = [&](auto act_c, auto z_c, auto h_c, auto before) {
         constexpr int kAct = decltype(act_c)::value, h = decltype(h_c)::value;
         constexpr bool kZ = decltype(z_c)::value, kHalf = !kZ && kAct == GPIC_ACT_SWIGLU;
+        constexpr bool kBoth = kKeepZ && !kAdd && kBNt == 256;   // z and y in one pass
         constexpr int kRowOut = kHalf ? 64 : 128, kLPR = kRowOut / 16, kRPI = 64 / kLPR, kNI = 16 * kRM / kRPI;
         // (an opaque lane per block: the blocks' addresses are computed in them, not shared by all and held throughout)
         const int bl = opaque_v(el), wr = bl & 15, wg = bl >> 4;
@@ -797,6 +798,9 @@ __global__ __launch_bounds__(kThreads) void gemm_tn_kernel(const uint8_t *__rest
             asm volatile("" : "+v"(sa_m));   // (the pass that stores z does not keep its values for the one that stores y)
 #pragma unroll
             for (int e = 0; e < 8; e++) v[e] = __builtin_fmaf(v[e] * sa_m, e_sb[h >> 1][q][e], e_b[h >> 1][q][e]);
+            if constexpr (kBoth)   // (z beside y, through the other 4 KiB)
+              *(GPIC_LDS st16_t *)(cst + 4096 + r * 128 + 16 * ((4 * q + wg) ^ ((r >> 1) & 7))) =
+                  st16_t{pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3]), pack_bf16(v[4], v[5]), pack_bf16(v[6], v[7])};
             if (!kZ) {
               act8<kAct>(v);
               if constexpr (kAdd) {
@@ -835,9 +839,22 @@ __global__ __launch_bounds__(kThreads) void gemm_tn_kernel(const uint8_t *__rest
           const int r = kRPI * j + rr;
           wv[j] = *(const GPIC_LDS st16_t *)(cst + r * kRowOut + 16 * (rc ^ (kHalf ? (r >> 2) & 3 : (r >> 1) & 7)));
         }
+        constexpr int kNZ = kBoth ? 4 : 0;
+        st16_t zv[kNZ + 1];
+#pragma unroll
+        for (int j = 0; j < kNZ; j++) {
+          const int r = 8 * j + (bl >> 3);
+          zv[j] = *(const GPIC_LDS st16_t *)(cst + 4096 + r * 128 + 16 * ((bl & 7) ^ ((r >> 1) & 7)));
+        }
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // read back before the next block overwrites it
         before();
         const int n = cur.n0 + wn * kWTNt + 64 * (h >> 1);
+#pragma unroll
+        for (int j = 0; j < kNZ; j++) {
+          const int r = wm * kWTM + 32 * (h & 1) + 8 * j + (bl >> 3), nz = n + 8 * (bl & 7);
+          __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, zv[j]), rZ,
+                                                 r < rows_c && nz < N ? (r * ep.ldz + nz) * 2 : kOOB, 0, kStoreNT);
+        }
         const int no = (kHalf ? n >> 1 : n) + 8 * rc, ld = kZ ? ep.ldz : (int)ldc;
         const int rl = wm * kWTM + 32 * (h & 1) + rr;
 #pragma unroll
@@ -849,7 +866,7 @@ __global__ __launch_bounds__(kThreads) void gemm_tn_kernel(const uint8_t *__rest
       with_act(ep.act, [&](auto act) {
         auto both = [&](auto h) {
           constexpr int next = decltype(h)::value + 1;
-          if (kKeepZ && (!kAdd || ep.z)) block(act, std::bool_constant<kKeepZ>(), h, []() {});
+          if (kKeepZ && !(!kAdd && kBNt == 256) && (!kAdd || ep.z)) block(act, std::bool_constant<kKeepZ>(), h, []() {});
           block(act, std::false_type(), h, [&]() {
             if constexpr (kLdsRes && next + 1 < kBlocks) res_load(next + 1);
             if constexpr (!kLdsRes && next < kBlocks) res_load(next);
@@ -1170,24 +1187,29 @@ __global__ __launch_bounds__(256) void splitk_rows_kernel(const float *__restric
   }
 }
 
-// Few rows (kF blocks of 16): the weight's bytes bound it, each read once. A workgroup takes 16 columns, its kW waves every
-// kW-th K tile, straight from memory into the MFMA's operand registers (lane l: row l & 15, 32 bytes at K 32 (l / 16): whole
-// 128-byte lines), and the waves' sums are added in their order through LDS. Rows past M read the last row.
-template <int kF, int kW>
+// Few rows (kF blocks of 16): the weight's bytes bound it, each read once. A workgroup takes kC tiles of 16 columns, its kW waves
+// every kW-th K tile, straight from memory into the MFMA's operand registers (lane l: row l & 15, 32 bytes at K 32 (l / 16):
+// whole 128-byte lines), and the waves' sums are added in their order through LDS. Rows past M read the last row. Device time in
+// a graph, us, the weight not in L2 (the small tiles in brackets): one row [4096 x 1024] 3.4 (4.8), [1024 x 8192] 7.4 (26),
+// [4096 x 4096] 6.0 (17), [8192 x 8192] 15.2 (24; its 64 MiB at the copy's rate 13.2); 32 rows [4096 x 4096] 8.9 (10.6).
+template <int kF, int kC, int kW>
 __global__ __launch_bounds__(64 * kW) void gemm_few_kernel(const uint8_t *__restrict__ A, int64_t lda,
                                                            const uint8_t *__restrict__ B, int64_t ldb,
-                                                           uint16_t *__restrict__ C, int64_t ldc, int M, int K, RowsEpi ep) {
-  __shared__ __attribute__((aligned(16))) f4a_t red[kW][kF][64];
+                                                           uint16_t *__restrict__ C, int64_t ldc, int M, int N, int K,
+                                                           RowsEpi ep) {
+  static_assert(kF * kC <= kW, "a wave for each 16 x 16 tile's epilogue");
+  __shared__ __attribute__((aligned(16))) f4a_t red[kW][kF * kC][64];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int n0 = blockIdx.x * 16, row = lane & 15, kl = 32 * (lane >> 4);
-  const uint8_t *b = B + (n0 + row) * ldb + kl;
-  const uint8_t *a[kF];
+  const int n0 = blockIdx.x * (16 * kC), row = lane & 15, kl = 32 * (lane >> 4);
+  const uint8_t *a[kF], *b[kC];
 #pragma unroll
-  for (int f = 0; f < kF; f++) a[f] = A + (int64_t)min(16 * f + row, M - 1) * lda + kl;
-  // the epilogue's operands (wave f < kF, the lanes that will store), requested before the weight's bytes
-  const int em = 16 * wave + row, en = n0 + 4 * (lane >> 4);
-  const bool stores = wave < kF && !(lane & 16) && em < M;
+  for (int c = 0; c < kC; c++) b[c] = B + min(n0 + 16 * c + row, N - 1) * ldb + kl;   // (N % 16 == 0: a whole tile past it)
+#pragma unroll
+  for (int f = 0; f < kF; f++) a[f] = A + min(16 * f + row, M - 1) * lda + kl;
+  // the epilogue's operands (wave w: tile w, the lanes that will store), requested before the weight's bytes
+  const int em = 16 * (wave % kF) + row, en = n0 + 16 * (wave / kF) + 4 * (lane >> 4);
+  const bool stores = wave < kF * kC && !(lane & 16) && em < M && en < N;
   float sb8[8], b8[8], sa_m = 1.0f;
   u32x4 res{0u, 0u, 0u, 0u};
   if (stores) {
@@ -1196,9 +1218,9 @@ __global__ __launch_bounds__(64 * kW) void gemm_few_kernel(const uint8_t *__rest
     if (ep.sa) sa_m = ep.sa[em];
     res = epi8_res(ep, em, en);
   }
-  v4f acc[kF];
+  v4f acc[kF * kC];
 #pragma unroll
-  for (int f = 0; f < kF; f++) acc[f] = v4f{};
+  for (int f = 0; f < kF * kC; f++) acc[f] = v4f{};
   auto frag = [&](const uint8_t *p, int k0) {   // (K % 16 == 0: a 16-byte half lies in K or past it)
     u32x4 x{0u, 0u, 0u, 0u}, y{0u, 0u, 0u, 0u};
     if (k0 + kl < K) x = *reinterpret_cast<const u32x4 *>(p + k0);
@@ -1206,27 +1228,30 @@ __global__ __launch_bounds__(64 * kW) void gemm_few_kernel(const uint8_t *__rest
     return v8i{(int)x.x, (int)x.y, (int)x.z, (int)x.w, (int)y.x, (int)y.y, (int)y.z, (int)y.w};
   };
   const int nk = (K + kBK - 1) / kBK;
-  constexpr int kU = kF == 1 ? 4 : 2;   // K tiles in flight
+  constexpr int kU = kF * kC == 1 ? 4 : 2;   // K tiles in flight
   for (int kt = wave; kt < nk; kt += kU * kW) {
-    v8i fb[kU], fa[kU][kF];
+    v8i fb[kU][kC], fa[kU][kF];
 #pragma unroll
     for (int u = 0; u < kU; u++) {   // (tiles past K: zeros)
       const int k0 = (kt + u * kW) * kBK;
-      fb[u] = frag(b, k0);
+#pragma unroll
+      for (int c = 0; c < kC; c++) fb[u][c] = frag(b[c], k0);
 #pragma unroll
       for (int f = 0; f < kF; f++) fa[u][f] = frag(a[f], k0);
     }
 #pragma unroll
     for (int u = 0; u < kU; u++)
 #pragma unroll
-      for (int f = 0; f < kF; f++)
-        acc[f] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(fb[u], fa[u][f], acc[f], 0, 0, 0, 0, 0, 0);
+      for (int c = 0; c < kC; c++)
+#pragma unroll
+        for (int f = 0; f < kF; f++)
+          acc[c * kF + f] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(fb[u][c], fa[u][f], acc[c * kF + f], 0, 0, 0, 0, 0, 0);
   }
 #pragma unroll
-  for (int f = 0; f < kF; f++) red[wave][f][lane] = acc[f];
+  for (int f = 0; f < kF * kC; f++) red[wave][f][lane] = acc[f];
   __syncthreads();
-  if (wave >= kF) return;
-  // wave f: lane l holds C[16 f + (l & 15)][n0 + 4 (l / 16) + [0, 4)]; with lane l ^ 16, runs of 8
+  if (wave >= kF * kC) return;
+  // lane l of tile `wave` holds row l & 15, columns 4 (l / 16) + [0, 4); with lane l ^ 16, runs of 8
   f4a_t s = red[0][wave][lane];
 #pragma unroll
   for (int w = 1; w < kW; w++) s += red[w][wave][lane];
@@ -1461,10 +1486,21 @@ static int launch_gemm_rows(const uint8_t *A, int64_t lda, const uint8_t *B, int
     P = static_cast<float *>(ws);
   }
   if (M <= 32) {
-    auto *few = M <= 16 ? (K <= 512 ? gemm_few_kernel<1, 4> : K <= 2048 ? gemm_few_kernel<1, 8> : gemm_few_kernel<1, 16>)
-                        : (K <= 512 ? gemm_few_kernel<2, 4> : K <= 2048 ? gemm_few_kernel<2, 8> : gemm_few_kernel<2, 16>);
-    const int threads = K <= 512 ? 256 : K <= 2048 ? 512 : 1024;
-    few<<<(unsigned)(N / 16), threads, 0, st>>>(A, lda, B, ldb, C, ldc, (int)M, (int)K, ep);
+    // (waves by K, so that each has a few K tiles)
+    auto few = [&](auto rows, auto cols) {
+      constexpr int f = decltype(rows)::value, c = decltype(cols)::value;
+      auto *k = K <= 512 ? gemm_few_kernel<f, c, 4> : K <= 2048 ? gemm_few_kernel<f, c, 8> : gemm_few_kernel<f, c, 16>;
+      k<<<(unsigned)((N + 16 * c - 1) / (16 * c)), K <= 512 ? 256 : K <= 2048 ? 512 : 1024, 0, st>>>(
+          A, lda, B, ldb, C, ldc, (int)M, (int)N, (int)K, ep);
+    };
+    typedef std::integral_constant<int, 1> One;
+    typedef std::integral_constant<int, 2> Two;
+    // Two column tiles a workgroup, which reads A's rows half as often, where that still leaves one for every CU and there are
+    // rows to read ([8192 x 8192], two tiles / one: 32 rows 20.1 us / 27.5, 8 rows 16.9 / 17.4, one 16.1 / 15.2; with fewer columns
+    // the workgroups are missed: 32 rows [4096 x 4096] 10.8 / 9.1).
+    const bool wide = M > 4 && N >= 32 * num_cus();
+    if (M <= 16) wide ? few(One(), Two()) : few(One(), One());
+    else wide ? few(Two(), Two()) : few(Two(), One());
     return (int)hipGetLastError();
   }
   if (launch_small_class<RowsEpi>(A, lda, nullptr, B, ldb, nullptr, nullptr, 0, C, ldc, M, N, K, p, st, ep))

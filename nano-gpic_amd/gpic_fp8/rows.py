@@ -412,6 +412,7 @@ class _LinearRows(torch.autograd.Function):
             wq, sw = L.call(tcast_rows_op, w)
             y, z = L.call(gemm_rows_op, xq, sx, wq, sw, b, act, r2, None, want_z)
         ctx.save_for_backward(x2, z, wq, sw)
+        ctx.set_materialize_grads(False)
         ctx.act, ctx.wdt, ctx.bdt, ctx.shape = act, w.dtype, None if b is None else b.dtype, x.shape
         return y.view(*x.shape[:-1], w.shape[0])
 
@@ -421,6 +422,8 @@ class _LinearRows(torch.autograd.Function):
         x2, z, wq, sw = ctx.saved_tensors
         need = ctx.needs_input_grad
         dx = dw = db = None
+        if dy is None:
+            return None, None, None, None, None
         if any(need[:3]):
             dx, dw, db = _linear_bwd(ctx, dy.reshape(-1, dy.shape[-1]).to(BF), z, wq, sw, x2, *need[:3])
         return dx.view(ctx.shape) if need[0] else None, dw, db, None, dy if need[4] else None
@@ -442,6 +445,7 @@ class _NormLinearRows(torch.autograd.Function):
         xs = x if a is None else xn
         ctx.save_for_backward(xs, a if gate is not None else None, gate, wn, shift, scale, rstd,
                               h.view(-1, C) if train else None, z, wq, sw)
+        ctx.set_materialize_grads(False)
         ctx.act, ctx.wdt, ctx.bdt = act, w.dtype, None if b is None else b.dtype
         y = y.view(*x.shape[:-1], w.shape[0])
         return y if a is None else (xn, y)
@@ -452,6 +456,10 @@ class _NormLinearRows(torch.autograd.Function):
         xs, a, gate, wn, shift, scale, rstd, h, z, wq, sw = ctx.saved_tensors
         dxn, dy = grads if len(grads) == 2 else (None, grads[0])
         need = ctx.needs_input_grad
+        if dy is None:   # (x_new alone was used)
+            if dxn is None:
+                return (None,) * 10
+            dy = dxn.new_zeros(*dxn.shape[:-1], wq.shape[0])
         below = any(need[:6])   # a gradient through the norm
         dy2 = dy.reshape(-1, dy.shape[-1]).to(BF)
         dx = da = dgate = dwn = dshift = dscale = None
