@@ -113,7 +113,7 @@ struct CastArgs {
 
 // The row cast of p's rows first, first + step, ... by one team. red: two sets of T / 64 words, in turn.
 template <int T, int kV>
-__device__ __forceinline__ void cast_team(const CastArgs &p, int C, int64_t first, int64_t step,
+__device__ __forceinline__ void cast_team(const CastArgs &p, bool f32, int C, int64_t first, int64_t step,
                                           uint32_t (&red)[2][T > 64 ? T / 64 : 1]) {
   const int t = threadIdx.x % T, nv = C / 8;
   int turn = 0;
@@ -123,7 +123,7 @@ __device__ __forceinline__ void cast_team(const CastArgs &p, int C, int64_t firs
 #pragma unroll
     for (int j = 0; j < kV; j++) {
       const int v = t + T * j;
-      if (v < nv) load8(p.x, p.f32, row * p.ld + 8 * v, H[j]);
+      if (v < nv) load8(p.x, f32, row * p.ld + 8 * v, H[j]);
     }
 #pragma unroll
     for (int j = 0; j < kV; j++)
@@ -147,14 +147,21 @@ __device__ __forceinline__ int64_t team_row_in(int first) {
 }
 
 // One matrix by the first `blocks` workgroups, another (a linear's input and its weight: rows of one length) by the rest.
-template <int T, int kV>
+// (kKind: one bf16 matrix, one fp32, or two: instances of their own, as for the norm, whose plain one the test and the second
+// set of arguments cost 6%)
+enum { kOneBF16, kOneF32, kTwo };
+template <int T, int kV, int kKind>
 __global__ __launch_bounds__(kWG<T>) void tcast_rows_kernel(CastArgs a, CastArgs b, int C, int blocks) {
   __shared__ uint32_t red[2][T > 64 ? T / 64 : 1];
   constexpr int R = kWG<T> / T;
-  const bool first = (int)blockIdx.x < blocks;
-  const CastArgs p = first ? a : b;
-  cast_team<T, kV>(p, C, team_row_in<T>(first ? 0 : blocks),
-                   (int64_t)(first ? blocks : (int)gridDim.x - blocks) * R, red);
+  if constexpr (kKind != kTwo) {
+    cast_team<T, kV>(a, kKind == kOneF32, C, team_row<T>(), team_step<T>(), red);
+  } else {
+    const bool first = (int)blockIdx.x < blocks;
+    const CastArgs p = first ? a : b;
+    cast_team<T, kV>(p, p.f32, C, team_row_in<T>(first ? 0 : blocks),
+                     (int64_t)(first ? blocks : (int)gridDim.x - blocks) * R, red);
+  }
 }
 
 struct NormRowsArgs {
@@ -170,13 +177,13 @@ struct NormRowsArgs {
 
 // A team takes `chunk` rows one after another: the row after the current one is requested before the current one's sums, and
 // w, and gate, shift and scale while the batch entry stays the same, are kept in registers.
-template <int T, int kV, bool kRes, bool kMod>
+template <int T, int kV, bool kRes, bool kMod, bool kWeight>
 __global__ __launch_bounds__(kWG<T>) void rmsnorm_rows_kernel(NormRowsArgs p, CastArgs weight, int blocks) {
   __shared__ float red_s[T > 64 ? T / 64 : 1];
   __shared__ uint32_t red_w[2][T > 64 ? T / 64 : 1];
   uint32_t (&red_m)[T > 64 ? T / 64 : 1] = red_w[0];
-  if ((int)blockIdx.x >= blocks) {   // (the weight of the linear that reads the norm: its cast, beside it)
-    cast_team<T, kV>(weight, p.C, team_row_in<T>(blocks), (int64_t)((int)gridDim.x - blocks) * (kWG<T> / T), red_w);
+  if (kWeight && (int)blockIdx.x >= blocks) {   // (the weight of the linear that reads the norm: its cast, beside it)
+    cast_team<T, kV>(weight, weight.f32, p.C, team_row_in<T>(blocks), (int64_t)((int)gridDim.x - blocks) * (kWG<T> / T), red_w);
     return;
   }
   const int t = threadIdx.x % T, nv = p.C / 8;
@@ -632,7 +639,8 @@ int gpic_fp8_tcast_rows(const void *x, int dtype, int64_t ldx, int64_t rows, int
   with_team(cols, [&](auto T, auto V) {
     constexpr int t = decltype(T)::value, v = decltype(V)::value;
     const unsigned ga = row_blocks(rows, kWG<t> / t), gb = row_blocks(rows2, kWG<t> / t);
-    tcast_rows_kernel<t, v><<<ga + gb, kWG<t>, 0, (hipStream_t)stream>>>(a, b, (int)cols, (int)ga);
+    auto *k = x2 ? tcast_rows_kernel<t, v, kTwo> : a.f32 ? tcast_rows_kernel<t, v, kOneF32> : tcast_rows_kernel<t, v, kOneBF16>;
+    k<<<ga + gb, kWG<t>, 0, (hipStream_t)stream>>>(a, b, (int)cols, (int)ga);
   });
   return (int)hipGetLastError();
 }
@@ -669,8 +677,12 @@ int gpic_fp8_rmsnorm_rows(const uint16_t *x, int64_t ldx, const uint16_t *a, int
       NormRowsArgs q = p;
       q.chunk = norm_chunk(rows, kWG<t> / t);
       const unsigned g = (unsigned)((rows + (int64_t)q.chunk * (kWG<t> / t) - 1) / ((int64_t)q.chunk * (kWG<t> / t)));
-      auto *k = a ? (shift ? rmsnorm_rows_kernel<t, v, true, true> : rmsnorm_rows_kernel<t, v, true, false>)
-                  : (shift ? rmsnorm_rows_kernel<t, v, false, true> : rmsnorm_rows_kernel<t, v, false, false>);
+      auto pick = [&](auto two) {
+        constexpr bool w = decltype(two)::value;
+        return a ? (shift ? rmsnorm_rows_kernel<t, v, true, true, w> : rmsnorm_rows_kernel<t, v, true, false, w>)
+                 : (shift ? rmsnorm_rows_kernel<t, v, false, true, w> : rmsnorm_rows_kernel<t, v, false, false, w>);
+      };
+      auto *k = wt ? pick(std::true_type()) : pick(std::false_type());
       k<<<g + row_blocks(N, kWG<t> / t), kWG<t>, 0, st>>>(q, weight, (int)g);
     }
   });
