@@ -693,11 +693,12 @@ __global__ __launch_bounds__(kThreads) void gemm_tn_kernel(const uint8_t *__rest
         if (!ep.res) return;
         const bool half = ep.act == GPIC_ACT_SWIGLU;
         const int l = opaque_v(lane), rows = min(M - cur.m0, kBM);
-        const v4i rR = buffer_rsrc(ep.res + (int64_t)cur.m0 * ep.ldr, rows * ep.ldr * 2);
+        // (to the end of the last row and no further: lanes past N read the next row's values, or zeros, and store nothing)
+        const v4i rR = buffer_rsrc(ep.res + (int64_t)cur.m0 * ep.ldr, ((rows - 1) * ep.ldr + (half ? N >> 1 : N)) * 2);
         const uint32_t to =
             lds_addr(smem) + (group == 0 ? a_half(2) : b_half(1)) + (wave & 3) * kCStage + 4096 * (h & 1);
         const int n = cur.n0 + wn * kWTNt + 64 * (h >> 1), row0 = wm * kWTM + 32 * (h & 1);
-        const int lr = half ? l >> 2 : l >> 3;   // (columns past N: the next row's, or zeros; never stored)
+        const int lr = half ? l >> 2 : l >> 3;
         for (int i = 0; i < (half ? 2 : 4); i++) {
           const int r = (half ? 16 : 8) * i + lr;
           const int c = half ? (l & 3) ^ ((r >> 2) & 3) : (l & 7) ^ ((r >> 1) & 7);

@@ -37,10 +37,18 @@ def _act(act, train=False):
     return ACTS[act]
 
 
-def _run(op, *args):
-    """op(*args) for a public call: its function directly (L.call) unless a gradient is recorded, when the op itself says
-    that it has none."""
-    if torch.is_grad_enabled() and any(isinstance(t, torch.Tensor) and t.requires_grad for t in args):
+_PLAIN = (torch.Tensor, torch.nn.Parameter)
+
+
+def _run(op, name, x, *args):
+    """A public call of op: the native host module's function `name` on args, else the op's function (L.call); the op itself
+    where a gradient is recorded (it says that it has none) and for tensors without memory of their own (fake ones)."""
+    if type(x) in _PLAIN:
+        o = L.native(name, x, *(ACTS[a] if type(a) is str else a for a in args))
+        if o is not None:
+            return o
+    tensors = [t for t in args if isinstance(t, torch.Tensor)]
+    if any(type(t) not in _PLAIN for t in tensors) or (torch.is_grad_enabled() and any(t.requires_grad for t in tensors)):
         return op(*args)
     return L.call(op, *args)
 
@@ -109,8 +117,7 @@ def _(x):
 def tcast_rows(x):
     """x [..., C] (any float dtype, C % 8 == 0, C <= 32768) -> (q e4m3, x's shape; s [rows] fp32): tcast with one amax, and
     one scale, a row. A NaN in a row makes its scale NaN."""
-    o = L.native("cast_rows", x, x)
-    return o if o is not None else _run(tcast_rows_op, x)
+    return _run(tcast_rows_op, "cast_rows", x, x)
 
 
 class RowsWeight(NamedTuple):
@@ -201,8 +208,7 @@ def rmsnorm_rows(x, w, eps, a=None, gate=None, shift=None, scale=None, want_h=Fa
     (x_new bf16, empty without a; h bf16, empty unless want_h; h's e4m3 bytes; their scales [rows]; rstd [rows]).
     x, a [..., C] bf16, C % 8 == 0, C <= 16384; w [C]; gate, shift, scale [B, 1, C] for x [B, N, C] (or one row for all;
     for x [M, C] any number of rows that divides M). h is rounded once, to e4m3 (and once, to bf16, for want_h)."""
-    o = L.native("norm_rows", x, x, w, eps, a, gate, shift, scale, want_h)
-    return o if o is not None else _run(rmsnorm_rows_op, x, w, eps, a, gate, shift, scale, want_h)
+    return _run(rmsnorm_rows_op, "norm_rows", x, x, w, eps, a, gate, shift, scale, want_h)
 
 
 @L.step_op("gpic::fp8_rmsnorm_rows_bwd")
@@ -247,8 +253,7 @@ def rmsnorm_rows_bwd(dh, dxn, xs, w, rstd):
     """The backward of rmsnorm_rows without gate, shift and scale: dh (of h) and dxn (of x_new, or None) like xs (x_new, or
     x without a) [..., C] bf16, rstd [rows] -> (dx, which is a's gradient too, bf16; dw [C] of w's dtype, summed in fp32 in a
     fixed order)."""
-    o = L.native("norm_rows_bwd", xs, dh, dxn, xs, w, rstd)
-    return o if o is not None else _run(rmsnorm_rows_bwd_op, dh, dxn, xs, w, rstd)
+    return _run(rmsnorm_rows_bwd_op, "norm_rows_bwd", xs, dh, dxn, xs, w, rstd)
 
 
 # ------------------------------------------------------------------------------------------------ GEMM
@@ -320,8 +325,8 @@ def fp8_gemm_rows(a, sa, b, sb, bias=None, act="none", residual=None, gate=None)
     y [M, N] bf16 = residual + gate act(sa sb a b^T + bias), in fp32 and rounded once. act: "none", "silu", "gelu_tanh", or
     "swiglu" (b's rows as rows_weight(w12, "swiglu") lays them out; y [M, N / 2]). bias [N] bf16 or fp32; residual [M, N]
     bf16; gate [B, 1, N] bf16, B dividing M: a block's gate, one row for M / B rows of y."""
-    o = L.native("gemm_rows", a, a, sa, b, sb, bias, _act(act), residual, gate, False)
-    return (o if o is not None else _run(gemm_rows_op, a, sa, b, sb, bias, act, residual, gate))[0]
+    _act(act)
+    return _run(gemm_rows_op, "gemm_rows", a, a, sa, b, sb, bias, act, residual, gate, False)[0]
 
 
 @L.step_op("gpic::fp8_act_bwd_rows")
@@ -376,7 +381,7 @@ def act_bwd_rows(dy, z, act, sw):
     """dy [M, N] bf16 and the forward's z [M, N] bf16 (unused for act="none") -> (dz = dy act'(z) as bf16, dy itself for
     "none"; dz sw as e4m3; its scales [M]): the operands of the weight's gradient and, against the weight's bytes
     transposed, of the dgrad (sw [N]: the weight's scales, which lie on its reduction)."""
-    dz, q, s, _, _ = _run(act_bwd_rows_op, dy, z, act, sw)
+    dz, q, s, _, _ = _run(act_bwd_rows_op, None, None, dy, z, act, sw)
     return (dy if act == "none" else dz), q, s
 
 
@@ -520,10 +525,14 @@ def fp8_linear_rows(x, weight, bias=None, act="none", residual=None, gate=None):
                 raise ValueError(f"residual must be {(*x.shape[:-1], weight.shape[0])}, got {tuple(residual.shape)}")
             return _LinearRows.apply(x, weight, bias, act, residual)
         _no_gradient(x, bias, residual, gate)
-        K = x.shape[-1]
+        K, N = x.shape[-1], weight.q.shape[0] // (2 if weight.swiglu else 1)
+        if residual is not None:
+            if residual.shape != (*x.shape[:-1], N):
+                raise ValueError(f"residual must be {(*x.shape[:-1], N)}, got {tuple(residual.shape)}")
+            residual = residual.reshape(-1, N)
         q, s = L.call(tcast_rows_op, x.reshape(-1, K))
         y = L.call(gemm_rows_op, q, s, weight.q, weight.s, bias, act, residual, gate)[0]
-        return y.view(*x.shape[:-1], y.shape[-1])
+        return y.view(*x.shape[:-1], N)
 
 
 def fp8_rmsnorm_linear_rows(x, w_norm, eps, weight, bias=None, act="none", a=None, gate=None, shift=None, scale=None):

@@ -274,6 +274,27 @@ def test_gemm_rows_strides_and_empty(dev):
     assert G.fp8_gemm_rows(a, None, B[:0, :128], None).shape == (35, 0)
 
 
+@pytest.mark.parametrize("M,N,K,act", [(20, 96, 64, "none"), (300, 96, 512, "silu"), (4099, 1040, 256, "none"),
+                                       (4099, 1056, 256, "swiglu"), (9000, 2064, 400, "gelu_tanh"), (9001, 2080, 384, "swiglu"),
+                                       (700, 1040, 8192, "silu")])
+def test_gemm_rows_strided_residual_and_gate(dev, M, N, K, act):
+    """A residual that is a column range ending with its storage, a gate whose rows change within and between the waves' 64
+    rows, with and without z, in every tile class."""
+    g = gen(dev, M + N)
+    a, sa, b, sb = (t.to(dev) for t in (*R.rowq(randn(g, M, K)), *R.rowq(randn(g, N, K, std=K ** -0.5))))
+    No = N // 2 if act == "swiglu" else N
+    res = randn(g, M, No + 72)[:, 72:]
+    bias = randn(g, N)
+    for B in {1, 3 if M % 3 == 0 else 1, M // 50 if M % 50 == 0 else 1, M}:
+        gate = randn(g, B, 1, 3 * No).chunk(3, dim=-1)[1]
+        y = G.fp8_gemm_rows(a, sa, b, sb, bias, act, res, gate)
+        R.within(y, *R.gemm(a, sa, b, sb, bias, act, res, gate), f"gate of {B}")
+    y, z = GR.gemm_rows_op(a, sa, b, sb, bias, act, res, gate, True)
+    R.within(y, *R.gemm(a, sa, b, sb, bias, act, res, gate), "y beside z")
+    R.within(z, *R.gemm(a, sa, b, sb, bias), "z")
+    R.within(G.fp8_gemm_rows(a, sa, b, sb, bias, act, res), *R.gemm(a, sa, b, sb, bias, act, res), "residual alone")
+
+
 def test_gemm_rows_not_finite(dev):
     """A NaN scale reaches its own row alone, and so does an infinite one; an infinite residual stays."""
     g = gen(dev)
@@ -403,6 +424,16 @@ def test_linear_rows_some_gradients(dev):
     y = G.fp8_linear_rows(x32[:, :0], w, b, "gelu_tanh")
     gx, gw, gb = torch.autograd.grad(y.sum(), (x32, w, b))
     assert y.shape == (2, 0, 32) and not gw.any() and not gb.any() and not gx.any()
+    a = randn(g, 2, 9, 64).requires_grad_()
+    wn = torch.ones(64, device=dev, requires_grad=True)
+    xn, y = G.fp8_rmsnorm_linear_rows(x32, wn, 1e-6, w, b, "silu", a)   # one output alone
+    ga, gw0 = torch.autograd.grad(xn.float().sum(), (a, wn), retain_graph=True)
+    assert (ga == 1).all() and not gw0.any()
+    ga, gx = torch.autograd.grad(y.float().sum(), (a, x32))
+    assert torch.equal(ga.float(), gx) and ga.any()
+    y = G.fp8_linear_rows(x32, w, b, "silu").expand(3, 2, 9, 32)        # an expanded gradient
+    (gx,) = torch.autograd.grad(y.sum(), x32)
+    assert torch.isfinite(gx).all()
     with pytest.raises(RuntimeError):
         y = G.fp8_linear_rows(x32, w, b, "silu")
         (gx,) = torch.autograd.grad(y.float().sum(), x32, create_graph=True)

@@ -165,6 +165,8 @@ def test_refusals(no_gpu_check):
         lambda: G.fp8_linear_rows(z(4, 64), G.RowsWeight(z(32, 64, dt=F32).to(E4), torch.ones(32), True)),
         lambda: G.fp8_linear_rows(z(4, 64), G.RowsWeight(z(32, 64, dt=F32).to(E4), torch.ones(32), False), None, "swiglu"),
         lambda: G.fp8_linear_rows(z(4, 64).requires_grad_(), G.RowsWeight(z(32, 64, dt=F32).to(E4), torch.ones(32), False)),
+        lambda: G.fp8_linear_rows(z(4, 64), G.RowsWeight(z(32, 64, dt=F32).to(E4), torch.ones(32), False), None, "none", z(2, 32)),
+        lambda: G.fp8_linear_rows(z(4, 64), G.RowsWeight(z(32, 64, dt=F32).to(E4), torch.ones(32), True), None, "swiglu", z(4, 32)),
         lambda: G.fp8_rmsnorm_linear_rows(z(4, 64), w, 1e-6, z(16, 64), None, "none", None, None, z(1, 64), z(1, 64)),
         lambda: G.fp8_rmsnorm_linear_rows(z(1, 4, 64), w, 1e-6, z(16, 64), None, "none", z(1, 4, 64), z(1, 1, 64)),
         lambda: G.fp8_rmsnorm_linear_rows(z(1, 4, 64), w, 1e-6, z(16, 64), None, "none", z(1, 4, 64), None, z(1, 1, 64),
@@ -226,3 +228,15 @@ def test_host_module_takes_no_cpu_tensors():
     assert h.linear_rows_bwd(x, x, 0, q, v, x, True, True, True, True, True, 0, 0, 0) is None
     assert h.norm_linear_rows_fwd(x, v, 1e-6, n, n, n, n, w, n, 0, True, True, 0, 0, 0) is None
     assert h.norm_linear_rows_bwd(x, n, x, 0, q, v, x, x, v, v, True, True, True, True, 0, 0, 0) is None
+
+
+def test_public_calls_on_fake_tensors():
+    """Tensors without memory (a shape pass over a program) go to the ops' fake kernels."""
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    with FakeTensorMode():
+        e = lambda *s, dt=BF: torch.empty(*s, dtype=dt, device="cuda")  # noqa: E731
+        q, s = G.tcast_rows(e(6, 64))
+        assert G.rmsnorm_rows(e(2, 3, 64), e(64), 1e-6, e(2, 3, 64))[0].shape == (2, 3, 64)
+        assert G.rmsnorm_rows_bwd(e(3, 64), None, e(3, 64), e(64), e(3, dt=F32))[1].shape == (64,)
+        assert G.fp8_gemm_rows(q, s, e(32, 64, dt=E4), e(32, dt=F32), act="swiglu").shape == (6, 16)
+        assert G.act_bwd_rows(e(3, 64), e(3, 64), "silu", e(64, dt=F32))[1].dtype == E4
