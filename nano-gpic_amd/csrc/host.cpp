@@ -10,7 +10,10 @@
 // allocates and launches, as ctypes and torch's own operations release it: a launch waits where the queue is full.
 #include <ATen/ATen.h>
 #include <c10/core/GradMode.h>
+#include <c10/hip/HIPStream.h>
 #include <torch/csrc/Exceptions.h>
+#include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/utils.h>
 #include <torch/csrc/utils/pybind.h>
 
 #include <optional>
@@ -446,57 +449,64 @@ bool rows_weight_ok(const at::Tensor &w, int64_t K, int dev) {
   return w.dim() == 2 && w.size(1) == K && w.size(0) >= 16 && w.size(0) % 16 == 0 && K % 16 == 0 && row_castable(w, dev);
 }
 
-// x [M, K] bf16, w [N, K], bias [N] or None, residual [M, N] bf16 or None -> (y [M, N], z [M, N] or empty, w's bytes and scales)
-py::object linear_rows_fwd(const at::Tensor &x, const at::Tensor &w, const opt &bias, int act, const opt &res, bool want_z,
-                           int dev, handle, handle stream) {
-  if (x.dim() != 2 || x.size(0) < 1 || !bf16(x, dev) || !row_castable(x, dev) || !rows_weight_ok(w, x.size(1), dev) ||
-      !bias_ok(bias, w.size(0), dev) ||
-      (res && (!bf16(*res, dev) || res->dim() != 2 || res->size(0) != x.size(0) || res->size(1) != w.size(0))))
-    return py::none();
-  const int64_t M = x.size(0), K = x.size(1), N = w.size(0);
-  at::Tensor wq, sw, y, z;
-  {
-    NoGil no_gil;
-    wq = make(w, w.sizes(), kE4);
-    sw = make(w, {N}, at::kFloat);
-    y = make(x, {M, N}, at::kBFloat16);
-    z = want_z ? make(x, {M, N}, at::kBFloat16) : none_of(x, at::kBFloat16);
-    Arena m;
-    const size_t bytes = gpic_fp8_gemm_workspace_bytes(M, N, K), q = m.add(M * K), s = m.add(4 * M), ws = m.add(bytes);
-    m.make_like(x);
-    check(gpic_fp8_tcast_rows(x.data_ptr(), GPIC_DTYPE_BF16, K, M, K, m.at<uint8_t>(q), m.at<float>(s), w.data_ptr(),
-                              dtype_code(w), K, N, ptr<uint8_t>(wq), ptr<float>(sw), vp(stream)),
-          "gpic_fp8_tcast_rows");
-    const GemmIn g{m.at<uint8_t>(q), ptr<uint8_t>(wq), m.at<float>(s), ptr<float>(sw), M, N, K, &bias, act, u16(res)};
-    gemm_rows_call(g, ptr<uint16_t>(y), want_z ? ptr<uint16_t>(z) : nullptr, m.at<uint8_t>(ws), bytes, vp(stream));
-  }
-  return py::make_tuple(y, z, wq, sw);
+// A linear's tensors: x [..., K] or the norm's input, w [N, K]; y [..., N], z [M, N] (or empty), w's bytes and scales.
+struct LinearOut {
+  at::Tensor y, z, wq, sw;
+};
+LinearOut linear_out(const at::Tensor &x, const at::Tensor &w, bool want_z) {
+  std::vector<int64_t> size = x.sizes().vec();
+  size.back() = w.size(0);
+  LinearOut o;
+  o.y = make(x, size, at::kBFloat16);
+  o.z = want_z ? make(x, {x.numel() / x.size(-1), w.size(0)}, at::kBFloat16) : none_of(x, at::kBFloat16);
+  o.wq = make(w, w.sizes(), kE4);
+  o.sw = make(w, {w.size(0)}, at::kFloat);
+  return o;
+}
+LinearOut linear_run(const at::Tensor &x, const at::Tensor &w, const opt &bias, int act, const opt &res, bool want_z,
+                     void *stream) {
+  const int64_t K = x.size(-1), M = x.numel() / K, N = w.size(0);
+  LinearOut o = linear_out(x, w, want_z);
+  Arena m;
+  const size_t bytes = gpic_fp8_gemm_workspace_bytes(M, N, K), q = m.add(M * K), s = m.add(4 * M), ws = m.add(bytes);
+  m.make_like(x);
+  check(gpic_fp8_tcast_rows(x.data_ptr(), GPIC_DTYPE_BF16, K, M, K, m.at<uint8_t>(q), m.at<float>(s), w.data_ptr(),
+                            dtype_code(w), K, N, ptr<uint8_t>(o.wq), ptr<float>(o.sw), stream),
+        "gpic_fp8_tcast_rows");
+  const GemmIn g{m.at<uint8_t>(q), ptr<uint8_t>(o.wq), m.at<float>(s), ptr<float>(o.sw), M, N, K, &bias, act, u16(res)};
+  gemm_rows_call(g, ptr<uint16_t>(o.y), want_z ? ptr<uint16_t>(o.z) : nullptr, m.at<uint8_t>(ws), bytes, stream);
+  return o;
+}
+// The norm and the linear that reads its bytes.
+std::pair<NormOut, LinearOut> norm_linear_run(const at::Tensor &x, const at::Tensor &wn, double eps, const opt &a,
+                                              const NormIn &in, const at::Tensor &w, const opt &bias, int act, bool want_h,
+                                              bool want_z, void *stream) {
+  const int64_t K = x.size(-1), M = x.numel() / K, N = w.size(0);
+  LinearOut o = linear_out(x, w, want_z);
+  Arena m;
+  const size_t bytes = gpic_fp8_gemm_workspace_bytes(M, N, K), q = m.add(M * K), s = m.add(4 * M), ws = m.add(bytes);
+  m.make_like(x);
+  NormOut n = norm_run(x, wn, eps, a, in, want_h, m.at<uint8_t>(q), m.at<float>(s), &w, ptr<uint8_t>(o.wq), ptr<float>(o.sw),
+                       stream);
+  const GemmIn g{m.at<uint8_t>(q), ptr<uint8_t>(o.wq), m.at<float>(s), ptr<float>(o.sw), M, N, K, &bias, act};
+  gemm_rows_call(g, ptr<uint16_t>(o.y), want_z ? ptr<uint16_t>(o.z) : nullptr, m.at<uint8_t>(ws), bytes, stream);
+  return {n, o};
 }
 
-// The norm and the linear that reads its bytes -> (x_new or empty, h as bf16 or empty, rstd, y, z or empty, w's bytes, scales)
+// (x_new or empty, h as bf16 or empty, rstd, y, z or empty, w's bytes, scales)
 py::object norm_linear_rows_fwd(const at::Tensor &x, const at::Tensor &wn, double eps, const opt &a, const opt &gate,
                                 const opt &shift, const opt &scale, const at::Tensor &w, const opt &bias, int act, bool want_h,
                                 bool want_z, int dev, handle, handle stream) {
   NormIn in;
   if (!norm_ok(x, wn, a, gate, shift, scale, dev, in) || !rows_weight_ok(w, x.size(-1), dev) || !bias_ok(bias, w.size(0), dev))
     return py::none();
-  const int64_t K = x.size(-1), M = x.numel() / K, N = w.size(0);
-  at::Tensor wq, sw, y, z;
-  NormOut n;
+  std::pair<NormOut, LinearOut> r;
   {
     NoGil no_gil;
-    wq = make(w, w.sizes(), kE4);
-    sw = make(w, {N}, at::kFloat);
-    y = make(x, {M, N}, at::kBFloat16);
-    z = want_z ? make(x, {M, N}, at::kBFloat16) : none_of(x, at::kBFloat16);
-    Arena m;
-    const size_t bytes = gpic_fp8_gemm_workspace_bytes(M, N, K), q = m.add(M * K), s = m.add(4 * M), ws = m.add(bytes);
-    m.make_like(x);
-    n = norm_run(x, wn, eps, a, in, want_h, m.at<uint8_t>(q), m.at<float>(s), &w, ptr<uint8_t>(wq), ptr<float>(sw), vp(stream));
-    const GemmIn g{m.at<uint8_t>(q), ptr<uint8_t>(wq), m.at<float>(s), ptr<float>(sw), M, N, K, &bias, act};
-    gemm_rows_call(g, ptr<uint16_t>(y), want_z ? ptr<uint16_t>(z) : nullptr, m.at<uint8_t>(ws), bytes, vp(stream));
+    r = norm_linear_run(x, wn, eps, a, in, w, bias, act, want_h, want_z, vp(stream));
   }
-  return py::make_tuple(n.xn, n.h, n.rstd, y, z, wq, sw);
+  const auto &[n, o] = r;
+  return py::make_tuple(n.xn, n.h, n.rstd, o.y, o.z, o.wq, o.sw);
 }
 
 struct LinearGrads {
@@ -580,33 +590,180 @@ py::object linear_rows_bwd(const at::Tensor &dy, const at::Tensor &z, int act, c
   return py::make_tuple(or_none(o.dx), or_none(o.dw), or_none(o.db));
 }
 
-// The same and the norm's backward (without gate, shift and scale): (dx like xs, dwn, dw, db)
-py::object norm_linear_rows_bwd(const at::Tensor &dy, const opt &dxn, const at::Tensor &z, int act, const at::Tensor &wq,
-                                const at::Tensor &sw, const at::Tensor &h, const at::Tensor &xs, const at::Tensor &wn,
-                                const at::Tensor &rstd, bool need_dw, bool need_db, bool w32, bool b32, int dev, handle,
-                                handle stream) {
-  const BwdIn in{dy, z, wq, sw, h, act, true, need_dw, need_db, w32, b32};
-  if (!linear_bwd_ok(in, dev) || xs.dim() < 1 || xs.size(-1) != wq.size(1) ||
-      !norm_bwd_ok(dy.size(0), dxn, xs, wn, rstd, dev))
+// ---- the row-scaled linears in their usual form as nodes of the graph: the calls that the Python Functions of
+// gpic_fp8/rows.py make, without a Python frame on either of the engine's threads.
+
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+
+// An output's gradient as the kernels take it: [M, N] bf16, contiguous, 16-byte aligned.
+at::Tensor usual(const at::Tensor &g, int64_t N) {
+  at::Tensor t = g.reshape({-1, N}).to(at::kBFloat16).contiguous();
+  return (reinterpret_cast<uintptr_t>(t.data_ptr()) & 15u) ? t.clone() : t;
+}
+// The current stream of t's device: in a backward the engine has made the forward's current.
+void *current_stream(const at::Tensor &t) { return c10::hip::getCurrentHIPStream(t.get_device()).stream(); }
+// The gradients as they are; in a backward that is itself recorded, as outputs of a node that refuses to be differentiated.
+variable_list once(const variable_list &out, variable_list grads) {
+  bool recorded = false;
+  if (c10::GradMode::is_enabled())
+    for (const auto &g : out) recorded = recorded || (g.defined() && g.requires_grad());
+  if (!recorded) return grads;
+  struct Refuse : torch::autograd::Node {
+    using Node::Node;
+    variable_list apply(variable_list &&) override {
+      throw std::runtime_error("the row-scaled linears are differentiable once");
+    }
+  };
+  const std::shared_ptr<Refuse> node(new Refuse(torch::autograd::collect_next_edges(out)), torch::autograd::deleteNode);
+  for (auto &g : grads)
+    if (g.defined()) torch::autograd::set_history(g = g.detach(), node);
+  return grads;
+}
+// What a node keeps beside its tensors, in one number.
+enum : int64_t { kActMask = 7, kFlagW32 = 8, kFlagB32 = 16, kFlagBias = 32, kFlagMore = 64 };   // (more: residual, or a)
+int64_t node_flags(int64_t act, const at::Tensor &w, const opt &bias, bool more) {
+  return act | (w.scalar_type() == at::kFloat ? kFlagW32 : 0) | (bias ? kFlagBias : 0) |
+         (bias && bias->scalar_type() == at::kFloat ? kFlagB32 : 0) | (more ? kFlagMore : 0);
+}
+
+struct LinearNode : torch::autograd::Function<LinearNode> {
+  // (the order of the arguments is the order of backward's gradients; a tensor that is not there has no edge)
+  static at::Tensor forward(AutogradContext *ctx, const at::Tensor &x, const at::Tensor &w, const opt &bias, const opt &res,
+                            int64_t act) {
+    const LinearOut o = linear_run(x, w, bias, (int)act, res, act != GPIC_ACT_NONE, current_stream(x));
+    ctx->save_for_backward({x, o.z, o.wq, o.sw});
+    ctx->set_materialize_grads(false);
+    ctx->saved_data["flags"] = node_flags(act, w, bias, res.has_value());
+    return o.y;
+  }
+  static variable_list backward(AutogradContext *ctx, const variable_list &out) {
+    variable_list g(5);
+    if (!out[0].defined()) return g;
+    const variable_list s = ctx->get_saved_variables();
+    const at::Tensor &x = s[0], &z = s[1], &wq = s[2], &sw = s[3];
+    const int64_t f = ctx->saved_data["flags"].toInt();
+    size_t edge = 2;
+    const bool db = f & kFlagBias && ctx->needs_input_grad(edge++), dres = f & kFlagMore && ctx->needs_input_grad(edge);
+    {
+      at::AutoGradMode off(false);
+      const at::Tensor dy = usual(out[0], wq.size(0));
+      const BwdIn in{dy, z, wq, sw, x, (int)(f & kActMask), ctx->needs_input_grad(0), ctx->needs_input_grad(1), db,
+                     (f & kFlagW32) != 0, (f & kFlagB32) != 0};
+      if (in.need_dx || in.need_dw || in.need_db) {
+        Arena m;
+        const BwdParts p = linear_bwd_parts(in, m);
+        m.make_like(dy);
+        if (in.need_dx) g[0] = make(x, x.sizes(), at::kBFloat16);
+        const LinearGrads o = linear_bwd_run(in, p, m, in.need_dx ? ptr<uint16_t>(g[0]) : nullptr, current_stream(dy));
+        g[1] = o.dw;
+        g[2] = o.db;
+      }
+    }
+    if (dres) g[3] = out[0];
+    return once(out, std::move(g));
+  }
+};
+
+struct NormLinearNode : torch::autograd::Function<NormLinearNode> {
+  // (x_new, y), or y alone without a
+  static variable_list forward(AutogradContext *ctx, const at::Tensor &x, const at::Tensor &wn, const at::Tensor &w,
+                               const opt &a, const opt &bias, double eps, int64_t act) {
+    const auto [n, o] = norm_linear_run(x, wn, eps, a, NormIn(), w, bias, (int)act, w.requires_grad(), act != GPIC_ACT_NONE,
+                                        current_stream(x));
+    ctx->save_for_backward({a ? n.xn : x, wn, n.rstd, n.h, o.z, o.wq, o.sw});
+    ctx->set_materialize_grads(false);
+    ctx->saved_data["flags"] = node_flags(act, w, bias, a.has_value());
+    if (a) return {n.xn, o.y};
+    return {o.y};
+  }
+  static variable_list backward(AutogradContext *ctx, const variable_list &out) {
+    variable_list g(7);
+    const int64_t f = ctx->saved_data["flags"].toInt();
+    const bool has_a = f & kFlagMore;
+    const at::Tensor &dxn_ = has_a ? out[0] : at::Tensor(), &dy_ = out[has_a ? 1 : 0];
+    if (!dy_.defined() && !dxn_.defined()) return g;
+    const variable_list s = ctx->get_saved_variables();
+    const at::Tensor &xs = s[0], &wn = s[1], &rstd = s[2], &h = s[3], &z = s[4], &wq = s[5], &sw = s[6];
+    size_t edge = 3;
+    const bool da = has_a && ctx->needs_input_grad(edge++), db = f & kFlagBias && ctx->needs_input_grad(edge);
+    const bool dx = ctx->needs_input_grad(0), dwn = ctx->needs_input_grad(1), below = dx || da || dwn;
+    {
+      at::AutoGradMode off(false);
+      const int64_t K = wq.size(1), M = xs.numel() / K, N = wq.size(0);
+      const at::Tensor dy = dy_.defined() ? usual(dy_, N) : at::zeros({M, N}, xs.options());   // (x_new alone was used)
+      const opt dxn = dxn_.defined() ? opt(usual(dxn_, K)) : std::nullopt;
+      const BwdIn in{dy, z, wq, sw, h, (int)(f & kActMask), below, ctx->needs_input_grad(2), db, (f & kFlagW32) != 0,
+                     (f & kFlagB32) != 0};
+      Arena m;
+      const BwdParts p = linear_bwd_parts(in, m);
+      const size_t bytes = below ? gpic_fp8_rmsnorm_rows_bwd_workspace_bytes(M, K) : 0, dh = below ? m.add(2 * M * K) : 0,
+                   ws = m.add(bytes);
+      m.make_like(dy);
+      void *stream = current_stream(dy);
+      const LinearGrads o = linear_bwd_run(in, p, m, below ? m.at<uint16_t>(dh) : nullptr, stream);
+      g[2] = o.dw;
+      g[4] = o.db;
+      if (below) {
+        const at::Tensor d = make(xs, xs.sizes(), at::kBFloat16), dw = make(xs, {K}, wn.scalar_type());
+        check(gpic_fp8_rmsnorm_rows_bwd(m.at<uint16_t>(dh), u16(dxn), ptr<uint16_t>(xs), wn.data_ptr(), dtype_code(wn),
+                                        ptr<float>(rstd), M, K, ptr<uint16_t>(d), dw.data_ptr(), dtype_code(dw),
+                                        m.at<uint8_t>(ws), bytes, stream),
+              "gpic_fp8_rmsnorm_rows_bwd");
+        if (dx) g[0] = d;
+        if (da) g[3] = d;
+        if (dwn) g[1] = dw;
+      }
+    }
+    return once(out, std::move(g));
+  }
+};
+
+// Whether the backward takes these sizes (linear_bwd_ok's, from the forward's side).
+bool trainable(int64_t M, int64_t N, int64_t K) {
+  return N <= kRowsMaxCast && 2 * M * std::max(N, K) < (int64_t(1) << 31) && K < (1 << 21);
+}
+
+// residual + act(x w^T + bias), x [..., K] bf16, w [N, K], residual [..., N] bf16; a node of the graph where it records
+py::object linear_rows(const at::Tensor &x, const at::Tensor &w, const opt &bias, int act, const opt &res, int dev, handle,
+                       handle stream) {
+  const opt ox = x, ow = w;
+  if (x.dim() < 1 || x.numel() < 1 || !bf16(x, dev) || !row_castable(x, dev) || !rows_weight_ok(w, x.size(-1), dev) ||
+      !bias_ok(bias, w.size(0), dev) || !trainable(x.numel() / x.size(-1), w.size(0), x.size(-1)) ||
+      (res && (!bf16(*res, dev) || res->dim() != x.dim() || res->size(-1) != w.size(0) ||
+               res->sizes().slice(0, x.dim() - 1) != x.sizes().slice(0, x.dim() - 1))))
     return py::none();
-  const int64_t M = dy.size(0), K = wq.size(1);
-  LinearGrads o;
-  at::Tensor dx, dwn;
+  at::Tensor y;
   {
     NoGil no_gil;
-    Arena m;
-    const BwdParts p = linear_bwd_parts(in, m);
-    const size_t bytes = gpic_fp8_rmsnorm_rows_bwd_workspace_bytes(M, K), dh = m.add(2 * M * K), ws = m.add(bytes);
-    m.make_like(dy);
-    o = linear_bwd_run(in, p, m, m.at<uint16_t>(dh), vp(stream));
-    dx = make(xs, xs.sizes(), at::kBFloat16);
-    dwn = make(xs, {K}, wn.scalar_type());
-    check(gpic_fp8_rmsnorm_rows_bwd(m.at<uint16_t>(dh), u16(dxn), ptr<uint16_t>(xs), wn.data_ptr(), dtype_code(wn),
-                                    ptr<float>(rstd), M, K, ptr<uint16_t>(dx), dwn.data_ptr(), dtype_code(dwn),
-                                    m.at<uint8_t>(ws), bytes, vp(stream)),
-          "gpic_fp8_rmsnorm_rows_bwd");
+    if (records({&ox, &ow, &bias, &res})) y = LinearNode::apply(x, w, bias, res, (int64_t)act);
+    else y = linear_run(x, w, bias, act, res, false, vp(stream)).y;
   }
-  return py::make_tuple(dx, dwn, or_none(o.dw), or_none(o.db));
+  return py::cast(y);
+}
+
+// (x_new, act(h w^T + bias)) for the norm of x + a (x_new None without a), x [..., K] bf16
+py::object norm_linear_rows(const at::Tensor &x, const at::Tensor &wn, double eps, const opt &a, const at::Tensor &w,
+                            const opt &bias, int act, int dev, handle, handle stream) {
+  NormIn in;
+  const opt ox = x, own = wn, ow = w, none;
+  if (!norm_ok(x, wn, a, none, none, none, dev, in) || !rows_weight_ok(w, x.size(-1), dev) ||
+      !bias_ok(bias, w.size(0), dev) || !trainable(x.numel() / x.size(-1), w.size(0), x.size(-1)))
+    return py::none();
+  at::Tensor xn, y;
+  {
+    NoGil no_gil;
+    if (records({&ox, &own, &a, &ow, &bias})) {
+      variable_list o = NormLinearNode::apply(x, wn, w, a, bias, eps, (int64_t)act);
+      y = o.back();
+      if (a) xn = o[0];
+    } else {
+      const auto [n, o] = norm_linear_run(x, wn, eps, a, in, w, bias, act, false, false, vp(stream));
+      y = o.y;
+      if (a) xn = n.xn;
+    }
+  }
+  return py::make_tuple(or_none(xn), y);
 }
 
 }  // namespace
@@ -621,8 +778,8 @@ PYBIND11_MODULE(_gpic_host, m) {   // (wrapped: torch's own errors, out of memor
   m.def("norm_rows", torch::wrap_pybind_function(&norm_rows));
   m.def("norm_rows_bwd", torch::wrap_pybind_function(&norm_rows_bwd));
   m.def("gemm_rows", torch::wrap_pybind_function(&gemm_rows));
-  m.def("linear_rows_fwd", torch::wrap_pybind_function(&linear_rows_fwd));
   m.def("linear_rows_bwd", torch::wrap_pybind_function(&linear_rows_bwd));
   m.def("norm_linear_rows_fwd", torch::wrap_pybind_function(&norm_linear_rows_fwd));
-  m.def("norm_linear_rows_bwd", torch::wrap_pybind_function(&norm_linear_rows_bwd));
+  m.def("linear_rows", torch::wrap_pybind_function(&linear_rows));
+  m.def("norm_linear_rows", torch::wrap_pybind_function(&norm_linear_rows));
 }

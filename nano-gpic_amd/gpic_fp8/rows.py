@@ -407,15 +407,10 @@ class _LinearRows(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, w, b, act, residual):
         x2 = x.reshape(-1, x.shape[-1])
-        want_z = act != "none" and any(ctx.needs_input_grad)
-        r2 = None if residual is None else residual.reshape(-1, w.shape[0])
-        r = L.native("linear_rows_fwd", x2, x2, w, b, ACTS[act], r2, want_z)
-        if r is not None:
-            y, z, wq, sw = r
-        else:
-            xq, sx = L.call(tcast_rows_op, x2)
-            wq, sw = L.call(tcast_rows_op, w)
-            y, z = L.call(gemm_rows_op, xq, sx, wq, sw, b, act, r2, None, want_z)
+        xq, sx = L.call(tcast_rows_op, x2)
+        wq, sw = L.call(tcast_rows_op, w)
+        y, z = L.call(gemm_rows_op, xq, sx, wq, sw, b, act, None if residual is None else residual.reshape(-1, w.shape[0]), None,
+                      act != "none" and any(ctx.needs_input_grad))
         ctx.save_for_backward(x2, z, wq, sw)
         ctx.set_materialize_grads(False)
         ctx.act, ctx.wdt, ctx.bdt, ctx.shape = act, w.dtype, None if b is None else b.dtype, x.shape
@@ -468,24 +463,15 @@ class _NormLinearRows(torch.autograd.Function):
         below = any(need[:6])   # a gradient through the norm
         dy2 = dy.reshape(-1, dy.shape[-1]).to(BF)
         dx = da = dgate = dwn = dshift = dscale = None
-        r = None
+        dh, dw, db = _linear_bwd(ctx, dy2, z, wq, sw, h, below, need[7], need[8])
         if below and shift is None:
-            r = L.native("norm_linear_rows_bwd", dy2, dy2, dxn, z, ACTS[ctx.act], wq, sw, h, xs, wn, rstd, need[7], need[8],
-                         ctx.wdt == torch.float32, ctx.bdt == torch.float32)
-        if r is not None:
-            dx, dwn, dw, db = r
+            dx, dwn = L.call(rmsnorm_rows_bwd_op, dh.view(xs.shape), dxn, xs, wn, rstd)
             dwn, da = dwn.to(wn.dtype), dx
-            dw, db = dw if dw is None else dw.to(ctx.wdt), db if db is None else db.to(ctx.bdt)
-        else:
-            dh, dw, db = _linear_bwd(ctx, dy2, z, wq, sw, h, below, need[7], need[8])
-            if below and shift is None:
-                dx, dwn = L.call(rmsnorm_rows_bwd_op, dh.view(xs.shape), dxn, xs, wn, rstd)
-                dwn, da = dwn.to(wn.dtype), dx
-            elif below:
-                dx, da, dg, dwn, dsh, dsc = L.call(res_mod_rmsnorm_bwd_k, dh.view(xs.shape), dxn, xs, a, gate, wn, scale, rstd)
-                dwn = dwn.to(wn.dtype)
-                dshift, dscale = dsh.view(shift.shape).to(shift.dtype), dsc.view(scale.shape).to(scale.dtype)
-                dgate = dg.view(gate.shape).to(gate.dtype) if gate is not None else None
+        elif below:
+            dx, da, dg, dwn, dsh, dsc = L.call(res_mod_rmsnorm_bwd_k, dh.view(xs.shape), dxn, xs, a, gate, wn, scale, rstd)
+            dwn = dwn.to(wn.dtype)
+            dshift, dscale = dsh.view(shift.shape).to(shift.dtype), dsc.view(scale.shape).to(scale.dtype)
+            dgate = dg.view(gate.shape).to(gate.dtype) if gate is not None else None
         out = [dx, da, dgate, dwn, dshift, dscale, None, dw, db, None]
         return tuple(g if n else None for g, n in zip(out, need))
 
@@ -523,6 +509,10 @@ def fp8_linear_rows(x, weight, bias=None, act="none", residual=None, gate=None):
                 raise ValueError("gate needs a RowsWeight")
             if residual is not None and residual.shape != (*x.shape[:-1], weight.shape[0]):
                 raise ValueError(f"residual must be {(*x.shape[:-1], weight.shape[0])}, got {tuple(residual.shape)}")
+            if type(x) in _PLAIN and type(weight) in _PLAIN:   # (the usual form, recorded or not)
+                y = L.native("linear_rows", x, x, weight, bias, ACTS[act], residual)
+                if y is not None:
+                    return y
             return _LinearRows.apply(x, weight, bias, act, residual)
         _no_gradient(x, bias, residual, gate)
         K, N = x.shape[-1], weight.q.shape[0] // (2 if weight.swiglu else 1)
@@ -558,5 +548,9 @@ def fp8_rmsnorm_linear_rows(x, w_norm, eps, weight, bias=None, act="none", a=Non
                 raise ValueError("gate, shift and scale [B, 1, C] need x [B, N, C]")
             if x.shape[-1] > BWD_MAX_C:
                 raise ValueError(f"the modulated norm's backward takes rows of at most {BWD_MAX_C}, got C = {x.shape[-1]}")
+        elif type(x) in _PLAIN and type(weight) in _PLAIN:
+            r = L.native("norm_linear_rows", x, x, w_norm, eps, a, weight, bias, ACTS[act])
+            if r is not None:
+                return (x if a is None else r[0]), r[1]
         out = _NormLinearRows.apply(x, a, gate, w_norm, shift, scale, eps, weight, bias, act)
         return (x, out) if a is None else out

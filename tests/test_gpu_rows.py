@@ -623,3 +623,102 @@ def test_host_module_and_general_form(dev, monkeypatch, act):
     monkeypatch.setattr(L, "native", lambda *a: None)
     got = passes()
     assert len(want) == len(got) and all(torch.equal(p, q) for p, q in zip(want, got))
+
+
+def subsets(n):
+    return [[i >> k & 1 == 1 for k in range(n)] for i in range(1, 1 << n)]
+
+
+def grads_of(outs, dys, leaves, needs):
+    need = [t for t, r in zip(leaves, needs) if r and t is not None]
+    pairs = [(o, d) for o, d in zip(outs, dys) if o.requires_grad]
+    got = iter(torch.autograd.grad([o for o, _ in pairs], need, [d for _, d in pairs], allow_unused=True))
+    return [next(got) if r and t is not None else None for t, r in zip(leaves, needs)]
+
+
+@pytest.mark.parametrize("bias", [False, True])
+@pytest.mark.parametrize("res", [False, True])
+@pytest.mark.parametrize("act", ["none", "gelu_tanh"])
+def test_linear_rows_gradient_of_each_set(dev, bias, res, act):
+    """Every set of leaves that take a gradient, with and without bias and residual: the graph's native node gives the bits
+    of the general Function, which is fed an output's gradient of another layout too."""
+    g = gen(dev)
+    leaves = [randn(g, 2, 9, 64), randn(g, 48, 64, dtype=F32), randn(g, 48) if bias else None,
+              randn(g, 2, 9, 48) if res else None]
+    dy = randn(g, 9, 2, 48).transpose(0, 1)
+    for needs in subsets(4):
+        if not any(r and t is not None for t, r in zip(leaves, needs)):
+            continue
+        x, w, b, r = [t if t is None else t.detach().requires_grad_(n) for t, n in zip(leaves, needs)]
+        y = G.fp8_linear_rows(x, w, b, act, r)
+        y2 = GR._LinearRows.apply(x, w, b, act, r)
+        assert y.grad_fn.name() != y2.grad_fn.name() and torch.equal(y, y2)
+        for p, q in zip(grads_of([y], [dy], [x, w, b, r], needs), grads_of([y2], [dy], [x, w, b, r], needs)):
+            assert (p is None) == (q is None) and (p is None or (torch.equal(p, q) and p.dtype == q.dtype)), needs
+
+
+@pytest.mark.parametrize("bias", [False, True])
+@pytest.mark.parametrize("add", [False, True])
+def test_rmsnorm_linear_rows_gradient_of_each_set(dev, bias, add):
+    g = gen(dev)
+    leaves = [randn(g, 2, 9, 64), randn(g, 64, dtype=F32), randn(g, 48, 64), randn(g, 2, 9, 64) if add else None,
+              randn(g, 48, dtype=F32) if bias else None]
+    dxn, dy = randn(g, 2, 9, 64), randn(g, 2, 9, 48)
+    for needs in subsets(5):
+        if not any(r and t is not None for t, r in zip(leaves, needs)):
+            continue
+        x, wn, w, a, b = [t if t is None else t.detach().requires_grad_(n) for t, n in zip(leaves, needs)]
+        xn, y = G.fp8_rmsnorm_linear_rows(x, wn, 1e-6, w, b, "silu", a)
+        o = GR._NormLinearRows.apply(x, a, None, wn, None, None, 1e-6, w, b, "silu")
+        outs, outs2 = ([xn, y], list(o)) if add else ([y], [o])
+        assert y.grad_fn.name() != outs2[-1].grad_fn.name() and all(torch.equal(p, q) for p, q in zip(outs, outs2))
+        for keep in ([0, 1], [0], [1]) if add else ([0],):   # (both outputs used, or one)
+            dys = [dxn, dy] if add else [dy]
+            args = ([x, wn, w, a, b], needs)
+            o = G.fp8_rmsnorm_linear_rows(x, wn, 1e-6, w, b, "silu", a)
+            p = grads_of([o[i if add else 1] for i in keep], [dys[i] for i in keep], *args)
+            o = GR._NormLinearRows.apply(x, a, None, wn, None, None, 1e-6, w, b, "silu")
+            q = grads_of([o[i] if add else o for i in keep], [dys[i] for i in keep], *args)
+            for i, (s, t) in enumerate(zip(p, q)):
+                assert (s is None) == (t is None) and (s is None or (torch.equal(s, t) and s.dtype == t.dtype)), (needs, keep, i)
+
+
+def test_linear_rows_nodes_in_a_graph(dev):
+    """What a node of the graph owes: a gradient of a gradient is refused (and a recorded first one alone is not), an input
+    changed in place after the forward is refused, checkpointing and hooks work, two backward passes are the same."""
+    from torch.utils.checkpoint import checkpoint
+    g = gen(dev)
+    x, wn, w = randn(g, 5, 64).requires_grad_(), torch.ones(64, device=dev, requires_grad=True), randn(g, 64, 64).requires_grad_()
+    a = randn(g, 5, 64).requires_grad_()
+    calls = [lambda x: G.fp8_linear_rows(x, w, None, "silu"),
+             lambda x: G.fp8_rmsnorm_linear_rows(x, wn, 1e-6, w, None, "silu")[1],
+             lambda x: sum(G.fp8_rmsnorm_linear_rows(x, wn, 1e-6, w, None, "silu", a))]
+    for f in calls:
+        y = f(x)
+        dy = randn(g, *y.shape).requires_grad_()
+        gx, gw = torch.autograd.grad(y, (x, w), dy.detach(), retain_graph=True, create_graph=True)
+        assert not gx.requires_grad
+        rx, rw = torch.autograd.grad(y, (x, w), dy, retain_graph=True, create_graph=True)
+        assert torch.equal(rx, gx) and torch.equal(rw, gw) and rx.requires_grad
+        with pytest.raises(RuntimeError, match="differentiable once"):
+            rx.float().sum().backward()
+        p, q = torch.autograd.grad(checkpoint(f, x, use_reentrant=False), (x, w), dy.detach())
+        assert torch.equal(p, gx) and torch.equal(q, gw)
+        seen = []
+        h = x.register_hook(lambda t: seen.append(t.clone()))
+        y.backward(dy.detach())
+        h.remove()
+        assert torch.equal(seen[0], gx) and torch.equal(x.grad, gx) and torch.equal(w.grad, gw)
+        x.grad = w.grad = wn.grad = a.grad = None
+        x2 = x.detach().clone()
+        y = f(x2)
+        x2.add_(1)
+        if f is calls[2]:        # (it keeps x + a, not x)
+            torch.autograd.grad(y, w, dy.detach())
+        else:
+            with pytest.raises(RuntimeError, match="inplace"):
+                torch.autograd.grad(y, w, dy.detach())
+        with pytest.raises(RuntimeError):
+            torch.func.grad(lambda t: f(t).float().sum())(x.detach())
+        with pytest.raises(RuntimeError):
+            torch.func.vmap(f)(x.detach()[None])
