@@ -36,7 +36,8 @@ __device__ __forceinline__ float act_bwd(float z, int act) {
   }
   if (act == 2) {
     const float p = gelu_sig(z);
-    return __builtin_fmaf(z * p * (1.0f - p), __builtin_fmaf(3.0f * kGelu2C3, z * z, kGelu2C), p);
+    // (z^2 bounded: p (1 - p) is 0 long before, and 0 times the overflowed square would be NaN)
+    return __builtin_fmaf(z * p * (1.0f - p), __builtin_fmaf(3.0f * kGelu2C3, __builtin_fminf(z * z, 1e30f), kGelu2C), p);
   }
   return 1.0f;
 }
