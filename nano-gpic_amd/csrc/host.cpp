@@ -1,7 +1,9 @@
 // The host side of the path's calls in one native module (_gpic_host): output allocation and the C-ABI calls of a cast
-// group, a GEMM, a weight gradient, the whole forward or backward of a phase-3 linear, and the row-scaled operators with the
-// forward and backward of their linears, without a Python frame, a ctypes conversion and a tensor constructor for each piece. A linear of a few hundred rows is bound by that host time,
-// not by its kernels (~40 us of Python for 25 us of kernels in a sampler's proj).
+// group, a GEMM, a weight gradient, the whole forward or backward of a phase-3 linear, and the row-scaled operators, their
+// linears as nodes of the autograd graph, without a Python frame, a ctypes conversion and a tensor constructor for each piece.
+// A linear of a few hundred rows is bound by that host time, not by its kernels (~40 us of Python for 25 us of kernels in a
+// sampler's proj; the row-scaled norm and linear of 331 rows, forward and backward, 165 us with Python Functions and 74-114
+// with nodes, for 53 us of kernels).
 //
 // Every function takes tensors of the usual form only (on the current device, contiguous, 16-byte aligned, the types
 // the C ABI takes) and returns None for any other, for which the caller runs its general form. Outputs are ordinary
@@ -252,11 +254,12 @@ bool scales_ok(const opt &s, int64_t n, int dev) {
 }
 uint16_t *u16(const opt &t) { return t ? ptr<uint16_t>(*t) : nullptr; }
 at::Tensor none_of(const at::Tensor &like, at::ScalarType ty) { return make(like, {0}, ty); }
-// Whether a call on these records a gradient: the operators themselves have none, and the general form says so.
+// Whether a call on these records a gradient, or carries a forward-mode one: the operators themselves have none, and the
+// general form says so.
 bool records(std::initializer_list<const opt *> ts) {
-  if (!c10::GradMode::is_enabled()) return false;
+  const bool on = c10::GradMode::is_enabled();
   for (const opt *t : ts)
-    if (*t && (*t)->requires_grad()) return true;
+    if (*t && ((on && (*t)->requires_grad()) || (*t)->_fw_grad(0).defined())) return true;
   return false;
 }
 
@@ -521,8 +524,8 @@ bool linear_bwd_ok(const BwdIn &in, int dev) {
   if (in.dy.dim() != 2 || !bf16(in.dy, dev) || !operand_rows(in.wq, dev)) return false;
   const int64_t M = in.dy.size(0), N = in.dy.size(1), K = in.wq.size(1);
   return M >= 1 && N >= 16 && N % 16 == 0 && N <= kRowsMaxCast && in.wq.size(0) == N && scales_ok(in.sw, N, dev) &&
-         (in.act == GPIC_ACT_NONE || (bf16(in.z, dev) && in.z.sizes() == in.dy.sizes())) && bf16(in.x, dev) &&
-         in.x.numel() == M * K && 2 * M * std::max(N, K) < (int64_t(1) << 31) && K < (1 << 21);
+         (in.act == GPIC_ACT_NONE || (bf16(in.z, dev) && in.z.sizes() == in.dy.sizes())) &&
+         (!in.need_dw || (bf16(in.x, dev) && in.x.numel() == M * K)) && 2 * M * std::max(N, K) < (int64_t(1) << 31) && K < (1 << 21);
 }
 // The parts of a linear's backward in its call's arena, and the bytes of its workspaces.
 struct BwdParts {
@@ -620,6 +623,10 @@ variable_list once(const variable_list &out, variable_list grads) {
     if (g.defined()) torch::autograd::set_history(g = g.detach(), node);
   return grads;
 }
+// Saved tensors come back through the user's hooks, where there are any: on another device, or in another layout.
+void saved_ok(bool ok) {
+  if (!ok) throw std::runtime_error("the row-scaled linears' backward needs the tensors that the forward saved, as they were saved");
+}
 // What a node keeps beside its tensors, in one number.
 enum : int64_t { kActMask = 7, kFlagW32 = 8, kFlagB32 = 16, kFlagBias = 32, kFlagMore = 64 };   // (more: residual, or a)
 int64_t node_flags(int64_t act, const at::Tensor &w, const opt &bias, bool more) {
@@ -650,6 +657,7 @@ struct LinearNode : torch::autograd::Function<LinearNode> {
       const at::Tensor dy = usual(out[0], wq.size(0));
       const BwdIn in{dy, z, wq, sw, x, (int)(f & kActMask), ctx->needs_input_grad(0), ctx->needs_input_grad(1), db,
                      (f & kFlagW32) != 0, (f & kFlagB32) != 0};
+      saved_ok(linear_bwd_ok(in, dy.get_device()));
       if (in.need_dx || in.need_dw || in.need_db) {
         Arena m;
         const BwdParts p = linear_bwd_parts(in, m);
@@ -692,9 +700,10 @@ struct NormLinearNode : torch::autograd::Function<NormLinearNode> {
       at::AutoGradMode off(false);
       const int64_t K = wq.size(1), M = xs.numel() / K, N = wq.size(0);
       const at::Tensor dy = dy_.defined() ? usual(dy_, N) : at::zeros({M, N}, xs.options());   // (x_new alone was used)
-      const opt dxn = dxn_.defined() ? opt(usual(dxn_, K)) : std::nullopt;
+      const opt dxn = dxn_.defined() ? opt(usual(dxn_, K).view(xs.sizes())) : std::nullopt;
       const BwdIn in{dy, z, wq, sw, h, (int)(f & kActMask), below, ctx->needs_input_grad(2), db, (f & kFlagW32) != 0,
                      (f & kFlagB32) != 0};
+      saved_ok(linear_bwd_ok(in, dy.get_device()) && (!below || norm_bwd_ok(M, dxn, xs, wn, rstd, dy.get_device())));
       Arena m;
       const BwdParts p = linear_bwd_parts(in, m);
       const size_t bytes = below ? gpic_fp8_rmsnorm_rows_bwd_workspace_bytes(M, K) : 0, dh = below ? m.add(2 * M * K) : 0,

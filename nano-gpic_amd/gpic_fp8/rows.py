@@ -11,8 +11,9 @@ and over them
     fp8_linear_rows(x, weight, ...)               a linear with activation and residual
     fp8_rmsnorm_linear_rows(x, w_norm, ..., weight, ...)   the norm feeding one
 
-A row's scale needs no maximum over the chip, so one token's norm or linear is a short launch, and a token's result does not
-depend on the others of its batch. With weights that rows_weight has cast once (a sampler, a server) a linear is the cast of
+A row's scale needs no maximum over the chip, so one token's norm or linear is a short launch, and a token's bytes do not
+depend on the others of its batch (nor its linear on their values; their number chooses the GEMM's tiles, whose sums differ in
+the last bits). With weights that rows_weight has cast once (a sampler, a server) a linear is the cast of
 x and one GEMM; with ordinary weights the two are differentiable: the forward and the dgrad in FP8, the weight's gradient
 in bf16 (a token's scale lies on its reduction), from the bf16 input and the bf16 gradient of z.
 """

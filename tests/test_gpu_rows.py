@@ -378,6 +378,22 @@ def test_act_bwd_differences(dev):
 
 # ------------------------------------------------------------------------------------------------ linears
 
+@pytest.mark.parametrize("act", ["silu", "gelu_tanh"])
+def test_act_bwd_rows_far_values(dev, act):
+    """The activation's derivative where it is 0 or 1 to the last bit, up to the type's largest values, whose square
+    overflows; NaN stays NaN."""
+    z = torch.tensor([30., -300., 1e4, -1e9, 1e18, -1e20, 1e25, -3e38], dtype=BF, device=dev).repeat(2, 2)
+    dy = torch.full_like(z, 3.0)
+    sw = torch.ones(16, device=dev)
+    dz, q, s = G.act_bwd_rows(dy, z, act, sw)
+    assert torch.equal(dz, torch.where(z > 0, dy, torch.zeros_like(dy)))
+    ref = torch.where(z > 0, 3.0, 0.0).double()
+    assert ((R.deq(q, s) - ref).abs() <= 2 ** -24 * ref).all()   # (448 times the rounded 3 / 448)
+    z[1, 5] = float("nan")
+    dz, q, s = G.act_bwd_rows(dy, z, act, sw)
+    assert torch.isnan(dz[1, 5]) and torch.isnan(s[1]) and torch.isfinite(s[0]) and torch.isfinite(dz).sum() == 31
+
+
 def rel(x, ref):
     return (torch.linalg.norm(x.double() - ref) / torch.linalg.norm(ref)).item()
 
@@ -710,6 +726,22 @@ def test_linear_rows_nodes_in_a_graph(dev):
         h.remove()
         assert torch.equal(seen[0], gx) and torch.equal(x.grad, gx) and torch.equal(w.grad, gw)
         x.grad = w.grad = wn.grad = a.grad = None
+        with torch.autograd.graph.save_on_cpu():
+            y = f(x)
+        p, q = torch.autograd.grad(y, (x, w), dy.detach())
+        assert torch.equal(p, gx) and torch.equal(q, gw)
+        for back in (lambda t: t.cpu(), lambda t: t.t().contiguous().t() if t.dim() == 2 else t):   # (hooks that change them)
+            with torch.autograd.graph.saved_tensors_hooks(lambda t: t.clone(), back):
+                y = f(x)
+            with pytest.raises(RuntimeError, match="as they were saved"):
+                torch.autograd.grad(y, (x, w), dy.detach())
+        with torch.autograd.detect_anomaly(check_nan=False):
+            p, q = torch.autograd.grad(f(x), (x, w), dy.detach())
+        assert torch.equal(p, gx) and torch.equal(q, gw)
+        with torch.autograd.forward_ad.dual_level():
+            for leaf in (x.detach(), x):
+                with pytest.raises((RuntimeError, NotImplementedError)):
+                    f(torch.autograd.forward_ad.make_dual(leaf, torch.ones_like(leaf)))
         x2 = x.detach().clone()
         y = f(x2)
         x2.add_(1)
@@ -722,3 +754,7 @@ def test_linear_rows_nodes_in_a_graph(dev):
             torch.func.grad(lambda t: f(t).float().sum())(x.detach())
         with pytest.raises(RuntimeError):
             torch.func.vmap(f)(x.detach()[None])
+    xn, y = G.fp8_rmsnorm_linear_rows(x, wn, 1e-6, w, None, "silu", a)   # (an output that is kept, changed in place)
+    xn.mul_(2)
+    with pytest.raises(RuntimeError, match="inplace"):
+        y.float().sum().backward()
