@@ -146,6 +146,8 @@ __device__ __forceinline__ int64_t team_row_in(int first) {
   return ((int64_t)blockIdx.x - first) * R + (R == 1 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x / T));
 }
 
+// Bound by memory: [32768 x 4096] bf16 71 us, 5.7 TB/s of the 3 bytes an element; [8192 x 1024] fp32 8.2 us, 5.1 TB/s (a copy of
+// 1 GiB: 5.1).
 // One matrix by the first `blocks` workgroups, another (a linear's input and its weight: rows of one length) by the rest.
 // (kKind: one bf16 matrix, one fp32, or two: instances of their own, as for the norm, whose plain one the test and the second
 // set of arguments cost 6%)
@@ -175,6 +177,8 @@ struct NormRowsArgs {
   float eps;
 };
 
+// Bound by memory, one row alone by the launch: x_new and the bytes of [32768 x 1024] with residual, gate, shift and scale, 7 bytes
+// an element, 46 us, 5.1 TB/s; one row 2.6 us.
 // A team takes `chunk` rows one after another: the row after the current one is requested before the current one's sums, and
 // w, and gate, shift and scale while the batch entry stays the same, are kept in registers.
 template <int T, int kV, bool kRes, bool kMod, bool kWeight>
@@ -356,6 +360,8 @@ __device__ __forceinline__ void store_column_partials(float (&D)[kV][8], float *
   }
 }
 
+// Bound by memory: 7 bytes an element, [16384 x 7168] with db and the weight's transpose 166 us, 5.2 TB/s of what it moves; the
+// derivative's arithmetic passes under the loads ([6592 x 4096] 39 us).
 // The epilogue's backward, and beside it, in workgroups of their own, the transposed bytes of the weight that the dgrad reads
 // (independent work: a launch less in the chain). kDb: each thread also sums its columns' dz, as rounded, over its rows, for
 // column_sum_kernel: the same order in every run.
@@ -455,6 +461,8 @@ struct NormBwdRowsArgs {
   int C, w32;
 };
 
+// Bound by memory: 8 bytes an element with dx_new, [16381 x 4096] 96 us, 5.7 TB/s, and 5 us for the column sums; [6528 x 1024] 11
+// and 4.
 // The rows of a workgroup in their order, each thread's columns' dw in registers; a workgroup's teams are added in their
 // order, then the workgroups in theirs (column_sum_kernel): the same sums in every run.
 template <int T, int kV>
@@ -554,7 +562,11 @@ __global__ __launch_bounds__(256) void column_sum_kernel(const float *__restrict
 
 // ------------------------------------------------------------------------------------------- host side
 
-// Calls f(T, kV) with the team and the steps for rows of C elements (C <= 8 T kV).
+// Calls f(T, kV) with the team and the steps for rows of C elements (C <= 8 T kV): the smallest team that holds a row in four
+// steps, since a wave alone needs no barrier. us, norm / cast / norm's backward: rows of 1024 by a wave 9.8 / 4.8 / 14.1 (6528
+// rows), by four 12.8 / 7.0 / 18.8; 4096 by four waves 19.8 / 71.4 / 102 (4096, 32768, 16381 rows), by one 30.2 / 79.2 / 114; 8192
+// by four 22.3 / 33 / 51.0 (2048, 8192, 4096 rows), by sixteen 28.3 / 36.4 / 56.1. (Rows of 2048 by four waves cost the cast 3%
+// and the norm 6%.)
 template <class F>
 static void with_team(int64_t C, F f) {
   typedef std::integral_constant<int, 64> W;
@@ -572,7 +584,8 @@ static void with_team(int64_t C, F f) {
   else f(S(), V4());
 }
 
-// The same for the epilogue's backward, which holds dy, z, db and two rows' loads: at most two steps a thread up to 16384.
+// The same for the epilogue's backward, which holds dy, z, db and two rows' loads: at most two steps a thread up to 16384. us,
+// with db, against twice the steps: [6592 x 2048] 24.0 / 27.2, [16384 x 7168] 165 / 184, [8192 x 8192] 99 / 113.
 template <class F>
 static void with_short_team(int64_t C, F f) {
   typedef std::integral_constant<int, 1> V1;
@@ -593,19 +606,27 @@ static unsigned row_blocks(int64_t rows, int teams) {
 
 static bool dtype_ok(int d) { return d == GPIC_DTYPE_BF16 || d == GPIC_DTYPE_F32; }
 
-// Rows a team of the norm takes: one while the workgroups do not fill the device twice over, then up to 8.
-static int norm_chunk(int64_t rows, int teams) {
-  const int64_t c = std::min<int64_t>(rows / (2048 * teams), 8);
+// Rows a team of the norm takes one after another: one while the workgroups would not fill the device, then up to `most`, by what
+// it keeps from row to row. Short runs spread a launch's stores over its time, long ones read shift, scale and gate less often.
+// us, at most 1 / 2 / 4 / 8 rows: [16384 x 4096] with a residual alone 82.4 / 85.0 / 88.4 / 92.6, with residual, gate, shift and
+// scale 96.4 / 89.1 / 89.3 / 94.2, with shift and scale alone 48.5 / 42.4 / 39.7 / 39.8, with neither 34.7 / 33.9 / 33.8 / 35.5;
+// [32768 x 1024] in that order 35.2 / 36.6 / 37.5 / 37.5, 39.5 / 38.0 / 39.0 / 39.0, 25.3 / 22.2 / 22.4 / 22.5 and four times 20
+// (the rule's worst: [8192 x 8192] with all of them 95.3 at 2 against 92.7).
+static int norm_chunk(int64_t rows, int teams, int most) {
+  const int64_t c = std::min<int64_t>(rows / (2048 * teams), most);
   return (int)std::max<int64_t>(std::max<int64_t>(c, 1), rows / ((int64_t)teams << 21) + 1);
 }
 
-// Workgroups of the epilogue's backward: with db each leaves a partial row of it.
+// Workgroups of the epilogue's backward: with db each leaves a partial row of it, so no more than fill the device. us, 256 / 512 /
+// 768 / 1024: [6592 x 4096] 66 / 43.2 / 39.6 / 40.7, [32768 x 4096] 322 / 198 / 185 / 180, [16384 x 7168] (512 threads each)
+// 191 / 165 / 196 / 172. Without db a workgroup a row: [32768 x 4096] 166, 2048 workgroups 189.
 static int act_bwd_blocks(int64_t rows, int64_t N, bool db) {
   const int teams = N <= 1024 ? 4 : 1;
   return (int)std::min<int64_t>((rows + teams - 1) / teams, db ? N <= 4096 ? 768 : 512 : kMaxRowBlocks);
 }
 
-// Workgroups of the norm's backward: each leaves a partial row of dw.
+// Workgroups of the norm's backward: each leaves a partial row of dw. us, 256 / 512 / 1024: [6528 x 1024] 15.5 / 14.1 / 16.0,
+// [16381 x 4096] 113 / 102 / 111, [4096 x 8192] 57 / 51 / 61.
 static int norm_bwd_blocks(int64_t rows, int64_t C) {
   const int teams = C <= 2048 ? 4 : 1;
   return (int)std::min<int64_t>((rows + teams - 1) / teams, 512);
@@ -675,7 +696,7 @@ int gpic_fp8_rmsnorm_rows(const uint16_t *x, int64_t ldx, const uint16_t *a, int
     constexpr int t = decltype(T)::value, v = decltype(V)::value;
     if constexpr (t * v * 8 <= kMaxNormC) {
       NormRowsArgs q = p;
-      q.chunk = norm_chunk(rows, kWG<t> / t);
+      q.chunk = norm_chunk(rows, kWG<t> / t, a ? (gate || shift ? 2 : 1) : shift ? 4 : 2);
       const unsigned g = (unsigned)((rows + (int64_t)q.chunk * (kWG<t> / t) - 1) / ((int64_t)q.chunk * (kWG<t> / t)));
       auto pick = [&](auto two) {
         constexpr bool w = decltype(two)::value;
