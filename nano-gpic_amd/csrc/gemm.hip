@@ -1189,7 +1189,8 @@ __global__ __launch_bounds__(256) void splitk_rows_kernel(const float *__restric
   }
 }
 
-// Few rows (kF blocks of 16): the weight's bytes bound it, each read once. A workgroup takes kC tiles of 16 columns, its kW waves
+// Few rows (kF blocks of 16): the weight's bytes bound it, each read once. A workgroup takes kC tiles of 16 columns (of kF row
+// blocks: small products of more rows come here too, for the K tiles of a small tile follow one another), its kW waves
 // every kW-th K tile, straight from memory into the MFMA's operand registers (lane l: row l & 15, 32 bytes at K 32 (l / 16):
 // whole 128-byte lines), and the waves' sums are added in their order through LDS. Rows past M read the last row. Device time in
 // a graph, us, the weight not in L2 (the small tiles in brackets): one row [4096 x 1024] 3.4 (4.8), [1024 x 8192] 7.4 (26),
@@ -1203,14 +1204,14 @@ __global__ __launch_bounds__(64 * kW) void gemm_few_kernel(const uint8_t *__rest
   __shared__ __attribute__((aligned(16))) f4a_t red[kW][kF * kC][64];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int n0 = blockIdx.x * (16 * kC), row = lane & 15, kl = 32 * (lane >> 4);
+  const int n0 = blockIdx.x * (16 * kC), m0 = blockIdx.y * (16 * kF), row = lane & 15, kl = 32 * (lane >> 4);
   const uint8_t *a[kF], *b[kC];
 #pragma unroll
   for (int c = 0; c < kC; c++) b[c] = B + min(n0 + 16 * c + row, N - 1) * ldb + kl;   // (N % 16 == 0: a whole tile past it)
 #pragma unroll
-  for (int f = 0; f < kF; f++) a[f] = A + min(16 * f + row, M - 1) * lda + kl;
+  for (int f = 0; f < kF; f++) a[f] = A + min(m0 + 16 * f + row, M - 1) * lda + kl;
   // the epilogue's operands (wave w: tile w, the lanes that will store), requested before the weight's bytes
-  const int em = 16 * (wave % kF) + row, en = n0 + 16 * (wave / kF) + 4 * (lane >> 4);
+  const int em = m0 + 16 * (wave % kF) + row, en = n0 + 16 * (wave / kF) + 4 * (lane >> 4);
   const bool stores = wave < kF * kC && !(lane & 16) && em < M && en < N;
   float sb8[8], b8[8], sa_m = 1.0f;
   u32x4 res{0u, 0u, 0u, 0u};
@@ -1487,21 +1488,27 @@ static int launch_gemm_rows(const uint8_t *A, int64_t lda, const uint8_t *B, int
     if (!aligned16(ws)) return GPIC_EALIGN;
     P = static_cast<float *>(ws);
   }
-  if (M <= 32) {
-    // Waves by K, so that each has a few K tiles. N = 4096, us with 4 / 16: one row, K 1024 3.7 / 4.0, 2048 4.3 / 4.6, 4096 6.8 / 6.1,
-    // 8192 11.6 / 8.8; 32 rows 4.5 / 4.8, 6.1 / 6.1, 9.5 / 8.9, 15.2 / 15.0 (8 lies between).
+  // Few rows, and products of so few tiles that each CU has one at most: there the waves that share K beat the small tiles, whose
+  // K tiles follow one another. us, this / the other classes: [64 x 64 x 4096] 7.9 / 17.2, [256 x 256 x 8192] 13.9 / 22.6,
+  // [128 x 1024 x 2048] 5.4 / 6.7, [512 x 256 x 512] 3.5 / 3.7; past one a CU [64 x 4096 x 2048] 8.7 / 6.8; past K = 8192 level.
+  // Two column tiles a workgroup, which reads A's rows half as often: where few rows still leave one for every CU ([8192 x 8192],
+  // two tiles / one: 32 rows 20.1 us / 27.5, 8 rows 16.9 / 17.4, one 16.1 / 15.2; with fewer columns the workgroups are missed:
+  // 32 rows [4096 x 4096] 10.8 / 9.1), and up to one a CU where the other classes' K loops are longest ([128 x 1536 x 6144] 14.3 /
+  // 18.9, [64 x 4096 x 8192] 19.0 / 23.7, [256 x 1024 x 6144] 14.5 / 21.8; K = 5120 12.4 / 12.1).
+  const int64_t cus = num_cus(), few_tiles = (M + 31) / 32 * (N / 16);
+  const bool one = few_tiles <= cus && K <= 8192, two = few_tiles <= 2 * cus && K > 5120 && K <= 8192;
+  if (M <= 32 || one || two) {
+    // Waves by K, so that each has a few K tiles. N = 4096, us with 4 / 16: one row, K 1024 3.7 / 4.0, 2048 4.3 / 4.6, 4096 6.8 /
+    // 6.1, 8192 11.6 / 8.8; 32 rows 4.5 / 4.8, 6.1 / 6.1, 9.5 / 8.9, 15.2 / 15.0 (8 lies between).
     auto few = [&](auto rows, auto cols) {
       constexpr int f = decltype(rows)::value, c = decltype(cols)::value;
       auto *k = K <= 2048 ? gemm_few_kernel<f, c, 4> : gemm_few_kernel<f, c, 16>;
-      k<<<(unsigned)((N + 16 * c - 1) / (16 * c)), K <= 2048 ? 256 : 1024, 0, st>>>(A, lda, B, ldb, C, ldc, (int)M, (int)N, (int)K,
-                                                                                     ep);
+      k<<<dim3((unsigned)((N + 16 * c - 1) / (16 * c)), (unsigned)((M + 16 * f - 1) / (16 * f))), K <= 2048 ? 256 : 1024, 0, st>>>(
+          A, lda, B, ldb, C, ldc, (int)M, (int)N, (int)K, ep);
     };
     typedef std::integral_constant<int, 1> One;
     typedef std::integral_constant<int, 2> Two;
-    // Two column tiles a workgroup, which reads A's rows half as often, where that still leaves one for every CU and there are
-    // rows to read ([8192 x 8192], two tiles / one: 32 rows 20.1 us / 27.5, 8 rows 16.9 / 17.4, one 16.1 / 15.2; with fewer columns
-    // the workgroups are missed: 32 rows [4096 x 4096] 10.8 / 9.1).
-    const bool wide = M > 4 && N >= 32 * num_cus();
+    const bool wide = M > 32 ? !one : M > 4 && N >= 32 * cus;
     if (M <= 16) wide ? few(One(), Two()) : few(One(), One());
     else wide ? few(Two(), Two()) : few(Two(), One());
     return (int)hipGetLastError();

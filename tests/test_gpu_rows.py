@@ -201,6 +201,9 @@ SHAPES = [(1, 16, 16), (1, 64, 128), (1, 4096, 1024), (2, 48, 400), (15, 80, 528
           (32, 256, 4112), (33, 64, 64), (33, 1040, 1008), (100, 96, 144), (257, 528, 1024), (512, 1024, 1024),
           (512, 272, 8192), (1000, 2064, 272), (2049, 1024, 1024), (4097, 2064, 528), (700, 4112, 2064),
           (2500, 512, 8208), (6592, 4096, 256), (9000, 1040, 400)]
+# more rows than 32 in few tiles of 16 columns: one a workgroup, two; and the small tiles past them
+SHAPES += [(33, 16, 16), (45, 208, 8176), (250, 512, 2064), (1000, 112, 400), (2048, 16, 2048), (8190, 16, 48), (64, 4080, 5632),
+           (1021, 240, 8112), (130, 1520, 6160), (333, 1040, 272), (700, 2064, 400), (1500, 2064, 400)]
 
 
 @pytest.mark.parametrize("M,N,K", SHAPES)
@@ -230,7 +233,8 @@ def test_gemm_rows_exact(dev, M, N, K):
 
 @pytest.mark.parametrize("act", ["none", "silu", "gelu_tanh", "swiglu"])
 @pytest.mark.parametrize("M,N,K", [(1, 4096, 1024), (1, 32, 16), (5, 96, 272), (31, 512, 4096), (64, 160, 48), (300, 1024, 1024),
-                                   (2049, 1056, 1024), (4100, 2080, 528), (520, 1024, 8192)])
+                                   (2049, 1056, 1024), (4100, 2080, 528), (520, 1024, 8192), (205, 96, 272), (130, 1536, 6160),
+                                   (335, 1056, 272)])
 def test_gemm_rows_epilogue(dev, M, N, K, act):
     g = gen(dev, N + K)
     a, sa = R.rowq(randn(g, M, K))
@@ -248,7 +252,7 @@ def test_gemm_rows_epilogue(dev, M, N, K, act):
         assert torch.equal(y, G.fp8_gemm_rows(a, sa, b, sb, kw.get("bias"), act, kw.get("res"), kw.get("gate")))
 
 
-@pytest.mark.parametrize("M,N,K", [(3, 64, 64), (300, 512, 512), (5000, 2048, 528), (700, 1024, 8192)])
+@pytest.mark.parametrize("M,N,K", [(3, 64, 64), (300, 512, 512), (5000, 2048, 528), (700, 1024, 8192), (100, 256, 4112)])
 def test_gemm_rows_keeps_z(dev, M, N, K):
     g = gen(dev, M)
     a, sa, b, sb = (t.to(dev) for t in (*R.rowq(randn(g, M, K)), *R.rowq(randn(g, N, K, std=K ** -0.5))))
@@ -276,7 +280,7 @@ def test_gemm_rows_strides_and_empty(dev):
 
 @pytest.mark.parametrize("M,N,K,act", [(20, 96, 64, "none"), (300, 96, 512, "silu"), (4099, 1040, 256, "none"),
                                        (4099, 1056, 256, "swiglu"), (9000, 2064, 400, "gelu_tanh"), (9001, 2080, 384, "swiglu"),
-                                       (700, 1040, 8192, "silu")])
+                                       (700, 1040, 8192, "silu"), (90, 96, 2064, "swiglu"), (100, 2080, 5136, "silu")])
 def test_gemm_rows_strided_residual_and_gate(dev, M, N, K, act):
     """A residual that is a column range ending with its storage, a gate whose rows change within and between the waves' 64
     rows, with and without z, in every tile class."""
