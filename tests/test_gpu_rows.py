@@ -762,3 +762,65 @@ def test_linear_rows_nodes_in_a_graph(dev):
     xn.mul_(2)
     with pytest.raises(RuntimeError, match="inplace"):
         y.float().sum().backward()
+
+
+def test_linear_rows_inference_mode_and_threads(dev):
+    """Under inference mode, and from four threads at once, each on a stream of its own: the bits of a call alone."""
+    import threading
+    g = gen(dev)
+    x, a, wn = randn(g, 70, 256), randn(g, 70, 256), torch.ones(256, device=dev)
+    w, w2 = randn(g, 512, 256, std=1 / 16), randn(g, 256, 512, std=1 / 22)
+
+    def step(train):
+        leaves = [t.detach().requires_grad_(train) for t in (x, a, wn, w, w2)]
+        X, A, WN, W, W2 = leaves
+        xn, h = G.fp8_rmsnorm_linear_rows(X, WN, 1e-6, W, None, "gelu_tanh", A)
+        y = G.fp8_linear_rows(h, W2, None, "none", xn)
+        return [y.detach(), *torch.autograd.grad(y, leaves, x)] if train else [y]
+
+    want = step(True)
+    with torch.inference_mode():
+        (y,) = step(False)
+        assert y.is_inference() and torch.equal(y, want[0])
+        q, s = G.tcast_rows(x)
+        assert q.is_inference() and torch.equal(u8(q), u8(G.tcast_rows(x)[0]))
+    torch.cuda.synchronize()
+    bad = []
+
+    def work():
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                for _ in range(10):
+                    got = step(True)
+                    torch.cuda.current_stream().synchronize()
+                    bad.extend(i for i, (p, q) in enumerate(zip(got, want)) if not torch.equal(p, q))
+        except Exception as e:   # noqa: BLE001 (reported by the thread that waits)
+            bad.append(e)
+    threads = [threading.Thread(target=work) for _ in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not bad
+
+
+def test_linear_rows_past_32_bits(dev):
+    """A linear whose output has more than 2^31 bytes, and its gradients: the last rows, and the sums over all."""
+    M, K, N = 140000, 64, 8192
+    g = gen(dev)
+    x, w, b = (randn(g, *s).requires_grad_() for s in ((M, K), (N, K), (N,)))
+    y = G.fp8_linear_rows(x, w, b, "silu")
+    dy = randn(g, N, std=0.1).expand(M, N)
+    gx, gw, gb = torch.autograd.grad(y, (x, w, b), dy)
+    with torch.no_grad():
+        (xq, sx), (wq, sw) = G.tcast_rows(x), G.tcast_rows(w)
+        X, W = R.deq(xq, sx), R.deq(wq, sw)
+        dw, db = torch.zeros(N, K, dtype=torch.float64, device=dev), torch.zeros(N, dtype=torch.float64, device=dev)
+        for i in range(0, M, 10000):
+            z = X[i:i + 10000] @ W.t() + b.double()
+            dz = dy[i:i + 10000].double() * R.dact(z.to(BF).double(), "silu")
+            dw += dz.t() @ x[i:i + 10000].double()
+            db += dz.sum(0)
+        assert rel(y[-1000:], R.act(z, "silu")[-1000:]) < 1e-2 and rel(gw, dw) < 1e-2 and rel(gb, db) < 1e-2
+        dq, sd = R.rowq((dz[-1000:]).float() * sw)
+        assert rel(gx[-1000:], R.deq(dq.to(dev), sd.to(dev)) @ wq.double()) < 1e-2
