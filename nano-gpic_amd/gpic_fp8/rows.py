@@ -501,6 +501,10 @@ def fp8_linear_rows(x, weight, bias=None, act="none", residual=None, gate=None):
     weight a RowsWeight (rows_weight): forward only, with act="swiglu" (N / 2 columns) and gate as well."""
     serving = isinstance(weight, RowsWeight)
     _check_linear(x, weight, act, not serving)
+    if serving and type(x) in _PLAIN:
+        y = L.native("linear_served", x, x, weight.q, weight.s, bias, ACTS[act], residual, gate)
+        if y is not None:
+            return y
     with _no_autocast():
         x = x.to(BF)
         if residual is not None:
@@ -532,6 +536,10 @@ def fp8_rmsnorm_linear_rows(x, w_norm, eps, weight, bias=None, act="none", a=Non
     or a alone, or neither, or shift and scale alone (then C <= 2048)."""
     serving = isinstance(weight, RowsWeight)
     _check_linear(x, weight, act, not serving)
+    if serving and type(x) in _PLAIN:
+        r = L.native("norm_linear_served", x, x, w_norm, eps, a, gate, shift, scale, weight.q, weight.s, bias, ACTS[act])
+        if r is not None:
+            return (x if a is None else r[0]), r[1]
     with _no_autocast():
         x = x.to(BF)
         if a is not None:

@@ -824,3 +824,34 @@ def test_linear_rows_past_32_bits(dev):
         assert rel(y[-1000:], R.act(z, "silu")[-1000:]) < 1e-2 and rel(gw, dw) < 1e-2 and rel(gb, db) < 1e-2
         dq, sd = R.rowq((dz[-1000:]).float() * sw)
         assert rel(gx[-1000:], R.deq(dq.to(dev), sd.to(dev)) @ wq.double()) < 1e-2
+
+
+@pytest.mark.parametrize("shape", [(256,), (1, 256), (2, 3, 5, 256), (40, 256)])
+def test_served_linears_native_and_general(dev, monkeypatch, shape):
+    """Linears on a RowsWeight: the native call gives the general form's bits, and what neither takes is refused."""
+    g = gen(dev)
+    x, a, wn = randn(g, *shape), randn(g, *shape), 1 + 0.1 * torch.randn(256, generator=g, device=dev)
+    M = x.numel() // 256
+    w, w12 = G.rows_weight(randn(g, 96, 256)), G.rows_weight(randn(g, 192, 256), "swiglu")
+    b, b12, res = randn(g, 96), randn(g, 192, dtype=F32), randn(g, *shape[:-1], 96)
+    gate = randn(g, 2 if M % 2 == 0 else 1, 1, 192).chunk(2, dim=-1)[1]
+
+    def calls():
+        out = [G.fp8_linear_rows(x, w, b, "gelu_tanh", res, gate), G.fp8_linear_rows(x, w), G.fp8_linear_rows(x, w, None, "silu", res),
+               G.fp8_linear_rows(x, w12, b12, "swiglu", res, gate), G.fp8_linear_rows(x.float(), w12, None, "swiglu")]
+        if len(shape) > 1:
+            out += [*G.fp8_rmsnorm_linear_rows(x, wn, 1e-6, w, b, "silu"), *G.fp8_rmsnorm_linear_rows(x, wn, 1e-6, w12, b12, "swiglu", a)]
+        return out
+    for r in (res[..., :80], res.reshape(1, *res.shape)):
+        with pytest.raises(ValueError, match="residual"):
+            G.fp8_linear_rows(x, w, None, "none", r)
+    with pytest.raises(ValueError):
+        G.fp8_linear_rows(x, w, None, "none", res, gate.repeat(M + 1, 1, 1))
+    with pytest.raises(ValueError, match="RowsWeight"):
+        G.fp8_linear_rows(x.requires_grad_(), w)
+    x.requires_grad_(False)
+    want = calls()
+    assert all(y.shape == (*shape[:-1], 96) for y in want[:5])
+    monkeypatch.setattr(L, "native", lambda *a: None)
+    got = calls()
+    assert len(want) == len(got) and all(torch.equal(p, q) for p, q in zip(want, got))

@@ -226,6 +226,8 @@ def test_host_module_takes_no_cpu_tensors():
     assert h.gemm_rows(q, n, q, n, n, 0, n, n, False, 0, 0, 0) is None
     assert h.linear_rows(x, w, n, 0, n, 0, 0, 0) is None
     assert h.norm_linear_rows(x, v, 1e-6, n, w, n, 0, 0, 0, 0) is None
+    assert h.linear_served(x, q, v, n, 0, n, n, 0, 0, 0) is None
+    assert h.norm_linear_served(x, v, 1e-6, n, n, n, n, q, v, n, 0, 0, 0, 0) is None
     assert h.linear_rows_bwd(x, x, 0, q, v, x, True, True, True, True, True, 0, 0, 0) is None
     assert h.norm_linear_rows_fwd(x, v, 1e-6, n, n, n, n, w, n, 0, True, True, 0, 0, 0) is None
 
