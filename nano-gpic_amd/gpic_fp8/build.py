@@ -32,7 +32,7 @@ def _host_command(out):
     from torch.utils import cpp_extension
     inc = [f for p in cpp_extension.include_paths() + [sysconfig.get_paths()["include"]] for f in ("-isystem", p)]
     return [CXX, "-O2", "-std=c++17", "-fPIC", "-shared", "-Wall", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}",
-            "-D__HIP_PLATFORM_AMD__", "-isystem", os.path.join(os.path.dirname(os.path.dirname(HIPCC)), "include"), *inc,
+            "-D__HIP_PLATFORM_AMD__", "-isystem", os.path.join(cpp_extension.ROCM_HOME or "/opt/rocm", "include"), *inc,
             "-o", out, os.path.join(CSRC, "host.cpp"), *[f"-L{p}" for p in cpp_extension.library_paths()],
             "-lc10", "-lc10_hip", "-ltorch_cpu", "-ltorch_python", f"-L{HERE}", "-l:libgpic_fp8.so", "-Wl,-rpath,$ORIGIN"]
 
