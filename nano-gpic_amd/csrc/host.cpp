@@ -406,13 +406,14 @@ py::object norm_rows(const at::Tensor &x, const at::Tensor &w, double eps, const
 
 py::object gemm_rows(const at::Tensor &a, const opt &sa, const at::Tensor &b, const opt &sb, const opt &bias, int act,
                      const opt &res, const opt &gate, bool want_z, int dev, handle, handle stream) {
+  const opt oa = a, ob = b;
   if (!operand_rows(a, dev) || !operand_rows(b, dev) || a.size(1) != b.size(1)) return py::none();
   const int64_t M = a.size(0), K = a.size(1), N = b.size(0), No = act == GPIC_ACT_SWIGLU ? N / 2 : N;
   GemmIn g{ptr<uint8_t>(a), ptr<uint8_t>(b), sa ? ptr<float>(*sa) : nullptr, sb ? ptr<float>(*sb) : nullptr, M, N, K,
            &bias, act, u16(res)};
   if (M < 1 || N < 16 || N % (act == GPIC_ACT_SWIGLU ? 32 : 16) || !scales_ok(sa, M, dev) || !scales_ok(sb, N, dev) ||
       !bias_ok(bias, N, dev) || (res && (!bf16(*res, dev) || res->dim() != 2 || res->size(0) != M || res->size(1) != No)) ||
-      !mod_ok(gate, No, 0, M, dev, g.gate) || records({&sa, &sb, &bias, &res, &gate}))
+      !mod_ok(gate, No, 0, M, dev, g.gate) || records({&oa, &sa, &ob, &sb, &bias, &res, &gate}))
     return py::none();
   at::Tensor y, z;
   {
@@ -795,8 +796,9 @@ at::Tensor served_out(const at::Tensor &x, const at::Tensor &wq, int act) {
 // residual + gate act(x w^T + bias), x [..., K] bf16
 py::object linear_served(const at::Tensor &x, const at::Tensor &wq, const at::Tensor &sw, const opt &bias, int act,
                          const opt &res, const opt &gate, int dev, handle, handle stream) {
-  const opt ox = x, osw = sw;
-  if (!served_ok(x, wq, sw, bias, act, dev) || !bf16(x, dev) || !row_castable(x, dev) || records({&ox, &osw, &bias, &res, &gate}))
+  const opt ox = x, owq = wq, osw = sw;
+  if (!served_ok(x, wq, sw, bias, act, dev) || !bf16(x, dev) || !row_castable(x, dev) ||
+      records({&ox, &owq, &osw, &bias, &res, &gate}))
     return py::none();
   const int64_t K = x.size(-1), M = x.numel() / K, N = wq.size(0), No = act == GPIC_ACT_SWIGLU ? N / 2 : N;
   GemmIn g{nullptr, ptr<uint8_t>(wq), nullptr, ptr<float>(sw), M, N, K, &bias, act, u16(res)};
@@ -826,9 +828,9 @@ py::object norm_linear_served(const at::Tensor &x, const at::Tensor &wn, double 
                               const opt &shift, const opt &scale, const at::Tensor &wq, const at::Tensor &sw, const opt &bias,
                               int act, int dev, handle, handle stream) {
   NormIn in;
-  const opt ox = x, own = wn, osw = sw;
+  const opt ox = x, own = wn, owq = wq, osw = sw;
   if (!norm_ok(x, wn, a, gate, shift, scale, dev, in) || !served_ok(x, wq, sw, bias, act, dev) ||
-      records({&ox, &own, &a, &gate, &shift, &scale, &osw, &bias}))
+      records({&ox, &own, &a, &gate, &shift, &scale, &owq, &osw, &bias}))
     return py::none();
   const int64_t K = x.size(-1), M = x.numel() / K, N = wq.size(0);
   at::Tensor y;

@@ -519,7 +519,7 @@ def fp8_linear_rows(x, weight, bias=None, act="none", residual=None, gate=None):
                 if y is not None:
                     return y
             return _LinearRows.apply(x, weight, bias, act, residual)
-        _no_gradient(x, bias, residual, gate)
+        _no_gradient(x, weight.q, weight.s, bias, residual, gate)
         K, N = x.shape[-1], weight.q.shape[0] // (2 if weight.swiglu else 1)
         if residual is not None:
             if residual.shape != (*x.shape[:-1], N):
@@ -545,7 +545,7 @@ def fp8_rmsnorm_linear_rows(x, w_norm, eps, weight, bias=None, act="none", a=Non
         if a is not None:
             a = a.to(BF)
         if serving:
-            _no_gradient(x, w_norm, bias, a, gate, shift, scale)
+            _no_gradient(x, w_norm, weight.q, weight.s, bias, a, gate, shift, scale)
             xn, _, q, s, _ = L.call(rmsnorm_rows_op, x, w_norm, eps, a, gate, shift, scale)
             y = L.call(gemm_rows_op, q.view(-1, x.shape[-1]), s, weight.q, weight.s, bias, act)[0]
             return (x if a is None else xn), y.view(*x.shape[:-1], y.shape[-1])

@@ -855,3 +855,22 @@ def test_served_linears_native_and_general(dev, monkeypatch, shape):
     monkeypatch.setattr(L, "native", lambda *a: None)
     got = calls()
     assert len(want) == len(got) and all(torch.equal(p, q) for p, q in zip(want, got))
+
+
+def test_operands_that_take_a_gradient(dev):
+    """A gradient asked of the GEMM through any of its operands is an error, not a silent loss, also through the e4m3 ones."""
+    g = gen(dev)
+    a, b = randn(g, 4, 64).to(E4), randn(g, 32, 64).to(E4)
+    ins = [a, torch.ones(4, device=dev), b, torch.ones(32, device=dev), randn(g, 32), randn(g, 4, 32), randn(g, 1, 32)]
+    for i in range(len(ins)):
+        t = [v.detach().requires_grad_(k == i) for k, v in enumerate(ins)]
+        y = G.fp8_gemm_rows(*t[:5], "none", t[5], t[6])
+        with pytest.raises(RuntimeError):
+            y.float().sum().backward()
+        with torch.no_grad():
+            assert not G.fp8_gemm_rows(*t[:5], "none", t[5], t[6]).requires_grad
+    for w in (G.RowsWeight(b.detach().requires_grad_(), ins[3], False), G.RowsWeight(b, ins[3].detach().requires_grad_(), False)):
+        with pytest.raises(ValueError, match="RowsWeight"):
+            G.fp8_linear_rows(randn(g, 4, 64), w)
+        with pytest.raises(ValueError, match="RowsWeight"):
+            G.fp8_rmsnorm_linear_rows(randn(g, 4, 64), torch.ones(64, device=dev), 1e-6, w)

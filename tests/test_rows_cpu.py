@@ -242,3 +242,13 @@ def test_public_calls_on_fake_tensors():
         assert G.rmsnorm_rows_bwd(e(3, 64), None, e(3, 64), e(64), e(3, dt=F32))[1].shape == (64,)
         assert G.fp8_gemm_rows(q, s, e(32, 64, dt=E4), e(32, dt=F32), act="swiglu").shape == (6, 16)
         assert G.act_bwd_rows(e(3, 64), e(3, 64), "silu", e(64, dt=F32))[1].dtype == E4
+
+
+def test_served_weights_that_take_a_gradient(no_gpu_check):
+    z = lambda *s, dt=BF: torch.zeros(*s, dtype=dt)  # noqa: E731
+    q, s = z(32, 64, dt=F32).to(E4), torch.ones(32)
+    for w in (G.RowsWeight(q.clone().requires_grad_(), s, False), G.RowsWeight(q, s.clone().requires_grad_(), False)):
+        with pytest.raises(ValueError, match="RowsWeight"):
+            G.fp8_linear_rows(z(4, 64), w)
+        with pytest.raises(ValueError, match="RowsWeight"):
+            G.fp8_rmsnorm_linear_rows(z(4, 64), torch.ones(64), 1e-6, w)
