@@ -804,7 +804,7 @@ py::object linear_served(const at::Tensor &x, const at::Tensor &wq, const at::Te
   GemmIn g{nullptr, ptr<uint8_t>(wq), nullptr, ptr<float>(sw), M, N, K, &bias, act, u16(res)};
   if ((res && (!bf16(*res, dev) || res->dim() != x.dim() || res->size(-1) != No ||
                res->sizes().slice(0, x.dim() - 1) != x.sizes().slice(0, x.dim() - 1))) ||
-      !mod_ok(gate, No, 0, M, dev, g.gate))
+      !mod_ok(gate, No, x.dim() > 2 ? x.size(0) : 0, M, dev, g.gate))
     return py::none();
   at::Tensor y;
   {

@@ -498,7 +498,8 @@ def _no_gradient(*tensors):
 def fp8_linear_rows(x, weight, bias=None, act="none", residual=None, gate=None):
     """residual + gate act(x weight^T + bias), x [..., K] -> [..., N] bf16, with row-scaled e4m3 operands. weight [N, K]:
     differentiable (the forward and the dgrad in FP8, the weight's gradient in bf16; act none, silu or gelu_tanh; no gate).
-    weight a RowsWeight (rows_weight): forward only, with act="swiglu" (N / 2 columns) and gate as well."""
+    weight a RowsWeight (rows_weight): forward only, with act="swiglu" (N / 2 columns) and gate as well: [B, 1, N] for x
+    [B, ..., K], or one row for all; for x [M, K] any number of rows that divides M."""
     serving = isinstance(weight, RowsWeight)
     _check_linear(x, weight, act, not serving)
     if serving and type(x) in _PLAIN:
@@ -525,6 +526,8 @@ def fp8_linear_rows(x, weight, bias=None, act="none", residual=None, gate=None):
             if residual.shape != (*x.shape[:-1], N):
                 raise ValueError(f"residual must be {(*x.shape[:-1], N)}, got {tuple(residual.shape)}")
             residual = residual.reshape(-1, N)
+        if gate is not None and x.dim() > 2 and gate.numel() not in (N, x.shape[0] * N):
+            raise ValueError(f"gate has {gate.numel() // N} rows of {N} for a batch of {x.shape[0]}")
         q, s = L.call(tcast_rows_op, x.reshape(-1, K))
         y = L.call(gemm_rows_op, q, s, weight.q, weight.s, bias, act, residual, gate)[0]
         return y.view(*x.shape[:-1], N)

@@ -874,3 +874,24 @@ def test_operands_that_take_a_gradient(dev):
             G.fp8_linear_rows(randn(g, 4, 64), w)
         with pytest.raises(ValueError, match="RowsWeight"):
             G.fp8_rmsnorm_linear_rows(randn(g, 4, 64), torch.ones(64, device=dev), 1e-6, w)
+
+
+def test_gate_rows_follow_the_batch(dev, monkeypatch):
+    """A gate of a linear on a RowsWeight: one row, or x's batch's; for a 2-D x any number that divides its rows."""
+    g = gen(dev)
+    x, w, gates = randn(g, 2, 6, 64), G.rows_weight(randn(g, 32, 64)), randn(g, 12, 1, 32)
+    z = G.fp8_linear_rows(x, w).double()
+    for native in (True, False):
+        if not native:
+            monkeypatch.setattr(L, "native", lambda *a: None)
+        for n in (3, 4, 6, 12):
+            with pytest.raises(ValueError, match="gate has"):
+                G.fp8_linear_rows(x, w, gate=gates[:n])
+        with pytest.raises(ValueError, match="gate has"):
+            G.fp8_linear_rows(x.view(1, 12, 64), w, gate=gates[:2])
+        for n in (1, 2, 3, 4, 6, 12):
+            y = G.fp8_linear_rows(x.view(12, 64), w, gate=gates[:n])
+            ref = z.view(12, 32) * gates[:n].double().view(n, 32).repeat_interleave(12 // n, 0)
+            assert rel(y, ref) < 2 * R.UBF
+            if n <= 2:
+                assert torch.equal(G.fp8_linear_rows(x, w, gate=gates[:n]).view(12, 32), y)

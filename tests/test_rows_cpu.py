@@ -252,3 +252,11 @@ def test_served_weights_that_take_a_gradient(no_gpu_check):
             G.fp8_linear_rows(z(4, 64), w)
         with pytest.raises(ValueError, match="RowsWeight"):
             G.fp8_rmsnorm_linear_rows(z(4, 64), torch.ones(64), 1e-6, w)
+
+
+def test_gate_rows_follow_the_batch(no_gpu_check):
+    z = lambda *s, dt=BF: torch.zeros(*s, dtype=dt)  # noqa: E731
+    w = G.RowsWeight(z(32, 64, dt=F32).to(E4), torch.ones(32), False)
+    for x, gate in ((z(2, 3, 64), z(3, 1, 32)), (z(2, 3, 64), z(6, 32)), (z(1, 6, 64), z(2, 1, 32)), (z(2, 3, 4, 64), z(6, 32))):
+        with pytest.raises(ValueError, match="gate has"):
+            G.fp8_linear_rows(x, w, None, "none", None, gate)
