@@ -672,8 +672,8 @@ int gpic_fp8_rmsnorm_rows(const uint16_t *x, int64_t ldx, const uint16_t *a, int
                           float *rstd, uint8_t *q, float *s, const void *wt, int wt_dtype, int64_t N, uint8_t *wq, float *sw,
                           void *stream) {
   status_scope();
-  if (rows < 0 || C <= 0 || ntok <= 0 || (gate && !a) || !shift != !scale) return GPIC_EINVAL;
-  if (rows > 0 && (!x || !w || !rstd || !q || !s || (a && !xn))) return GPIC_EINVAL;
+  if (rows < 0 || C <= 0 || ntok <= 0 || !shift != !scale) return GPIC_EINVAL;
+  if (rows > 0 && (!x || !w || !rstd || !q || !s || (a && !xn) || (gate && !a))) return GPIC_EINVAL;   // (no rows: null)
   if (!dtype_ok(w_dtype)) return GPIC_EDTYPE;
   if (C % 8 || C > kMaxNormC || rows >= (int64_t(1) << 31) || rows % ntok || ldx % 8 || ldx < C || (a && (lda % 8 || lda < C)) ||
       (gate && (sg % 8 || sg < C)) || (shift && (ssh % 8 || ssh < C || ssc % 8 || ssc < C)))

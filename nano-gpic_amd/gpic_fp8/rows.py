@@ -67,7 +67,7 @@ def _vec(t, C, batch, rows, name):
         raise ValueError(f"{name} must have {C} columns, got {tuple(t.shape)}")
     t = t.reshape(-1, C)
     B = t.shape[0]
-    if B != 1 and (B != batch if batch is not None else B == 0 or rows % B):
+    if B != 1 and (B != batch if batch is not None else rows % B if B else rows):
         raise ValueError(f"{name} has {B} rows for a batch of {batch if batch is not None else rows}")
     if t.dtype != BF:
         t = t.to(BF)

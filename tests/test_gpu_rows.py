@@ -895,3 +895,28 @@ def test_gate_rows_follow_the_batch(dev, monkeypatch):
             assert rel(y, ref) < 2 * R.UBF
             if n <= 2:
                 assert torch.equal(G.fp8_linear_rows(x, w, gate=gates[:n]).view(12, 32), y)
+
+
+@pytest.mark.parametrize("B,N", [(0, 3), (2, 0), (0, 0)])
+def test_no_rows(dev, B, N):
+    """An empty batch, and entries without tokens, with a block's gate, shift and scale: outputs without rows, zero gradients."""
+    g = gen(dev)
+    leaves = [randn(g, *s) for s in ((B, N, 64), (64,), (32, 64), (32,), (B, N, 64), (B, 1, 64), (B, 1, 64), (B, 1, 64))]
+    w, w12, res = G.rows_weight(leaves[2]), G.rows_weight(randn(g, 64, 64), "swiglu"), randn(g, B, N, 32)
+    x, wn, _, b, a, gate, shift, scale = leaves
+    for kw in (dict(), dict(a=a), dict(a=a, gate=gate), dict(shift=shift, scale=scale), dict(a=a, gate=gate, shift=shift, scale=scale)):
+        xn, h, q, s, rstd = G.rmsnorm_rows(x, wn, 1e-6, want_h=True, **kw)
+        assert h.shape == q.shape == (B, N, 64) and s.numel() == rstd.numel() == 0 and xn.numel() == 0
+        for weight, act in ((w, "silu"), (w12, "swiglu")):
+            xn, y = G.fp8_rmsnorm_linear_rows(x, wn, 1e-6, weight, None, act, **kw)
+            assert xn.shape == x.shape and y.shape == (B, N, 32)
+            assert G.fp8_linear_rows(x, weight, None, act, res, randn(g, B, 1, 32)).shape == (B, N, 32)
+        if "gate" not in kw or "shift" in kw:
+            t = {k: v.detach().requires_grad_() for k, v in dict(x=x, wn=wn, w=leaves[2], b=b, **kw).items()}
+            xn, y = G.fp8_rmsnorm_linear_rows(t["x"], t["wn"], 1e-6, t["w"], t["b"], "silu", *[t.get(k) for k in ("a", "gate", "shift", "scale")])
+            grads = torch.autograd.grad(xn.float().sum() + y.float().sum(), list(t.values()))
+            assert all(d.shape == v.shape and d.dtype == v.dtype and not d.any() for d, v in zip(grads, t.values()))
+    for rows in (0, 1, 3):   # (x without a batch: any number of modulation rows that divides none)
+        mod = randn(g, rows, 64)
+        assert G.rmsnorm_rows(x.reshape(-1, 64), wn, 1e-6, a.reshape(-1, 64), mod, mod, mod)[2].shape == (0, 64)
+        assert G.fp8_linear_rows(x.reshape(-1, 64), w, gate=randn(g, rows, 32)).shape == (0, 32)

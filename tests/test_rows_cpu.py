@@ -260,3 +260,12 @@ def test_gate_rows_follow_the_batch(no_gpu_check):
     for x, gate in ((z(2, 3, 64), z(3, 1, 32)), (z(2, 3, 64), z(6, 32)), (z(1, 6, 64), z(2, 1, 32)), (z(2, 3, 4, 64), z(6, 32))):
         with pytest.raises(ValueError, match="gate has"):
             G.fp8_linear_rows(x, w, None, "none", None, gate)
+
+
+def test_no_rows_need_no_memory(p):
+    """No rows: their tensors have no memory, and the modulation's may have some."""
+    def f(x=None, a=None, gate=p, sh=p, sc=p, rows=0, xn=None):
+        return L.lib().gpic_fp8_rmsnorm_rows(x, 64, a, 64, gate, 64, p, 1, sh, 64, sc, 64, rows, 1, 64, 1e-6, xn, None, None, None,
+                                             None, None, 0, 0, None, None, None)
+    assert f() == 0 and f(gate=None) == 0 and f(gate=None, sh=None, sc=None) == 0 and f(sh=None) == EINVAL
+    assert f(x=p, rows=4) == EINVAL
