@@ -701,14 +701,22 @@ struct NormLinearNode : torch::autograd::Function<NormLinearNode> {
     const at::Tensor &xs = s[0], &wn = s[1], &rstd = s[2], &h = s[3], &z = s[4], &wq = s[5], &sw = s[6];
     size_t edge = 3;
     const bool da = has_a && ctx->needs_input_grad(edge++), db = f & kFlagBias && ctx->needs_input_grad(edge);
-    const bool dx = ctx->needs_input_grad(0), dwn = ctx->needs_input_grad(1), below = dx || da || dwn;
+    const bool dx = ctx->needs_input_grad(0), dwn = ctx->needs_input_grad(1), dw = ctx->needs_input_grad(2),
+               below = dx || da || dwn;
     {
       at::AutoGradMode off(false);
       const int64_t K = wq.size(1), M = xs.numel() / K, N = wq.size(0);
-      const at::Tensor dy = dy_.defined() ? usual(dy_, N) : at::zeros({M, N}, xs.options());   // (x_new alone was used)
       const opt dxn = dxn_.defined() ? opt(usual(dxn_, K).view(xs.sizes())) : std::nullopt;
-      const BwdIn in{dy, z, wq, sw, h, (int)(f & kActMask), below, ctx->needs_input_grad(2), db, (f & kFlagW32) != 0,
-                     (f & kFlagB32) != 0};
+      if (!dy_.defined()) {   // (x_new alone was used: its gradient as it is, and zeros that no value of h or z can spoil)
+        if (dx) g[0] = *dxn;
+        if (da) g[3] = *dxn;
+        if (dwn) g[1] = at::zeros({K}, dxn->options().dtype(wn.scalar_type()));
+        if (dw) g[2] = at::zeros({N, K}, dxn->options().dtype(f & kFlagW32 ? at::kFloat : at::kBFloat16));
+        if (db) g[4] = at::zeros({N}, dxn->options().dtype(f & kFlagB32 ? at::kFloat : at::kBFloat16));
+        return once(out, std::move(g));
+      }
+      const at::Tensor dy = usual(dy_, N);
+      const BwdIn in{dy, z, wq, sw, h, (int)(f & kActMask), below, dw, db, (f & kFlagW32) != 0, (f & kFlagB32) != 0};
       saved_ok(linear_bwd_ok(in, dy.get_device()) && (!below || norm_bwd_ok(M, dxn, xs, wn, rstd, dy.get_device())));
       Arena m;
       const BwdParts p = linear_bwd_parts(in, m);
@@ -720,14 +728,14 @@ struct NormLinearNode : torch::autograd::Function<NormLinearNode> {
       g[2] = o.dw;
       g[4] = o.db;
       if (below) {
-        const at::Tensor d = make(xs, xs.sizes(), at::kBFloat16), dw = make(xs, {K}, wn.scalar_type());
+        const at::Tensor d = make(xs, xs.sizes(), at::kBFloat16), dn = make(xs, {K}, wn.scalar_type());
         check(gpic_fp8_rmsnorm_rows_bwd(m.at<uint16_t>(dh), u16(dxn), ptr<uint16_t>(xs), wn.data_ptr(), dtype_code(wn),
-                                        ptr<float>(rstd), M, K, ptr<uint16_t>(d), dw.data_ptr(), dtype_code(dw),
+                                        ptr<float>(rstd), M, K, ptr<uint16_t>(d), dn.data_ptr(), dtype_code(dn),
                                         m.at<uint8_t>(ws), bytes, stream),
               "gpic_fp8_rmsnorm_rows_bwd");
         if (dx) g[0] = d;
         if (da) g[3] = d;
-        if (dwn) g[1] = dw;
+        if (dwn) g[1] = dn;
       }
     }
     return once(out, std::move(g));

@@ -457,10 +457,22 @@ class _NormLinearRows(torch.autograd.Function):
         xs, a, gate, wn, shift, scale, rstd, h, z, wq, sw = ctx.saved_tensors
         dxn, dy = grads if len(grads) == 2 else (None, grads[0])
         need = ctx.needs_input_grad
-        if dy is None:   # (x_new alone was used)
+        if dy is None:
             if dxn is None:
                 return (None,) * 10
-            dy = dxn.new_zeros(*dxn.shape[:-1], wq.shape[0])
+            # x_new alone was used: its gradient as it is, and zeros that no value of h or z can spoil (gate's and a's by the
+            # norm's backward of zero rows, whose dx is dxn)
+            zeros = lambda t, dtype=None: torch.zeros_like(t, dtype=dtype)  # noqa: E731
+            dx = da = dxn.to(BF)
+            dgate = None
+            if gate is not None and (need[1] or need[2]):
+                none = zeros(xs)
+                _, da, dg, *_ = L.call(res_mod_rmsnorm_bwd_k, none, dx, none, a, gate, zeros(wn), zeros(scale), zeros(rstd))
+                dgate = dg.view(gate.shape).to(gate.dtype)
+            return (dx if need[0] else None, da if need[1] else None, dgate if need[2] else None,
+                    *[zeros(t) if n else None for t, n in zip((wn, shift, scale), need[3:6])], None,
+                    zeros(wq, ctx.wdt) if need[7] else None,
+                    sw.new_zeros(wq.shape[0], dtype=ctx.bdt) if need[8] else None, None)
         below = any(need[:6])   # a gradient through the norm
         dy2 = dy.reshape(-1, dy.shape[-1]).to(BF)
         dx = da = dgate = dwn = dshift = dscale = None

@@ -920,3 +920,33 @@ def test_no_rows(dev, B, N):
         mod = randn(g, rows, 64)
         assert G.rmsnorm_rows(x.reshape(-1, 64), wn, 1e-6, a.reshape(-1, 64), mod, mod, mod)[2].shape == (0, 64)
         assert G.fp8_linear_rows(x.reshape(-1, 64), w, gate=randn(g, rows, 32)).shape == (0, 32)
+
+
+@pytest.mark.parametrize("form", ["native", "general", "gated"])
+def test_x_new_alone(dev, form):
+    """Only x_new in the loss: its gradient as it is, and zeros for what the norm and the linear have, also where h is not finite."""
+    g = gen(dev)
+    x, a, wn, w, b = randn(g, 2, 9, 64), randn(g, 2, 9, 64), randn(g, 64), randn(g, 48, 64), randn(g, 48, dtype=F32)
+    x[0, 3, 7], x[1, 2, 0] = math.inf, math.nan
+    mod = randn(g, 2, 1, 3 * 64, std=0.3).chunk(3, -1) if form == "gated" else (None, None, None)
+    leaves = [t if t is None else t.detach().requires_grad_() for t in (x, a, wn, w, b, *mod)]
+    x, a, wn, w, b, gate, shift, scale = leaves
+    if form == "general":
+        xn, y = GR._NormLinearRows.apply(x, a, None, wn, None, None, 1e-6, w, b, "silu")
+    else:
+        xn, y = G.fp8_rmsnorm_linear_rows(x, wn, 1e-6, w, b, "silu", a, gate, shift, scale)
+    dxn = randn(g, 9, 2, 64).transpose(0, 1)
+    need = [t for t in leaves if t is not None]
+    grads = dict(zip(map(id, need), torch.autograd.grad(xn, need, dxn, retain_graph=True)))
+    assert torch.equal(grads[id(x)], dxn)
+    for t in (wn, w, b, shift, scale):
+        if t is not None:
+            assert grads[id(t)].shape == t.shape and grads[id(t)].dtype == t.dtype and not grads[id(t)].any()
+    if gate is None:
+        assert torch.equal(grads[id(a)], dxn)
+    else:
+        assert torch.equal(grads[id(a)], (gate.double() * dxn.double()).to(BF))
+        assert rel(grads[id(gate)], (dxn.double() * a.double()).sum(1, keepdim=True)) < R.UBF
+    for t in need:   # (and each alone)
+        (got,) = torch.autograd.grad(xn, t, dxn, retain_graph=True)
+        assert torch.equal(got, grads[id(t)])
