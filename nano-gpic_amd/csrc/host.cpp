@@ -37,8 +37,10 @@ void check(int status, const char *what) {
                              std::to_string(status) + ")");
 }
 
+// Whether t has memory of its own: a fake tensor, or a subclass that wraps others, has none to read.
+bool has_memory(const at::Tensor &t) { return !t.key_set().has(c10::DispatchKey::Python); }
 bool plain(const at::Tensor &t, int dev) {
-  return t.is_cuda() && t.get_device() == dev && t.layout() == at::kStrided && t.is_contiguous() &&
+  return t.is_cuda() && t.get_device() == dev && has_memory(t) && t.layout() == at::kStrided && t.is_contiguous() &&
          (reinterpret_cast<uintptr_t>(t.data_ptr()) & 15u) == 0;
 }
 bool castable(const at::Tensor &t, int dev) {
@@ -293,7 +295,7 @@ struct Mod {
 bool mod_ok(const opt &t, int64_t C, int64_t batch, int64_t rows, int dev, Mod &m) {
   if (!t) return true;
   const int64_t d = t->dim();
-  if (d < 1 || d > 3 || t->scalar_type() != at::kBFloat16 || !t->is_cuda() || t->get_device() != dev ||
+  if (d < 1 || d > 3 || t->scalar_type() != at::kBFloat16 || !t->is_cuda() || t->get_device() != dev || !has_memory(*t) ||
       t->layout() != at::kStrided || t->size(d - 1) != C || t->stride(d - 1) != 1 || (d == 3 && t->size(1) != 1))
     return false;
   m.B = d == 1 ? 1 : t->size(0);

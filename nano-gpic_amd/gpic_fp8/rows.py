@@ -54,6 +54,13 @@ def _run(op, name, x, *args):
     return L.call(op, *args)
 
 
+def _call(op, *args):
+    """L.call for a linear's own calls; the op itself, with its fake kernel, for tensors without memory of their own."""
+    if torch.compiler.is_compiling() or not any(isinstance(t, torch.Tensor) and type(t) not in _PLAIN for t in args):
+        return L.call(op, *args)
+    return op(*args)
+
+
 def _same_device(dev, **named):
     for name, t in named.items():
         if t is not None and t.device != dev:
@@ -390,17 +397,19 @@ def act_bwd_rows(dy, z, act, sw):
 
 def _linear_bwd(ctx, dy2, z, wq, sw, x2, need_dx, need_dw, need_db):
     """(dx [M, K] bf16, dw, db) of y = act(x w^T + b), each None unless needed."""
-    r = L.native("linear_rows_bwd", dy2, dy2, z, ACTS[ctx.act], wq, sw, x2, need_dx, need_dw, need_db,
-                 ctx.wdt == torch.float32, ctx.bdt == torch.float32)
+    r = None
+    if type(dy2) in _PLAIN:
+        r = L.native("linear_rows_bwd", dy2, dy2, z, ACTS[ctx.act], wq, sw, x2, need_dx, need_dw, need_db,
+                     ctx.wdt == torch.float32, ctx.bdt == torch.float32)
     if r is not None:
         dx, dw, db = r
         return dx, dw if dw is None else dw.to(ctx.wdt), db if db is None else db.to(ctx.bdt)
-    dz, dq, sd, wqt, db = L.call(act_bwd_rows_op, dy2, z, ctx.act, sw, wq if need_dx else None, need_db,
-                                 ctx.bdt == torch.float32)
+    dz, dq, sd, wqt, db = _call(act_bwd_rows_op, dy2, z, ctx.act, sw, wq if need_dx else None, need_db,
+                                ctx.bdt == torch.float32)
     if ctx.act == "none":
         dz = dy2
-    dx = L.call(gemm_rows_op, dq, sd, wqt, None)[0] if need_dx else None
-    dw = L.call(bf16_wgrad, dz, x2, ctx.wdt == torch.float32).to(ctx.wdt) if need_dw else None
+    dx = _call(gemm_rows_op, dq, sd, wqt, None)[0] if need_dx else None
+    dw = _call(bf16_wgrad, dz, x2, ctx.wdt == torch.float32).to(ctx.wdt) if need_dw else None
     return dx, dw, db.to(ctx.bdt) if need_db else None
 
 
@@ -408,10 +417,10 @@ class _LinearRows(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, w, b, act, residual):
         x2 = x.reshape(-1, x.shape[-1])
-        xq, sx = L.call(tcast_rows_op, x2)
-        wq, sw = L.call(tcast_rows_op, w)
-        y, z = L.call(gemm_rows_op, xq, sx, wq, sw, b, act, None if residual is None else residual.reshape(-1, w.shape[0]), None,
-                      act != "none" and any(ctx.needs_input_grad))
+        xq, sx = _call(tcast_rows_op, x2)
+        wq, sw = _call(tcast_rows_op, w)
+        y, z = _call(gemm_rows_op, xq, sx, wq, sw, b, act, None if residual is None else residual.reshape(-1, w.shape[0]), None,
+                     act != "none" and any(ctx.needs_input_grad))
         ctx.save_for_backward(x2, z, wq, sw)
         ctx.set_materialize_grads(False)
         ctx.act, ctx.wdt, ctx.bdt, ctx.shape = act, w.dtype, None if b is None else b.dtype, x.shape
@@ -436,13 +445,15 @@ class _NormLinearRows(torch.autograd.Function):
         C = x.shape[-1]
         train = any(ctx.needs_input_grad)
         want_z = train and act != "none"
-        r = L.native("norm_linear_rows_fwd", x, x, wn, eps, a, gate, shift, scale, w, b, ACTS[act], train, want_z)
+        r = None
+        if type(x) in _PLAIN:
+            r = L.native("norm_linear_rows_fwd", x, x, wn, eps, a, gate, shift, scale, w, b, ACTS[act], train, want_z)
         if r is not None:
             xn, h, rstd, y, z, wq, sw = r
         else:
-            xn, h, hq, sh, rstd = L.call(rmsnorm_rows_op, x, wn, eps, a, gate, shift, scale, train)
-            wq, sw = L.call(tcast_rows_op, w)
-            y, z = L.call(gemm_rows_op, hq.view(-1, C), sh, wq, sw, b, act, None, None, want_z)
+            xn, h, hq, sh, rstd = _call(rmsnorm_rows_op, x, wn, eps, a, gate, shift, scale, train)
+            wq, sw = _call(tcast_rows_op, w)
+            y, z = _call(gemm_rows_op, hq.view(-1, C), sh, wq, sw, b, act, None, None, want_z)
         xs = x if a is None else xn
         ctx.save_for_backward(xs, a if gate is not None else None, gate, wn, shift, scale, rstd,
                               h.view(-1, C) if train else None, z, wq, sw)
@@ -467,7 +478,7 @@ class _NormLinearRows(torch.autograd.Function):
             dgate = None
             if gate is not None and (need[1] or need[2]):
                 none = zeros(xs)
-                _, da, dg, *_ = L.call(res_mod_rmsnorm_bwd_k, none, dx, none, a, gate, zeros(wn), zeros(scale), zeros(rstd))
+                _, da, dg, *_ = _call(res_mod_rmsnorm_bwd_k, none, dx, none, a, gate, zeros(wn), zeros(scale), zeros(rstd))
                 dgate = dg.view(gate.shape).to(gate.dtype)
             return (dx if need[0] else None, da if need[1] else None, dgate if need[2] else None,
                     *[zeros(t) if n else None for t, n in zip((wn, shift, scale), need[3:6])], None,
@@ -478,10 +489,10 @@ class _NormLinearRows(torch.autograd.Function):
         dx = da = dgate = dwn = dshift = dscale = None
         dh, dw, db = _linear_bwd(ctx, dy2, z, wq, sw, h, below, need[7], need[8])
         if below and shift is None:
-            dx, dwn = L.call(rmsnorm_rows_bwd_op, dh.view(xs.shape), dxn, xs, wn, rstd)
+            dx, dwn = _call(rmsnorm_rows_bwd_op, dh.view(xs.shape), dxn, xs, wn, rstd)
             dwn, da = dwn.to(wn.dtype), dx
         elif below:
-            dx, da, dg, dwn, dsh, dsc = L.call(res_mod_rmsnorm_bwd_k, dh.view(xs.shape), dxn, xs, a, gate, wn, scale, rstd)
+            dx, da, dg, dwn, dsh, dsc = _call(res_mod_rmsnorm_bwd_k, dh.view(xs.shape), dxn, xs, a, gate, wn, scale, rstd)
             dwn = dwn.to(wn.dtype)
             dshift, dscale = dsh.view(shift.shape).to(shift.dtype), dsc.view(scale.shape).to(scale.dtype)
             dgate = dg.view(gate.shape).to(gate.dtype) if gate is not None else None
@@ -540,8 +551,8 @@ def fp8_linear_rows(x, weight, bias=None, act="none", residual=None, gate=None):
             residual = residual.reshape(-1, N)
         if gate is not None and x.dim() > 2 and gate.numel() not in (N, x.shape[0] * N):
             raise ValueError(f"gate has {gate.numel() // N} rows of {N} for a batch of {x.shape[0]}")
-        q, s = L.call(tcast_rows_op, x.reshape(-1, K))
-        y = L.call(gemm_rows_op, q, s, weight.q, weight.s, bias, act, residual, gate)[0]
+        q, s = _call(tcast_rows_op, x.reshape(-1, K))
+        y = _call(gemm_rows_op, q, s, weight.q, weight.s, bias, act, residual, gate)[0]
         return y.view(*x.shape[:-1], N)
 
 
@@ -561,8 +572,8 @@ def fp8_rmsnorm_linear_rows(x, w_norm, eps, weight, bias=None, act="none", a=Non
             a = a.to(BF)
         if serving:
             _no_gradient(x, w_norm, weight.q, weight.s, bias, a, gate, shift, scale)
-            xn, _, q, s, _ = L.call(rmsnorm_rows_op, x, w_norm, eps, a, gate, shift, scale)
-            y = L.call(gemm_rows_op, q.view(-1, x.shape[-1]), s, weight.q, weight.s, bias, act)[0]
+            xn, _, q, s, _ = _call(rmsnorm_rows_op, x, w_norm, eps, a, gate, shift, scale)
+            y = _call(gemm_rows_op, q.view(-1, x.shape[-1]), s, weight.q, weight.s, bias, act)[0]
             return (x if a is None else xn), y.view(*x.shape[:-1], y.shape[-1])
         if shift is not None or gate is not None:
             if shift is None or (a is not None and gate is None):

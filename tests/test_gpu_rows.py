@@ -950,3 +950,20 @@ def test_x_new_alone(dev, form):
     for t in need:   # (and each alone)
         (got,) = torch.autograd.grad(xn, t, dxn, retain_graph=True)
         assert torch.equal(got, grads[id(t)])
+
+
+def test_linears_on_fake_tensors(dev):
+    """Forward and backward as a shape pass over a program makes them."""
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    with FakeTensorMode():
+        e = lambda *s, dt=BF: torch.empty(*s, dtype=dt, device=dev)  # noqa: E731
+        x, a, w, b = e(2, 9, 64).requires_grad_(), e(2, 9, 64).requires_grad_(), e(48, 64).requires_grad_(), e(48, dt=F32).requires_grad_()
+        wn, m = e(64, dt=F32).requires_grad_(), [t.requires_grad_() for t in (e(2, 1, 64), e(2, 1, 64), e(2, 1, 64))]
+        y = G.fp8_linear_rows(x, w, b, "silu", e(2, 9, 48))
+        assert [t.shape for t in torch.autograd.grad(y, (x, w, b), e(2, 9, 48))] == [x.shape, w.shape, b.shape]
+        for mod in ((None, None, None), m):
+            leaves = [t for t in (x, wn, w, b, a, *mod) if t is not None]
+            xn, y = G.fp8_rmsnorm_linear_rows(x, wn, 1e-6, w, b, "gelu_tanh", a, *mod)
+            for outs, dys in (((xn, y), (e(2, 9, 64), e(2, 9, 48))), ((y,), (e(2, 9, 48),)), ((xn,), (e(2, 9, 64),))):
+                got = torch.autograd.grad(outs, leaves, dys, retain_graph=True)
+                assert [(t.shape, t.dtype) for t in got] == [(t.shape, t.dtype) for t in leaves]

@@ -269,3 +269,37 @@ def test_no_rows_need_no_memory(p):
                                              None, None, 0, 0, None, None, None)
     assert f() == 0 and f(gate=None) == 0 and f(gate=None, sh=None, sc=None) == 0 and f(sh=None) == EINVAL
     assert f(x=p, rows=4) == EINVAL
+
+
+def test_linears_on_fake_tensors():
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    with FakeTensorMode():
+        e = lambda *s, dt=BF: torch.empty(*s, dtype=dt, device="cuda")  # noqa: E731
+        w, b, wn = e(32, 64).requires_grad_(), e(32), e(64, dt=F32)
+        served = G.RowsWeight(e(32, 64, dt=E4), e(32, dt=F32), True)
+        assert G.fp8_linear_rows(e(2, 3, 64), w, b, "silu", e(2, 3, 32)).shape == (2, 3, 32)
+        assert G.fp8_linear_rows(e(2, 3, 64), served, None, "swiglu", e(2, 3, 16), e(2, 1, 16)).shape == (2, 3, 16)
+        assert [t.shape for t in G.fp8_rmsnorm_linear_rows(e(2, 3, 64), wn, 1e-6, w, b, "silu", e(2, 3, 64))] == [(2, 3, 64), (2, 3, 32)]
+        m = e(2, 1, 6 * 64).chunk(6, -1)
+        for weight, act, n in ((w, "gelu_tanh", 32), (served, "swiglu", 16)):
+            xn, y = G.fp8_rmsnorm_linear_rows(e(2, 3, 64), wn, 1e-6, weight, None, act, e(2, 3, 64), m[2], m[3], m[4])
+            assert xn.shape == (2, 3, 64) and y.shape == (2, 3, n) and y.dtype == BF
+
+
+def test_host_module_takes_no_fake_tensors():
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    with FakeTensorMode():
+        e = lambda *s, dt=BF: torch.empty(*s, dtype=dt, device="cuda")  # noqa: E731
+        x, w, v, q = e(16, 16), e(16, 16), e(16, dt=F32), e(16, 16, dt=E4)
+    h, n = L.host(), None
+    assert h.cast_rows(x, 0, 0, 0) is None
+    assert h.gemm_rows(q, n, q, n, n, 0, n, n, False, 0, 0, 0) is None
+    assert h.linear_served(x, q, v, n, 0, n, n, 0, 0, 0) is None
+    for mod in ((n, n, n), (x, v, v)):   # (the modulation's rows are looked at apart)
+        assert h.norm_rows(x, v, 1e-6, x, *mod, False, 0, 0, 0) is None
+    assert h.norm_rows_bwd(x, n, x, v, v, 0, 0, 0) is None
+    assert h.linear_rows(x, w, n, 0, n, 0, 0, 0) is None
+    assert h.norm_linear_rows(x, v, 1e-6, n, w, n, 0, 0, 0, 0) is None
+    assert h.norm_linear_served(x, v, 1e-6, n, n, n, n, q, v, n, 0, 0, 0, 0) is None
+    assert h.linear_rows_bwd(x, x, 0, q, v, x, True, True, True, True, True, 0, 0, 0) is None
+    assert h.norm_linear_rows_fwd(x, v, 1e-6, n, n, n, n, w, n, 0, True, True, 0, 0, 0) is None
