@@ -614,11 +614,16 @@ at::Tensor usual(const at::Tensor &g, int64_t N) {
 }
 // The current stream of t's device: in a backward the engine has made the forward's current.
 void *current_stream(const at::Tensor &t) { return c10::hip::getCurrentHIPStream(t.get_device()).stream(); }
-// The gradients as they are; in a backward that is itself recorded, as outputs of a node that refuses to be differentiated.
-variable_list once(const variable_list &out, variable_list grads) {
+// The gradients as they are; in a backward that is itself recorded, as outputs of a node that refuses to be differentiated, where
+// an output's gradient is of the graph, else as constants, with a warning where they are not (torch's once_differentiable too
+// returns constants then, without a word: a term made of them is lost from a sum whose other terms have a gradient).
+variable_list once(const variable_list &out, variable_list grads, bool constant = false) {
   bool recorded = false;
-  if (c10::GradMode::is_enabled())
-    for (const auto &g : out) recorded = recorded || (g.defined() && g.requires_grad());
+  if (!c10::GradMode::is_enabled()) return grads;
+  for (const auto &g : out) recorded = recorded || (g.defined() && g.requires_grad());
+  if (!recorded && !constant)
+    TORCH_WARN("the row-scaled linears are differentiable once: the gradients of a backward under create_graph=True do not "
+               "require a gradient, and a loss made of them has none through these linears");
   if (!recorded) return grads;
   struct Refuse : torch::autograd::Node {
     using Node::Node;
@@ -676,8 +681,9 @@ struct LinearNode : torch::autograd::Function<LinearNode> {
         g[2] = o.db;
       }
     }
+    const bool only_res = !(ctx->needs_input_grad(0) || ctx->needs_input_grad(1) || db);
     if (dres) g[3] = out[0];
-    return once(out, std::move(g));
+    return once(out, std::move(g), only_res);
   }
 };
 
@@ -715,7 +721,7 @@ struct NormLinearNode : torch::autograd::Function<NormLinearNode> {
         if (dwn) g[1] = at::zeros({K}, dxn->options().dtype(wn.scalar_type()));
         if (dw) g[2] = at::zeros({N, K}, dxn->options().dtype(f & kFlagW32 ? at::kFloat : at::kBFloat16));
         if (db) g[4] = at::zeros({N}, dxn->options().dtype(f & kFlagB32 ? at::kFloat : at::kBFloat16));
-        return once(out, std::move(g));
+        return once(out, std::move(g), true);
       }
       const at::Tensor dy = usual(dy_, N);
       const BwdIn in{dy, z, wq, sw, h, (int)(f & kActMask), below, dw, db, (f & kFlagW32) != 0, (f & kFlagB32) != 0};

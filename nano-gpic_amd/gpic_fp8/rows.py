@@ -15,8 +15,11 @@ A row's scale needs no maximum over the chip, so one token's norm or linear is a
 depend on the others of its batch (nor its linear on their values; their number chooses the GEMM's tiles, whose sums differ in
 the last bits). With weights that rows_weight has cast once (a sampler, a server) a linear is the cast of
 x and one GEMM; with ordinary weights the two are differentiable: the forward and the dgrad in FP8, the weight's gradient
-in bf16 (a token's scale lies on its reduction), from the bf16 input and the bf16 gradient of z.
+in bf16 (a token's scale lies on its reduction), from the bf16 input and the bf16 gradient of z. They are differentiable
+once: under create_graph=True their gradients are constants, with a warning.
 """
+import functools
+import warnings
 from typing import NamedTuple, Optional
 
 import torch
@@ -413,6 +416,22 @@ def _linear_bwd(ctx, dy2, z, wq, sw, x2, need_dx, need_dw, need_db):
     return dx, dw, db.to(ctx.bdt) if need_db else None
 
 
+def _once(backward):
+    """once_differentiable, with a warning where a backward under create_graph=True returns constants that are none (the last
+    input's gradient, a residual's, is y's own): a term made of them would be lost without a word from a sum whose other terms
+    have a gradient."""
+    inner = once_differentiable(backward)
+
+    @functools.wraps(backward)
+    def call(ctx, *grads):
+        if (torch.is_grad_enabled() and not torch.compiler.is_compiling() and grads[-1] is not None
+                and any(ctx.needs_input_grad[:-1]) and not any(g is not None and g.requires_grad for g in grads)):
+            warnings.warn("the row-scaled linears are differentiable once: the gradients of a backward under create_graph=True "
+                          "do not require a gradient, and a loss made of them has none through these linears")
+        return inner(ctx, *grads)
+    return call
+
+
 class _LinearRows(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, w, b, act, residual):
@@ -427,7 +446,7 @@ class _LinearRows(torch.autograd.Function):
         return y.view(*x.shape[:-1], w.shape[0])
 
     @staticmethod
-    @once_differentiable
+    @_once
     def backward(ctx, dy):
         x2, z, wq, sw = ctx.saved_tensors
         need = ctx.needs_input_grad
@@ -463,7 +482,7 @@ class _NormLinearRows(torch.autograd.Function):
         return y if a is None else (xn, y)
 
     @staticmethod
-    @once_differentiable
+    @_once
     def backward(ctx, *grads):
         xs, a, gate, wn, shift, scale, rstd, h, z, wq, sw = ctx.saved_tensors
         dxn, dy = grads if len(grads) == 2 else (None, grads[0])

@@ -1,5 +1,6 @@
 """The row-scaled operators (gpic_fp8.rows) against their 64-bit statements (rows_ref.py), on the GPU."""
 import math
+import warnings
 
 import pytest
 import torch
@@ -967,3 +968,35 @@ def test_linears_on_fake_tensors(dev):
             for outs, dys in (((xn, y), (e(2, 9, 64), e(2, 9, 48))), ((y,), (e(2, 9, 48),)), ((xn,), (e(2, 9, 64),))):
                 got = torch.autograd.grad(outs, leaves, dys, retain_graph=True)
                 assert [(t.shape, t.dtype) for t in got] == [(t.shape, t.dtype) for t in leaves]
+
+
+@pytest.mark.parametrize("form", ["native", "general"])
+def test_recorded_backward_warns(dev, form, monkeypatch):
+    """A backward that is itself recorded, from an output's gradient that is a constant: what comes back is a constant too (as
+    torch's once_differentiable has it), and a warning says so. The usual backward gives none."""
+    g = gen(dev)
+    x, w, a = (randn(g, *s).requires_grad_() for s in ((5, 64), (64, 64), (5, 64)))
+    wn = torch.ones(64, device=dev, requires_grad=True)
+    if form == "general":
+        monkeypatch.setattr(L, "native", lambda *a: None)
+    res = randn(g, 5, 64).requires_grad_()
+    calls = [lambda: G.fp8_linear_rows(x, w, None, "silu", res), lambda: G.fp8_rmsnorm_linear_rows(x, wn, 1e-6, w, None, "silu")[1],
+             lambda: sum(G.fp8_rmsnorm_linear_rows(x, wn, 1e-6, w, None, "silu", a))]
+    for f in calls:
+        y = f()
+        dy = randn(g, 5, 64)
+        with pytest.warns(UserWarning, match="differentiable once"):
+            gx, gw = torch.autograd.grad(y, (x, w), dy, create_graph=True)
+        with warnings.catch_warnings():
+            warnings.simplefilter("error")
+            px, pw = torch.autograd.grad(y, (x, w), dy, retain_graph=True)
+            rx, rw = torch.autograd.grad(y, (x, w), dy.detach().requires_grad_(), create_graph=True)   # (refused by rx's node)
+        assert all(torch.equal(p, q) for p, q in ((gx, px), (gw, pw), (rx, px), (rw, pw)))
+        with pytest.raises(RuntimeError):
+            rx.float().sum().backward()
+    with warnings.catch_warnings():   # (gradients that are constants: a residual's, and x_new's own)
+        warnings.simplefilter("error")
+        y = G.fp8_linear_rows(x.detach(), w.detach(), None, "silu", res)
+        assert torch.equal(torch.autograd.grad(y, res, dy, create_graph=True)[0], dy)
+        xn, _ = G.fp8_rmsnorm_linear_rows(x, wn, 1e-6, w, None, "silu", a)
+        assert torch.equal(torch.autograd.grad(xn, x, dy, create_graph=True)[0], dy)
