@@ -384,7 +384,8 @@ int gpic_fp8_rmsnorm_rows_bwd(const uint16_t *dh, const uint16_t *dxn, const uin
  * The GEMM of row-scaled operands with bias, activation and residual in its epilogue (fp32, one rounding):
  *   z[m, n] = sa[m] * sb[n] * sum_k A[m, k] * B[n, k] + bias[n];  C = bf16(res + gate * act(z))
  *   A [M, K], B [N, K] e4m3 (row strides lda, ldb); sa [M], sb [N] fp32, or NULL (ones); bias [N] of bias_dtype, or NULL
- *   act: GPIC_ACT_*; SWIGLU (N % 32 == 0) makes N / 2 columns, column 4 i + j of z columns 8 i + j and 8 i + 4 + j
+ *   act: GPIC_ACT_*; SWIGLU (N % 32 == 0) makes N / 2 columns, column 4 i + j of z columns 8 i + j and 8 i + 4 + j (B's rows,
+ *       and sb's and bias's entries with them, in that order)
  *   res: bf16, C's shape (row stride ldr), or NULL; gate: bf16 rows of C's width (stride sg), row m uses row m / ntok
  *       (M % ntok == 0), or NULL
  *   C bf16 (row stride ldc); z: where to keep z as bf16 [M, N] (row stride ldz; for the activation's backward), or NULL

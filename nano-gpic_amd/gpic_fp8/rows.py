@@ -147,7 +147,8 @@ def swiglu_layout(t):
 
 
 def rows_weight(w, act="none"):
-    """A linear's weight [N, K] (w12 [2 H, K] for act="swiglu") cast once, for forward calls."""
+    """A linear's weight [N, K] (w12 [2 H, K] for act="swiglu") cast once, for forward calls. A SwiGLU's rows are reordered
+    (swiglu_layout), so its calls take the bias in that order too: swiglu_layout(b12), made once beside the weight."""
     if w.dim() != 2 or w.shape[0] % 16 or w.shape[1] % 16:
         raise ValueError(f"rows_weight needs w [N, K] with N % 16 == 0 and K % 16 == 0, got {tuple(w.shape)}")
     swiglu = _act(act) == ACTS["swiglu"]
@@ -334,7 +335,8 @@ def _(a, sa, b, sb, bias=None, act="none", residual=None, gate=None, want_z=Fals
 def fp8_gemm_rows(a, sa, b, sb, bias=None, act="none", residual=None, gate=None):
     """a [M, K], b [N, K] e4m3 with their rows' scales sa [M], sb [N] fp32 (None: ones) ->
     y [M, N] bf16 = residual + gate act(sa sb a b^T + bias), in fp32 and rounded once. act: "none", "silu", "gelu_tanh", or
-    "swiglu" (b's rows as rows_weight(w12, "swiglu") lays them out; y [M, N / 2]). bias [N] bf16 or fp32; residual [M, N]
+    "swiglu" (b's rows as rows_weight(w12, "swiglu") lays them out, and sb and bias in the same order: swiglu_layout(b12);
+    y [M, N / 2]). bias [N] bf16 or fp32; residual [M, N]
     bf16; gate [B, 1, N] bf16, B dividing M: a block's gate, one row for M / B rows of y."""
     _act(act)
     return _run(gemm_rows_op, "gemm_rows", a, a, sa, b, sb, bias, act, residual, gate, False)[0]
@@ -541,7 +543,8 @@ def fp8_linear_rows(x, weight, bias=None, act="none", residual=None, gate=None):
     """residual + gate act(x weight^T + bias), x [..., K] -> [..., N] bf16, with row-scaled e4m3 operands. weight [N, K]:
     differentiable (the forward and the dgrad in FP8, the weight's gradient in bf16; act none, silu or gelu_tanh; no gate).
     weight a RowsWeight (rows_weight): forward only, with act="swiglu" (N / 2 columns) and gate as well: [B, 1, N] for x
-    [B, ..., K], or one row for all; for x [M, K] any number of rows that divides M."""
+    [B, ..., K], or one row for all; for x [M, K] any number of rows that divides M. act="swiglu": bias is
+    swiglu_layout(b12), w12's bias in the order of the RowsWeight's rows."""
     serving = isinstance(weight, RowsWeight)
     _check_linear(x, weight, act, not serving)
     if serving and type(x) in _PLAIN:
@@ -578,7 +581,7 @@ def fp8_linear_rows(x, weight, bias=None, act="none", residual=None, gate=None):
 def fp8_rmsnorm_linear_rows(x, w_norm, eps, weight, bias=None, act="none", a=None, gate=None, shift=None, scale=None):
     """(x_new, act(h weight^T + bias)) for x_new, h of rmsnorm_rows(x, w_norm, eps, a, gate, shift, scale); x_new is x without
     a. h goes to the GEMM as the norm's bytes. weight as in fp8_linear_rows; with a gradient: a with gate, shift and scale,
-    or a alone, or neither, or shift and scale alone (then C <= 2048)."""
+    or a alone, or neither, or shift and scale alone (then C <= 2048). act="swiglu": bias is swiglu_layout(b12)."""
     serving = isinstance(weight, RowsWeight)
     _check_linear(x, weight, act, not serving)
     if serving and type(x) in _PLAIN:

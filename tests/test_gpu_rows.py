@@ -1000,3 +1000,23 @@ def test_recorded_backward_warns(dev, form, monkeypatch):
         assert torch.equal(torch.autograd.grad(y, res, dy, create_graph=True)[0], dy)
         xn, _ = G.fp8_rmsnorm_linear_rows(x, wn, 1e-6, w, None, "silu", a)
         assert torch.equal(torch.autograd.grad(xn, x, dy, create_graph=True)[0], dy)
+
+
+@pytest.mark.parametrize("M", [5, 700])
+def test_swiglu_bias_order(dev, M):
+    """w12 and its bias through swiglu_layout and rows_weight: the plain silu(x w1^T + b1) (x w2^T + b2)."""
+    g = gen(dev, M)
+    K, H = 256, 512
+    x, w12, b12 = randn(g, M, K), randn(g, 2 * H, K, std=K ** -0.5), randn(g, 2 * H)
+    w = G.rows_weight(w12, "swiglu")
+    (xq, sx), (wq, sw) = G.tcast_rows(x), G.tcast_rows(w12)
+    z = R.deq(xq, sx) @ R.deq(wq, sw).t() + b12.double()
+    ref = R.act(z[:, :H], "silu") * z[:, H:]
+    assert rel(G.fp8_linear_rows(x, w, G.swiglu_layout(b12), "swiglu"), ref) < 2 * R.UBF
+    assert rel(G.fp8_linear_rows(x, w, b12, "swiglu"), ref) > 0.1   # (in w12's own order it is another bias)
+    assert rel(G.fp8_gemm_rows(xq, sx, w.q, w.s, G.swiglu_layout(b12), "swiglu"), ref) < 2 * R.UBF
+    wn = torch.ones(K, device=dev)
+    _, _, hq, sh, _ = G.rmsnorm_rows(x, wn, 1e-6)
+    z = R.deq(hq, sh) @ R.deq(wq, sw).t() + b12.double()
+    _, y = G.fp8_rmsnorm_linear_rows(x, wn, 1e-6, w, G.swiglu_layout(b12), "swiglu")
+    assert rel(y, R.act(z[:, :H], "silu") * z[:, H:]) < 2 * R.UBF
