@@ -1532,7 +1532,8 @@ static int launch_gemm_rows(const uint8_t *A, int64_t lda, const uint8_t *B, int
   const bool add = ep.res || ep.gate;
   if (P || (!add && !ep.z)) launch(RowsEpiT<false, false>{ep});   // (partials carry no epilogue)
   else if (!add) launch(RowsEpiT<false, true>{ep});
-  else if (!ep.z && (!ep.gate || ep.ntok % kWTM == 0)) launch(RowsEpiT<true, false>{ep});
+  else if (!ep.z && (!ep.gate || ep.ntok % kWTM == 0 || ep.ntok >= M))   // (or one gate row for all: M need not be whole waves)
+    launch(RowsEpiT<true, false>{ep});
   else launch(RowsEpiT<true, true>{ep});
   if (P) {
     const int64_t g = (M * (N / 8) + 255) / 256;

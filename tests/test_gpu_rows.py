@@ -1020,3 +1020,18 @@ def test_swiglu_bias_order(dev, M):
     z = R.deq(hq, sh) @ R.deq(wq, sw).t() + b12.double()
     _, y = G.fp8_rmsnorm_linear_rows(x, wn, 1e-6, w, G.swiglu_layout(b12), "swiglu")
     assert rel(y, R.act(z[:, :H], "silu") * z[:, H:]) < 2 * R.UBF
+
+
+@pytest.mark.parametrize("M,N,K,act", [(4099, 1040, 256, "none"), (4099, 2080, 128, "swiglu"), (16500, 1008, 1024, "silu"),
+                                       (6529, 1024, 1024, "gelu_tanh"), (6529, 1024, 1024, "swiglu")])
+def test_gemm_rows_one_gate_row(dev, M, N, K, act):
+    """One gate row for all rows, whose number no tile divides."""
+    g = gen(dev, M)
+    a, b = randn(g, M, K).to(E4), randn(g, N, K).to(E4)
+    sa, sb = torch.rand(M, generator=g, device=dev) / K ** 0.5, torch.rand(N, generator=g, device=dev) + 0.5
+    No = N // 2 if act == "swiglu" else N
+    gate, res = randn(g, 1, No), randn(g, M, No)
+    for r in (None, res):
+        y = G.fp8_gemm_rows(a, sa, b, sb, None, act, r, gate)
+        ref, bound = R.gemm(a, sa, b, sb, None, act, r, gate)
+        R.within(y, ref, bound)
