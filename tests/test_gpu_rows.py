@@ -1035,3 +1035,58 @@ def test_gemm_rows_one_gate_row(dev, M, N, K, act):
         y = G.fp8_gemm_rows(a, sa, b, sb, None, act, r, gate)
         ref, bound = R.gemm(a, sa, b, sb, None, act, r, gate)
         R.within(y, ref, bound)
+
+
+@pytest.mark.parametrize("mode", ["plain", "res", "mod", "res_gate_mod"])
+@pytest.mark.parametrize("B,N,C,O,act", [(2, 5, 64, 96, "silu"), (3, 100, 896, 512, "gelu_tanh"), (1, 1, 1024, 64, "none")])
+def test_rmsnorm_linear_rows_train_same_bytes(dev, mode, B, N, C, O, act):
+    """The norm feeding a linear: outputs, z and all gradients against 64 bits from the forward's bytes (norm's, weight's and z's
+    roundings as they are, the gradient's row cast and dh's rounding to bf16 made again). An output is off by half a step of bf16,
+    and by another where dh rounds the other way: 2 UBF. The norm's backward without the mean of dt t, its smallest term, is
+    further off than that wherever there are rows to average over."""
+    g = gen(dev, C + N)
+    x, a = randn(g, B, N, C).requires_grad_(), randn(g, B, N, C).requires_grad_()
+    wn, w = randn(g, C, std=0.1).add_(1).requires_grad_(), randn(g, O, C, std=C ** -0.5).requires_grad_()
+    b = randn(g, O).requires_grad_()
+    gate, shift, scale = (randn(g, B, 1, C, std=0.3).requires_grad_() for _ in range(3))
+    kw = dict(a=a if "res" in mode else None, gate=gate if "gate" in mode else None,
+              shift=shift if "mod" in mode else None, scale=scale if "mod" in mode else None)
+    res = kw["a"] is not None
+    xn, y = G.fp8_rmsnorm_linear_rows(x, wn, 1e-6, w, b, act, **kw)
+    names = ["x", "wn", "w", "b"] + [k for k, t in kw.items() if t is not None]
+    leaves = [x, wn, w, b] + [t for t in kw.values() if t is not None]
+    dxn, dy = randn(g, B, N, C, std=0.1), randn(g, B, N, O)
+    got = dict(zip(names, torch.autograd.grad((xn, y) if res else (y,), leaves, (dxn, dy) if res else (dy,))))
+    with torch.no_grad():
+        xn2, h16, hq, sh, _ = G.rmsnorm_rows(x, wn, 1e-6, want_h=True, **kw)
+        wq, sw = G.tcast_rows(w)
+        y2, z = GR.gemm_rows_op(hq.view(-1, C), sh, wq, sw, b, act, None, None, True)
+        rz, bound = R.gemm(hq.view(-1, C), sh, wq, sw, b)
+        R.within(z, rz, bound, "z")
+        R.within(y2, *R.gemm(hq.view(-1, C), sh, wq, sw, b, act), "y")
+        assert torch.equal(y.view(-1, O), y2) and (not res or torch.equal(xn, xn2))
+        xs, M, z, d = xn if res else x, B * N, z.double(), dy.double().view(-1, O)
+        dz = d * R.dact(z, act)
+        dq, sd = R.rowq(dz.float() * sw)
+        dh = (R.deq(dq.to(dev), sd.to(dev)) @ wq.double()).to(BF).double().view(B, N, C)
+        dz16 = dz.to(BF).double()
+        ref = {"w": dz16.t() @ h16.double().view(M, C), "b": dz16.sum(0)}
+        v = xs.double()
+        rstd = (v.square().mean(-1, keepdim=True) + 1e-6) ** -0.5
+        t = v * rstd
+        dn = dh
+        if kw["shift"] is not None:
+            n = wn.double() * t
+            dn = dh * (1 + scale.double())
+            ref["shift"], ref["scale"] = dh.sum(1, keepdim=True), (dh * n).sum(1, keepdim=True)
+        dt = dn * wn.double()
+        ref["wn"] = (dn * t).sum((0, 1))
+        base = dxn.double() if res else 0.0
+        ref["x"] = rstd * (dt - t * (dt * t).mean(-1, keepdim=True)) + base
+        if res:
+            ref["a"] = ref["x"] * (gate.double() if kw["gate"] is not None else 1.0)
+        if kw["gate"] is not None:
+            ref["gate"] = (ref["x"] * a.double()).sum(1, keepdim=True)
+        for k in got:
+            assert rel(got[k], ref[k]) < 2 * R.UBF, (k, rel(got[k], ref[k]))
+        assert set(ref) == set(got) and (M == 1 or rel(rstd * dt + base, ref["x"]) > 3 * R.UBF)
