@@ -57,11 +57,14 @@ def _run(op, name, x, *args):
     return L.call(op, *args)
 
 
-def _call(op, *args):
-    """L.call for a linear's own calls; the op itself, with its fake kernel, for tensors without memory of their own."""
-    if torch.compiler.is_compiling() or not any(isinstance(t, torch.Tensor) and type(t) not in _PLAIN for t in args):
-        return L.call(op, *args)
-    return op(*args)
+def _has_memory(t):
+    """Whether t has memory of its own: a fake tensor, or a subclass that wraps others, has none to read."""
+    return type(t).__torch_dispatch__ is torch.Tensor.__torch_dispatch__
+
+
+def _call(op, t, *args):
+    """L.call for a linear's own calls; the op itself, with its fake kernel, for tensors without memory (t says it for all)."""
+    return L.call(op, t, *args) if torch.compiler.is_compiling() or _has_memory(t) else op(t, *args)
 
 
 def _same_device(dev, **named):
@@ -403,7 +406,7 @@ def act_bwd_rows(dy, z, act, sw):
 def _linear_bwd(ctx, dy2, z, wq, sw, x2, need_dx, need_dw, need_db):
     """(dx [M, K] bf16, dw, db) of y = act(x w^T + b), each None unless needed."""
     r = None
-    if type(dy2) in _PLAIN:
+    if _has_memory(dy2):
         r = L.native("linear_rows_bwd", dy2, dy2, z, ACTS[ctx.act], wq, sw, x2, need_dx, need_dw, need_db,
                      ctx.wdt == torch.float32, ctx.bdt == torch.float32)
     if r is not None:
@@ -467,7 +470,7 @@ class _NormLinearRows(torch.autograd.Function):
         train = any(ctx.needs_input_grad)
         want_z = train and act != "none"
         r = None
-        if type(x) in _PLAIN:
+        if _has_memory(x):
             r = L.native("norm_linear_rows_fwd", x, x, wn, eps, a, gate, shift, scale, w, b, ACTS[act], train, want_z)
         if r is not None:
             xn, h, rstd, y, z, wq, sw = r
