@@ -43,6 +43,7 @@ extern "C" {
 
 #define GPIC_DTYPE_BF16 0
 #define GPIC_DTYPE_F32 1
+#define GPIC_DTYPE_F16 2  /* where an entry point says so */
 
 /* Activations of the row-scaled linears: silu(z) = z sigmoid(z); gelu_tanh(z) = z (1 + tanh(sqrt(2 / pi) (z + 0.044715 z^3))) / 2;
  * SwiGLU: silu of 4 columns times the next 4, in runs of 8 (half as many columns come out). */
@@ -411,6 +412,30 @@ size_t gpic_fp8_act_bwd_rows_workspace_bytes(int64_t rows, int64_t N);
 int gpic_fp8_act_bwd_rows(const uint16_t *dy, int64_t lddy, const uint16_t *z, int64_t ldz, int act, const float *sw,
                           int64_t rows, int64_t N, uint16_t *dz, uint8_t *q, float *s, const uint8_t *wq, int64_t K,
                           uint8_t *wqt, int64_t ldt, void *db, int db_dtype, void *ws, size_t ws_bytes, void *stream);
+
+/*
+ * Layer norm with the residual's addition, beside the root-mean-square norms. No counterpart in the reference, whose norms take no
+ * mean. dtype: x's, a's, xn's and h's type (bf16, fp32 or fp16); w, b [C] of any of them, or NULL (1 and 0).
+ *   x_new = x + a, rounded to dtype -> xn (a != NULL), else x_new = x
+ *   mu = mean(x_new) -> mean [rows];  1 / sqrt(mean((x_new - mu)^2) + eps) -> rstd [rows]  (both or neither; NULL: not kept)
+ *   h = (x_new - mu) rstd w + b, fp32 -> h, rounded to dtype; and (bf16 only) -> q [rows, C], s [rows] by the row cast's rule.
+ *       h or q may be NULL.
+ *   x, a [rows, C] (row strides ldx, lda); outputs contiguous. C % 8 == 0, C <= 16384, rows < 2^31.
+ */
+int gpic_fp8_layer_norm(const void *x, int dtype, int64_t ldx, const void *a, int64_t lda, const void *w, int w_dtype,
+                        const void *b, int b_dtype, int64_t rows, int64_t C, float eps, void *xn, void *h, float *mean,
+                        float *rstd, uint8_t *q, float *s, void *stream);
+
+/*
+ * Its backward, dh the gradient of h and dxn (or NULL) of x_new, xs x_new or x:
+ *   t = (xs - mean) rstd, dt = dh w;  dx = rstd (dt - mean(dt) - t mean(dt t)) + dxn, rounded to dtype (a's gradient too)
+ *   dw = sum over the rows of dh t;  db = sum of dh: fp32 in a fixed order, rounded once (NULL: not asked for)
+ *   every matrix [rows, C] contiguous, of dtype. ws: gpic_fp8_layer_norm_bwd_workspace_bytes(rows, C) bytes, scratch of this call.
+ */
+size_t gpic_fp8_layer_norm_bwd_workspace_bytes(int64_t rows, int64_t C);
+int gpic_fp8_layer_norm_bwd(const void *dh, const void *dxn, const void *xs, int dtype, const void *w, int w_dtype,
+                            const float *mean, const float *rstd, int64_t rows, int64_t C, void *dx, void *dw, int dw_dtype,
+                            void *db, int db_dtype, void *ws, size_t ws_bytes, void *stream);
 
 #ifdef __cplusplus
 }

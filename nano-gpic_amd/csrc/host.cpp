@@ -864,6 +864,106 @@ py::object norm_linear_served(const at::Tensor &x, const at::Tensor &wn, double 
   return py::make_tuple(a ? py::cast(n.xn) : py::none(), y);
 }
 
+// ------------------------------------------------------------------------------------------- layer norm
+
+int dtype_code3(const at::Tensor &t) { return t.scalar_type() == at::kHalf ? GPIC_DTYPE_F16 : dtype_code(t); }
+bool float3(at::ScalarType t) { return t == at::kBFloat16 || t == at::kFloat || t == at::kHalf; }
+// A weight or bias of n elements, or none
+bool vector3_ok(const opt &t, int64_t n, int dev) {
+  return !t || (float3(t->scalar_type()) && plain(*t, dev) && t->dim() == 1 && t->size(0) == n);
+}
+bool layer_norm_ok(const at::Tensor &x, const opt &w, const opt &b, const opt &a, bool bf16_only, int dev) {
+  if (x.dim() < 1 || (bf16_only ? x.scalar_type() != at::kBFloat16 : !float3(x.scalar_type())) || !plain(x, dev)) return false;
+  const int64_t C = x.size(-1);
+  return C > 0 && C % 8 == 0 && C <= kRowsMaxNorm && x.numel() > 0 && vector3_ok(w, C, dev) && vector3_ok(b, C, dev) &&
+         (!a || (a->scalar_type() == x.scalar_type() && a->sizes() == x.sizes() && plain(*a, dev)));
+}
+struct LayerNormOut {
+  at::Tensor xn, h, mean, rstd, q, s;
+};
+LayerNormOut layer_norm_run(const at::Tensor &x, const opt &w, const opt &b, double eps, const opt &a, bool want_h, bool stats,
+                            bool rows, void *stream) {
+  const int64_t C = x.size(-1), M = x.numel() / C;
+  LayerNormOut o;
+  o.xn = a ? make(x, x.sizes(), x.scalar_type()) : none_of(x, x.scalar_type());
+  o.h = want_h ? make(x, x.sizes(), x.scalar_type()) : none_of(x, x.scalar_type());
+  if (stats) o.mean = make(x, {M}, at::kFloat), o.rstd = make(x, {M}, at::kFloat);
+  if (rows) o.q = make(x, x.sizes(), kE4), o.s = make(x, {M}, at::kFloat);
+  check(gpic_fp8_layer_norm(x.data_ptr(), dtype_code3(x), C, a ? a->data_ptr() : nullptr, C, w ? w->data_ptr() : nullptr,
+                            w ? dtype_code3(*w) : 0, b ? b->data_ptr() : nullptr, b ? dtype_code3(*b) : 0, M, C, (float)eps,
+                            a ? o.xn.data_ptr() : nullptr, want_h ? o.h.data_ptr() : nullptr,
+                            stats ? ptr<float>(o.mean) : nullptr, stats ? ptr<float>(o.rstd) : nullptr,
+                            rows ? ptr<uint8_t>(o.q) : nullptr, rows ? ptr<float>(o.s) : nullptr, stream),
+        "gpic_fp8_layer_norm");
+  return o;
+}
+
+// (x_new, h, mean, rstd), the last two empty unless stats; for the op and the autograd Function, which have looked whether a
+// gradient is recorded
+py::object layer_norm(const at::Tensor &x, const opt &w, const opt &b, double eps, const opt &a, bool stats, int dev, handle,
+                      handle stream) {
+  if (!layer_norm_ok(x, w, b, a, false, dev)) return py::none();
+  LayerNormOut o;
+  {
+    NoGil no_gil;
+    o = layer_norm_run(x, w, b, eps, a, true, stats, false, vp(stream));
+    if (!stats) o.mean = none_of(x, at::kFloat), o.rstd = none_of(x, at::kFloat);
+  }
+  return py::make_tuple(o.xn, o.h, o.mean, o.rstd);
+}
+
+// The public call where no gradient is recorded: h, or (x_new, h)
+py::object layer_norm_served(const at::Tensor &x, const opt &w, const opt &b, double eps, const opt &a, int dev, handle,
+                             handle stream) {
+  const opt ox = x;
+  if (!layer_norm_ok(x, w, b, a, false, dev) || records({&ox, &w, &b, &a})) return py::none();
+  LayerNormOut o;
+  {
+    NoGil no_gil;
+    o = layer_norm_run(x, w, b, eps, a, true, false, false, vp(stream));
+  }
+  if (!a) return py::cast(o.h);
+  return py::make_tuple(o.xn, o.h);
+}
+
+py::object layer_norm_rows(const at::Tensor &x, const opt &w, const opt &b, double eps, const opt &a, bool want_h, int dev, handle,
+                           handle stream) {
+  const opt ox = x;
+  if (!layer_norm_ok(x, w, b, a, true, dev) || records({&ox, &w, &b, &a})) return py::none();
+  LayerNormOut o;
+  {
+    NoGil no_gil;
+    o = layer_norm_run(x, w, b, eps, a, want_h, false, true, vp(stream));
+  }
+  return py::make_tuple(o.xn, o.h, o.q, o.s);
+}
+
+py::object layer_norm_bwd(const at::Tensor &dh, const opt &dxn, const at::Tensor &xs, const opt &w, const at::Tensor &mean,
+                          const at::Tensor &rstd, const std::optional<at::ScalarType> &bias_dtype, int dev, handle,
+                          handle stream) {
+  const opt odh = dh, oxs = xs, om = mean, ors = rstd;
+  if (!layer_norm_ok(xs, w, std::nullopt, dxn, false, dev) || dh.scalar_type() != xs.scalar_type() || dh.sizes() != xs.sizes() ||
+      !plain(dh, dev) || (bias_dtype && !float3(*bias_dtype)))
+    return py::none();
+  const int64_t C = xs.size(-1), M = xs.numel() / C;
+  if (!scales_ok(om, M, dev) || !scales_ok(ors, M, dev) || records({&odh, &dxn, &oxs, &w, &om, &ors})) return py::none();
+  at::Tensor dx, dw, db;
+  {
+    NoGil no_gil;
+    dx = make(xs, xs.sizes(), xs.scalar_type());
+    dw = w ? make(xs, {C}, w->scalar_type()) : none_of(xs, at::kFloat);
+    db = bias_dtype ? make(xs, {C}, *bias_dtype) : none_of(xs, at::kFloat);
+    const size_t bytes = gpic_fp8_layer_norm_bwd_workspace_bytes(M, C);
+    const at::Tensor ws = make(xs, {(int64_t)bytes}, at::kByte);
+    check(gpic_fp8_layer_norm_bwd(dh.data_ptr(), dxn ? dxn->data_ptr() : nullptr, xs.data_ptr(), dtype_code3(xs),
+                                  w ? w->data_ptr() : nullptr, w ? dtype_code3(*w) : 0, ptr<float>(mean), ptr<float>(rstd), M, C,
+                                  dx.data_ptr(), w ? dw.data_ptr() : nullptr, dtype_code3(dw),
+                                  bias_dtype ? db.data_ptr() : nullptr, dtype_code3(db), ws.data_ptr(), bytes, vp(stream)),
+          "gpic_fp8_layer_norm_bwd");
+  }
+  return py::make_tuple(dx, dw, db);
+}
+
 }  // namespace
 
 PYBIND11_MODULE(_gpic_host, m) {   // (wrapped: torch's own errors, out of memory among them, stay what they are)
@@ -876,6 +976,10 @@ PYBIND11_MODULE(_gpic_host, m) {   // (wrapped: torch's own errors, out of memor
   m.def("norm_rows", torch::wrap_pybind_function(&norm_rows));
   m.def("norm_rows_bwd", torch::wrap_pybind_function(&norm_rows_bwd));
   m.def("gemm_rows", torch::wrap_pybind_function(&gemm_rows));
+  m.def("layer_norm", torch::wrap_pybind_function(&layer_norm));
+  m.def("layer_norm_served", torch::wrap_pybind_function(&layer_norm_served));
+  m.def("layer_norm_rows", torch::wrap_pybind_function(&layer_norm_rows));
+  m.def("layer_norm_bwd", torch::wrap_pybind_function(&layer_norm_bwd));
   m.def("linear_rows_bwd", torch::wrap_pybind_function(&linear_rows_bwd));
   m.def("norm_linear_rows_fwd", torch::wrap_pybind_function(&norm_linear_rows_fwd));
   m.def("linear_rows", torch::wrap_pybind_function(&linear_rows));

@@ -9,6 +9,7 @@ from .fp8_native import (E4, FMAX, TINY, Fp8Linear, Fp8LinearF8, convert_native,
                          tcast_t, tcast_t_group, weight_casts, _mm)
 from .fp8 import KEEP, convert_fp8, fp8_filter
 from .heads import Fp8HeadsLinearF8, convert_fused_heads
+from .layernorm import layer_norm, layer_norm_bwd, layer_norm_rows
 from .norm import (Fp8NormLinearF8, convert_fused_norm, fp8_mod_rmsnorm_linear, fp8_res_mod_rmsnorm_mlp,
                    mod_rmsnorm, res_mod_rmsnorm, res_mod_rmsnorm_bwd, res_mod_rmsnorm_fwd, res_mod_rmsnorm_q)
 from .norm import reference as norm_reference
@@ -23,4 +24,5 @@ __all__ = ["E4", "FMAX", "TINY", "Fp8Linear", "Fp8LinearF8", "convert_native", "
            "fp8_res_mod_rmsnorm_mlp", "Fp8NormLinearF8", "convert_fused_norm", "tcast_heads", "fp8_heads_linear_f8",
            "Fp8HeadsLinearF8", "convert_fused_heads", "res_mod_rmsnorm_fwd", "res_mod_rmsnorm_bwd",
            "RowsWeight", "act_bwd_rows", "fp8_gemm_rows", "fp8_linear_rows", "fp8_rmsnorm_linear_rows", "rmsnorm_rows",
-           "rmsnorm_rows_bwd", "rows_weight", "swiglu_layout", "tcast_rows"]
+           "rmsnorm_rows_bwd", "rows_weight", "swiglu_layout", "tcast_rows",
+           "layer_norm", "layer_norm_rows", "layer_norm_bwd"]

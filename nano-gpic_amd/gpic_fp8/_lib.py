@@ -63,10 +63,16 @@ SIGNATURES = {
     "gpic_fp8_act_bwd_rows_workspace_bytes": (_sz, [_i64, _i64]),
     "gpic_fp8_act_bwd_rows": (_int, [_vp, _i64, _vp, _i64, _int, _vp, _i64, _i64, _vp, _vp, _vp, _vp, _i64, _vp, _i64, _vp,
                                       _int, _vp, _sz, _vp]),
+    "gpic_fp8_layer_norm": (_int, [_vp, _int, _i64, _vp, _i64, _vp, _int, _vp, _int, _i64, _i64, ctypes.c_float, _vp, _vp, _vp,
+                                    _vp, _vp, _vp, _vp]),
+    "gpic_fp8_layer_norm_bwd_workspace_bytes": (_sz, [_i64, _i64]),
+    "gpic_fp8_layer_norm_bwd": (_int, [_vp, _vp, _vp, _int, _vp, _int, _vp, _vp, _i64, _i64, _vp, _vp, _int, _vp, _int, _vp, _sz,
+                                        _vp]),
     "gpic_fp8_bf16_gemm_mn": (_int, [_vp, _i64, _vp, _i64, _vp, _int, _i64, _i64, _i64, _i64, _vp, _sz, _vp]),
 }
 
 DTYPE_CODE = {torch.bfloat16: 0, torch.float32: 1}
+DTYPE_CODE_3 = {**DTYPE_CODE, torch.float16: 2}   # of the entry points that take fp16 too
 
 _lib = None
 
