@@ -437,6 +437,42 @@ int gpic_fp8_layer_norm_bwd(const void *dh, const void *dxn, const void *xs, int
                             const float *mean, const float *rstd, int64_t rows, int64_t C, void *dx, void *dw, int dw_dtype,
                             void *db, int db_dtype, void *ws, size_t ws_bytes, void *stream);
 
+/*
+ * Attention of queries to an encoder's states of another length. (The reference calls torch's scaled_dot_product_attention,
+ * attention_op.py:4, and casts its output for proj, JiT_T2I.py:183-185.)
+ *   q, o [B, H, N, D], k, v [B, Hk, L, D] of dtype (bf16 or fp16), H a multiple of Hk (query head h reads key head h / (H / Hk))
+ *   S = scale q k^T over the valid keys of the batch entry;  P = softmax(S);  o = P v, rounded once
+ *   A key j is valid below lens[b] (NULL: L; taken into 0..L) and where mask[b ldm + j] is not 0 (NULL: everywhere). What the
+ *   others' rows of k and v hold is not used, not even an infinity or NaN. A row without a valid key, or whose scores are all
+ *   -inf, gives zeros.
+ *   lse [B, H, N] (NULL: not kept): log2 of the sum of 2^(S log2 e), +inf for such a row; for the backward.
+ *   *s: host arrays of 3: the strides, in elements, of a batch entry, a head and a row (elements of a row are contiguous);
+ *       multiples of 8, not negative; 0 where a dimension is broadcast (inputs only).
+ *   D % 8 == 0, D <= 128; scale > 0; B, H, N, L, H N / Hk <= 2^30; B Hk times the 64-row tiles of H N / Hk and of L < 2^23.
+ *   ws: gpic_fp8_attention_workspace_bytes bytes, scratch of this call. P is rounded to dtype as the second product's operand;
+ *   scores, maxima, sums and o are fp32 until the end. Deterministic.
+ */
+size_t gpic_fp8_attention_workspace_bytes(int64_t B, int64_t H, int64_t Hk, int64_t N, int64_t L, int64_t D);
+int gpic_fp8_attention(const uint16_t *q, const int64_t *qs, const uint16_t *k, const int64_t *ks, const uint16_t *v,
+                       const int64_t *vs, int dtype, const int *lens, const uint8_t *mask, int64_t ldm, int64_t B, int64_t H,
+                       int64_t Hk, int64_t N, int64_t L, int64_t D, float scale, uint16_t *o, const int64_t *os, float *lse,
+                       void *ws, size_t ws_bytes, void *stream);
+
+/*
+ * Its backward, dout the gradient of o; o and lse the forward's:
+ *   delta = sum(dout o);  dv = P^T dout;  dS = P (dout v^T - delta);  dq = scale dS k;  dk = scale dS^T q
+ *   dk and dv sum over the heads that share theirs, and are zeros for keys that are not valid; both NULL: not asked for.
+ *   P and dS are rounded to dtype as the products' operands (fp16: times powers of two that keep them among its normal numbers);
+ *   sums are fp32, in a fixed order. ws: gpic_fp8_attention_bwd_workspace_bytes bytes, scratch of this call.
+ */
+size_t gpic_fp8_attention_bwd_workspace_bytes(int64_t B, int64_t H, int64_t Hk, int64_t N, int64_t L, int64_t D);
+int gpic_fp8_attention_bwd(const uint16_t *dout, const int64_t *ds, const uint16_t *q, const int64_t *qs, const uint16_t *k,
+                           const int64_t *ks, const uint16_t *v, const int64_t *vs, const uint16_t *o, const int64_t *os,
+                           const float *lse, int dtype, const int *lens, const uint8_t *mask, int64_t ldm, int64_t B, int64_t H,
+                           int64_t Hk, int64_t N, int64_t L, int64_t D, float scale, uint16_t *dq, const int64_t *dqs,
+                           uint16_t *dk, const int64_t *dks, uint16_t *dv, const int64_t *dvs, void *ws, size_t ws_bytes,
+                           void *stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,1000 @@
+// Attention of queries to an encoder's states of another length, forward and backward, for gfx950.
+//
+//   S = scale q k^T over the valid keys of the query's batch entry;  P = softmax(S) (zeros where no key is valid);  o = P v
+//   lse = log2 sum 2^(S log2 e) (kept for the backward; +inf where nothing is valid)
+//   delta = sum(do o);  dv = P^T do;  dP = do v^T;  dS = P (dP - delta);  dq = scale dS k;  dk = scale dS^T q
+//
+// A key is valid below its batch entry's length and where its mask is true. Rows of k and v that are not are never used: they are
+// taken as zeros when a tile is staged, so that an infinity or NaN in padding reaches nothing, and their gradients are zeros.
+// The heads that share a key's head (H = G Hk) are rows beside each other: a (batch entry, key head) pair has G N rows of q.
+//
+// All products run on v_mfma_f32_16x16x32 (bf16 or fp16 operands, fp32 sums): lane l gives row (column) l & 15 and the 8 terms
+// from 8 (l / 16), and holds rows 4 (l / 16) + v of column l & 15 of the result. Each kernel takes the product that yields P (or
+// dS) with the index that is summed next as its rows, so that the result, rounded to 16 bits, is the next product's right operand
+// as it lies in its lane: terms 8 g + e of group g = l / 16 are rows 4 g + e of two 16-row tiles (e < 4 the first's), and the left
+// operand, read from the staged tile by columns (ds_read_b64_tr_b16: four rows' 16 columns, one column a lane), takes its rows in
+// that same order. A softmax's maximum and sum are then over a lane's own values and two exchanges between the four groups.
+//
+// Staged tiles hold rows of DP elements (head dimensions up to DP, the rest zeros) in 16-byte chunks, chunk c of row r in place
+// c ^ swz(r), where swz permutes the row's lowest bits so that both the reads by rows (16 rows, one chunk) and the reads by columns
+// (8 rows, two chunks) touch every bank once.
+#include <algorithm>
+#include <type_traits>
+
+#include "gpic_device.h"
+#include "gpic_launch.h"
+
+namespace gpic {
+
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef short s16x8 __attribute__((ext_vector_type(8)));
+typedef float f32x4_t __attribute__((ext_vector_type(4)));
+typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x8v __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x2v __attribute__((ext_vector_type(2)));
+typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
+
+constexpr int kTile = 64;   // rows of a staged tile
+constexpr float kInf = __builtin_huge_valf();
+
+struct AttnArgs {
+  const uint16_t *q, *k, *v, *o, *dout;
+  uint16_t *out, *dq, *dk, *dv;
+  int64_t qs[3], ks[3], vs[3], os[3], ds[3], dqs[3], dks[3], dvs[3];   // strides: batch entry, head, row
+  const int *lens;                                                     // [B] or null
+  const uint8_t *mask;                                                 // [B, L] or null
+  int64_t ldm;
+  float *lse, *delta, *rowmax, *part;
+  int B, H, Hk, N, L, D, G, rows, tiles, splits;   // rows: G N; tiles: row (or key) tiles of a (batch entry, key head) pair
+  int rtiles;                                      // row tiles of the dq kernel
+  float c, scale;                                  // c: scale log2 e
+};
+
+template <bool F16>
+__device__ __forceinline__ f32x4_t mfma16(s16x8 a, s16x8 b, f32x4_t c) {
+  if constexpr (F16)
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8v, a), __builtin_bit_cast(f16x8v, b), c, 0, 0, 0);
+  else
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, a), __builtin_bit_cast(bf16x8_t, b), c, 0, 0, 0);
+}
+template <bool F16>
+__device__ __forceinline__ uint32_t pack16(float lo, float hi) {
+  if constexpr (F16) return __builtin_bit_cast(uint32_t, f16x2v{(_Float16)lo, (_Float16)hi});
+  else return pack_bf16(lo, hi);
+}
+// Two result tiles as a right operand.
+template <bool F16>
+__device__ __forceinline__ s16x8 operand(f32x4_t a, f32x4_t b) {
+  return __builtin_bit_cast(s16x8, u32x4{pack16<F16>(a[0], a[1]), pack16<F16>(a[2], a[3]), pack16<F16>(b[0], b[1]),
+                                         pack16<F16>(b[2], b[3])});
+}
+template <bool F16>
+__device__ __forceinline__ void floats8(s16x8 x, float (&f)[8]) {
+  if constexpr (F16) {
+    const f16x8v h = __builtin_bit_cast(f16x8v, x);
+#pragma unroll
+    for (int e = 0; e < 8; e++) f[e] = (float)h[e];
+  } else {
+    const u32x4 w = __builtin_bit_cast(u32x4, x);
+#pragma unroll
+    for (int e = 0; e < 8; e++) f[e] = e & 1 ? bf16_hi(w[e >> 1]) : bf16_lo(w[e >> 1]);
+  }
+}
+
+// Sum, or maximum, of a value over the four groups of 16 lanes, in every lane.
+__device__ __forceinline__ float groups_sum(float v) {
+  v += __shfl_xor(v, 16, 64);
+  return v + __shfl_xor(v, 32, 64);
+}
+__device__ __forceinline__ float groups_max(float v) {
+  v = fmaxf(v, __shfl_xor(v, 16, 64));
+  return fmaxf(v, __shfl_xor(v, 32, 64));
+}
+
+// The workgroup's number with the workgroups of one XCD (every eighth) next to each other: they share k and v in its L2.
+__device__ __forceinline__ uint32_t xcd_order(uint32_t id, uint32_t n) {
+  const uint32_t x = id & 7, q = n >> 3, r = n & 7;
+  return x * q + min(x, r) + (id >> 3);
+}
+
+template <int DP>
+__device__ __forceinline__ int swz(int r) {
+  return DP == 64 ? ((r >> 1) & 3) << 1 | ((r >> 3) & 1) : (r & 7) << 1 | ((r >> 3) & 1);
+}
+
+// A lane's places in a staged tile (element offsets): for the read by rows of 16-row tile t and step ks, add t 16 DP to row[ks];
+// for the read by columns of tile t and columns 16 dt.., add t 16 DP to col[dt].
+template <int DP>
+struct Places {
+  int row[DP / 32], col[DP / 16];
+  __device__ __forceinline__ Places(int lane) {
+    const int l15 = lane & 15, g = lane >> 4;
+#pragma unroll
+    for (int k = 0; k < DP / 32; k++) row[k] = l15 * DP + ((4 * k + g) ^ swz<DP>(l15)) * 8;
+    const int r = 4 * g + (l15 >> 2);
+#pragma unroll
+    for (int d = 0; d < DP / 16; d++) col[d] = r * DP + ((2 * d + ((l15 >> 1) & 1)) ^ swz<DP>(r)) * 8 + (l15 & 1) * 4;
+  }
+};
+template <int DP>
+__device__ __forceinline__ s16x8 by_rows(const uint16_t *tile, int t, int place) {
+  return *reinterpret_cast<const s16x8 *>(tile + t * 16 * DP + place);
+}
+// Columns of 16-row tiles t and t + 1
+template <int DP>
+__device__ __forceinline__ s16x8 by_columns(uint16_t *tile, int t, int place) {
+  const s16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)(tile + t * 16 * DP + place));
+  const s16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)(tile + (t + 1) * 16 * DP + place));
+  return s16x8{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
+}
+
+// A tile of kTile rows on its way through registers: 256 threads, kU chunks each.
+template <int DP>
+struct Stage {
+  static constexpr int kC = DP / 8, kU = kTile * kC / 256;
+  u32x4 r[kU];
+  // Row i of the tile at base + i stride where bit i of rows is set; zeros elsewhere and past column D.
+  __device__ __forceinline__ void load(const uint16_t *base, int64_t stride, uint64_t rows, int D) {
+#pragma unroll
+    for (int u = 0; u < kU; u++) {
+      const int i = threadIdx.x + 256 * u, row = i / kC, c = i % kC;
+      r[u] = u32x4{0u, 0u, 0u, 0u};
+      if ((rows >> row & 1) && 8 * c < D) r[u] = *reinterpret_cast<const u32x4 *>(base + row * stride + 8 * c);
+    }
+  }
+  __device__ __forceinline__ void store(uint16_t *tile) const {
+#pragma unroll
+    for (int u = 0; u < kU; u++) {
+      const int i = threadIdx.x + 256 * u, row = i / kC, c = i % kC;
+      *reinterpret_cast<u32x4 *>(tile + row * DP + (c ^ swz<DP>(row)) * 8) = r[u];
+    }
+  }
+};
+
+// The keys of a batch entry: those below len, and of them those whose mask is true.
+struct Keys {
+  const uint8_t *mask;
+  int len;
+  __device__ __forceinline__ Keys(const AttnArgs &p, int b) {
+    len = p.lens ? min(max(p.lens[b], 0), p.L) : p.L;
+    mask = p.mask ? p.mask + b * p.ldm : nullptr;
+  }
+  __device__ __forceinline__ bool valid(int j) const { return j < len && (!mask || mask[j]); }
+  // Bit i: whether key j0 + i is valid
+  __device__ __forceinline__ uint64_t tile(int j0) const { return __ballot(valid(j0 + (int)(threadIdx.x & 63))); }
+  // The first tile at or after i (of kTile keys) that has a valid key, and its bits; at `end`, none.
+  __device__ __forceinline__ int next(int i, int end, uint64_t &bits) const {
+    for (; i < end; i++) {
+      bits = tile(i * kTile);
+      if (bits) return i;
+    }
+    return end;
+  }
+};
+
+// The heads and rows of a (batch entry, key head) pair: row r is row r % N of head hk G + r / N.
+__device__ __forceinline__ int64_t row_at(const AttnArgs &p, const int64_t (&s)[3], int b, int hk, int r) {
+  const int h = p.G == 1 ? 0 : r / p.N;
+  return b * s[0] + (hk * p.G + h) * s[1] + (r - h * p.N) * s[2];
+}
+// A row's 8 elements from 8 (4 ks + g), zeros past D and past the last row.
+__device__ __forceinline__ s16x8 row_chunk(const uint16_t *row, int chunk, int D, bool on) {
+  s16x8 z = {0, 0, 0, 0, 0, 0, 0, 0};
+  if (on && 8 * chunk < D) z = *reinterpret_cast<const s16x8 *>(row + 8 * chunk);
+  return z;
+}
+
+// The scores of a key tile as powers of two below the running maximum: p = 2^(c s - use), and what the sums so far shrink by.
+struct Softmax {
+  float m = -kInf, l = 0.0f, use = 0.0f;
+  // mx: the tile's maximum, the same in all groups; the factor for l and o
+  __device__ __forceinline__ float step(float mx, float c) {
+    const float before = m;
+    m = fmaxf(m, mx);
+    const float old = use;
+    use = m == -kInf ? 0.0f : m * c;
+    const float f = before == -kInf ? 0.0f : __builtin_amdgcn_exp2f(old - use);
+    l *= f;
+    return f;
+  }
+};
+
+// ------------------------------------------------------------------------------------------- forward
+
+// A workgroup's four waves take 16 QT rows each and walk the pair's keys (or its split's part of them) by tiles of 64, k and v
+// staged through two buffers: the next tile's loads are under way during the current one's products.
+template <bool F16, int DP, int QT>
+__global__ __launch_bounds__(256, 2) void attn_fwd_kernel(AttnArgs p) {
+  constexpr int KS = DP / 32, DT = DP / 16;
+  __shared__ __attribute__((aligned(16))) uint16_t kt[2][kTile * DP], vt[2][kTile * DP];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l15 = lane & 15, g = lane >> 4;
+  uint32_t id = xcd_order(blockIdx.x, gridDim.x);
+  const int rt = id % p.tiles, split = id / p.tiles % p.splits, pair = id / p.tiles / p.splits;
+  const int b = pair / p.Hk, hk = pair - b * p.Hk;
+  const Keys keys(p, b);
+  const Places<DP> at(lane);
+  const int row0 = rt * 64 * QT + wave * 16 * QT;
+  s16x8 qf[QT][KS];
+#pragma unroll
+  for (int i = 0; i < QT; i++) {
+    const int r = row0 + 16 * i + l15;
+    const uint16_t *row = p.q + row_at(p, p.qs, b, hk, min(r, p.rows - 1));
+#pragma unroll
+    for (int k = 0; k < KS; k++) qf[i][k] = row_chunk(row, 4 * k + g, p.D, r < p.rows);
+  }
+  f32x4_t O[QT][DT];
+  Softmax sm[QT];
+#pragma unroll
+  for (int i = 0; i < QT; i++)
+#pragma unroll
+    for (int d = 0; d < DT; d++) O[i][d] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+  const uint16_t *kb = p.k + b * p.ks[0] + hk * p.ks[1], *vb = p.v + b * p.vs[0] + hk * p.vs[1];
+  const int n = (keys.len + kTile - 1) / kTile, per = (n + p.splits - 1) / p.splits;
+  const int end = min(n, (split + 1) * per);
+  uint64_t bits = 0, nbits = 0;
+  int i = keys.next(split * per, end, bits);
+  Stage<DP> sk, sv;
+  if (i < end) {
+    sk.load(kb + (int64_t)i * kTile * p.ks[2], p.ks[2], bits, p.D);
+    sv.load(vb + (int64_t)i * kTile * p.vs[2], p.vs[2], bits, p.D);
+    sk.store(kt[0]);
+    sv.store(vt[0]);
+  }
+  __syncthreads();
+  for (int cur = 0; i < end; cur ^= 1, bits = nbits) {
+    const int j = keys.next(i + 1, end, nbits);
+    if (j < end) {
+      sk.load(kb + (int64_t)j * kTile * p.ks[2], p.ks[2], nbits, p.D);
+      sv.load(vb + (int64_t)j * kTile * p.vs[2], p.vs[2], nbits, p.D);
+    }
+    f32x4_t S[QT][4];
+#pragma unroll
+    for (int t = 0; t < 4; t++) {
+#pragma unroll
+      for (int q = 0; q < QT; q++) S[q][t] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+      for (int k = 0; k < KS; k++) {
+        const s16x8 a = by_rows<DP>(kt[cur], t, at.row[k]);
+#pragma unroll
+        for (int q = 0; q < QT; q++) S[q][t] = mfma16<F16>(a, qf[q][k], S[q][t]);
+      }
+    }
+    if (bits != ~0ull) {
+#pragma unroll
+      for (int t = 0; t < 4; t++) {
+        const uint32_t on = (uint32_t)(bits >> (16 * t)) >> (4 * g);
+#pragma unroll
+        for (int q = 0; q < QT; q++)
+#pragma unroll
+          for (int v = 0; v < 4; v++) S[q][t][v] = on >> v & 1 ? S[q][t][v] : -kInf;
+      }
+    }
+    s16x8 pf[QT][2];
+#pragma unroll
+    for (int q = 0; q < QT; q++) {
+      float mx = -kInf;
+#pragma unroll
+      for (int t = 0; t < 4; t++)
+#pragma unroll
+        for (int v = 0; v < 4; v++) mx = fmaxf(mx, S[q][t][v]);
+      const float before = sm[q].m;
+      const float f = sm[q].step(groups_max(mx), p.c);
+      if (__ballot(sm[q].m > before)) {
+#pragma unroll
+        for (int d = 0; d < DT; d++)
+#pragma unroll
+          for (int v = 0; v < 4; v++) O[q][d][v] *= f;
+      }
+#pragma unroll
+      for (int t = 0; t < 4; t++)
+#pragma unroll
+        for (int v = 0; v < 4; v++) {
+          S[q][t][v] = __builtin_amdgcn_exp2f(__builtin_fmaf(S[q][t][v], p.c, -sm[q].use));
+          sm[q].l += S[q][t][v];
+        }
+      pf[q][0] = operand<F16>(S[q][0], S[q][1]);
+      pf[q][1] = operand<F16>(S[q][2], S[q][3]);
+    }
+#pragma unroll
+    for (int h = 0; h < 2; h++)
+#pragma unroll
+      for (int d = 0; d < DT; d++) {
+        const s16x8 a = by_columns<DP>(vt[cur], 2 * h, at.col[d]);
+#pragma unroll
+        for (int q = 0; q < QT; q++) O[q][d] = mfma16<F16>(a, pf[q][h], O[q][d]);
+      }
+    if (j < end) {
+      sk.store(kt[cur ^ 1]);
+      sv.store(vt[cur ^ 1]);
+    }
+    __syncthreads();
+    i = j;
+  }
+#pragma unroll
+  for (int q = 0; q < QT; q++) {
+    const int r = row0 + 16 * q + l15;
+    const float l = groups_sum(sm[q].l);
+    if (r >= p.rows) continue;
+    if (p.splits > 1) {
+      // (partial o, its maximum and sum: joined by attn_join_kernel)
+      const int64_t at_row = ((int64_t)split * p.B * p.Hk + pair) * p.rows + r;
+      float *o = p.part + at_row * (DP + 2);
+#pragma unroll
+      for (int d = 0; d < DT; d++)
+#pragma unroll
+        for (int v = 0; v < 4; v++) o[16 * d + 4 * g + v] = O[q][d][v];
+      if (g == 0) o[DP] = l == 0.0f ? -kInf : sm[q].use, o[DP + 1] = l;
+      continue;
+    }
+    const float inv = l == 0.0f ? 0.0f : __fdiv_rn(1.0f, l);
+    uint16_t *o = p.out + row_at(p, p.os, b, hk, r);
+#pragma unroll
+    for (int d = 0; d < DT; d++)
+      if (16 * d + 4 * g < p.D)
+        *reinterpret_cast<u32x2 *>(o + 16 * d + 4 * g) = u32x2{pack16<F16>(O[q][d][0] * inv, O[q][d][1] * inv),
+                                                               pack16<F16>(O[q][d][2] * inv, O[q][d][3] * inv)};
+    if (p.lse && g == 0)
+      p.lse[(int64_t)pair * p.rows + r] = l == 0.0f ? kInf : sm[q].use + __builtin_amdgcn_logf(l);
+  }
+}
+
+// Up to 16 rows a pair (a token's heads): memory bounds it, k and v once. Each wave walks keys of its own, 32 a step: k goes from
+// memory to the lanes as they multiply it, v through the wave's own staged tile, both requested a step ahead; no barrier until the
+// waves' results are joined.
+template <bool F16, int DP>
+__global__ __launch_bounds__(256, 2) void attn_few_kernel(AttnArgs p) {
+  constexpr int KS = DP / 32, DT = DP / 16, kC = DP / 8, kU = 32 * kC / 64;
+  __shared__ __attribute__((aligned(16))) uint16_t vt[4][32 * DP];
+  __shared__ __attribute__((aligned(16))) float joined[4][16][DP + 4];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l15 = lane & 15, g = lane >> 4;
+  const uint32_t id = xcd_order(blockIdx.x, gridDim.x);
+  const int split = id % p.splits, pair = id / p.splits;
+  const int b = pair / p.Hk, hk = pair - b * p.Hk;
+  const Keys keys(p, b);
+  const Places<DP> at(lane);
+  s16x8 qf[KS];
+  const uint16_t *row = p.q + row_at(p, p.qs, b, hk, min(l15, p.rows - 1));
+#pragma unroll
+  for (int k = 0; k < KS; k++) qf[k] = row_chunk(row, 4 * k + g, p.D, l15 < p.rows);
+  f32x4_t O[DT];
+#pragma unroll
+  for (int d = 0; d < DT; d++) O[d] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+  Softmax sm;
+  const uint16_t *kb = p.k + b * p.ks[0] + hk * p.ks[1], *vb = p.v + b * p.vs[0] + hk * p.vs[1];
+  const int n = (keys.len + 31) / 32, per = (n + 4 * p.splits - 1) / (4 * p.splits);
+  const int first = (split * 4 + wave) * per, end = min(n, first + per);
+  s16x8 K[2][KS], Kn[2][KS];
+  u32x4 V[kU];
+  auto fetch = [&](int i, uint32_t bits) {
+#pragma unroll
+    for (int t = 0; t < 2; t++)
+#pragma unroll
+      for (int k = 0; k < KS; k++)
+        Kn[t][k] = row_chunk(kb + (int64_t)(32 * i + 16 * t + l15) * p.ks[2], 4 * k + g, p.D, bits >> (16 * t + l15) & 1);
+#pragma unroll
+    for (int u = 0; u < kU; u++) {
+      const int w = lane + 64 * u, r = w / kC, c = w % kC;
+      V[u] = __builtin_bit_cast(u32x4, row_chunk(vb + (int64_t)(32 * i + r) * p.vs[2], c, p.D, bits >> r & 1));
+    }
+  };
+  auto next = [&](int i, uint32_t &bits) {
+    for (; i < end; i++) {
+      bits = (uint32_t)__ballot(lane < 32 && keys.valid(32 * i + lane));
+      if (bits) return i;
+    }
+    return end;
+  };
+  uint32_t bits = 0, nbits = 0;
+  int i = next(first, bits);
+  if (i < end) fetch(i, bits);
+  while (i < end) {
+#pragma unroll
+    for (int t = 0; t < 2; t++)
+#pragma unroll
+      for (int k = 0; k < KS; k++) K[t][k] = Kn[t][k];
+#pragma unroll
+    for (int u = 0; u < kU; u++) {
+      const int w = lane + 64 * u, r = w / kC, c = w % kC;
+      *reinterpret_cast<u32x4 *>(vt[wave] + r * DP + (c ^ swz<DP>(r)) * 8) = V[u];
+    }
+    const int j = next(i + 1, nbits);
+    if (j < end) fetch(j, nbits);
+    f32x4_t S[2];
+#pragma unroll
+    for (int t = 0; t < 2; t++) {
+      S[t] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+      for (int k = 0; k < KS; k++) S[t] = mfma16<F16>(K[t][k], qf[k], S[t]);
+    }
+    float mx = -kInf;
+#pragma unroll
+    for (int t = 0; t < 2; t++)
+#pragma unroll
+      for (int v = 0; v < 4; v++) {
+        if (!(bits >> (16 * t + 4 * g + v) & 1)) S[t][v] = -kInf;
+        mx = fmaxf(mx, S[t][v]);
+      }
+    const float f = sm.step(groups_max(mx), p.c);
+#pragma unroll
+    for (int t = 0; t < 2; t++)
+#pragma unroll
+      for (int v = 0; v < 4; v++) {
+        S[t][v] = __builtin_amdgcn_exp2f(__builtin_fmaf(S[t][v], p.c, -sm.use));
+        sm.l += S[t][v];
+      }
+    const s16x8 pf = operand<F16>(S[0], S[1]);
+#pragma unroll
+    for (int d = 0; d < DT; d++) {
+#pragma unroll
+      for (int v = 0; v < 4; v++) O[d][v] *= f;
+      O[d] = mfma16<F16>(by_columns<DP>(vt[wave], 0, at.col[d]), pf, O[d]);
+    }
+    i = j;
+    bits = nbits;
+  }
+  const float l = groups_sum(sm.l);
+#pragma unroll
+  for (int d = 0; d < DT; d++)
+#pragma unroll
+    for (int v = 0; v < 4; v++) joined[wave][l15][16 * d + 4 * g + v] = O[d][v];
+  if (g == 0) joined[wave][l15][DP] = l == 0.0f ? -kInf : sm.use, joined[wave][l15][DP + 1] = l;
+  __syncthreads();
+  for (int w = threadIdx.x; w < p.rows * DP; w += 256) {
+    const int r = w / DP, d = w % DP;
+    float m = -kInf, sum = 0.0f, o = 0.0f;
+#pragma unroll
+    for (int x = 0; x < 4; x++) m = fmaxf(m, joined[x][r][DP]);
+#pragma unroll
+    for (int x = 0; x < 4; x++) {
+      if (joined[x][r][DP] == -kInf) continue;
+      const float f = __builtin_amdgcn_exp2f(joined[x][r][DP] - m);
+      sum = __builtin_fmaf(f, joined[x][r][DP + 1], sum);
+      o = __builtin_fmaf(f, joined[x][r][d], o);
+    }
+    if (p.splits > 1) {
+      float *out = p.part + (((int64_t)split * p.B * p.Hk + pair) * p.rows + r) * (DP + 2);
+      out[d] = o;
+      if (d == 0) out[DP] = m, out[DP + 1] = sum;
+      continue;
+    }
+    const float inv = sum == 0.0f ? 0.0f : __fdiv_rn(1.0f, sum);
+    if (d < p.D) p.out[row_at(p, p.os, b, hk, r) + d] = (uint16_t)pack16<F16>(o * inv, 0.0f);
+    if (p.lse && d == 0) p.lse[(int64_t)pair * p.rows + r] = sum == 0.0f ? kInf : m + __builtin_amdgcn_logf(sum);
+  }
+}
+
+// The splits' parts of a row, joined in their order: a thread a column, 256 / DP rows a workgroup.
+template <bool F16, int DP>
+__global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs p) {
+  const int64_t all = (int64_t)p.B * p.Hk * p.rows, row = (int64_t)blockIdx.x * (256 / DP) + threadIdx.x / DP;
+  const int d = threadIdx.x % DP;
+  if (row >= all) return;
+  float m = -kInf, sum = 0.0f, o = 0.0f;
+  for (int s = 0; s < p.splits; s++) m = fmaxf(m, p.part[(s * all + row) * (DP + 2) + DP]);
+  for (int s = 0; s < p.splits; s++) {
+    const float *x = p.part + (s * all + row) * (DP + 2);
+    if (x[DP] == -kInf) continue;
+    const float f = __builtin_amdgcn_exp2f(x[DP] - m);
+    sum = __builtin_fmaf(f, x[DP + 1], sum);
+    o = __builtin_fmaf(f, x[d], o);
+  }
+  const int pair = (int)(row / p.rows), r = (int)(row - (int64_t)pair * p.rows), b = pair / p.Hk;
+  const float inv = sum == 0.0f ? 0.0f : __fdiv_rn(1.0f, sum);
+  if (d < p.D) p.out[row_at(p, p.os, b, pair - b * p.Hk, r) + d] = (uint16_t)pack16<F16>(o * inv, 0.0f);
+  if (p.lse && d == 0) p.lse[row] = sum == 0.0f ? kInf : m + __builtin_amdgcn_logf(sum);
+}
+
+// ------------------------------------------------------------------------------------------- backward
+
+// fp16 holds nothing below 2^-24, where the probabilities of long states and their products with small gradients lie: P is held
+// 2^10 times itself, and dS times a power of two that brings the gradients' largest row norm (for dq each row's own) to 16 .. 32.
+// Exact factors, taken off the fp32 sums again.
+constexpr float kPUp = 10.0f;
+__device__ __forceinline__ float norm_factor(float norm2) {
+  if (!(norm2 > 0.0f) || norm2 == kInf) return 1.0f;
+  const int e = (int)((__float_as_uint(__builtin_sqrtf(norm2)) >> 23) & 255) - 127;
+  return __builtin_ldexpf(1.0f, min(max(4 - e, -60), 60));
+}
+
+// dq, delta and (fp16) the largest row norm of the workgroup's do; the forward's walk over the keys.
+template <bool F16, int DP, int QT>
+__global__ __launch_bounds__(256, 2) void attn_dq_kernel(AttnArgs p) {
+  constexpr int KS = DP / 32, DT = DP / 16;
+  __shared__ __attribute__((aligned(16))) uint16_t kt[2][kTile * DP], vt[2][kTile * DP];
+  __shared__ float norms[4];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l15 = lane & 15, g = lane >> 4;
+  const uint32_t id = xcd_order(blockIdx.x, gridDim.x);
+  const int rt = id % p.tiles, pair = id / p.tiles;
+  const int b = pair / p.Hk, hk = pair - b * p.Hk;
+  const Keys keys(p, b);
+  const Places<DP> at(lane);
+  const int row0 = rt * 64 * QT + wave * 16 * QT;
+  s16x8 qf[QT][KS], df[QT][KS];
+  float delta[QT], lse[QT], up[QT];
+  float most = 0.0f;
+#pragma unroll
+  for (int i = 0; i < QT; i++) {
+    const int r = row0 + 16 * i + l15, rc = min(r, p.rows - 1);
+    const bool on = r < p.rows;
+    const uint16_t *qr = p.q + row_at(p, p.qs, b, hk, rc), *dr = p.dout + row_at(p, p.ds, b, hk, rc),
+                   *orow = p.o + row_at(p, p.os, b, hk, rc);
+    float sum = 0.0f, n2 = 0.0f;
+#pragma unroll
+    for (int k = 0; k < KS; k++) {
+      qf[i][k] = row_chunk(qr, 4 * k + g, p.D, on);
+      df[i][k] = row_chunk(dr, 4 * k + g, p.D, on);
+      float d[8], o[8];
+      floats8<F16>(df[i][k], d);
+      floats8<F16>(row_chunk(orow, 4 * k + g, p.D, on), o);
+#pragma unroll
+      for (int e = 0; e < 8; e++) {
+        sum = __builtin_fmaf(d[e], o[e], sum);
+        if (F16) n2 = __builtin_fmaf(d[e], d[e], n2);
+      }
+    }
+    delta[i] = groups_sum(sum);
+    lse[i] = on ? p.lse[(int64_t)pair * p.rows + r] : kInf;
+    if (on && g == 0) p.delta[(int64_t)pair * p.rows + r] = delta[i];
+    up[i] = 1.0f;
+    if (F16) {
+      n2 = groups_sum(n2);
+      up[i] = norm_factor(n2);
+      most = fmaxf(most, n2);
+    }
+  }
+  if (F16) {
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor(most, o, 64));
+    if (lane == 0) norms[wave] = most;
+    __syncthreads();
+    if (threadIdx.x == 0) p.rowmax[id] = fmaxf(fmaxf(norms[0], norms[1]), fmaxf(norms[2], norms[3]));
+  }
+  f32x4_t dQ[QT][DT];
+#pragma unroll
+  for (int i = 0; i < QT; i++)
+#pragma unroll
+    for (int d = 0; d < DT; d++) dQ[i][d] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+  const uint16_t *kb = p.k + b * p.ks[0] + hk * p.ks[1], *vb = p.v + b * p.vs[0] + hk * p.vs[1];
+  const int end = (keys.len + kTile - 1) / kTile;
+  uint64_t bits = 0, nbits = 0;
+  int i = keys.next(0, end, bits);
+  Stage<DP> sk, sv;
+  if (i < end) {
+    sk.load(kb + (int64_t)i * kTile * p.ks[2], p.ks[2], bits, p.D);
+    sv.load(vb + (int64_t)i * kTile * p.vs[2], p.vs[2], bits, p.D);
+    sk.store(kt[0]);
+    sv.store(vt[0]);
+  }
+  __syncthreads();
+  for (int cur = 0; i < end; cur ^= 1, bits = nbits) {
+    const int j = keys.next(i + 1, end, nbits);
+    if (j < end) {
+      sk.load(kb + (int64_t)j * kTile * p.ks[2], p.ks[2], nbits, p.D);
+      sv.load(vb + (int64_t)j * kTile * p.vs[2], p.vs[2], nbits, p.D);
+    }
+#pragma unroll
+    for (int h = 0; h < 2; h++) {
+      f32x4_t S[QT][2], P[QT][2];
+#pragma unroll
+      for (int t = 0; t < 2; t++) {
+#pragma unroll
+        for (int q = 0; q < QT; q++) S[q][t] = P[q][t] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int k = 0; k < KS; k++) {
+          const s16x8 a = by_rows<DP>(kt[cur], 2 * h + t, at.row[k]), c = by_rows<DP>(vt[cur], 2 * h + t, at.row[k]);
+#pragma unroll
+          for (int q = 0; q < QT; q++) {
+            S[q][t] = mfma16<F16>(a, qf[q][k], S[q][t]);
+            P[q][t] = mfma16<F16>(c, df[q][k], P[q][t]);
+          }
+        }
+      }
+      s16x8 sf[QT];
+#pragma unroll
+      for (int q = 0; q < QT; q++) {
+#pragma unroll
+        for (int t = 0; t < 2; t++)
+#pragma unroll
+          for (int v = 0; v < 4; v++) {
+            float x = __builtin_amdgcn_exp2f(__builtin_fmaf(S[q][t][v], p.c, -lse[q]));
+            if (bits != ~0ull && !(bits >> (32 * h + 16 * t + 4 * g + v) & 1)) x = 0.0f;
+            x *= P[q][t][v] - delta[q];
+            S[q][t][v] = F16 ? x * up[q] : x;
+          }
+        sf[q] = operand<F16>(S[q][0], S[q][1]);
+      }
+#pragma unroll
+      for (int d = 0; d < DT; d++) {
+        const s16x8 a = by_columns<DP>(kt[cur], 2 * h, at.col[d]);
+#pragma unroll
+        for (int q = 0; q < QT; q++) dQ[q][d] = mfma16<F16>(a, sf[q], dQ[q][d]);
+      }
+    }
+    if (j < end) {
+      sk.store(kt[cur ^ 1]);
+      sv.store(vt[cur ^ 1]);
+    }
+    __syncthreads();
+    i = j;
+  }
+#pragma unroll
+  for (int q = 0; q < QT; q++) {
+    const int r = row0 + 16 * q + l15;
+    if (r >= p.rows) continue;
+    const float f = F16 ? p.scale / up[q] : p.scale;
+    uint16_t *o = p.dq + row_at(p, p.dqs, b, hk, r);
+#pragma unroll
+    for (int d = 0; d < DT; d++)
+      if (16 * d + 4 * g < p.D)
+        *reinterpret_cast<u32x2 *>(o + 16 * d + 4 * g) = u32x2{pack16<F16>(dQ[q][d][0] * f, dQ[q][d][1] * f),
+                                                               pack16<F16>(dQ[q][d][2] * f, dQ[q][d][3] * f)};
+  }
+}
+
+// dk and dv of 64 KT keys: the waves' k and v stay in registers, the pair's rows (or the split's part of them) pass by in staged
+// tiles of q and do. A shared key's gradient sums over its heads here, in a fixed order.
+template <bool F16, int DP, int KT>
+__global__ __launch_bounds__(256, 2) void attn_dkv_kernel(AttnArgs p) {
+  constexpr int KS = DP / 32, DT = DP / 16;
+  __shared__ __attribute__((aligned(16))) uint16_t qt[2][kTile * DP], dt[2][kTile * DP];
+  __shared__ __attribute__((aligned(16))) float lse[2][kTile], delta[2][kTile];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l15 = lane & 15, g = lane >> 4;
+  const uint32_t id = xcd_order(blockIdx.x, gridDim.x);
+  const int kt = id % p.tiles, split = id / p.tiles % p.splits, pair = id / p.tiles / p.splits;
+  const int b = pair / p.Hk, hk = pair - b * p.Hk;
+  const Keys keys(p, b);
+  const Places<DP> at(lane);
+  const int key0 = kt * 64 * KT + wave * 16 * KT;
+  s16x8 kf[KT][KS], vf[KT][KS];
+  bool on[KT];
+  bool any = false;
+#pragma unroll
+  for (int i = 0; i < KT; i++) {
+    const int j = key0 + 16 * i + l15;
+    on[i] = keys.valid(j);
+    any |= on[i];
+    const int64_t jc = min(j, p.L - 1);
+    const uint16_t *kr = p.k + b * p.ks[0] + hk * p.ks[1] + jc * p.ks[2], *vr = p.v + b * p.vs[0] + hk * p.vs[1] + jc * p.vs[2];
+#pragma unroll
+    for (int k = 0; k < KS; k++) {
+      kf[i][k] = row_chunk(kr, 4 * k + g, p.D, on[i]);
+      vf[i][k] = row_chunk(vr, 4 * k + g, p.D, on[i]);
+    }
+  }
+  f32x4_t dK[KT][DT], dV[KT][DT];
+#pragma unroll
+  for (int i = 0; i < KT; i++)
+#pragma unroll
+    for (int d = 0; d < DT; d++) dK[i][d] = dV[i][d] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+  float up = 1.0f;
+  if (F16) {   // (every row tile's largest norm: of the dq kernel's workgroups)
+    const int n = p.rtiles;
+    float m = 0.0f;
+    for (int x = lane; x < n; x += 64) m = fmaxf(m, p.rowmax[pair * (int64_t)n + x]);
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
+    up = norm_factor(m);
+  }
+  const int n = (p.rows + kTile - 1) / kTile, per = (n + p.splits - 1) / p.splits;
+  int i = split * per;
+  const int end = __syncthreads_or(any) ? min(n, i + per) : 0;
+  Stage<DP> sq, sd;
+  float sl = 0.0f;
+  // A tile's rows may belong to several heads: each staged row finds its own.
+  auto fetch = [&](int tile) {
+#pragma unroll
+    for (int u = 0; u < Stage<DP>::kU; u++) {
+      const int x = threadIdx.x + 256 * u, r = tile * kTile + x / Stage<DP>::kC, c = x % Stage<DP>::kC;
+      const int rc = min(r, p.rows - 1);
+      sq.r[u] = __builtin_bit_cast(u32x4, row_chunk(p.q + row_at(p, p.qs, b, hk, rc), c, p.D, r < p.rows));
+      sd.r[u] = __builtin_bit_cast(u32x4, row_chunk(p.dout + row_at(p, p.ds, b, hk, rc), c, p.D, r < p.rows));
+    }
+    const int r = tile * kTile + (threadIdx.x & 63);
+    if (threadIdx.x < 128) {
+      const float *src = threadIdx.x < 64 ? p.lse : p.delta;
+      sl = r < p.rows ? src[(int64_t)pair * p.rows + r] : threadIdx.x < 64 ? kInf : 0.0f;
+      if (F16 && threadIdx.x < 64) sl -= kPUp;
+    }
+  };
+  auto put = [&](int buf) {
+    sq.store(qt[buf]);
+    sd.store(dt[buf]);
+    if (threadIdx.x < 64) lse[buf][threadIdx.x] = sl;
+    else if (threadIdx.x < 128) delta[buf][threadIdx.x - 64] = sl;
+  };
+  if (i < end) {
+    fetch(i);
+    put(0);
+  }
+  __syncthreads();
+  const float us = F16 ? up * __builtin_ldexpf(1.0f, -(int)kPUp) : 1.0f;
+  for (int cur = 0; i < end; cur ^= 1, i++) {
+    if (i + 1 < end) fetch(i + 1);
+#pragma unroll
+    for (int h = 0; h < 2; h++) {
+      f32x4_t S[KT][2], P[KT][2];
+#pragma unroll
+      for (int t = 0; t < 2; t++) {
+#pragma unroll
+        for (int x = 0; x < KT; x++) S[x][t] = P[x][t] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int k = 0; k < KS; k++) {
+          const s16x8 a = by_rows<DP>(qt[cur], 2 * h + t, at.row[k]), c = by_rows<DP>(dt[cur], 2 * h + t, at.row[k]);
+#pragma unroll
+          for (int x = 0; x < KT; x++) {
+            S[x][t] = mfma16<F16>(a, kf[x][k], S[x][t]);
+            P[x][t] = mfma16<F16>(c, vf[x][k], P[x][t]);
+          }
+        }
+        const f32x4_t ls = *reinterpret_cast<const f32x4_t *>(&lse[cur][32 * h + 16 * t + 4 * g]),
+                      de = *reinterpret_cast<const f32x4_t *>(&delta[cur][32 * h + 16 * t + 4 * g]);
+#pragma unroll
+        for (int x = 0; x < KT; x++)
+#pragma unroll
+          for (int v = 0; v < 4; v++) {
+            const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(S[x][t][v], p.c, -ls[v]));
+            float d = P[x][t][v] - de[v];
+            if (F16) d *= us;
+            S[x][t][v] = e;
+            P[x][t][v] = e * d;
+          }
+      }
+      s16x8 pf[KT], sf[KT];
+#pragma unroll
+      for (int x = 0; x < KT; x++) {
+        pf[x] = operand<F16>(S[x][0], S[x][1]);
+        sf[x] = operand<F16>(P[x][0], P[x][1]);
+      }
+#pragma unroll
+      for (int d = 0; d < DT; d++) {
+        const s16x8 a = by_columns<DP>(dt[cur], 2 * h, at.col[d]), c = by_columns<DP>(qt[cur], 2 * h, at.col[d]);
+#pragma unroll
+        for (int x = 0; x < KT; x++) {
+          dV[x][d] = mfma16<F16>(a, pf[x], dV[x][d]);
+          dK[x][d] = mfma16<F16>(c, sf[x], dK[x][d]);
+        }
+      }
+    }
+    if (i + 1 < end) put(cur ^ 1);
+    __syncthreads();
+  }
+  const float fk = F16 ? p.scale / up : p.scale, fv = F16 ? __builtin_ldexpf(1.0f, -(int)kPUp) : 1.0f;
+#pragma unroll
+  for (int x = 0; x < KT; x++) {
+    const int j = key0 + 16 * x + l15;
+    if (j >= p.L) continue;
+    if (p.splits > 1) {
+      float *o = p.part + (((int64_t)split * p.B * p.Hk + pair) * p.L + j) * 2 * p.D;
+#pragma unroll
+      for (int d = 0; d < DT; d++)
+        if (16 * d + 4 * g < p.D) {
+          f32x4_t a, c;
+#pragma unroll
+          for (int v = 0; v < 4; v++) a[v] = on[x] ? dK[x][d][v] * fk : 0.0f, c[v] = on[x] ? dV[x][d][v] * fv : 0.0f;
+          *reinterpret_cast<f32x4_t *>(o + 16 * d + 4 * g) = a;
+          *reinterpret_cast<f32x4_t *>(o + p.D + 16 * d + 4 * g) = c;
+        }
+      continue;
+    }
+    uint16_t *ok = p.dk + b * p.dks[0] + hk * p.dks[1] + j * p.dks[2], *ov = p.dv + b * p.dvs[0] + hk * p.dvs[1] + j * p.dvs[2];
+#pragma unroll
+    for (int d = 0; d < DT; d++)
+      if (16 * d + 4 * g < p.D) {
+        u32x2 a{0u, 0u}, c{0u, 0u};
+        if (on[x]) {
+          a = u32x2{pack16<F16>(dK[x][d][0] * fk, dK[x][d][1] * fk), pack16<F16>(dK[x][d][2] * fk, dK[x][d][3] * fk)};
+          c = u32x2{pack16<F16>(dV[x][d][0] * fv, dV[x][d][1] * fv), pack16<F16>(dV[x][d][2] * fv, dV[x][d][3] * fv)};
+        }
+        *reinterpret_cast<u32x2 *>(ok + 16 * d + 4 * g) = a;
+        *reinterpret_cast<u32x2 *>(ov + 16 * d + 4 * g) = c;
+      }
+  }
+}
+
+// The splits' dk and dv added in their order: a thread four columns of one key's dk or dv.
+template <bool F16>
+__global__ __launch_bounds__(256) void attn_dkv_join_kernel(AttnArgs p) {
+  const int64_t n4 = (int64_t)p.B * p.Hk * p.L * 2 * (p.D / 4), x = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (x >= n4) return;
+  f32x4_t a{0.0f, 0.0f, 0.0f, 0.0f};
+  for (int s = 0; s < p.splits; s++) a += *reinterpret_cast<const f32x4_t *>(p.part + 4 * (s * n4 + x));
+  const int q = p.D / 4, c = (int)(x % q);
+  int64_t r = x / q;
+  const bool v = r & 1;
+  r >>= 1;
+  const int j = (int)(r % p.L), pair = (int)(r / p.L), b = pair / p.Hk, hk = pair - b * p.Hk;
+  const int64_t (&s)[3] = v ? p.dvs : p.dks;
+  *reinterpret_cast<u32x2 *>((v ? p.dv : p.dk) + b * s[0] + hk * s[1] + j * s[2] + 4 * c) =
+      u32x2{pack16<F16>(a[0], a[1]), pack16<F16>(a[2], a[3])};
+}
+
+// ------------------------------------------------------------------------------------------- host side
+
+constexpr int kMaxAttnD = 128;
+constexpr int kFewRows = 16;
+constexpr int64_t kMaxBlocks = int64_t(1) << 23;   // (a launch's threads are counted in 32 bits)
+
+struct AttnPlan {
+  bool few;
+  int qt, tiles, splits;        // forward: 16-row tiles a wave, row tiles, key splits
+  int bqt, btiles, kt, ktiles, ksplits;
+};
+static AttnPlan attn_plan(int64_t B, int64_t H, int64_t Hk, int64_t N, int64_t L, int64_t D) {
+  AttnPlan a;
+  const int64_t pairs = B * Hk, rows = H / Hk * N;
+  a.few = rows <= kFewRows;
+  if (a.few) {
+    a.qt = 1, a.tiles = 1;
+    const int64_t want = (1024 + pairs - 1) / pairs, most = (L + 255) / 256;
+    a.splits = (int)std::max<int64_t>(std::min(want, most), 1);
+  } else {
+    a.qt = pairs * ((rows + 127) / 128) >= 512 ? 2 : 1;
+    a.tiles = (int)((rows + 64 * a.qt - 1) / (64 * a.qt));
+    const int64_t want = 512 / (pairs * a.tiles), most = (L + 511) / 512;
+    a.splits = (int)std::max<int64_t>(std::min(want, most), 1);
+  }
+  a.bqt = pairs * ((rows + 127) / 128) >= 512 ? 2 : 1;
+  a.btiles = (int)((rows + 64 * a.bqt - 1) / (64 * a.bqt));
+  a.kt = D <= 64 && pairs * ((L + 127) / 128) >= 512 ? 2 : 1;
+  a.ktiles = (int)((L + 64 * a.kt - 1) / (64 * a.kt));
+  const int64_t want = 512 / std::max<int64_t>(pairs * a.ktiles, 1), most = (rows + 255) / 256;
+  a.ksplits = (int)std::max<int64_t>(std::min(want, most), 1);
+  return a;
+}
+static int attn_dp(int64_t D) { return D <= 64 ? 64 : 128; }
+
+// The extents' status
+static int attn_shape(int dtype, int64_t B, int64_t H, int64_t Hk, int64_t N, int64_t L, int64_t D) {
+  if (B < 0 || H <= 0 || Hk <= 0 || N < 0 || L < 0 || D <= 0) return GPIC_EINVAL;
+  if (dtype != GPIC_DTYPE_BF16 && dtype != GPIC_DTYPE_F16) return GPIC_EDTYPE;
+  if (H % Hk || D % 8 || D > kMaxAttnD) return GPIC_ESHAPE;
+  const int64_t most = int64_t(1) << 30;
+  if (B > most || H > most || N > most || L > most || H / Hk * N > most || B * H > most) return GPIC_ESHAPE;
+  if (B * Hk * ((H / Hk * N + 63) / 64) * 32 >= kMaxBlocks * 32 || B * Hk * ((L + 63) / 64) >= kMaxBlocks) return GPIC_ESHAPE;
+  return GPIC_OK;
+}
+static int strides_ok(const void *p, const int64_t *s, int64_t (&out)[3]) {
+  if (!s) return GPIC_EINVAL;
+  for (int i = 0; i < 3; i++) {
+    if (s[i] < 0) return GPIC_EINVAL;
+    if (s[i] % 8) return GPIC_EALIGN;
+    out[i] = s[i];
+  }
+  return aligned16(p) ? GPIC_OK : GPIC_EALIGN;
+}
+
+template <class F>
+static void with_attn(int dtype, int64_t D, F f) {
+  auto dp = [&](auto f16) {
+    if (D <= 64) f(f16, std::integral_constant<int, 64>());
+    else f(f16, std::integral_constant<int, 128>());
+  };
+  if (dtype == GPIC_DTYPE_F16) dp(std::true_type());
+  else dp(std::false_type());
+}
+
+}  // namespace gpic
+
+using namespace gpic;
+
+extern "C" {
+
+size_t gpic_fp8_attention_workspace_bytes(int64_t B, int64_t H, int64_t Hk, int64_t N, int64_t L, int64_t D) {
+  if (attn_shape(GPIC_DTYPE_BF16, B, H, Hk, N, L, D) != GPIC_OK || B * N == 0) return 0;
+  const AttnPlan a = attn_plan(B, H, Hk, N, L, D);
+  return a.splits > 1 ? (size_t)a.splits * B * H * N * (attn_dp(D) + 2) * sizeof(float) : 0;
+}
+
+int gpic_fp8_attention(const uint16_t *q, const int64_t *qs, const uint16_t *k, const int64_t *ks, const uint16_t *v,
+                       const int64_t *vs, int dtype, const int *lens, const uint8_t *mask, int64_t ldm, int64_t B, int64_t H,
+                       int64_t Hk, int64_t N, int64_t L, int64_t D, float scale, uint16_t *o, const int64_t *os, float *lse,
+                       void *ws, size_t ws_bytes, void *stream) {
+  status_scope();
+  int e = attn_shape(dtype, B, H, Hk, N, L, D);
+  if (e != GPIC_OK) return e;
+  if (!(scale > 0.0f) || scale == kInf) return GPIC_EINVAL;
+  if (B * N == 0) return GPIC_OK;
+  if (!q || !o || (L > 0 && (!k || !v)) || (mask && ldm < 0)) return GPIC_EINVAL;
+  AttnArgs p{};
+  if ((e = strides_ok(q, qs, p.qs)) || (e = strides_ok(k, ks, p.ks)) || (e = strides_ok(v, vs, p.vs)) ||
+      (e = strides_ok(o, os, p.os)))
+    return e;
+  if (!aligned16(ws)) return GPIC_EALIGN;
+  if (ws_bytes < gpic_fp8_attention_workspace_bytes(B, H, Hk, N, L, D)) return GPIC_EWORKSPACE;
+  const AttnPlan a = attn_plan(B, H, Hk, N, L, D);
+  if (a.splits > 1 && !ws) return GPIC_EWORKSPACE;
+  p.q = q, p.k = k, p.v = v, p.out = o, p.lens = lens, p.mask = mask, p.ldm = ldm, p.lse = lse;
+  p.part = static_cast<float *>(ws);
+  p.B = (int)B, p.H = (int)H, p.Hk = (int)Hk, p.N = (int)N, p.L = (int)L, p.D = (int)D, p.G = (int)(H / Hk);
+  p.rows = p.G * p.N, p.tiles = a.tiles, p.splits = a.splits, p.scale = scale, p.c = scale * 1.44269504f;
+  const hipStream_t st = (hipStream_t)stream;
+  const unsigned grid = (unsigned)(B * Hk * a.tiles * a.splits);
+  with_attn(dtype, D, [&](auto f, auto dp) {
+    constexpr bool F = decltype(f)::value;
+    constexpr int DP = decltype(dp)::value;
+    if (a.few) attn_few_kernel<F, DP><<<grid, 256, 0, st>>>(p);
+    else if (a.qt == 2) attn_fwd_kernel<F, DP, 2><<<grid, 256, 0, st>>>(p);
+    else attn_fwd_kernel<F, DP, 1><<<grid, 256, 0, st>>>(p);
+    if (a.splits > 1) {
+      const int64_t per = 256 / DP;
+      attn_join_kernel<F, DP><<<(unsigned)((B * Hk * p.rows + per - 1) / per), 256, 0, st>>>(p);
+    }
+  });
+  return (int)hipGetLastError();
+}
+
+// delta, the row tiles' largest norms, the splits' parts of dk and dv: bytes before each, and of all
+struct AttnBwdSpace {
+  size_t rowmax, part, all;
+};
+static AttnBwdSpace attn_bwd_space(const AttnPlan &a, int64_t B, int64_t H, int64_t Hk, int64_t N, int64_t L, int64_t D) {
+  auto up = [](size_t n) { return (n + 255) & ~size_t(255); };
+  AttnBwdSpace s;
+  s.rowmax = up((size_t)B * H * N * sizeof(float));
+  s.part = s.rowmax + up((size_t)B * Hk * a.btiles * sizeof(float));
+  s.all = s.part + (a.ksplits > 1 ? (size_t)a.ksplits * B * Hk * L * 2 * D * sizeof(float) : 0);
+  return s;
+}
+
+size_t gpic_fp8_attention_bwd_workspace_bytes(int64_t B, int64_t H, int64_t Hk, int64_t N, int64_t L, int64_t D) {
+  if (attn_shape(GPIC_DTYPE_BF16, B, H, Hk, N, L, D) != GPIC_OK) return 0;
+  return attn_bwd_space(attn_plan(B, H, Hk, N, L, D), B, H, Hk, N, L, D).all;
+}
+
+int gpic_fp8_attention_bwd(const uint16_t *dout, const int64_t *ds, const uint16_t *q, const int64_t *qs, const uint16_t *k,
+                           const int64_t *ks, const uint16_t *v, const int64_t *vs, const uint16_t *o, const int64_t *os,
+                           const float *lse, int dtype, const int *lens, const uint8_t *mask, int64_t ldm, int64_t B, int64_t H,
+                           int64_t Hk, int64_t N, int64_t L, int64_t D, float scale, uint16_t *dq, const int64_t *dqs,
+                           uint16_t *dk, const int64_t *dks, uint16_t *dv, const int64_t *dvs, void *ws, size_t ws_bytes,
+                           void *stream) {
+  status_scope();
+  int e = attn_shape(dtype, B, H, Hk, N, L, D);
+  if (e != GPIC_OK) return e;
+  if (!(scale > 0.0f) || scale == kInf) return GPIC_EINVAL;
+  if (!dk != !dv) return GPIC_EINVAL;
+  const bool rows = B * N > 0, keys = B * L > 0;
+  if (!rows && !keys) return GPIC_OK;
+  if ((rows && (!q || !dout || !o || !lse || !dq)) || (keys && (!k || !v)) || (mask && ldm < 0)) return GPIC_EINVAL;
+  AttnArgs p{};
+  if ((e = strides_ok(dout, ds, p.ds)) || (e = strides_ok(q, qs, p.qs)) || (e = strides_ok(k, ks, p.ks)) ||
+      (e = strides_ok(v, vs, p.vs)) || (e = strides_ok(o, os, p.os)) || (e = strides_ok(dq, dqs, p.dqs)) ||
+      (dk && ((e = strides_ok(dk, dks, p.dks)) || (e = strides_ok(dv, dvs, p.dvs)))))
+    return e;
+  if (!aligned16(ws)) return GPIC_EALIGN;
+  const AttnPlan a = attn_plan(B, H, Hk, N, L, D);
+  const AttnBwdSpace space = attn_bwd_space(a, B, H, Hk, N, L, D);
+  if (ws_bytes < space.all || (space.all && !ws)) return GPIC_EWORKSPACE;
+  p.q = q, p.k = k, p.v = v, p.o = o, p.dout = dout, p.dq = dq, p.dk = dk, p.dv = dv, p.lens = lens, p.mask = mask, p.ldm = ldm;
+  p.lse = const_cast<float *>(lse);
+  char *w = static_cast<char *>(ws);
+  p.delta = reinterpret_cast<float *>(w), p.rowmax = reinterpret_cast<float *>(w + space.rowmax);
+  p.part = reinterpret_cast<float *>(w + space.part);
+  p.B = (int)B, p.H = (int)H, p.Hk = (int)Hk, p.N = (int)N, p.L = (int)L, p.D = (int)D, p.G = (int)(H / Hk);
+  p.rows = p.G * p.N, p.scale = scale, p.c = scale * 1.44269504f, p.rtiles = a.btiles;
+  const hipStream_t st = (hipStream_t)stream;
+  with_attn(dtype, D, [&](auto f, auto dp) {
+    constexpr bool F = decltype(f)::value;
+    constexpr int DP = decltype(dp)::value;
+    if (rows) {
+      p.tiles = a.btiles, p.splits = 1;
+      const unsigned grid = (unsigned)(B * Hk * a.btiles);
+      if (a.bqt == 2) attn_dq_kernel<F, DP, 2><<<grid, 256, 0, st>>>(p);
+      else attn_dq_kernel<F, DP, 1><<<grid, 256, 0, st>>>(p);
+    }
+    if (keys && dk) {
+      p.tiles = a.ktiles, p.splits = a.ksplits;
+      const unsigned grid = (unsigned)(B * Hk * a.ktiles * a.ksplits);
+      if constexpr (DP == 64) {
+        if (a.kt == 2) attn_dkv_kernel<F, DP, 2><<<grid, 256, 0, st>>>(p);
+        else attn_dkv_kernel<F, DP, 1><<<grid, 256, 0, st>>>(p);
+      } else {
+        attn_dkv_kernel<F, DP, 1><<<grid, 256, 0, st>>>(p);
+      }
+      if (a.ksplits > 1)
+        attn_dkv_join_kernel<F><<<(unsigned)((B * Hk * L * (D / 2) + 255) / 256), 256, 0, st>>>(p);
+    }
+  });
+  return (int)hipGetLastError();
+}
+
+}  // extern "C"

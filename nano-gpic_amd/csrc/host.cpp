@@ -13,6 +13,7 @@
 #include <ATen/ATen.h>
 #include <ATen/EmptyTensor.h>
 #include <ATen/hip/impl/HIPCachingAllocatorMasqueradingAsCUDA.h>
+#include <ATen/core/LegacyTypeDispatch.h>
 #include <c10/core/GradMode.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/Exceptions.h>
@@ -20,6 +21,7 @@
 #include <torch/csrc/autograd/functions/utils.h>
 #include <torch/csrc/utils/pybind.h>
 
+#include <cmath>
 #include <optional>
 #include <string>
 
@@ -964,6 +966,129 @@ py::object layer_norm_bwd(const at::Tensor &dh, const opt &dxn, const at::Tensor
   return py::make_tuple(dx, dw, db);
 }
 
+// ------------------------------------------------------------------------------------------- attention
+
+// [B, H, N, D] as the kernels read it, and its strides (0 for an extent of one)
+bool heads_ok(const at::Tensor &t, at::ScalarType ty, int dev, int64_t (&s)[3]) {
+  if (t.dim() != 4 || t.scalar_type() != ty || !t.is_cuda() || t.get_device() != dev || !has_memory(t) ||
+      t.layout() != at::kStrided || t.numel() == 0 || t.stride(3) != 1 || (reinterpret_cast<uintptr_t>(t.data_ptr()) & 15u))
+    return false;
+  for (int i = 0; i < 3; i++) {
+    s[i] = t.size(i) > 1 ? t.stride(i) : 0;
+    if (s[i] % 8) return false;
+  }
+  return true;
+}
+struct AttnIn {
+  int64_t B, H, Hk, N, L, D, qs[3], ks[3], vs[3], ldm = 0;
+  const int *lens = nullptr;
+  const uint8_t *mask = nullptr;
+  int dtype;
+};
+bool attn_ok(const at::Tensor &q, const at::Tensor &k, const at::Tensor &v, const opt &lens, const opt &mask, double scale, int dev,
+             AttnIn &in) {
+  const at::ScalarType ty = q.scalar_type();
+  if ((ty != at::kBFloat16 && ty != at::kHalf) || !heads_ok(q, ty, dev, in.qs) || !heads_ok(k, ty, dev, in.ks) ||
+      !heads_ok(v, ty, dev, in.vs) || k.sizes() != v.sizes() || q.size(0) != k.size(0) || q.size(3) != k.size(3))
+    return false;
+  in.B = q.size(0), in.H = q.size(1), in.N = q.size(2), in.D = q.size(3), in.Hk = k.size(1), in.L = k.size(2);
+  in.dtype = ty == at::kHalf ? GPIC_DTYPE_F16 : GPIC_DTYPE_BF16;
+  if (in.D > 128 || in.D % 8 || in.H % in.Hk || !(scale > 0.0) || !((float)scale < INFINITY)) return false;
+  if (lens) {
+    if (lens->scalar_type() != at::kInt || lens->dim() != 1 || lens->size(0) != in.B || !lens->is_cuda() ||
+        lens->get_device() != dev || !has_memory(*lens) || !lens->is_contiguous())
+      return false;
+    in.lens = ptr<int>(*lens);
+  }
+  if (mask) {
+    if (mask->scalar_type() != at::kBool || mask->dim() != 2 || mask->size(0) != in.B || mask->size(1) != in.L || !mask->is_cuda() ||
+        mask->get_device() != dev || !has_memory(*mask) || mask->layout() != at::kStrided || mask->stride(1) != 1 ||
+        mask->stride(0) < 0)
+      return false;
+    in.mask = static_cast<const uint8_t *>(mask->data_ptr());
+    in.ldm = mask->stride(0);
+  }
+  return true;
+}
+// [B, H, N, D], [B, N, H, D] in memory: a view of a new tensor, as the general form makes it
+at::Tensor make_heads(const at::Tensor &like, int64_t B, int64_t H, int64_t N, int64_t D, int64_t (&s)[3]) {
+  s[0] = N * H * D, s[1] = D, s[2] = H * D;
+  return make(like, {B, N, H, D}, like.scalar_type()).transpose(1, 2);
+}
+at::Tensor attn_run(const at::Tensor &q, const at::Tensor &k, const at::Tensor &v, const AttnIn &in, double scale, float *lse,
+                    void *stream) {
+  int64_t os[3];
+  at::Tensor o = make_heads(q, in.B, in.H, in.N, in.D, os);
+  const size_t bytes = gpic_fp8_attention_workspace_bytes(in.B, in.H, in.Hk, in.N, in.L, in.D);
+  at::Tensor ws;
+  if (bytes) ws = make(q, {(int64_t)bytes}, at::kByte);
+  check(gpic_fp8_attention(ptr<uint16_t>(q), in.qs, ptr<uint16_t>(k), in.ks, ptr<uint16_t>(v), in.vs, in.dtype, in.lens, in.mask,
+                           in.ldm, in.B, in.H, in.Hk, in.N, in.L, in.D, (float)scale, ptr<uint16_t>(o), os, lse,
+                           bytes ? ws.data_ptr() : nullptr, bytes, stream),
+        "gpic_fp8_attention");
+  return o;
+}
+
+// (o, lse, empty unless asked for); for the op and the autograd Function, which have looked whether a gradient is recorded
+py::object attention(const at::Tensor &q, const at::Tensor &k, const at::Tensor &v, const opt &lens, const opt &mask, double scale,
+                     bool want_lse, int dev, handle, handle stream) {
+  AttnIn in;
+  const opt oq = q, ok = k, ov = v;
+  if (!attn_ok(q, k, v, lens, mask, scale, dev, in) || records({&oq, &ok, &ov})) return py::none();
+  at::Tensor o, lse;
+  {
+    NoGil no_gil;
+    at::AutoDispatchBelowADInplaceOrView below;
+    lse = want_lse ? make(q, {in.B, in.H, in.N}, at::kFloat) : none_of(q, at::kFloat);
+    o = attn_run(q, k, v, in, scale, want_lse ? ptr<float>(lse) : nullptr, vp(stream));
+  }
+  return py::make_tuple(o, lse);
+}
+
+py::object attention_served(const at::Tensor &q, const at::Tensor &k, const at::Tensor &v, const opt &lens, const opt &mask,
+                            double scale, int dev, handle, handle stream) {
+  AttnIn in;
+  const opt oq = q, ok = k, ov = v;
+  if (!attn_ok(q, k, v, lens, mask, scale, dev, in) || records({&oq, &ok, &ov})) return py::none();
+  at::Tensor o;
+  {
+    NoGil no_gil;
+    at::AutoDispatchBelowADInplaceOrView below;
+    o = attn_run(q, k, v, in, scale, nullptr, vp(stream));
+  }
+  return py::cast(o);
+}
+
+py::object attention_bwd(const at::Tensor &dout, const at::Tensor &q, const at::Tensor &k, const at::Tensor &v, const at::Tensor &o,
+                         const at::Tensor &lse, const opt &lens, const opt &mask, double scale, bool want_kv, int dev, handle,
+                         handle stream) {
+  AttnIn in;
+  int64_t ds[3], os[3], dqs[3], dks[3], dvs[3];
+  const opt od = dout, oq = q, ok = k, ov = v, oo = o, ol = lse;
+  const at::ScalarType ty = q.scalar_type();
+  if (!attn_ok(q, k, v, lens, mask, scale, dev, in) || !heads_ok(dout, ty, dev, ds) || !heads_ok(o, ty, dev, os) ||
+      dout.sizes() != q.sizes() || o.sizes() != q.sizes() || lse.dim() != 3 || lse.scalar_type() != at::kFloat || !plain(lse, dev) ||
+      lse.numel() != in.B * in.H * in.N || lse.size(0) != in.B || lse.size(1) != in.H ||
+      records({&od, &oq, &ok, &ov, &oo, &ol}))
+    return py::none();
+  at::Tensor dq, dk, dv;
+  {
+    NoGil no_gil;
+    at::AutoDispatchBelowADInplaceOrView below;
+    dq = make_heads(q, in.B, in.H, in.N, in.D, dqs);
+    dk = want_kv ? make_heads(q, in.B, in.Hk, in.L, in.D, dks) : none_of(q, ty);
+    dv = want_kv ? make_heads(q, in.B, in.Hk, in.L, in.D, dvs) : none_of(q, ty);
+    const size_t bytes = gpic_fp8_attention_bwd_workspace_bytes(in.B, in.H, in.Hk, in.N, in.L, in.D);
+    const at::Tensor ws = make(q, {std::max<int64_t>((int64_t)bytes, 16)}, at::kByte);
+    check(gpic_fp8_attention_bwd(ptr<uint16_t>(dout), ds, ptr<uint16_t>(q), in.qs, ptr<uint16_t>(k), in.ks, ptr<uint16_t>(v), in.vs,
+                                 ptr<uint16_t>(o), os, ptr<float>(lse), in.dtype, in.lens, in.mask, in.ldm, in.B, in.H, in.Hk, in.N,
+                                 in.L, in.D, (float)scale, ptr<uint16_t>(dq), dqs, want_kv ? ptr<uint16_t>(dk) : nullptr, dks,
+                                 want_kv ? ptr<uint16_t>(dv) : nullptr, dvs, ws.data_ptr(), bytes, vp(stream)),
+          "gpic_fp8_attention_bwd");
+  }
+  return py::make_tuple(dq, dk, dv);
+}
+
 }  // namespace
 
 PYBIND11_MODULE(_gpic_host, m) {   // (wrapped: torch's own errors, out of memory among them, stay what they are)
@@ -980,6 +1105,9 @@ PYBIND11_MODULE(_gpic_host, m) {   // (wrapped: torch's own errors, out of memor
   m.def("layer_norm_served", torch::wrap_pybind_function(&layer_norm_served));
   m.def("layer_norm_rows", torch::wrap_pybind_function(&layer_norm_rows));
   m.def("layer_norm_bwd", torch::wrap_pybind_function(&layer_norm_bwd));
+  m.def("attention", torch::wrap_pybind_function(&attention));
+  m.def("attention_served", torch::wrap_pybind_function(&attention_served));
+  m.def("attention_bwd", torch::wrap_pybind_function(&attention_bwd));
   m.def("linear_rows_bwd", torch::wrap_pybind_function(&linear_rows_bwd));
   m.def("norm_linear_rows_fwd", torch::wrap_pybind_function(&norm_linear_rows_fwd));
   m.def("linear_rows", torch::wrap_pybind_function(&linear_rows));

@@ -68,6 +68,11 @@ SIGNATURES = {
     "gpic_fp8_layer_norm_bwd_workspace_bytes": (_sz, [_i64, _i64]),
     "gpic_fp8_layer_norm_bwd": (_int, [_vp, _vp, _vp, _int, _vp, _int, _vp, _vp, _i64, _i64, _vp, _vp, _int, _vp, _int, _vp, _sz,
                                         _vp]),
+    "gpic_fp8_attention_workspace_bytes": (_sz, [_i64] * 6),
+    "gpic_fp8_attention": (_int, [_vp] * 6 + [_int, _vp, _vp, _i64] + [_i64] * 6 + [ctypes.c_float, _vp, _vp, _vp, _vp, _sz,
+                                                                                     _vp]),
+    "gpic_fp8_attention_bwd_workspace_bytes": (_sz, [_i64] * 6),
+    "gpic_fp8_attention_bwd": (_int, [_vp] * 11 + [_int, _vp, _vp, _i64] + [_i64] * 6 + [ctypes.c_float] + [_vp] * 7 + [_sz, _vp]),
     "gpic_fp8_bf16_gemm_mn": (_int, [_vp, _i64, _vp, _i64, _vp, _int, _i64, _i64, _i64, _i64, _vp, _sz, _vp]),
 }
 
