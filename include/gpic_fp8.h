@@ -473,6 +473,20 @@ int gpic_fp8_attention_bwd(const uint16_t *dout, const int64_t *ds, const uint16
                            uint16_t *dk, const int64_t *dks, uint16_t *dv, const int64_t *dvs, void *ws, size_t ws_bytes,
                            void *stream);
 
+/*
+ * Low-rank adapters of many requests beside a shared projection. No counterpart in the reference.
+ *   out[m] = y[m] + scales[i] (x[m] A_i^T) B_i^T, i = ids[m / per];  a row whose i is none of 0 .. n - 1: out[m] = y[m]
+ *   y [M, N] (row stride ldy; the shared projection's output), x [M, K] (row stride ldx), A [n, R, K], B [n, N, R], out [M, N], of
+ *   dtype (bf16 or fp16); scales [n] fp32 (NULL: ones); ids int32, or int64 with wide_ids: one for every `per` rows.
+ *   Sums are fp32, x A_i^T is kept to 2^-16 and better, out is rounded once; what an adapter holds reaches no row but its own.
+ *   N, K, R % 8 == 0, R <= 128; M, N, K, n < 2^30. out may not overlap the inputs. Deterministic.
+ *   ws: gpic_fp8_lora_rows_workspace_bytes(M, N, K, R, n) bytes, scratch of this call.
+ */
+size_t gpic_fp8_lora_rows_workspace_bytes(int64_t M, int64_t N, int64_t K, int64_t R, int64_t n);
+int gpic_fp8_lora_rows(const uint16_t *y, int64_t ldy, const uint16_t *x, int64_t ldx, const uint16_t *A, const uint16_t *B,
+                       const float *scales, const void *ids, int wide_ids, int64_t per, int dtype, int64_t M, int64_t N, int64_t K,
+                       int64_t R, int64_t n, uint16_t *out, void *ws, size_t ws_bytes, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -23,19 +23,13 @@
 
 #include "gpic_device.h"
 #include "gpic_launch.h"
+#include "gpic_mfma.h"
 
 namespace gpic {
 
-typedef short s16x4 __attribute__((ext_vector_type(4)));
-typedef short s16x8 __attribute__((ext_vector_type(8)));
-typedef float f32x4_t __attribute__((ext_vector_type(4)));
-typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
-typedef _Float16 f16x8v __attribute__((ext_vector_type(8)));
-typedef _Float16 f16x2v __attribute__((ext_vector_type(2)));
 typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
 
 constexpr int kTile = 64;   // rows of a staged tile
-constexpr float kInf = __builtin_huge_valf();
 
 struct AttnArgs {
   const uint16_t *q, *k, *v, *o, *dout;
@@ -50,37 +44,12 @@ struct AttnArgs {
   float c, scale;                                  // c: scale log2 e
 };
 
-template <bool F16>
-__device__ __forceinline__ f32x4_t mfma16(s16x8 a, s16x8 b, f32x4_t c) {
-  if constexpr (F16)
-    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8v, a), __builtin_bit_cast(f16x8v, b), c, 0, 0, 0);
-  else
-    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, a), __builtin_bit_cast(bf16x8_t, b), c, 0, 0, 0);
-}
-template <bool F16>
-__device__ __forceinline__ uint32_t pack16(float lo, float hi) {
-  if constexpr (F16) return __builtin_bit_cast(uint32_t, f16x2v{(_Float16)lo, (_Float16)hi});
-  else return pack_bf16(lo, hi);
-}
 // Two result tiles as a right operand.
 template <bool F16>
 __device__ __forceinline__ s16x8 operand(f32x4_t a, f32x4_t b) {
   return __builtin_bit_cast(s16x8, u32x4{pack16<F16>(a[0], a[1]), pack16<F16>(a[2], a[3]), pack16<F16>(b[0], b[1]),
                                          pack16<F16>(b[2], b[3])});
 }
-template <bool F16>
-__device__ __forceinline__ void floats8(s16x8 x, float (&f)[8]) {
-  if constexpr (F16) {
-    const f16x8v h = __builtin_bit_cast(f16x8v, x);
-#pragma unroll
-    for (int e = 0; e < 8; e++) f[e] = (float)h[e];
-  } else {
-    const u32x4 w = __builtin_bit_cast(u32x4, x);
-#pragma unroll
-    for (int e = 0; e < 8; e++) f[e] = e & 1 ? bf16_hi(w[e >> 1]) : bf16_lo(w[e >> 1]);
-  }
-}
-
 // Sum, or maximum, of a value over the four groups of 16 lanes, in every lane.
 __device__ __forceinline__ float groups_sum(float v) {
   v += __shfl_xor(v, 16, 64);

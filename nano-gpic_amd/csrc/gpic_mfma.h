@@ -1,0 +1,49 @@
+// The 16-bit matrix instruction of the attention and adapter kernels, and what its operands and results are made of:
+// v_mfma_f32_16x16x32 with bf16 or fp16 operands and fp32 sums. Lane l gives row (column) l & 15 and the 8 terms from 8 (l / 16) of
+// its operand, and holds rows 4 (l / 16) + v, v = 0 .. 3, of column l & 15 of the result.
+#pragma once
+#include "gpic_device.h"
+
+namespace gpic {
+
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef short s16x8 __attribute__((ext_vector_type(8)));
+typedef float f32x4_t __attribute__((ext_vector_type(4)));
+typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x8v __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x2v __attribute__((ext_vector_type(2)));
+
+constexpr float kInf = __builtin_huge_valf();
+
+template <bool F16>
+__device__ __forceinline__ f32x4_t mfma16(s16x8 a, s16x8 b, f32x4_t c) {
+  if constexpr (F16)
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8v, a), __builtin_bit_cast(f16x8v, b), c, 0, 0, 0);
+  else
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, a), __builtin_bit_cast(bf16x8_t, b), c, 0, 0, 0);
+}
+template <bool F16>
+__device__ __forceinline__ uint32_t pack16(float lo, float hi) {
+  if constexpr (F16) return __builtin_bit_cast(uint32_t, f16x2v{(_Float16)lo, (_Float16)hi});
+  else return pack_bf16(lo, hi);
+}
+template <bool F16>
+__device__ __forceinline__ void floats8(s16x8 x, float (&f)[8]) {
+  if constexpr (F16) {
+    const f16x8v h = __builtin_bit_cast(f16x8v, x);
+#pragma unroll
+    for (int e = 0; e < 8; e++) f[e] = (float)h[e];
+  } else {
+    const u32x4 w = __builtin_bit_cast(u32x4, x);
+#pragma unroll
+    for (int e = 0; e < 8; e++) f[e] = e & 1 ? bf16_hi(w[e >> 1]) : bf16_lo(w[e >> 1]);
+  }
+}
+// Rounded to the type and back.
+template <bool F16>
+__device__ __forceinline__ float round16(float f) {
+  if constexpr (F16) return (float)(_Float16)f;
+  else return bf16_round(f);
+}
+
+}  // namespace gpic

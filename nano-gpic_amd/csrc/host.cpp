@@ -1089,6 +1089,41 @@ py::object attention_bwd(const at::Tensor &dout, const at::Tensor &q, const at::
   return py::make_tuple(dq, dk, dv);
 }
 
+// ------------------------------------------------------------------------------------------- adapters
+
+py::object lora_rows(const at::Tensor &y, const at::Tensor &x, const at::Tensor &A, const at::Tensor &B, const at::Tensor &ids,
+                     const opt &scale, int dev, handle, handle stream) {
+  const at::ScalarType ty = y.scalar_type();
+  const opt oy = y, ox = x, oA = A, oB = B;
+  if ((ty != at::kBFloat16 && ty != at::kHalf) || x.scalar_type() != ty || A.scalar_type() != ty || B.scalar_type() != ty ||
+      y.dim() < 2 || x.dim() != y.dim() || A.dim() != 3 || B.dim() != 3 || !plain(y, dev) || !plain(x, dev) || !plain(A, dev) ||
+      !plain(B, dev) || !plain(ids, dev) || (ids.scalar_type() != at::kInt && ids.scalar_type() != at::kLong))
+    return py::none();
+  const int64_t N = y.size(-1), K = x.size(-1), n = A.size(0), R = A.size(1);
+  if (N <= 0 || K <= 0 || n <= 0 || R <= 0 || N % 8 || K % 8 || R % 8 || R > 128 || A.size(2) != K || B.size(0) != n ||
+      B.size(1) != N || B.size(2) != R || !scales_ok(scale, n, dev))
+    return py::none();
+  for (int64_t i = 0; i + 1 < y.dim(); i++)
+    if (x.size(i) != y.size(i)) return py::none();
+  const int64_t M = x.numel() / K;
+  if (M < 1 || (ids.sizes() != x.sizes().slice(0, x.dim() - 1) && !(ids.dim() == 1 && ids.size(0) == x.size(0))) ||
+      records({&oy, &ox, &oA, &oB, &scale}))
+    return py::none();
+  at::Tensor out;
+  {
+    NoGil no_gil;
+    out = make(y, y.sizes(), ty);
+    const size_t bytes = gpic_fp8_lora_rows_workspace_bytes(M, N, K, R, n);
+    const at::Tensor ws = make(y, {(int64_t)bytes}, at::kByte);
+    check(gpic_fp8_lora_rows(ptr<uint16_t>(y), N, ptr<uint16_t>(x), K, ptr<uint16_t>(A), ptr<uint16_t>(B),
+                             scale ? ptr<float>(*scale) : nullptr, ids.data_ptr(), ids.scalar_type() == at::kLong,
+                             M / ids.numel(), ty == at::kHalf ? GPIC_DTYPE_F16 : GPIC_DTYPE_BF16, M, N, K, R, n, ptr<uint16_t>(out),
+                             ws.data_ptr(), bytes, vp(stream)),
+          "gpic_fp8_lora_rows");
+  }
+  return py::cast(out);
+}
+
 }  // namespace
 
 PYBIND11_MODULE(_gpic_host, m) {   // (wrapped: torch's own errors, out of memory among them, stay what they are)
@@ -1108,6 +1143,7 @@ PYBIND11_MODULE(_gpic_host, m) {   // (wrapped: torch's own errors, out of memor
   m.def("attention", torch::wrap_pybind_function(&attention));
   m.def("attention_served", torch::wrap_pybind_function(&attention_served));
   m.def("attention_bwd", torch::wrap_pybind_function(&attention_bwd));
+  m.def("lora_rows", torch::wrap_pybind_function(&lora_rows));
   m.def("linear_rows_bwd", torch::wrap_pybind_function(&linear_rows_bwd));
   m.def("norm_linear_rows_fwd", torch::wrap_pybind_function(&norm_linear_rows_fwd));
   m.def("linear_rows", torch::wrap_pybind_function(&linear_rows));

@@ -7,6 +7,7 @@ from .fp8_native import (E4, FMAX, TINY, Fp8Linear, Fp8LinearF8, convert_native,
                          fp8_heads_linear_f8, fp8_linear, fp8_linear_f8, fp8_mlp, fp8_mlp_f8, fp8_swiglu_w3, reference,
                          swiglu_bwd, swiglu_bwd_q, swiglu_bwd_t, swiglu_tcast, swiglu_tcast_t, tcast, tcast_heads,
                          tcast_t, tcast_t_group, weight_casts, _mm)
+from .adapters import lora_rows
 from .attention import cross_attention, cross_attention_bwd, cross_attention_fwd
 from .fp8 import KEEP, convert_fp8, fp8_filter
 from .heads import Fp8HeadsLinearF8, convert_fused_heads
@@ -27,4 +28,4 @@ __all__ = ["E4", "FMAX", "TINY", "Fp8Linear", "Fp8LinearF8", "convert_native", "
            "RowsWeight", "act_bwd_rows", "fp8_gemm_rows", "fp8_linear_rows", "fp8_rmsnorm_linear_rows", "rmsnorm_rows",
            "rmsnorm_rows_bwd", "rows_weight", "swiglu_layout", "tcast_rows",
            "layer_norm", "layer_norm_rows", "layer_norm_bwd", "cross_attention",
-           "cross_attention_fwd", "cross_attention_bwd"]
+           "cross_attention_fwd", "cross_attention_bwd", "lora_rows"]

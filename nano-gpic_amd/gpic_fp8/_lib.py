@@ -73,6 +73,8 @@ SIGNATURES = {
                                                                                      _vp]),
     "gpic_fp8_attention_bwd_workspace_bytes": (_sz, [_i64] * 6),
     "gpic_fp8_attention_bwd": (_int, [_vp] * 11 + [_int, _vp, _vp, _i64] + [_i64] * 6 + [ctypes.c_float] + [_vp] * 7 + [_sz, _vp]),
+    "gpic_fp8_lora_rows_workspace_bytes": (_sz, [_i64] * 5),
+    "gpic_fp8_lora_rows": (_int, [_vp, _i64, _vp, _i64, _vp, _vp, _vp, _vp, _int, _i64, _int] + [_i64] * 5 + [_vp, _vp, _sz, _vp]),
     "gpic_fp8_bf16_gemm_mn": (_int, [_vp, _i64, _vp, _i64, _vp, _int, _i64, _i64, _i64, _i64, _vp, _sz, _vp]),
 }
 

@@ -10,7 +10,7 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(os.path.dirname(HERE), "csrc")
 INCLUDE = os.path.join(os.path.dirname(os.path.dirname(HERE)), "include")
 LIB = os.path.join(HERE, "libgpic_fp8.so")
-SOURCES = ["api.hip", "attention.hip", "cast.hip", "gemm.hip", "layernorm.hip", "norm.hip", "rows.hip"]
+SOURCES = ["api.hip", "attention.hip", "cast.hip", "gemm.hip", "layernorm.hip", "lora.hip", "norm.hip", "rows.hip"]
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 
 FLAGS = [
