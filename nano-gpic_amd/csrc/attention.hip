@@ -60,12 +60,6 @@ __device__ __forceinline__ float groups_max(float v) {
   return fmaxf(v, __shfl_xor(v, 32, 64));
 }
 
-// The workgroup's number with the workgroups of one XCD (every eighth) next to each other: they share k and v in its L2.
-__device__ __forceinline__ uint32_t xcd_order(uint32_t id, uint32_t n) {
-  const uint32_t x = id & 7, q = n >> 3, r = n & 7;
-  return x * q + min(x, r) + (id >> 3);
-}
-
 template <int DP>
 __device__ __forceinline__ int swz(int r) {
   return DP == 64 ? ((r >> 1) & 3) << 1 | ((r >> 3) & 1) : (r & 7) << 1 | ((r >> 3) & 1);

@@ -111,6 +111,12 @@ __device__ __forceinline__ float exp_cw(float t) {
 
 __device__ __forceinline__ float sigmoid(float x) { return __fdiv_rn(1.0f, 1.0f + exp_cw(-x)); }
 
+// The workgroup's number with the workgroups of one XCD (every eighth) next to each other: what neighbours share stays in its L2.
+__device__ __forceinline__ uint32_t xcd_order(uint32_t id, uint32_t n) {
+  const uint32_t x = id & 7, q = n >> 3, r = n & 7;
+  return x * q + min(x, r) + (id >> 3);
+}
+
 // ------------------------------------------------------------------------------------------- reductions
 
 __device__ __forceinline__ uint32_t wave_max_u32(uint32_t v) {

@@ -31,7 +31,7 @@ struct LoraArgs {
   float *up;   // fp16: the factors of t's rows
   int64_t ldx, ldy;
   int M, per, N, K, R, n, wide_ids;   // wide_ids: 64-bit ids
-  int splits, groups, cols;           // parts of K; workgroups that share a tile's passes; columns of a workgroup
+  int splits, groups, blocks, cols;   // parts of K; workgroups that share a tile's passes; column blocks, of cols columns each
 };
 constexpr int kMaxSplits = 4;
 
@@ -43,7 +43,8 @@ __device__ __forceinline__ int adapter_of(const LoraArgs &p, int m) {
   return i >= 0 && i < p.n ? (int)i : -1;
 }
 
-// Sixteen bytes of a row from element 8 c, zeros where off.
+// Sixteen bytes of a row from element 8 c, or zeros.
+__device__ __forceinline__ s16x8 chunk16(const uint16_t *row, int c) { return *reinterpret_cast<const s16x8 *>(row + 8 * c); }
 __device__ __forceinline__ s16x8 chunk16(const uint16_t *row, int c, bool on) {
   s16x8 z = {0, 0, 0, 0, 0, 0, 0, 0};
   if (on) z = *reinterpret_cast<const s16x8 *>(row + 8 * c);
@@ -71,18 +72,40 @@ __device__ __forceinline__ void row_factor(float most, float &down, float &up) {
   }
 }
 
-// t of 16 RT rows (NT tiles of 16 of the rank): the workgroups' parts of K (kParts), and in them the four waves', added in their
-// order. The next step's loads are under way during a step's products.
+// t of 16 RT rows (NT tiles of 16 of the rank): the workgroups' parts of K (kParts), and in them the waves', added in their
+// order.
+template <int NT>
+constexpr int kShrinkWaves = NT == 8 ? 4 : 8;
+
 template <bool F16, int RT, int NT, bool kParts>
-__global__ __launch_bounds__(256) void lora_shrink_kernel(LoraArgs p) {
-  __shared__ float red[16 * RT][16 * NT + 1];
+__global__ __launch_bounds__(64 * kShrinkWaves<NT>) void lora_shrink_kernel(LoraArgs p) {
+  constexpr int W = kShrinkWaves<NT>;
+  __shared__ float red[W][16 * RT][16 * NT + 1];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l15 = lane & 15, g = lane >> 4;
   const int row0 = blockIdx.x * 16 * RT;
   const int split = blockIdx.y, group = blockIdx.z;
+  const int steps = (p.K + 63) / 64, per = (steps + W * p.splits - 1) / (W * p.splits);
+  const int first = (split * W + wave) * per, end = min(steps, first + per), whole = min(end, p.K / 64);
+  // 64 of K a step, 16 from 16 g for group g: whole lines of x and A at a time. Loads have no conditions, so that they stay in
+  // flight behind the products of the step before: rows past the last and of other passes, and the rank's past R, are read from
+  // rows that are there, and what they give is not kept. K's last step, where it is none of 64, loads zeros past K.
+  const uint16_t *xr[RT];
+#pragma unroll
+  for (int i = 0; i < RT; i++) xr[i] = p.x + (int64_t)min(row0 + 16 * i + l15, p.M - 1) * p.ldx;
+  struct Step {
+    s16x8 a[RT][2], b[NT][2];
+  };
+  auto fetch_x = [&](int s, Step &f) {
+#pragma unroll
+    for (int h = 0; h < 2; h++)
+#pragma unroll
+      for (int i = 0; i < RT; i++) f.a[i][h] = chunk16(xr[i], 8 * s + 2 * g + h);
+  };
+  Step f0, f1;
+  if (first < whole) fetch_x(first, f0);   // (before the ids are known, which A waits for)
   const int id = lane < 16 * RT ? adapter_of(p, row0 + lane) : -1;
-  const int steps = (p.K + 31) / 32, per = (steps + 4 * p.splits - 1) / (4 * p.splits);
-  const int first = (split * 4 + wave) * per, end = min(steps, first + per);
   uint64_t todo = __ballot(id >= 0);
+  bool again = false;
   for (int pass = 0; todo; pass++) {
     const int cur = __builtin_amdgcn_readlane(id, __builtin_ctzll(todo));
     const uint64_t mine = __ballot(id == cur);
@@ -93,55 +116,83 @@ __global__ __launch_bounds__(256) void lora_shrink_kernel(LoraArgs p) {
     for (int i = 0; i < RT; i++)
 #pragma unroll
       for (int j = 0; j < NT; j++) acc[i][j] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
-    const uint16_t *A = p.A + (int64_t)cur * p.R * p.K;
-    s16x8 a[RT], b[NT];
-    auto fetch = [&](int s) {
-      const int c = 4 * s + g;
-      const bool in = s < end && 8 * c < p.K;
+    const uint16_t *Ar[NT];
 #pragma unroll
-      for (int i = 0; i < RT; i++)
-        a[i] = chunk16(p.x + (int64_t)(row0 + 16 * i + l15) * p.ldx, c, in && (mine >> (16 * i + l15) & 1));
+    for (int j = 0; j < NT; j++) Ar[j] = p.A + ((int64_t)cur * p.R + min(16 * j + l15, p.R - 1)) * p.K;
+    auto fetch_A = [&](int s, Step &f) {
 #pragma unroll
-      for (int j = 0; j < NT; j++) b[j] = chunk16(A + (int64_t)(16 * j + l15) * p.K, c, in && 16 * j + l15 < p.R);
+      for (int h = 0; h < 2; h++)
+#pragma unroll
+        for (int j = 0; j < NT; j++) f.b[j][h] = chunk16(Ar[j], 8 * s + 2 * g + h);
     };
-    fetch(first);
-    for (int s = first; s < end; s++) {
-      s16x8 an[RT], bn[NT];
+    auto fetch = [&](int s, Step &f) {
+      fetch_x(s, f);
+      fetch_A(s, f);
+    };
+    auto multiply = [&](const Step &f) {
 #pragma unroll
-      for (int i = 0; i < RT; i++) an[i] = a[i];
-#pragma unroll
-      for (int j = 0; j < NT; j++) bn[j] = b[j];
-      fetch(s + 1);
-#pragma unroll
-      for (int i = 0; i < RT; i++)
-#pragma unroll
-        for (int j = 0; j < NT; j++) acc[i][j] = mfma16<F16>(an[i], bn[j], acc[i][j]);
-    }
-    for (int w = 0; w < 4; w++) {
-      if (wave == w) {
+      for (int h = 0; h < 2; h++)
 #pragma unroll
         for (int i = 0; i < RT; i++)
 #pragma unroll
-          for (int j = 0; j < NT; j++)
-#pragma unroll
-            for (int v = 0; v < 4; v++) {
-              float &r = red[16 * i + 4 * g + v][16 * j + l15];
-              r = w ? r + acc[i][j][v] : acc[i][j][v];
-            }
-      }
-      __syncthreads();
+          for (int j = 0; j < NT; j++) acc[i][j] = mfma16<F16>(f.a[i][h], f.b[j][h], acc[i][j]);
+    };
+    int s = first;
+    if (s < whole) {
+      if (again) fetch_x(s, f0);
+      fetch_A(s, f0);
     }
+    again = true;
+    for (; s + 2 < whole; s += 2) {
+      fetch(s + 1, f1);
+      multiply(f0);
+      fetch(s + 2, f0);
+      multiply(f1);
+    }
+    if (s + 1 < whole) {
+      fetch(s + 1, f1);
+      multiply(f0);
+      multiply(f1);
+      s += 2;
+    } else if (s < whole) {
+      multiply(f0);
+      s++;
+    }
+    if (s < end) {
+#pragma unroll
+      for (int h = 0; h < 2; h++) {
+        const int c = 8 * s + 2 * g + h;
+#pragma unroll
+        for (int i = 0; i < RT; i++) f0.a[i][h] = chunk16(xr[i], c, 8 * c < p.K);
+#pragma unroll
+        for (int j = 0; j < NT; j++) f0.b[j][h] = chunk16(Ar[j], c, 8 * c < p.K);
+      }
+      multiply(f0);
+    }
+#pragma unroll
+    for (int i = 0; i < RT; i++)
+#pragma unroll
+      for (int j = 0; j < NT; j++)
+#pragma unroll
+        for (int v = 0; v < 4; v++) red[wave][16 * i + 4 * g + v][16 * j + l15] = acc[i][j][v];
+    __syncthreads();
+    auto sum = [&](int m, int r) {
+      float x = red[0][m][r];
+#pragma unroll
+      for (int w = 1; w < W; w++) x += red[w][m][r];
+      return x;
+    };
     if constexpr (kParts) {
-      for (int e = threadIdx.x; e < 16 * RT * p.R; e += 256) {
+      for (int e = threadIdx.x; e < 16 * RT * p.R; e += 64 * W) {
         const int m = e / p.R, r = e - m * p.R;
-        if (mine >> m & 1) static_cast<float *>(p.t)[((int64_t)split * p.M + row0 + m) * p.R + r] = red[m][r];
+        if (mine >> m & 1) static_cast<float *>(p.t)[((int64_t)split * p.M + row0 + m) * p.R + r] = sum(m, r);
       }
     } else {
       const int c = threadIdx.x & 15;   // (16 threads a row, 8 of the rank each)
-      for (int m = threadIdx.x >> 4; m < 16 * RT; m += 16) {
+      for (int m = threadIdx.x >> 4; m < 16 * RT; m += 4 * W) {
         float t[8], most = 0.0f, down = 1.0f, up = 1.0f;
 #pragma unroll
-        for (int e = 0; e < 8; e++) t[e] = c < 2 * NT ? red[m][8 * c + e] : 0.0f;
+        for (int e = 0; e < 8; e++) t[e] = 8 * c < p.R ? sum(m, 8 * c + e) : 0.0f;
         if (F16) {
 #pragma unroll
           for (int e = 0; e < 8; e++) most = fmaxf(most, fabsf(t[e]));
@@ -172,45 +223,32 @@ __global__ __launch_bounds__(256) void lora_expand_kernel(LoraArgs p) {
   constexpr int RP = 16 * NS;             // the rank in tiles of 16
   constexpr int NB = NS > 1 ? NS / 2 : 1;   // steps over B's chunks (a rank of one tile: both halves in one step)
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l15 = lane & 15, g = lane >> 4;
-  const int row0 = blockIdx.x * 16 * RT;
-  const int group = blockIdx.z;
-  const int id = lane < 16 * RT ? adapter_of(p, row0 + lane) : -1;
-  uint64_t todo = __ballot(lane < 16 * RT && row0 + lane < p.M);
-  const int c0 = blockIdx.y * p.cols, c1 = min(p.N, c0 + p.cols);
-  for (int pass = 0; todo; pass++) {
-    const int cur = __builtin_amdgcn_readlane(id, __builtin_ctzll(todo));
-    const uint64_t mine = __ballot(id == cur) & todo;   // (rows without an adapter are a pass too)
-    todo &= ~mine;
-    if (pass % p.groups != group) continue;
-    const uint16_t *B = p.B + (int64_t)max(cur, 0) * p.N * p.R;
-    u32x4 Y[RT];
+  // (workgroups beside each other take columns beside each other: rows whose length is a power of two would otherwise meet in few
+  // of the memory's channels)
+  const int tile = blockIdx.x / p.blocks, block = blockIdx.x - tile * p.blocks;
+  const int row0 = tile * 16 * RT;
+  const int group = blockIdx.y;
+  const int c0 = block * p.cols, c1 = min(p.N, c0 + p.cols);
+  // (loads without conditions, as above: of rows past the last and of other passes nothing is kept; t is zero past R, and B's
+  // chunks there are taken as zeros; a step that runs past the last column reads its last columns again)
+  const uint16_t *yr[RT];
+#pragma unroll
+  for (int i = 0; i < RT; i++) yr[i] = p.y + (int64_t)min(row0 + 16 * i + l15, p.M - 1) * p.ldy;
+  struct Step {
+    u32x4 y[RT];
     s16x8 b[2][NB];
-    auto fetch = [&](int c) {
-      const int col = c + 8 * g;
+  };
+  auto fetch_y = [&](int c, Step &f) {
 #pragma unroll
-      for (int i = 0; i < RT; i++) {
-        Y[i] = u32x4{0u, 0u, 0u, 0u};
-        if ((mine >> (16 * i + l15) & 1) && col < c1)
-          Y[i] = *reinterpret_cast<const u32x4 *>(p.y + (int64_t)(row0 + 16 * i + l15) * p.ldy + col);
-      }
-#pragma unroll
-      for (int h = 0; h < 2; h++) {
-        const int n = c + 8 * (l15 >> 2) + 4 * h + (l15 & 3);
-#pragma unroll
-        for (int k = 0; k < NB; k++) {
-          const int r = NS > 1 ? 32 * k + 8 * g : 8 * (g & 1);
-          b[h][k] = chunk16(B + (int64_t)n * p.R, r / 8, cur >= 0 && n < c1 && r < p.R);
-        }
-      }
-    };
-    int c = c0 + 32 * wave;
-    fetch(c);
-    s16x8 tf[RT][NS];
-    float up[RT];
+    for (int i = 0; i < RT; i++) f.y[i] = *reinterpret_cast<const u32x4 *>(yr[i] + min(c + 8 * g, (c1 - 1) & ~7));
+  };
+  Step f0, f1;
+  s16x8 tf[RT][NS];
+  float up[RT];
+  auto fetch_t = [&]() {
 #pragma unroll
     for (int i = 0; i < RT; i++) {
-      const int row = row0 + 16 * i + l15;
-      const bool on = cur >= 0 && (mine >> (16 * i + l15) & 1);
+      const int row = min(row0 + 16 * i + l15, p.M - 1);
       up[i] = 1.0f;
       if constexpr (kParts) {
         float t[NS][8], most = 0.0f, down = 1.0f;
@@ -220,18 +258,17 @@ __global__ __launch_bounds__(256) void lora_expand_kernel(LoraArgs p) {
           float4 part[kMaxSplits][2];
 #pragma unroll
           for (int s = 0; s < kMaxSplits; s++) {
-            part[s][0] = part[s][1] = float4{0.0f, 0.0f, 0.0f, 0.0f};
-            if (on && r < p.R && s < p.splits) {
-              const float4 *src = reinterpret_cast<const float4 *>(static_cast<const float *>(p.t) + ((int64_t)s * p.M + row) * p.R + r);
-              part[s][0] = src[0], part[s][1] = src[1];
-            }
+            const float4 *src = reinterpret_cast<const float4 *>(static_cast<const float *>(p.t) +
+                                                                 ((int64_t)min(s, p.splits - 1) * p.M + row) * p.R + min(r, p.R - 8));
+            part[s][0] = src[0], part[s][1] = src[1];
           }
 #pragma unroll
           for (int e = 0; e < 8; e++) {
             auto of = [&](int s) { return reinterpret_cast<const float *>(&part[s][0])[e]; };
             t[k][e] = of(0);
 #pragma unroll
-            for (int s = 1; s < kMaxSplits; s++) t[k][e] += of(s);
+            for (int s = 1; s < kMaxSplits; s++) t[k][e] += s < p.splits ? of(s) : 0.0f;
+            if (r >= p.R) t[k][e] = 0.0f;
             most = fmaxf(most, fabsf(t[k][e]));
           }
         }
@@ -248,40 +285,80 @@ __global__ __launch_bounds__(256) void lora_expand_kernel(LoraArgs p) {
         }
       } else {
 #pragma unroll
-        for (int k = 0; k < NS; k++) tf[i][k] = chunk16(static_cast<const uint16_t *>(p.t) + (int64_t)row * 2 * RP, 4 * k + g, on);
-        if (F16 && on) up[i] = p.up[row];
+        for (int k = 0; k < NS; k++) tf[i][k] = chunk16(static_cast<const uint16_t *>(p.t) + (int64_t)row * 2 * RP, 4 * k + g);
+        if (F16) up[i] = p.up[row];
       }
     }
-    const float s = cur >= 0 && p.s ? p.s[cur] : 1.0f;
-    for (; c < c1; c += 128) {
-      u32x4 Yc[RT];
-      s16x8 bc[2][NB];
+  };
+  if (!kParts) {   // (before the ids are known, which B waits for; few rows' workgroups may have no pass)
+    if (c0 + 32 * wave < c1) fetch_y(c0 + 32 * wave, f0);
+    fetch_t();
+  }
+  const int id = lane < 16 * RT ? adapter_of(p, row0 + lane) : -1;
+  uint64_t todo = __ballot(lane < 16 * RT && row0 + lane < p.M);
+  bool again = false;
+  for (int pass = 0; todo; pass++) {
+    const int cur = __builtin_amdgcn_readlane(id, __builtin_ctzll(todo));
+    const uint64_t mine = __ballot(id == cur) & todo;   // (rows without an adapter are a pass too)
+    todo &= ~mine;
+    if (pass % p.groups != group) continue;
+    const uint16_t *B = p.B + (int64_t)max(cur, 0) * p.N * p.R;
+    auto fetch_B = [&](int c, Step &f) {
 #pragma unroll
-      for (int i = 0; i < RT; i++) Yc[i] = Y[i];
+      for (int h = 0; h < 2; h++) {
+        const int n = min(c + 8 * (l15 >> 2) + 4 * h + (l15 & 3), c1 - 1);
+#pragma unroll
+        for (int k = 0; k < NB; k++) {
+          const int r = NS > 1 ? 32 * k + 8 * g : 8 * (g & 1);
+          f.b[h][k] = chunk16(B + (int64_t)n * p.R, min(r, p.R - 8) / 8);
+        }
+      }
+    };
+    auto fetch = [&](int c, Step &f) {
+      fetch_y(c, f);
+      fetch_B(c, f);
+    };
+    int c = c0 + 32 * wave;
+    if (c < c1) {
+      if (kParts || again) fetch_y(c, f0);
+      fetch_B(c, f0);
+    }
+    if (kParts && !again) fetch_t();
+    again = true;
+    const float s = cur >= 0 && p.s ? p.s[cur] : 1.0f;
+    auto put = [&](int c, Step &f) {
+      const int col = c + 8 * g;
 #pragma unroll
       for (int h = 0; h < 2; h++)
 #pragma unroll
-        for (int k = 0; k < NB; k++) bc[h][k] = b[h][k];
-      if (c + 128 < c1) fetch(c + 128);
-      const int col = c + 8 * g;
+        for (int k = 0; k < NB; k++)
+          if ((NS > 1 ? 32 * k + 8 * g : 8 * (g & 1)) >= p.R) f.b[h][k] = s16x8{0, 0, 0, 0, 0, 0, 0, 0};
 #pragma unroll
       for (int i = 0; i < RT; i++) {
-        f32x4_t acc[2] = {f32x4_t{0.0f, 0.0f, 0.0f, 0.0f}, f32x4_t{0.0f, 0.0f, 0.0f, 0.0f}};
-#pragma unroll
-        for (int h = 0; h < 2; h++)
-#pragma unroll
-          for (int k = 0; k < NS; k++) acc[h] = mfma16<F16>(bc[h][k % NB], tf[i][k], acc[h]);
-        if (!(mine >> (16 * i + l15) & 1) || col >= c1) continue;
+        u32x4 out = f.y[i];
         if (cur >= 0) {
-          float f[8];
-          floats8<F16>(__builtin_bit_cast(s16x8, Yc[i]), f);
+          f32x4_t acc[2] = {f32x4_t{0.0f, 0.0f, 0.0f, 0.0f}, f32x4_t{0.0f, 0.0f, 0.0f, 0.0f}};
 #pragma unroll
-          for (int e = 0; e < 8; e++) f[e] = __builtin_fmaf(F16 ? acc[e >> 2][e & 3] * up[i] : acc[e >> 2][e & 3], s, f[e]);
-          Yc[i] = u32x4{pack16<F16>(f[0], f[1]), pack16<F16>(f[2], f[3]), pack16<F16>(f[4], f[5]), pack16<F16>(f[6], f[7])};
+          for (int h = 0; h < 2; h++)
+#pragma unroll
+            for (int k = 0; k < NS; k++) acc[h] = mfma16<F16>(f.b[h][k % NB], tf[i][k], acc[h]);
+          float v[8];
+          floats8<F16>(__builtin_bit_cast(s16x8, out), v);
+#pragma unroll
+          for (int e = 0; e < 8; e++) v[e] = __builtin_fmaf(F16 ? acc[e >> 2][e & 3] * up[i] : acc[e >> 2][e & 3], s, v[e]);
+          out = u32x4{pack16<F16>(v[0], v[1]), pack16<F16>(v[2], v[3]), pack16<F16>(v[4], v[5]), pack16<F16>(v[6], v[7])};
         }
-        *reinterpret_cast<u32x4 *>(p.out + (int64_t)(row0 + 16 * i + l15) * p.N + col) = Yc[i];
+        if ((mine >> (16 * i + l15) & 1) && col < c1)
+          *reinterpret_cast<u32x4 *>(p.out + (int64_t)(row0 + 16 * i + l15) * p.N + col) = out;
       }
+    };
+    for (; c + 128 < c1; c += 256) {
+      fetch(c + 128, f1);
+      put(c, f0);
+      if (c + 256 < c1) fetch(c + 256, f0);
+      put(c + 128, f1);
     }
+    if (c < c1) put(c, f0);
   }
 }
 
@@ -294,13 +371,13 @@ static LoraPlan lora_plan(int64_t M, int64_t K, int64_t N, int64_t R, int64_t n)
   LoraPlan a;
   a.nt = R <= 16 ? 1 : R <= 32 ? 2 : R <= 64 ? 4 : 8;
   const bool few = M <= 256;
-  a.shrink_rt = M >= 8192 ? 2 : 1;
+  a.shrink_rt = M >= 8192 || (a.nt == 8 && M >= 1024) ? 2 : 1;
   a.rt = M < 1024 ? 1 : a.nt == 8 ? 2 : 4;
   a.groups = few ? (int)std::min<int64_t>(std::min<int64_t>(n + 1, M), 16) : 1;
   a.splits = few ? (int)std::max<int64_t>(std::min<int64_t>(K / 512, kMaxSplits), 1) : 1;   // (a wave 128 of K at least)
   const int64_t tiles = (M + 16 * a.rt - 1) / (16 * a.rt);
   a.cols = 128;
-  while (a.cols < 1024 && tiles * ((N + 2 * a.cols - 1) / (2 * a.cols)) >= 2048) a.cols *= 2;
+  while (!few && a.cols < 1024 && tiles * ((N + 2 * a.cols - 1) / (2 * a.cols)) >= 256) a.cols *= 2;
   return a;
 }
 static size_t lora_t_bytes(const LoraPlan &a, int64_t M, int64_t R) {
@@ -345,21 +422,21 @@ int gpic_fp8_lora_rows(const uint16_t *y, int64_t ldy, const uint16_t *x, int64_
   const int64_t tiles = (M + 16 * a.rt - 1) / (16 * a.rt), blocks = (N + a.cols - 1) / a.cols;
   const int64_t stiles = (M + 16 * a.shrink_rt - 1) / (16 * a.shrink_rt);
   // (a launch's threads are counted in 32 bits)
-  if (blocks > 65535 || tiles * blocks * a.groups >= (int64_t(1) << 24) || stiles * a.splits * a.groups >= (int64_t(1) << 24))
+  if (tiles * blocks * a.groups >= (int64_t(1) << 24) || stiles * a.splits * a.groups >= (int64_t(1) << 24))
     return GPIC_ESHAPE;
   char *w = static_cast<char *>(ws);
   const LoraArgs p{y, x, A, B, scales, ids, out, w, reinterpret_cast<float *>(w + lora_t_bytes(a, M, R)), ldx, ldy, (int)M, (int)per,
-                   (int)N, (int)K, (int)R, (int)n, wide_ids, a.splits, a.groups, a.cols};
+                   (int)N, (int)K, (int)R, (int)n, wide_ids, a.splits, a.groups, (int)blocks, a.cols};
   const hipStream_t st = (hipStream_t)stream;
   const dim3 shrink((unsigned)stiles, (unsigned)a.splits, (unsigned)a.groups),
-      expand((unsigned)tiles, (unsigned)blocks, (unsigned)a.groups);
+      expand((unsigned)(tiles * blocks), (unsigned)a.groups);
   auto launch = [&](auto f16) {
     constexpr bool F = decltype(f16)::value;
     with_rank(a.nt, [&](auto nt) {
       constexpr int T = decltype(nt)::value, W = T == 8 ? 2 : 4;
-      if (a.splits > 1) lora_shrink_kernel<F, 1, T, true><<<shrink, 256, 0, st>>>(p);
-      else if (a.shrink_rt == 2) lora_shrink_kernel<F, 2, T, false><<<shrink, 256, 0, st>>>(p);
-      else lora_shrink_kernel<F, 1, T, false><<<shrink, 256, 0, st>>>(p);
+      if (a.splits > 1) lora_shrink_kernel<F, 1, T, true><<<shrink, 64 * kShrinkWaves<T>, 0, st>>>(p);
+      else if (a.shrink_rt == 2) lora_shrink_kernel<F, 2, T, false><<<shrink, 64 * kShrinkWaves<T>, 0, st>>>(p);
+      else lora_shrink_kernel<F, 1, T, false><<<shrink, 64 * kShrinkWaves<T>, 0, st>>>(p);
       if (a.splits > 1) lora_expand_kernel<F, 1, T, true><<<expand, 256, 0, st>>>(p);
       else if (a.rt == W) lora_expand_kernel<F, W, T, false><<<expand, 256, 0, st>>>(p);
       else lora_expand_kernel<F, 1, T, false><<<expand, 256, 0, st>>>(p);
