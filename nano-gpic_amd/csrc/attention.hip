@@ -50,19 +50,28 @@ __device__ __forceinline__ s16x8 operand(f32x4_t a, f32x4_t b) {
   return __builtin_bit_cast(s16x8, u32x4{pack16<F16>(a[0], a[1]), pack16<F16>(a[2], a[3]), pack16<F16>(b[0], b[1]),
                                          pack16<F16>(b[2], b[3])});
 }
-// Sum, or maximum, of a value over the four groups of 16 lanes, in every lane.
+// Sum, or maximum, of a value over the four groups of 16 lanes, in every lane: two exchanges of half the lanes, in registers.
+template <class F>
+__device__ __forceinline__ float over_groups(float v, F f) {
+  const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  v = f(__uint_as_float(a[0]), __uint_as_float(a[1]));
+  const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return f(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
 __device__ __forceinline__ float groups_sum(float v) {
-  v += __shfl_xor(v, 16, 64);
-  return v + __shfl_xor(v, 32, 64);
+  return over_groups(v, [](float a, float b) { return a + b; });
 }
 __device__ __forceinline__ float groups_max(float v) {
-  v = fmaxf(v, __shfl_xor(v, 16, 64));
-  return fmaxf(v, __shfl_xor(v, 32, 64));
+  return over_groups(v, [](float a, float b) { return fmaxf(a, b); });
 }
 
+// A read by rows takes 16 lanes at a time, those of one group with rows 0-3 and 12-15 and those of the next with rows 4-11: the
+// values for the former are pairs (x, x ^ 1), so that the latter's, one chunk on, are the other pairs. A read by columns takes 8
+// rows: the values of each half are of different pairs.
 template <int DP>
 __device__ __forceinline__ int swz(int r) {
-  return DP == 64 ? ((r >> 1) & 3) << 1 | ((r >> 3) & 1) : (r & 7) << 1 | ((r >> 3) & 1);
+  const int u = DP == 64 ? r >> 1 & 7 : r & 15, half = DP == 64 ? 4 : 8, high = u / half;
+  return ((u + high * half / 2) & (half - 1)) << 1 | high;
 }
 
 // A lane's places in a staged tile (element offsets): for the read by rows of 16-row tile t and step ks, add t 16 DP to row[ks];
@@ -91,26 +100,45 @@ __device__ __forceinline__ s16x8 by_columns(uint16_t *tile, int t, int place) {
   return s16x8{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
 }
 
-// A tile of kTile rows on its way through registers: 256 threads, kU chunks each.
+// Sixteen zero bytes, for the lanes of a staged tile that have none of their own.
+__device__ const u32x4 kZeros = {0u, 0u, 0u, 0u};
+
+__device__ __forceinline__ uint32_t lds_at(const void *p) {
+  return (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const void *)p;
+}
+// Sixteen bytes a lane from its own address to LDS [lds, lds + 1 KiB) in lane order, past the registers. The loads are counted in
+// vmcnt but not by the compiler, so staged() comes before the barrier that hands the tile on. (Through registers the next tile cost
+// 16 to 32 of them, which kept the backward for rows of 128 at half its tile.)
+__device__ __forceinline__ void to_lds(const void *src, uint32_t lds) {
+  asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" : : "v"(src), "s"(lds) : "memory", "m0");
+}
+__device__ __forceinline__ void staged() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+
+// How 256 threads stage a tile of kTile rows: kU loads each, load u of wave w to places 64 (4 u + w) + lane, of which place i is
+// place i % kC of row i / kC and takes that row's chunk (i % kC) ^ swz(row).
 template <int DP>
 struct Stage {
   static constexpr int kC = DP / 8, kU = kTile * kC / 256;
-  u32x4 r[kU];
-  // Row i of the tile at base + i stride where bit i of rows is set; zeros elsewhere and past column D.
-  __device__ __forceinline__ void load(const uint16_t *base, int64_t stride, uint64_t rows, int D) {
-#pragma unroll
-    for (int u = 0; u < kU; u++) {
-      const int i = threadIdx.x + 256 * u, row = i / kC, c = i % kC;
-      r[u] = u32x4{0u, 0u, 0u, 0u};
-      if ((rows >> row & 1) && 8 * c < D) r[u] = *reinterpret_cast<const u32x4 *>(base + row * stride + 8 * c);
-    }
+  __device__ __forceinline__ static int row(int u) { return (64 * (4 * u + (int)(threadIdx.x >> 6)) + (int)(threadIdx.x & 63)) / kC; }
+  __device__ __forceinline__ static int chunk(int u) { return ((int)(threadIdx.x & 63) % kC) ^ swz<DP>(row(u)); }
+  __device__ __forceinline__ static void put(uint16_t *tile, int u, const uint16_t *src, bool on) {
+    const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    to_lds(on ? (const void *)src : (const void *)&kZeros, lds_at(tile) + 1024 * (4 * u + w));
   }
-  __device__ __forceinline__ void store(uint16_t *tile) const {
+};
+// The same for rows at one stride: a lane's offsets are kept.
+template <int DP>
+struct RowStage {
+  int64_t at[Stage<DP>::kU];
+  __device__ __forceinline__ explicit RowStage(int64_t stride) {
 #pragma unroll
-    for (int u = 0; u < kU; u++) {
-      const int i = threadIdx.x + 256 * u, row = i / kC, c = i % kC;
-      *reinterpret_cast<u32x4 *>(tile + row * DP + (c ^ swz<DP>(row)) * 8) = r[u];
-    }
+    for (int u = 0; u < Stage<DP>::kU; u++) at[u] = Stage<DP>::row(u) * stride + 8 * Stage<DP>::chunk(u);
+  }
+  // Row i at base + i stride where bit i of rows is set; zeros elsewhere and past column D.
+  __device__ __forceinline__ void load(uint16_t *tile, const uint16_t *base, uint64_t rows, int D) const {
+#pragma unroll
+    for (int u = 0; u < Stage<DP>::kU; u++)
+      Stage<DP>::put(tile, u, base + at[u], (rows >> Stage<DP>::row(u) & 1) && 8 * Stage<DP>::chunk(u) < D);
   }
 };
 
@@ -147,21 +175,24 @@ __device__ __forceinline__ s16x8 row_chunk(const uint16_t *row, int chunk, int D
   return z;
 }
 
-// The scores of a key tile as powers of two below the running maximum: p = 2^(c s - use), and what the sums so far shrink by.
+// The scores of a key tile as powers of two relative to a running maximum: p = 2^(c s - use). The maximum is brought up to date, and
+// o and l shrunk, only when some row of the wave has passed its own by 2^8: p stays below that, which 16 bits hold as well, and
+// most tiles skip it. The sum l is of p before its rounding: a sum of the rounded p, by a matrix instruction with ones, would move
+// lse, and with it the backward's P, by as much as P's own rounding does. A lane sums its own keys, in four parts.
 struct Softmax {
-  float m = -kInf, l = 0.0f, use = 0.0f;
-  // mx: the tile's maximum, the same in all groups; the factor for l and o
-  __device__ __forceinline__ float step(float mx, float c) {
-    const float before = m;
-    m = fmaxf(m, mx);
+  float use = -kInf;
+  // mx: the tile's maximum, the same in all groups. Whether the wave moves.
+  __device__ __forceinline__ bool moves(float mx, float c) const { return __ballot(mx * c > use + kSlack) != 0; }
+  // The factor for o and l.
+  __device__ __forceinline__ float move(float mx, float c) {
     const float old = use;
-    use = m == -kInf ? 0.0f : m * c;
-    const float f = before == -kInf ? 0.0f : __builtin_amdgcn_exp2f(old - use);
-    l *= f;
-    return f;
+    use = fmaxf(old, mx * c);
+    return old == -kInf ? 0.0f : __builtin_amdgcn_exp2f(old - use);
   }
+  // Of a row without a score above -inf so far, 0: its p are 0 all the same.
+  __device__ __forceinline__ float base() const { return use == -kInf ? 0.0f : use; }
+  static constexpr float kSlack = 8.0f;
 };
-
 // ------------------------------------------------------------------------------------------- forward
 
 // A workgroup's four waves take 16 QT rows each and walk the pair's keys (or its split's part of them) by tiles of 64, k and v
@@ -185,30 +216,31 @@ __global__ __launch_bounds__(256, 2) void attn_fwd_kernel(AttnArgs p) {
 #pragma unroll
     for (int k = 0; k < KS; k++) qf[i][k] = row_chunk(row, 4 * k + g, p.D, r < p.rows);
   }
-  f32x4_t O[QT][DT];
+  f32x4_t O[QT][DT], l4[QT];
   Softmax sm[QT];
 #pragma unroll
-  for (int i = 0; i < QT; i++)
+  for (int i = 0; i < QT; i++) {
+    l4[i] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
     for (int d = 0; d < DT; d++) O[i][d] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+  }
   const uint16_t *kb = p.k + b * p.ks[0] + hk * p.ks[1], *vb = p.v + b * p.vs[0] + hk * p.vs[1];
   const int n = (keys.len + kTile - 1) / kTile, per = (n + p.splits - 1) / p.splits;
   const int end = min(n, (split + 1) * per);
   uint64_t bits = 0, nbits = 0;
   int i = keys.next(split * per, end, bits);
-  Stage<DP> sk, sv;
+  const RowStage<DP> sk(p.ks[2]), sv(p.vs[2]);
   if (i < end) {
-    sk.load(kb + (int64_t)i * kTile * p.ks[2], p.ks[2], bits, p.D);
-    sv.load(vb + (int64_t)i * kTile * p.vs[2], p.vs[2], bits, p.D);
-    sk.store(kt[0]);
-    sv.store(vt[0]);
+    sk.load(kt[0], kb + (int64_t)i * kTile * p.ks[2], bits, p.D);
+    sv.load(vt[0], vb + (int64_t)i * kTile * p.vs[2], bits, p.D);
   }
+  staged();
   __syncthreads();
   for (int cur = 0; i < end; cur ^= 1, bits = nbits) {
     const int j = keys.next(i + 1, end, nbits);
     if (j < end) {
-      sk.load(kb + (int64_t)j * kTile * p.ks[2], p.ks[2], nbits, p.D);
-      sv.load(vb + (int64_t)j * kTile * p.vs[2], p.vs[2], nbits, p.D);
+      sk.load(kt[cur ^ 1], kb + (int64_t)j * kTile * p.ks[2], nbits, p.D);
+      sv.load(vt[cur ^ 1], vb + (int64_t)j * kTile * p.vs[2], nbits, p.D);
     }
     f32x4_t S[QT][4];
 #pragma unroll
@@ -223,6 +255,7 @@ __global__ __launch_bounds__(256, 2) void attn_fwd_kernel(AttnArgs p) {
       }
     }
     if (bits != ~0ull) {
+      asm volatile("");   // (a branch: as selections in every tile it costs a third of the softmax)
 #pragma unroll
       for (int t = 0; t < 4; t++) {
         const uint32_t on = (uint32_t)(bits >> (16 * t)) >> (4 * g);
@@ -240,20 +273,23 @@ __global__ __launch_bounds__(256, 2) void attn_fwd_kernel(AttnArgs p) {
       for (int t = 0; t < 4; t++)
 #pragma unroll
         for (int v = 0; v < 4; v++) mx = fmaxf(mx, S[q][t][v]);
-      const float before = sm[q].m;
-      const float f = sm[q].step(groups_max(mx), p.c);
-      if (__ballot(sm[q].m > before)) {
+      mx = groups_max(mx);
+      if (sm[q].moves(mx, p.c)) {
+        const float f = sm[q].move(mx, p.c);
 #pragma unroll
-        for (int d = 0; d < DT; d++)
+        for (int v = 0; v < 4; v++) {
+          l4[q][v] *= f;
 #pragma unroll
-          for (int v = 0; v < 4; v++) O[q][d][v] *= f;
+          for (int d = 0; d < DT; d++) O[q][d][v] *= f;
+        }
       }
+      const float use = sm[q].base();
 #pragma unroll
       for (int t = 0; t < 4; t++)
 #pragma unroll
         for (int v = 0; v < 4; v++) {
-          S[q][t][v] = __builtin_amdgcn_exp2f(__builtin_fmaf(S[q][t][v], p.c, -sm[q].use));
-          sm[q].l += S[q][t][v];
+          S[q][t][v] = __builtin_amdgcn_exp2f(__builtin_fmaf(S[q][t][v], p.c, -use));
+          l4[q][v] += S[q][t][v];
         }
       pf[q][0] = operand<F16>(S[q][0], S[q][1]);
       pf[q][1] = operand<F16>(S[q][2], S[q][3]);
@@ -266,17 +302,14 @@ __global__ __launch_bounds__(256, 2) void attn_fwd_kernel(AttnArgs p) {
 #pragma unroll
         for (int q = 0; q < QT; q++) O[q][d] = mfma16<F16>(a, pf[q][h], O[q][d]);
       }
-    if (j < end) {
-      sk.store(kt[cur ^ 1]);
-      sv.store(vt[cur ^ 1]);
-    }
+    staged();
     __syncthreads();
     i = j;
   }
 #pragma unroll
   for (int q = 0; q < QT; q++) {
     const int r = row0 + 16 * q + l15;
-    const float l = groups_sum(sm[q].l);
+    const float l = groups_sum((l4[q][0] + l4[q][1]) + (l4[q][2] + l4[q][3]));
     if (r >= p.rows) continue;
     if (p.splits > 1) {
       // (partial o, its maximum and sum: joined by attn_join_kernel)
@@ -286,7 +319,7 @@ __global__ __launch_bounds__(256, 2) void attn_fwd_kernel(AttnArgs p) {
       for (int d = 0; d < DT; d++)
 #pragma unroll
         for (int v = 0; v < 4; v++) o[16 * d + 4 * g + v] = O[q][d][v];
-      if (g == 0) o[DP] = l == 0.0f ? -kInf : sm[q].use, o[DP + 1] = l;
+      if (g == 0) o[DP] = l == 0.0f ? -kInf : sm[q].base(), o[DP + 1] = l;
       continue;
     }
     const float inv = l == 0.0f ? 0.0f : __fdiv_rn(1.0f, l);
@@ -297,7 +330,7 @@ __global__ __launch_bounds__(256, 2) void attn_fwd_kernel(AttnArgs p) {
         *reinterpret_cast<u32x2 *>(o + 16 * d + 4 * g) = u32x2{pack16<F16>(O[q][d][0] * inv, O[q][d][1] * inv),
                                                                pack16<F16>(O[q][d][2] * inv, O[q][d][3] * inv)};
     if (p.lse && g == 0)
-      p.lse[(int64_t)pair * p.rows + r] = l == 0.0f ? kInf : sm[q].use + __builtin_amdgcn_logf(l);
+      p.lse[(int64_t)pair * p.rows + r] = l == 0.0f ? kInf : sm[q].base() + __builtin_amdgcn_logf(l);
   }
 }
 
@@ -319,7 +352,7 @@ __global__ __launch_bounds__(256, 2) void attn_few_kernel(AttnArgs p) {
   const uint16_t *row = p.q + row_at(p, p.qs, b, hk, min(l15, p.rows - 1));
 #pragma unroll
   for (int k = 0; k < KS; k++) qf[k] = row_chunk(row, 4 * k + g, p.D, l15 < p.rows);
-  f32x4_t O[DT];
+  f32x4_t O[DT], l4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
   for (int d = 0; d < DT; d++) O[d] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
   Softmax sm;
@@ -377,30 +410,36 @@ __global__ __launch_bounds__(256, 2) void attn_few_kernel(AttnArgs p) {
         if (!(bits >> (16 * t + 4 * g + v) & 1)) S[t][v] = -kInf;
         mx = fmaxf(mx, S[t][v]);
       }
-    const float f = sm.step(groups_max(mx), p.c);
+    mx = groups_max(mx);
+    if (sm.moves(mx, p.c)) {
+      const float f = sm.move(mx, p.c);
+#pragma unroll
+      for (int v = 0; v < 4; v++) l4[v] *= f;
+#pragma unroll
+      for (int d = 0; d < DT; d++)
+#pragma unroll
+        for (int v = 0; v < 4; v++) O[d][v] *= f;
+    }
+    const float use = sm.base();
 #pragma unroll
     for (int t = 0; t < 2; t++)
 #pragma unroll
       for (int v = 0; v < 4; v++) {
-        S[t][v] = __builtin_amdgcn_exp2f(__builtin_fmaf(S[t][v], p.c, -sm.use));
-        sm.l += S[t][v];
+        S[t][v] = __builtin_amdgcn_exp2f(__builtin_fmaf(S[t][v], p.c, -use));
+        l4[v] += S[t][v];
       }
     const s16x8 pf = operand<F16>(S[0], S[1]);
 #pragma unroll
-    for (int d = 0; d < DT; d++) {
-#pragma unroll
-      for (int v = 0; v < 4; v++) O[d][v] *= f;
-      O[d] = mfma16<F16>(by_columns<DP>(vt[wave], 0, at.col[d]), pf, O[d]);
-    }
+    for (int d = 0; d < DT; d++) O[d] = mfma16<F16>(by_columns<DP>(vt[wave], 0, at.col[d]), pf, O[d]);
     i = j;
     bits = nbits;
   }
-  const float l = groups_sum(sm.l);
+  const float l = groups_sum((l4[0] + l4[1]) + (l4[2] + l4[3]));
 #pragma unroll
   for (int d = 0; d < DT; d++)
 #pragma unroll
     for (int v = 0; v < 4; v++) joined[wave][l15][16 * d + 4 * g + v] = O[d][v];
-  if (g == 0) joined[wave][l15][DP] = l == 0.0f ? -kInf : sm.use, joined[wave][l15][DP + 1] = l;
+  if (g == 0) joined[wave][l15][DP] = l == 0.0f ? -kInf : sm.base(), joined[wave][l15][DP + 1] = l;
   __syncthreads();
   for (int w = threadIdx.x; w < p.rows * DP; w += 256) {
     const int r = w / DP, d = w % DP;
@@ -497,7 +536,6 @@ __global__ __launch_bounds__(256, 2) void attn_dq_kernel(AttnArgs p) {
     }
     delta[i] = groups_sum(sum);
     lse[i] = on ? p.lse[(int64_t)pair * p.rows + r] : kInf;
-    if (on && g == 0) p.delta[(int64_t)pair * p.rows + r] = delta[i];
     up[i] = 1.0f;
     if (F16) {
       n2 = groups_sum(n2);
@@ -521,37 +559,76 @@ __global__ __launch_bounds__(256, 2) void attn_dq_kernel(AttnArgs p) {
   const int end = (keys.len + kTile - 1) / kTile;
   uint64_t bits = 0, nbits = 0;
   int i = keys.next(0, end, bits);
-  Stage<DP> sk, sv;
+  const RowStage<DP> sk(p.ks[2]), sv(p.vs[2]);
   if (i < end) {
-    sk.load(kb + (int64_t)i * kTile * p.ks[2], p.ks[2], bits, p.D);
-    sv.load(vb + (int64_t)i * kTile * p.vs[2], p.vs[2], bits, p.D);
-    sk.store(kt[0]);
-    sv.store(vt[0]);
+    sk.load(kt[0], kb + (int64_t)i * kTile * p.ks[2], bits, p.D);
+    sv.load(vt[0], vb + (int64_t)i * kTile * p.vs[2], bits, p.D);
   }
+  staged();
   __syncthreads();
-  for (int cur = 0; i < end; cur ^= 1, bits = nbits) {
-    const int j = keys.next(i + 1, end, nbits);
+  f32x4_t S[QT][2], P[QT][2];
+  // P and dP of 32 keys of the tile, from the h-th half
+  auto scores = [&](int cur, int h) {
+#pragma unroll
+    for (int t = 0; t < 2; t++) {
+#pragma unroll
+      for (int q = 0; q < QT; q++) S[q][t] = P[q][t] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+      for (int k = 0; k < KS; k++) {
+        const s16x8 a = by_rows<DP>(kt[cur], 2 * h + t, at.row[k]), c = by_rows<DP>(vt[cur], 2 * h + t, at.row[k]);
+#pragma unroll
+        for (int q = 0; q < QT; q++) {
+          S[q][t] = mfma16<F16>(a, qf[q][k], S[q][t]);
+          P[q][t] = mfma16<F16>(c, df[q][k], P[q][t]);
+        }
+      }
+    }
+    if (bits != ~0ull) {
+      asm volatile("");   // (a branch, as in the forward)
+      const uint32_t on = (uint32_t)(bits >> (32 * h)) >> (4 * g);
+#pragma unroll
+      for (int t = 0; t < 2; t++)
+#pragma unroll
+        for (int q = 0; q < QT; q++)
+#pragma unroll
+          for (int v = 0; v < 4; v++) S[q][t][v] = on >> (16 * t + v) & 1 ? S[q][t][v] : -kInf;
+    }
+#pragma unroll
+    for (int q = 0; q < QT; q++)
+#pragma unroll
+      for (int t = 0; t < 2; t++)
+#pragma unroll
+        for (int v = 0; v < 4; v++) S[q][t][v] = __builtin_amdgcn_exp2f(__builtin_fmaf(S[q][t][v], p.c, -lse[q]));
+  };
+  int j = i < end ? keys.next(i + 1, end, nbits) : end;
+  if (i < end && j == end) {
+    // One tile alone: delta as the sum of P dP. The few keys' dP are as large as delta, which the rounding of o would move by
+    // as much as dS's own rounding does.
+#pragma unroll
+    for (int q = 0; q < QT; q++) delta[q] = 0.0f;
+    for (int h = 0; h < 2; h++) {
+      scores(0, h);
+#pragma unroll
+      for (int q = 0; q < QT; q++)
+#pragma unroll
+        for (int t = 0; t < 2; t++)
+#pragma unroll
+          for (int v = 0; v < 4; v++) delta[q] = __builtin_fmaf(S[q][t][v], P[q][t][v], delta[q]);
+    }
+#pragma unroll
+    for (int q = 0; q < QT; q++) delta[q] = groups_sum(delta[q]);
+  }
+#pragma unroll
+  for (int q = 0; q < QT; q++)
+    if (g == 0 && row0 + 16 * q + l15 < p.rows) p.delta[(int64_t)pair * p.rows + row0 + 16 * q + l15] = delta[q];
+  for (int cur = 0; i < end; cur ^= 1) {
     if (j < end) {
-      sk.load(kb + (int64_t)j * kTile * p.ks[2], p.ks[2], nbits, p.D);
-      sv.load(vb + (int64_t)j * kTile * p.vs[2], p.vs[2], nbits, p.D);
+      sk.load(kt[cur ^ 1], kb + (int64_t)j * kTile * p.ks[2], nbits, p.D);
+      sv.load(vt[cur ^ 1], vb + (int64_t)j * kTile * p.vs[2], nbits, p.D);
     }
 #pragma unroll
     for (int h = 0; h < 2; h++) {
-      f32x4_t S[QT][2], P[QT][2];
-#pragma unroll
-      for (int t = 0; t < 2; t++) {
-#pragma unroll
-        for (int q = 0; q < QT; q++) S[q][t] = P[q][t] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-        for (int k = 0; k < KS; k++) {
-          const s16x8 a = by_rows<DP>(kt[cur], 2 * h + t, at.row[k]), c = by_rows<DP>(vt[cur], 2 * h + t, at.row[k]);
-#pragma unroll
-          for (int q = 0; q < QT; q++) {
-            S[q][t] = mfma16<F16>(a, qf[q][k], S[q][t]);
-            P[q][t] = mfma16<F16>(c, df[q][k], P[q][t]);
-          }
-        }
-      }
+      scores(cur, h);
       s16x8 sf[QT];
 #pragma unroll
       for (int q = 0; q < QT; q++) {
@@ -559,9 +636,7 @@ __global__ __launch_bounds__(256, 2) void attn_dq_kernel(AttnArgs p) {
         for (int t = 0; t < 2; t++)
 #pragma unroll
           for (int v = 0; v < 4; v++) {
-            float x = __builtin_amdgcn_exp2f(__builtin_fmaf(S[q][t][v], p.c, -lse[q]));
-            if (bits != ~0ull && !(bits >> (32 * h + 16 * t + 4 * g + v) & 1)) x = 0.0f;
-            x *= P[q][t][v] - delta[q];
+            const float x = S[q][t][v] * (P[q][t][v] - delta[q]);
             S[q][t][v] = F16 ? x * up[q] : x;
           }
         sf[q] = operand<F16>(S[q][0], S[q][1]);
@@ -573,12 +648,10 @@ __global__ __launch_bounds__(256, 2) void attn_dq_kernel(AttnArgs p) {
         for (int q = 0; q < QT; q++) dQ[q][d] = mfma16<F16>(a, sf[q], dQ[q][d]);
       }
     }
-    if (j < end) {
-      sk.store(kt[cur ^ 1]);
-      sv.store(vt[cur ^ 1]);
-    }
+    staged();
     __syncthreads();
-    i = j;
+    i = j, bits = nbits;
+    if (i < end) j = keys.next(i + 1, end, nbits);
   }
 #pragma unroll
   for (int q = 0; q < QT; q++) {
@@ -638,41 +711,37 @@ __global__ __launch_bounds__(256, 2) void attn_dkv_kernel(AttnArgs p) {
     for (int o = 32; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
     up = norm_factor(m);
   }
-  const int n = (p.rows + kTile - 1) / kTile, per = (n + p.splits - 1) / p.splits;
+  // (tiles of a head's rows: one base a tile, where tiles across heads would need an address a row)
+  const int nt = (p.N + kTile - 1) / kTile, n = p.G * nt, per = (n + p.splits - 1) / p.splits;
   int i = split * per;
   const int end = __syncthreads_or(any) ? min(n, i + per) : 0;
-  Stage<DP> sq, sd;
+  const RowStage<DP> sq(p.qs[2]), sd(p.ds[2]);
   float sl = 0.0f;
-  // A tile's rows may belong to several heads: each staged row finds its own.
-  auto fetch = [&](int tile) {
-#pragma unroll
-    for (int u = 0; u < Stage<DP>::kU; u++) {
-      const int x = threadIdx.x + 256 * u, r = tile * kTile + x / Stage<DP>::kC, c = x % Stage<DP>::kC;
-      const int rc = min(r, p.rows - 1);
-      sq.r[u] = __builtin_bit_cast(u32x4, row_chunk(p.q + row_at(p, p.qs, b, hk, rc), c, p.D, r < p.rows));
-      sd.r[u] = __builtin_bit_cast(u32x4, row_chunk(p.dout + row_at(p, p.ds, b, hk, rc), c, p.D, r < p.rows));
-    }
-    const int r = tile * kTile + (threadIdx.x & 63);
+  auto fetch = [&](int item, int buf) {
+    const int h = item / nt, n0 = (item - h * nt) * kTile, rest = p.N - n0;
+    const uint64_t rows = rest < kTile ? (1ull << rest) - 1 : ~0ull;
+    sq.load(qt[buf], p.q + b * p.qs[0] + (hk * p.G + h) * p.qs[1] + n0 * p.qs[2], rows, p.D);
+    sd.load(dt[buf], p.dout + b * p.ds[0] + (hk * p.G + h) * p.ds[1] + n0 * p.ds[2], rows, p.D);
+    const int r = threadIdx.x & 63;
     if (threadIdx.x < 128) {
       const float *src = threadIdx.x < 64 ? p.lse : p.delta;
-      sl = r < p.rows ? src[(int64_t)pair * p.rows + r] : threadIdx.x < 64 ? kInf : 0.0f;
+      sl = r < rest ? src[(int64_t)pair * p.rows + h * p.N + n0 + r] : threadIdx.x < 64 ? kInf : 0.0f;
       if (F16 && threadIdx.x < 64) sl -= kPUp;
     }
   };
   auto put = [&](int buf) {
-    sq.store(qt[buf]);
-    sd.store(dt[buf]);
     if (threadIdx.x < 64) lse[buf][threadIdx.x] = sl;
     else if (threadIdx.x < 128) delta[buf][threadIdx.x - 64] = sl;
+    staged();
   };
   if (i < end) {
-    fetch(i);
+    fetch(i, 0);
     put(0);
   }
   __syncthreads();
   const float us = F16 ? up * __builtin_ldexpf(1.0f, -(int)kPUp) : 1.0f;
   for (int cur = 0; i < end; cur ^= 1, i++) {
-    if (i + 1 < end) fetch(i + 1);
+    if (i + 1 < end) fetch(i + 1, cur ^ 1);
 #pragma unroll
     for (int h = 0; h < 2; h++) {
       f32x4_t S[KT][2], P[KT][2];
@@ -800,7 +869,7 @@ static AttnPlan attn_plan(int64_t B, int64_t H, int64_t Hk, int64_t N, int64_t L
   a.btiles = (int)((rows + 64 * a.bqt - 1) / (64 * a.bqt));
   a.kt = D <= 64 && pairs * ((L + 127) / 128) >= 512 ? 2 : 1;
   a.ktiles = (int)((L + 64 * a.kt - 1) / (64 * a.kt));
-  const int64_t want = 512 / std::max<int64_t>(pairs * a.ktiles, 1), most = (rows + 255) / 256;
+  const int64_t want = 512 / std::max<int64_t>(pairs * a.ktiles, 1), most = (H / Hk * ((N + 63) / 64) + 3) / 4;
   a.ksplits = (int)std::max<int64_t>(std::min(want, most), 1);
   return a;
 }
@@ -947,12 +1016,8 @@ int gpic_fp8_attention_bwd(const uint16_t *dout, const int64_t *ds, const uint16
     if (keys && dk) {
       p.tiles = a.ktiles, p.splits = a.ksplits;
       const unsigned grid = (unsigned)(B * Hk * a.ktiles * a.ksplits);
-      if constexpr (DP == 64) {
-        if (a.kt == 2) attn_dkv_kernel<F, DP, 2><<<grid, 256, 0, st>>>(p);
-        else attn_dkv_kernel<F, DP, 1><<<grid, 256, 0, st>>>(p);
-      } else {
-        attn_dkv_kernel<F, DP, 1><<<grid, 256, 0, st>>>(p);
-      }
+      if (a.kt == 2) attn_dkv_kernel<F, DP, 2><<<grid, 256, 0, st>>>(p);
+      else attn_dkv_kernel<F, DP, 1><<<grid, 256, 0, st>>>(p);
       if (a.ksplits > 1)
         attn_dkv_join_kernel<F><<<(unsigned)((B * Hk * L * (D / 2) + 255) / 256), 256, 0, st>>>(p);
     }
