@@ -361,7 +361,18 @@ __global__ __launch_bounds__(256, 2) void attn_few_kernel(AttnArgs p) {
   const int first = (split * 4 + wave) * per, end = min(n, first + per);
   s16x8 K[2][KS], Kn[2][KS];
   u32x4 V[kU];
+  const uint16_t *kl = kb + l15 * p.ks[2] + 8 * g, *vl = vb + (lane / kC) * p.vs[2] + 8 * (lane % kC);
   auto fetch = [&](int i, uint32_t bits) {
+    if (bits == ~0u && p.D == DP) {   // (whole: loads without conditions, which stay in flight together)
+#pragma unroll
+      for (int t = 0; t < 2; t++)
+#pragma unroll
+        for (int k = 0; k < KS; k++)
+          Kn[t][k] = *reinterpret_cast<const s16x8 *>(kl + (int64_t)(32 * i + 16 * t) * p.ks[2] + 32 * k);
+#pragma unroll
+      for (int u = 0; u < kU; u++) V[u] = *reinterpret_cast<const u32x4 *>(vl + (int64_t)(32 * i + 64 / kC * u) * p.vs[2]);
+      return;
+    }
 #pragma unroll
     for (int t = 0; t < 2; t++)
 #pragma unroll
@@ -465,25 +476,49 @@ __global__ __launch_bounds__(256, 2) void attn_few_kernel(AttnArgs p) {
   }
 }
 
-// The splits' parts of a row, joined in their order: a thread a column, 256 / DP rows a workgroup.
+// The splits' parts of a row, joined in their order, by one wave: lane s holds split s's maximum and factor; the parts' columns are
+// read two a lane, eight splits at a time.
 template <bool F16, int DP>
-__global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs p) {
-  const int64_t all = (int64_t)p.B * p.Hk * p.rows, row = (int64_t)blockIdx.x * (256 / DP) + threadIdx.x / DP;
-  const int d = threadIdx.x % DP;
-  if (row >= all) return;
-  float m = -kInf, sum = 0.0f, o = 0.0f;
-  for (int s = 0; s < p.splits; s++) m = fmaxf(m, p.part[(s * all + row) * (DP + 2) + DP]);
-  for (int s = 0; s < p.splits; s++) {
-    const float *x = p.part + (s * all + row) * (DP + 2);
-    if (x[DP] == -kInf) continue;
-    const float f = __builtin_amdgcn_exp2f(x[DP] - m);
-    sum = __builtin_fmaf(f, x[DP + 1], sum);
-    o = __builtin_fmaf(f, x[d], o);
+__global__ __launch_bounds__(64) void attn_join_kernel(AttnArgs p) {
+  const int64_t all = (int64_t)p.B * p.Hk * p.rows, row = blockIdx.x;
+  const int lane = threadIdx.x;
+  const float *x = p.part + row * (DP + 2);
+  const int64_t step = all * (DP + 2);
+  const bool on = lane < p.splits;
+  const float2 ml = on ? *reinterpret_cast<const float2 *>(x + lane * step + DP) : float2{-kInf, 0.0f};
+  float m = ml.x;
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
+  const float f = ml.x == -kInf ? 0.0f : __builtin_amdgcn_exp2f(ml.x - m);
+  float sum = ml.x == -kInf ? 0.0f : f * ml.y;
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o, 64);
+  constexpr int kV = DP / 64;   // (columns lane, lane + 64)
+  float o[kV];
+#pragma unroll
+  for (int v = 0; v < kV; v++) o[v] = 0.0f;
+  for (int s0 = 0; s0 < p.splits; s0 += 8) {
+    float part[8][kV];
+#pragma unroll
+    for (int i = 0; i < 8; i++)
+#pragma unroll
+      for (int v = 0; v < kV; v++) part[i][v] = x[min(s0 + i, p.splits - 1) * step + lane + 64 * v];
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+      const float fs = __shfl(f, min(s0 + i, 63), 64);
+      if (s0 + i < p.splits && fs != 0.0f) {
+#pragma unroll
+        for (int v = 0; v < kV; v++) o[v] = __builtin_fmaf(fs, part[i][v], o[v]);
+      }
+    }
   }
   const int pair = (int)(row / p.rows), r = (int)(row - (int64_t)pair * p.rows), b = pair / p.Hk;
   const float inv = sum == 0.0f ? 0.0f : __fdiv_rn(1.0f, sum);
-  if (d < p.D) p.out[row_at(p, p.os, b, pair - b * p.Hk, r) + d] = (uint16_t)pack16<F16>(o * inv, 0.0f);
-  if (p.lse && d == 0) p.lse[row] = sum == 0.0f ? kInf : m + __builtin_amdgcn_logf(sum);
+  uint16_t *out = p.out + row_at(p, p.os, b, pair - b * p.Hk, r);
+#pragma unroll
+  for (int v = 0; v < kV; v++)
+    if (lane + 64 * v < p.D) out[lane + 64 * v] = (uint16_t)pack16<F16>(o[v] * inv, 0.0f);
+  if (p.lse && lane == 0) p.lse[row] = sum == 0.0f ? kInf : m + __builtin_amdgcn_logf(sum);
 }
 
 // ------------------------------------------------------------------------------------------- backward
@@ -844,6 +879,7 @@ __global__ __launch_bounds__(256) void attn_dkv_join_kernel(AttnArgs p) {
 
 constexpr int kMaxAttnD = 128;
 constexpr int kFewRows = 16;
+constexpr int kMaxKeySplits = 64;   // (a wave joins them)
 constexpr int64_t kMaxBlocks = int64_t(1) << 23;   // (a launch's threads are counted in 32 bits)
 
 struct AttnPlan {
@@ -853,21 +889,21 @@ struct AttnPlan {
 };
 static AttnPlan attn_plan(int64_t B, int64_t H, int64_t Hk, int64_t N, int64_t L, int64_t D) {
   AttnPlan a;
-  const int64_t pairs = B * Hk, rows = H / Hk * N;
+  const int64_t pairs = std::max<int64_t>(B * Hk, 1), rows = H / Hk * N;
   a.few = rows <= kFewRows;
   if (a.few) {
     a.qt = 1, a.tiles = 1;
-    const int64_t want = (1024 + pairs - 1) / pairs, most = (L + 255) / 256;
-    a.splits = (int)std::max<int64_t>(std::min(want, most), 1);
+    const int64_t want = (256 + pairs - 1) / pairs, most = (L + 255) / 256;
+    a.splits = (int)std::max<int64_t>(std::min<int64_t>(std::min(want, most), kMaxKeySplits), 1);
   } else {
     a.qt = pairs * ((rows + 127) / 128) >= 512 ? 2 : 1;
     a.tiles = (int)((rows + 64 * a.qt - 1) / (64 * a.qt));
     const int64_t want = 512 / (pairs * a.tiles), most = (L + 511) / 512;
-    a.splits = (int)std::max<int64_t>(std::min(want, most), 1);
+    a.splits = (int)std::max<int64_t>(std::min<int64_t>(std::min(want, most), kMaxKeySplits), 1);
   }
   a.bqt = pairs * ((rows + 127) / 128) >= 512 ? 2 : 1;
   a.btiles = (int)((rows + 64 * a.bqt - 1) / (64 * a.bqt));
-  a.kt = D <= 64 && pairs * ((L + 127) / 128) >= 512 ? 2 : 1;
+  a.kt = D <= 64 && L >= 1024 && pairs * ((L + 127) / 128) >= 512 ? 2 : 1;
   a.ktiles = (int)((L + 64 * a.kt - 1) / (64 * a.kt));
   const int64_t want = 512 / std::max<int64_t>(pairs * a.ktiles, 1), most = (H / Hk * ((N + 63) / 64) + 3) / 4;
   a.ksplits = (int)std::max<int64_t>(std::min(want, most), 1);
@@ -947,10 +983,7 @@ int gpic_fp8_attention(const uint16_t *q, const int64_t *qs, const uint16_t *k, 
     if (a.few) attn_few_kernel<F, DP><<<grid, 256, 0, st>>>(p);
     else if (a.qt == 2) attn_fwd_kernel<F, DP, 2><<<grid, 256, 0, st>>>(p);
     else attn_fwd_kernel<F, DP, 1><<<grid, 256, 0, st>>>(p);
-    if (a.splits > 1) {
-      const int64_t per = 256 / DP;
-      attn_join_kernel<F, DP><<<(unsigned)((B * Hk * p.rows + per - 1) / per), 256, 0, st>>>(p);
-    }
+    if (a.splits > 1) attn_join_kernel<F, DP><<<(unsigned)(B * Hk * p.rows), 64, 0, st>>>(p);
   });
   return (int)hipGetLastError();
 }

@@ -98,3 +98,9 @@ def test_backward_codes(p):
         assert call(**bad) == -4, bad
     n = L.lib().gpic_fp8_attention_bwd_workspace_bytes(1, 2, 1, 3, 5, 16)
     assert n >= 4 * 6 and call(n=n - 1) == call(ws=None, n=n) == -5
+
+
+def test_workspaces_of_nothing():
+    fwd, bwd = L.lib().gpic_fp8_attention_workspace_bytes, L.lib().gpic_fp8_attention_bwd_workspace_bytes
+    for B, N, n in ((0, 4, 5), (0, 100, 5), (2, 0, 5), (2, 4, 0), (0, 0, 0)):
+        assert fwd(B, 4, 4, N, n, 64) == 0 and bwd(B, 4, 2, N, n, 64) >= 0
