@@ -914,20 +914,6 @@ py::object layer_norm(const at::Tensor &x, const opt &w, const opt &b, double ep
   return py::make_tuple(o.xn, o.h, o.mean, o.rstd);
 }
 
-// The public call where no gradient is recorded: h, or (x_new, h)
-py::object layer_norm_served(const at::Tensor &x, const opt &w, const opt &b, double eps, const opt &a, int dev, handle,
-                             handle stream) {
-  const opt ox = x;
-  if (!layer_norm_ok(x, w, b, a, false, dev) || records({&ox, &w, &b, &a})) return py::none();
-  LayerNormOut o;
-  {
-    NoGil no_gil;
-    o = layer_norm_run(x, w, b, eps, a, true, false, false, vp(stream));
-  }
-  if (!a) return py::cast(o.h);
-  return py::make_tuple(o.xn, o.h);
-}
-
 py::object layer_norm_rows(const at::Tensor &x, const opt &w, const opt &b, double eps, const opt &a, bool want_h, int dev, handle,
                            handle stream) {
   const opt ox = x;
@@ -940,30 +926,131 @@ py::object layer_norm_rows(const at::Tensor &x, const opt &w, const opt &b, doub
   return py::make_tuple(o.xn, o.h, o.q, o.s);
 }
 
+struct LayerNormGrads {
+  at::Tensor dx, dw, db;
+};
+LayerNormGrads layer_norm_bwd_run(const at::Tensor &dh, const opt &dxn, const at::Tensor &xs, const opt &w, const at::Tensor &mean,
+                                  const at::Tensor &rstd, const std::optional<at::ScalarType> &bias_dtype, void *stream) {
+  const int64_t C = xs.size(-1), M = xs.numel() / C;
+  LayerNormGrads o;
+  o.dx = make(xs, xs.sizes(), xs.scalar_type());
+  if (w) o.dw = make(xs, {C}, w->scalar_type());
+  if (bias_dtype) o.db = make(xs, {C}, *bias_dtype);
+  const size_t bytes = gpic_fp8_layer_norm_bwd_workspace_bytes(M, C);
+  const at::Tensor ws = make(xs, {(int64_t)bytes}, at::kByte);
+  check(gpic_fp8_layer_norm_bwd(dh.data_ptr(), dxn ? dxn->data_ptr() : nullptr, xs.data_ptr(), dtype_code3(xs),
+                                w ? w->data_ptr() : nullptr, w ? dtype_code3(*w) : 0, ptr<float>(mean), ptr<float>(rstd), M, C,
+                                o.dx.data_ptr(), w ? o.dw.data_ptr() : nullptr, w ? dtype_code3(o.dw) : 0,
+                                bias_dtype ? o.db.data_ptr() : nullptr, bias_dtype ? dtype_code3(o.db) : 0, ws.data_ptr(), bytes,
+                                stream),
+        "gpic_fp8_layer_norm_bwd");
+  return o;
+}
+bool layer_norm_bwd_ok(const at::Tensor &dh, const opt &dxn, const at::Tensor &xs, const opt &w, const at::Tensor &mean,
+                       const at::Tensor &rstd, int dev) {
+  if (!layer_norm_ok(xs, w, std::nullopt, dxn, false, dev) || dh.scalar_type() != xs.scalar_type() || dh.sizes() != xs.sizes() ||
+      !plain(dh, dev))
+    return false;
+  const int64_t M = xs.numel() / xs.size(-1);
+  return scales_ok(mean, M, dev) && scales_ok(rstd, M, dev);
+}
+
 py::object layer_norm_bwd(const at::Tensor &dh, const opt &dxn, const at::Tensor &xs, const opt &w, const at::Tensor &mean,
                           const at::Tensor &rstd, const std::optional<at::ScalarType> &bias_dtype, int dev, handle,
                           handle stream) {
   const opt odh = dh, oxs = xs, om = mean, ors = rstd;
-  if (!layer_norm_ok(xs, w, std::nullopt, dxn, false, dev) || dh.scalar_type() != xs.scalar_type() || dh.sizes() != xs.sizes() ||
-      !plain(dh, dev) || (bias_dtype && !float3(*bias_dtype)))
+  if (!layer_norm_bwd_ok(dh, dxn, xs, w, mean, rstd, dev) || (bias_dtype && !float3(*bias_dtype)) ||
+      records({&odh, &dxn, &oxs, &w, &om, &ors}))
     return py::none();
-  const int64_t C = xs.size(-1), M = xs.numel() / C;
-  if (!scales_ok(om, M, dev) || !scales_ok(ors, M, dev) || records({&odh, &dxn, &oxs, &w, &om, &ors})) return py::none();
-  at::Tensor dx, dw, db;
+  LayerNormGrads o;
   {
     NoGil no_gil;
-    dx = make(xs, xs.sizes(), xs.scalar_type());
-    dw = w ? make(xs, {C}, w->scalar_type()) : none_of(xs, at::kFloat);
-    db = bias_dtype ? make(xs, {C}, *bias_dtype) : none_of(xs, at::kFloat);
-    const size_t bytes = gpic_fp8_layer_norm_bwd_workspace_bytes(M, C);
-    const at::Tensor ws = make(xs, {(int64_t)bytes}, at::kByte);
-    check(gpic_fp8_layer_norm_bwd(dh.data_ptr(), dxn ? dxn->data_ptr() : nullptr, xs.data_ptr(), dtype_code3(xs),
-                                  w ? w->data_ptr() : nullptr, w ? dtype_code3(*w) : 0, ptr<float>(mean), ptr<float>(rstd), M, C,
-                                  dx.data_ptr(), w ? dw.data_ptr() : nullptr, dtype_code3(dw),
-                                  bias_dtype ? db.data_ptr() : nullptr, dtype_code3(db), ws.data_ptr(), bytes, vp(stream)),
-          "gpic_fp8_layer_norm_bwd");
+    o = layer_norm_bwd_run(dh, dxn, xs, w, mean, rstd, bias_dtype, vp(stream));
+    if (!w) o.dw = none_of(xs, at::kFloat);
+    if (!bias_dtype) o.db = none_of(xs, at::kFloat);
   }
-  return py::make_tuple(dx, dw, db);
+  return py::make_tuple(o.dx, o.dw, o.db);
+}
+
+// The autograd Functions of gpic_fp8/layernorm.py and attention.py in their usual form as nodes of the graph, without a Python
+// frame on either of the engine's threads. Their gradients would be constants in a backward that is itself recorded: it throws.
+void differentiable_once(const char *what) {
+  if (c10::GradMode::is_enabled())
+    throw std::runtime_error(std::string(what) + " is differentiable once: its backward does not run under create_graph=True");
+}
+void saved_as_they_were(bool ok, const char *what) {
+  if (!ok) throw std::runtime_error(std::string(what) + "'s backward needs the tensors that the forward saved, as they were saved");
+}
+// An output's gradient of like's type, contiguous, 16-byte aligned.
+at::Tensor usual_as(const at::Tensor &g, const at::Tensor &like) {
+  at::Tensor t = g.to(like.scalar_type()).contiguous();
+  return (reinterpret_cast<uintptr_t>(t.data_ptr()) & 15u) ? t.clone() : t;
+}
+opt defined_or_none(const at::Tensor &t) { return t.defined() ? opt(t) : std::nullopt; }
+
+struct LayerNormNode : torch::autograd::Function<LayerNormNode> {
+  // (x_new, h), or h alone without a
+  static variable_list forward(AutogradContext *ctx, const at::Tensor &x, const opt &w, const opt &b, const opt &a, double eps) {
+    const LayerNormOut o = layer_norm_run(x, w, b, eps, a, true, true, false, current_stream(x));
+    ctx->save_for_backward({a ? o.xn : x, w ? *w : at::Tensor(), o.mean, o.rstd});
+    ctx->set_materialize_grads(false);
+    ctx->saved_data["parts"] = (int64_t)((w ? 1 : 0) | (a ? 2 : 0) | (b ? 4 + 8 * (int64_t)b->scalar_type() : 0));
+    if (a) return {o.xn, o.h};
+    return {o.h};
+  }
+  static variable_list backward(AutogradContext *ctx, const variable_list &out) {
+    differentiable_once("layer_norm");
+    variable_list g(5);
+    const int64_t parts = ctx->saved_data["parts"].toInt();
+    const bool has_w = parts & 1, has_a = parts & 2, has_b = parts & 4;
+    const at::Tensor &dxn_ = has_a ? out[0] : at::Tensor(), &dh_ = out.back();
+    if (!dh_.defined() && !dxn_.defined()) return g;
+    const variable_list s = ctx->get_saved_variables();
+    const at::Tensor &xs = s[0], &mean = s[2], &rstd = s[3];
+    const opt w = defined_or_none(s[1]);
+    size_t edge = 1;
+    const bool dx = ctx->needs_input_grad(0), dw = has_w && ctx->needs_input_grad(edge++),
+               db = has_b && ctx->needs_input_grad(edge++), da = has_a && ctx->needs_input_grad(edge);
+    const auto bt = (at::ScalarType)(parts >> 3);
+    const opt dxn = dxn_.defined() ? opt(usual_as(dxn_, xs)) : std::nullopt;
+    LayerNormGrads o;
+    if (!dh_.defined()) {   // (x_new alone was used: its gradient as it is, and zeros that no value of x can spoil)
+      o.dx = *dxn;
+      if (dw) o.dw = at::zeros({xs.size(-1)}, dxn->options().dtype(w->scalar_type()));
+      if (db) o.db = at::zeros({xs.size(-1)}, dxn->options().dtype(bt));
+    } else {
+      const at::Tensor dh = usual_as(dh_, xs);
+      saved_as_they_were(has_w == w.has_value() && layer_norm_bwd_ok(dh, dxn, xs, w, mean, rstd, dh.get_device()), "layer_norm");
+      o = layer_norm_bwd_run(dh, dxn, xs, w, mean, rstd, db ? std::optional<at::ScalarType>(bt) : std::nullopt,
+                             current_stream(dh));
+    }
+    if (dx) g[0] = o.dx;
+    if (dw) g[1] = o.dw;
+    if (db) g[2] = o.db;
+    if (da) g[3] = o.dx;
+    return g;
+  }
+};
+
+// The public call: h, or (x_new, h); a node of the graph where it records
+py::object layer_norm_call(const at::Tensor &x, const opt &w, const opt &b, double eps, const opt &a, int dev, handle,
+                           handle stream) {
+  const opt ox = x;
+  if (!layer_norm_ok(x, w, b, a, false, dev)) return py::none();
+  at::Tensor xn, h;
+  {
+    NoGil no_gil;
+    if (records({&ox, &w, &b, &a})) {
+      variable_list o = LayerNormNode::apply(x, w, b, a, eps);
+      h = o.back();
+      if (a) xn = o[0];
+    } else {
+      const LayerNormOut o = layer_norm_run(x, w, b, eps, a, true, false, false, vp(stream));
+      xn = o.xn, h = o.h;
+    }
+  }
+  if (!a) return py::cast(h);
+  return py::make_tuple(xn, h);
 }
 
 // ------------------------------------------------------------------------------------------- attention
@@ -1045,48 +1132,112 @@ py::object attention(const at::Tensor &q, const at::Tensor &k, const at::Tensor 
   return py::make_tuple(o, lse);
 }
 
-py::object attention_served(const at::Tensor &q, const at::Tensor &k, const at::Tensor &v, const opt &lens, const opt &mask,
-                            double scale, int dev, handle, handle stream) {
-  AttnIn in;
-  const opt oq = q, ok = k, ov = v;
-  if (!attn_ok(q, k, v, lens, mask, scale, dev, in) || records({&oq, &ok, &ov})) return py::none();
-  at::Tensor o;
-  {
-    NoGil no_gil;
-    at::AutoDispatchBelowADInplaceOrView below;
-    o = attn_run(q, k, v, in, scale, nullptr, vp(stream));
+struct AttnGrads {
+  at::Tensor dq, dk, dv;
+};
+bool attn_bwd_ok(const at::Tensor &dout, const at::Tensor &q, const at::Tensor &k, const at::Tensor &v, const at::Tensor &o,
+                 const at::Tensor &lse, const opt &lens, const opt &mask, double scale, int dev, AttnIn &in, int64_t (&ds)[3],
+                 int64_t (&os)[3]) {
+  const at::ScalarType ty = q.scalar_type();
+  return attn_ok(q, k, v, lens, mask, scale, dev, in) && heads_ok(dout, ty, dev, ds) && heads_ok(o, ty, dev, os) &&
+         dout.sizes() == q.sizes() && o.sizes() == q.sizes() && lse.dim() == 3 && lse.scalar_type() == at::kFloat &&
+         plain(lse, dev) && lse.size(0) == in.B && lse.size(1) == in.H && lse.size(2) == in.N;
+}
+AttnGrads attn_bwd_run(const at::Tensor &dout, const at::Tensor &q, const at::Tensor &k, const at::Tensor &v, const at::Tensor &o,
+                       const at::Tensor &lse, double scale, bool want_kv, const AttnIn &in, const int64_t (&ds)[3],
+                       const int64_t (&os)[3], void *stream) {
+  int64_t dqs[3], dks[3], dvs[3];
+  AttnGrads r;
+  r.dq = make_heads(q, in.B, in.H, in.N, in.D, dqs);
+  if (want_kv) {
+    r.dk = make_heads(q, in.B, in.Hk, in.L, in.D, dks);
+    r.dv = make_heads(q, in.B, in.Hk, in.L, in.D, dvs);
   }
-  return py::cast(o);
+  const size_t bytes = gpic_fp8_attention_bwd_workspace_bytes(in.B, in.H, in.Hk, in.N, in.L, in.D);
+  const at::Tensor ws = make(q, {std::max<int64_t>((int64_t)bytes, 16)}, at::kByte);
+  check(gpic_fp8_attention_bwd(ptr<uint16_t>(dout), ds, ptr<uint16_t>(q), in.qs, ptr<uint16_t>(k), in.ks, ptr<uint16_t>(v), in.vs,
+                               ptr<uint16_t>(o), os, ptr<float>(lse), in.dtype, in.lens, in.mask, in.ldm, in.B, in.H, in.Hk, in.N,
+                               in.L, in.D, (float)scale, ptr<uint16_t>(r.dq), dqs, want_kv ? ptr<uint16_t>(r.dk) : nullptr, dks,
+                               want_kv ? ptr<uint16_t>(r.dv) : nullptr, dvs, ws.data_ptr(), bytes, stream),
+        "gpic_fp8_attention_bwd");
+  return r;
 }
 
 py::object attention_bwd(const at::Tensor &dout, const at::Tensor &q, const at::Tensor &k, const at::Tensor &v, const at::Tensor &o,
                          const at::Tensor &lse, const opt &lens, const opt &mask, double scale, bool want_kv, int dev, handle,
                          handle stream) {
   AttnIn in;
-  int64_t ds[3], os[3], dqs[3], dks[3], dvs[3];
+  int64_t ds[3], os[3];
   const opt od = dout, oq = q, ok = k, ov = v, oo = o, ol = lse;
-  const at::ScalarType ty = q.scalar_type();
-  if (!attn_ok(q, k, v, lens, mask, scale, dev, in) || !heads_ok(dout, ty, dev, ds) || !heads_ok(o, ty, dev, os) ||
-      dout.sizes() != q.sizes() || o.sizes() != q.sizes() || lse.dim() != 3 || lse.scalar_type() != at::kFloat || !plain(lse, dev) ||
-      lse.numel() != in.B * in.H * in.N || lse.size(0) != in.B || lse.size(1) != in.H ||
-      records({&od, &oq, &ok, &ov, &oo, &ol}))
+  if (!attn_bwd_ok(dout, q, k, v, o, lse, lens, mask, scale, dev, in, ds, os) || records({&od, &oq, &ok, &ov, &oo, &ol}))
     return py::none();
-  at::Tensor dq, dk, dv;
+  AttnGrads r;
   {
     NoGil no_gil;
     at::AutoDispatchBelowADInplaceOrView below;
-    dq = make_heads(q, in.B, in.H, in.N, in.D, dqs);
-    dk = want_kv ? make_heads(q, in.B, in.Hk, in.L, in.D, dks) : none_of(q, ty);
-    dv = want_kv ? make_heads(q, in.B, in.Hk, in.L, in.D, dvs) : none_of(q, ty);
-    const size_t bytes = gpic_fp8_attention_bwd_workspace_bytes(in.B, in.H, in.Hk, in.N, in.L, in.D);
-    const at::Tensor ws = make(q, {std::max<int64_t>((int64_t)bytes, 16)}, at::kByte);
-    check(gpic_fp8_attention_bwd(ptr<uint16_t>(dout), ds, ptr<uint16_t>(q), in.qs, ptr<uint16_t>(k), in.ks, ptr<uint16_t>(v), in.vs,
-                                 ptr<uint16_t>(o), os, ptr<float>(lse), in.dtype, in.lens, in.mask, in.ldm, in.B, in.H, in.Hk, in.N,
-                                 in.L, in.D, (float)scale, ptr<uint16_t>(dq), dqs, want_kv ? ptr<uint16_t>(dk) : nullptr, dks,
-                                 want_kv ? ptr<uint16_t>(dv) : nullptr, dvs, ws.data_ptr(), bytes, vp(stream)),
-          "gpic_fp8_attention_bwd");
+    r = attn_bwd_run(dout, q, k, v, o, lse, scale, want_kv, in, ds, os, vp(stream));
+    if (!want_kv) r.dk = none_of(q, q.scalar_type()), r.dv = none_of(q, q.scalar_type());
   }
-  return py::make_tuple(dq, dk, dv);
+  return py::make_tuple(r.dq, r.dk, r.dv);
+}
+
+struct AttentionNode : torch::autograd::Function<AttentionNode> {
+  static at::Tensor forward(AutogradContext *ctx, const at::Tensor &q, const at::Tensor &k, const at::Tensor &v, const opt &lens,
+                            const opt &mask, double scale) {
+    at::AutoDispatchBelowADInplaceOrView below;   // (o is a tensor of its own, not a view)
+    AttnIn in;
+    saved_as_they_were(attn_ok(q, k, v, lens, mask, scale, q.get_device(), in), "cross_attention");
+    const at::Tensor lse = make(q, {in.B, in.H, in.N}, at::kFloat);
+    const at::Tensor o = attn_run(q, k, v, in, scale, ptr<float>(lse), current_stream(q));
+    ctx->save_for_backward({q, k, v, o, lse, lens ? *lens : at::Tensor(), mask ? *mask : at::Tensor()});
+    ctx->set_materialize_grads(false);
+    ctx->saved_data["scale"] = scale;
+    ctx->saved_data["keys"] = (int64_t)((lens ? 1 : 0) | (mask ? 2 : 0));
+    return o;
+  }
+  static variable_list backward(AutogradContext *ctx, const variable_list &out) {
+    differentiable_once("cross_attention");
+    variable_list g(6);
+    if (!out[0].defined()) return g;
+    const variable_list s = ctx->get_saved_variables();
+    const opt lens = defined_or_none(s[5]), mask = defined_or_none(s[6]);
+    const double scale = ctx->saved_data["scale"].toDouble();
+    const int64_t keys = ctx->saved_data["keys"].toInt();
+    at::AutoDispatchBelowADInplaceOrView below;
+    at::Tensor dout = out[0].to(s[0].scalar_type());
+    AttnIn in;
+    int64_t ds[3], os[3];
+    const int dev = dout.get_device();
+    if (!heads_ok(dout, dout.scalar_type(), dev, ds)) dout = usual_as(dout.transpose(1, 2), dout).transpose(1, 2);
+    saved_as_they_were(((keys & 1) != 0) == lens.has_value() && ((keys & 2) != 0) == mask.has_value() &&
+                           attn_bwd_ok(dout, s[0], s[1], s[2], s[3], s[4], lens, mask, scale, dev, in, ds, os),
+                       "cross_attention");
+    const bool nk = ctx->needs_input_grad(1), nv = ctx->needs_input_grad(2);
+    AttnGrads r = attn_bwd_run(dout, s[0], s[1], s[2], s[3], s[4], scale, nk || nv, in, ds, os, current_stream(dout));
+    if (ctx->needs_input_grad(0)) g[0] = r.dq;
+    if (nk) g[1] = r.dk;
+    if (nv) g[2] = r.dv;
+    return g;
+  }
+};
+
+// The public call; a node of the graph where it records
+py::object attention_call(const at::Tensor &q, const at::Tensor &k, const at::Tensor &v, const opt &lens, const opt &mask,
+                          double scale, int dev, handle, handle stream) {
+  AttnIn in;
+  const opt oq = q, ok = k, ov = v;
+  if (!attn_ok(q, k, v, lens, mask, scale, dev, in)) return py::none();
+  at::Tensor o;
+  {
+    NoGil no_gil;
+    if (records({&oq, &ok, &ov})) {
+      o = AttentionNode::apply(q, k, v, lens, mask, scale);
+    } else {
+      at::AutoDispatchBelowADInplaceOrView below;
+      o = attn_run(q, k, v, in, scale, nullptr, vp(stream));
+    }
+  }
+  return py::cast(o);
 }
 
 // ------------------------------------------------------------------------------------------- adapters
@@ -1137,11 +1288,11 @@ PYBIND11_MODULE(_gpic_host, m) {   // (wrapped: torch's own errors, out of memor
   m.def("norm_rows_bwd", torch::wrap_pybind_function(&norm_rows_bwd));
   m.def("gemm_rows", torch::wrap_pybind_function(&gemm_rows));
   m.def("layer_norm", torch::wrap_pybind_function(&layer_norm));
-  m.def("layer_norm_served", torch::wrap_pybind_function(&layer_norm_served));
+  m.def("layer_norm_call", torch::wrap_pybind_function(&layer_norm_call));
   m.def("layer_norm_rows", torch::wrap_pybind_function(&layer_norm_rows));
   m.def("layer_norm_bwd", torch::wrap_pybind_function(&layer_norm_bwd));
   m.def("attention", torch::wrap_pybind_function(&attention));
-  m.def("attention_served", torch::wrap_pybind_function(&attention_served));
+  m.def("attention_call", torch::wrap_pybind_function(&attention_call));
   m.def("attention_bwd", torch::wrap_pybind_function(&attention_bwd));
   m.def("lora_rows", torch::wrap_pybind_function(&lora_rows));
   m.def("linear_rows_bwd", torch::wrap_pybind_function(&linear_rows_bwd));

@@ -192,7 +192,7 @@ def cross_attention(q, k, v, kv_lens=None, mask=None, scale=None):
     Differentiable (once) in q, k and v."""
     scale = _scale(scale, q)
     if type(q) in _PLAIN:
-        o = L.native("attention_served", q, q, k, v, kv_lens, mask, scale)
+        o = L.native("attention_call", q, q, k, v, kv_lens, mask, scale)
         if o is not None:
             return o
     return _CrossAttention.apply(q, k, v, kv_lens, mask, scale)

@@ -229,7 +229,7 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5, a=None):
     if a is not None and a.shape != x.shape:
         raise ValueError(f"a must have x's shape {tuple(x.shape)}, got {tuple(a.shape)}")
     if type(x) in _PLAIN:
-        o = L.native("layer_norm_served", x, x, weight, bias, eps, a)
+        o = L.native("layer_norm_call", x, x, weight, bias, eps, a)
         if o is not None:
             return o
     return _LayerNorm.apply(x, weight, bias, eps, a)

@@ -316,3 +316,59 @@ def test_output_feeds_the_heads_linear(dev):
     assert torch.equal(G.fp8_heads_linear_f8(o, W, None), G.fp8_linear_f8(merged, W, None))
     y = G.fp8_linear_rows(merged, G.rows_weight(W))
     assert y.shape == (2, 32, 256) and y.isfinite().all()
+
+
+def test_saved_tensor_hooks_and_versions(dev):
+    """What the nodes owe autograd: hooks that bring the tensors back as they were change nothing, others raise; an input changed
+    in place after the forward raises."""
+    q, k, v, do = make(2, 4, 2, 30, 50, 64, BF, 18)
+    lens = torch.tensor([50, 20], dtype=torch.int32, device=dev)
+    leaves = [t.detach().requires_grad_() for t in (q, k, v)]
+    ref = torch.autograd.grad(G.cross_attention(*leaves, lens), leaves, do)
+    with torch.autograd.graph.save_on_cpu():
+        o = G.cross_attention(*leaves, lens)
+    assert all(torch.equal(a, b) for a, b in zip(torch.autograd.grad(o, leaves, do), ref))
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: t, lambda t: t.cpu()):
+        o = G.cross_attention(*leaves, lens)
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(o, leaves, do)
+    o = G.cross_attention(*leaves, lens)
+    with torch.no_grad():
+        leaves[1].mul_(2)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        torch.autograd.grad(o, leaves, do)
+
+
+def test_gradients_of_other_layouts(dev):
+    """o's gradient as autograd makes it: expanded (a sum's), transposed, fp32."""
+    q, k, v, do = make(2, 4, 2, 30, 50, 64, BF, 19)
+    leaves = [t.detach().requires_grad_() for t in (q, k, v)]
+    run = lambda d: torch.autograd.grad(G.cross_attention(*leaves), leaves, d)  # noqa: E731
+    ref = run(do)
+    last = do.transpose(2, 3).contiguous().transpose(2, 3)
+    odd = torch.empty(do.numel() + 1, dtype=BF, device=dev)[1:].view(do.shape).copy_(do)
+    for d in (do.contiguous(), last, odd):
+        assert all(torch.equal(a, b) for a, b in zip(run(d), ref))
+    one = torch.ones(2, 4, 30, 64, dtype=BF, device=dev)
+    total = torch.autograd.grad(G.cross_attention(*leaves).sum(), leaves)
+    assert all(torch.equal(a, b) for a, b in zip(total, run(one)))
+
+
+def test_retained_and_shared_graphs(dev):
+    q, k, v, do = make(2, 2, 2, 40, 60, 64, BF, 20)
+    leaves = [t.detach().requires_grad_() for t in (q, k, v)]
+    o = G.cross_attention(*leaves)
+    first = torch.autograd.grad(o, leaves, do, retain_graph=True)
+    again = torch.autograd.grad(o, leaves, do)
+    assert all(torch.equal(a, b) for a, b in zip(first, again))
+    same = q.detach().requires_grad_()   # the same tensor three times over: its gradient is the sum
+    (g,) = torch.autograd.grad(G.cross_attention(same, same, same), same, do)
+    o, lse = G.cross_attention_fwd(q, q, q)
+    dq, dk, dv = G.cross_attention_bwd(do, q, q, q, o, lse)
+    ref = dq.float() + dk.float() + dv.float()
+    assert ((g.float() - ref).abs() <= 3 * 2.0 ** -8 * (dq.float().abs() + dk.float().abs() + dv.float().abs())).all()
+    for t in leaves:
+        t.grad = None
+    for _ in range(2):
+        G.cross_attention(*leaves).backward(do)
+    assert all(((t.grad.float() - 2 * g.float()).abs() <= 2.0 ** -7 * g.float().abs()).all() for t, g in zip(leaves, first))

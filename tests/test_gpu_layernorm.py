@@ -301,3 +301,55 @@ def test_compiled(dev):
     assert torch.equal(h, ref)
     for p, q in zip(torch.autograd.grad(h, (x, w, b), dh), torch.autograd.grad(ref, (x, w, b), dh)):
         assert torch.equal(p, q)
+
+
+def test_saved_tensor_hooks_and_versions(dev):
+    x, a, w, b, dh, dxn = make((40, 256), BF, 15)
+    leaves = [t.requires_grad_() for t in (x, w, b)]
+    ref = torch.autograd.grad(G.layer_norm(*leaves), leaves, dh)
+    with torch.autograd.graph.save_on_cpu():
+        h = G.layer_norm(*leaves)
+    assert all(torch.equal(p, q) for p, q in zip(torch.autograd.grad(h, leaves, dh), ref))
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: t, lambda t: t.cpu()):
+        h = G.layer_norm(*leaves)
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(h, leaves, dh)
+    h = G.layer_norm(*leaves)
+    with torch.no_grad():
+        w.mul_(2)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        torch.autograd.grad(h, leaves, dh)
+
+
+@pytest.mark.parametrize("native", [True, False])
+def test_every_set_of_leaves(dev, native):
+    """The node of the usual form and the general form (a weight whose elements are not beside each other) give the same bits,
+    whichever leaves take a gradient, with either output's gradient missing."""
+    x, a, w, b, dh, dxn = make((33, 264), BF, 16)
+    if not native:
+        w = torch.stack([w, w], 1)[:, 0]
+    full = [t.detach().requires_grad_() for t in (x, a, w, b)]
+    xn, h = G.layer_norm(full[0], full[2], full[3], EPS, full[1])
+    ref = dict(zip("xawb", torch.autograd.grad((xn, h), full, (dxn, dh))))
+    only_h = dict(zip("xawb", torch.autograd.grad(G.layer_norm(full[0], full[2], full[3], EPS, full[1])[1], full, dh)))
+    for i in range(1, 16):
+        on = [n for j, n in enumerate("xawb") if i >> j & 1]
+        t = {n: v.detach().requires_grad_(n in on) for n, v in zip("xawb", (x, a, w, b))}
+        xn, h = G.layer_norm(t["x"], t["w"], t["b"], EPS, t["a"])
+        outs = [o for o in (xn, h) if o.requires_grad]
+        assert len(outs) == 2
+        got = torch.autograd.grad(outs, [t[n] for n in on], (dxn, dh), retain_graph=True)
+        assert all(torch.equal(g, ref[n]) for n, g in zip(on, got)), on
+        got = torch.autograd.grad(h, [t[n] for n in on], dh)
+        assert all(torch.equal(g, only_h[n]) for n, g in zip(on, got)), on
+
+
+def test_gradients_of_other_layouts_and_types(dev):
+    x, a, w, b, dh, dxn = make((30, 64), BF, 17)
+    leaves = [t.requires_grad_() for t in (x, w, b)]
+    run = lambda d: torch.autograd.grad(G.layer_norm(*leaves), leaves, d)  # noqa: E731
+    ref = run(dh)
+    for d in (dh.t().contiguous().t(), torch.empty(dh.numel() + 1, dtype=BF, device=dev)[1:].view(dh.shape).copy_(dh)):
+        assert all(torch.equal(p, q) for p, q in zip(run(d), ref))
+    total = torch.autograd.grad(G.layer_norm(*leaves).sum(), leaves)
+    assert all(torch.equal(p, q) for p, q in zip(total, run(torch.ones_like(x))))
