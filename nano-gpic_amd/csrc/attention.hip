@@ -103,17 +103,6 @@ __device__ __forceinline__ s16x8 by_columns(uint16_t *tile, int t, int place) {
 // Sixteen zero bytes, for the lanes of a staged tile that have none of their own.
 __device__ const u32x4 kZeros = {0u, 0u, 0u, 0u};
 
-__device__ __forceinline__ uint32_t lds_at(const void *p) {
-  return (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const void *)p;
-}
-// Sixteen bytes a lane from its own address to LDS [lds, lds + 1 KiB) in lane order, past the registers. The loads are counted in
-// vmcnt but not by the compiler, so staged() comes before the barrier that hands the tile on. (Through registers the next tile cost
-// 16 to 32 of them, which kept the backward for rows of 128 at half its tile.)
-__device__ __forceinline__ void to_lds(const void *src, uint32_t lds) {
-  asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" : : "v"(src), "s"(lds) : "memory", "m0");
-}
-__device__ __forceinline__ void staged() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
-
 // How 256 threads stage a tile of kTile rows: kU loads each, load u of wave w to places 64 (4 u + w) + lane, of which place i is
 // place i % kC of row i / kC and takes that row's chunk (i % kC) ^ swz(row).
 template <int DP>

@@ -39,11 +39,32 @@ __device__ __forceinline__ void floats8(s16x8 x, float (&f)[8]) {
     for (int e = 0; e < 8; e++) f[e] = e & 1 ? bf16_hi(w[e >> 1]) : bf16_lo(w[e >> 1]);
   }
 }
+// The two values of a word.
+template <bool F16>
+__device__ __forceinline__ float low16(uint32_t w) {
+  if constexpr (F16) return (float)__builtin_bit_cast(f16x2v, w)[0];
+  else return bf16_lo(w);
+}
+template <bool F16>
+__device__ __forceinline__ float high16(uint32_t w) {
+  if constexpr (F16) return (float)__builtin_bit_cast(f16x2v, w)[1];
+  else return bf16_hi(w);
+}
 // Rounded to the type and back.
 template <bool F16>
 __device__ __forceinline__ float round16(float f) {
   if constexpr (F16) return (float)(_Float16)f;
   else return bf16_round(f);
 }
+
+__device__ __forceinline__ uint32_t lds_at(const void *p) {
+  return (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const void *)p;
+}
+// Sixteen bytes a lane from its own address to LDS [lds, lds + 1 KiB) in lane order, past the registers. The loads are counted in
+// vmcnt but not by the compiler, so staged() comes before the reads of what they bring, or the barrier that hands it on.
+__device__ __forceinline__ void to_lds(const void *src, uint32_t lds) {
+  asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" : : "v"(src), "s"(lds) : "memory", "m0");
+}
+__device__ __forceinline__ void staged() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
 
 }  // namespace gpic

@@ -362,10 +362,117 @@ __global__ __launch_bounds__(256) void lora_expand_kernel(LoraArgs p) {
   }
 }
 
+// The same for many rows and ranks of at most two tiles: the product is t B^T with t's rows as the result's rows, and tile h of a
+// step of 16 HT columns takes B's rows HT l15 + h: a lane then holds HT columns beside each other, and 16 lanes one run of a row
+// of y and out, which the memory pipeline takes whole (rows across the lanes cost it four times as long). 16384 rows of rank 32,
+// 4096 columns: 50 us against 62; larger ranks, whose B's fragments are as many as y's runs, lose by it (2648 rows of rank 64 22
+// -> 26 us, 4096 of 128 17 -> 21).
+// NS: steps of 32 over t's two halves, which meet the same chunks of B.
+template <bool F16, int RT, int NS>
+__global__ __launch_bounds__(256) void lora_expand_runs_kernel(LoraArgs p) {
+  constexpr int RP = 16 * NS;               // the rank in tiles of 16
+  constexpr int NB = NS > 1 ? NS / 2 : 1;   // steps over B's chunks (a rank of one tile: both halves in one step)
+  constexpr int HT = 8;
+  typedef uint32_t Run __attribute__((ext_vector_type(HT / 2)));   // HT columns of y
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l15 = lane & 15, g = lane >> 4;
+  // (workgroups beside each other take columns beside each other: rows whose length is a power of two would otherwise meet in few
+  // of the memory's channels)
+  const int tile = blockIdx.x / p.blocks, block = blockIdx.x - tile * p.blocks;
+  const int row0 = tile * 16 * RT;
+  const int group = blockIdx.y;
+  const int c0 = block * p.cols, c1 = min(p.N, c0 + p.cols);
+  // (loads without conditions, as above: of rows past the last and of other passes nothing is kept; t is zero past R, and B's
+  // chunks there are taken as zeros; a step that runs past the last column reads its last columns again)
+  // (a tile's rows at 32-bit offsets from its first)
+  const uint16_t *yt = p.y + (int64_t)row0 * p.ldy;
+  uint16_t *ot = p.out + (int64_t)row0 * p.N;
+  const int last = p.M - 1 - row0;
+  auto fetch_y = [&](int c, int i, Run (&y)[4]) {
+#pragma unroll
+    for (int v = 0; v < 4; v++)
+      y[v] = *reinterpret_cast<const Run *>(yt + ((uint32_t)min(16 * i + 4 * g + v, last) * (uint32_t)p.ldy +
+                                                  (uint32_t)min(c + HT * l15, c1 - HT)));
+  };
+  Run y0[4], y1[4];
+  s16x8 tf[RT][NS];
+  float up[RT];
+  if (c0 + 16 * HT * wave < c1) fetch_y(c0 + 16 * HT * wave, 0, y0);   // (before the ids are known, which B waits for; t too)
+#pragma unroll
+  for (int i = 0; i < RT; i++) {
+    const int row = min(row0 + 16 * i + l15, p.M - 1);
+#pragma unroll
+    for (int k = 0; k < NS; k++) tf[i][k] = chunk16(static_cast<const uint16_t *>(p.t) + (int64_t)row * 2 * RP, 4 * k + g);
+    up[i] = F16 ? p.up[row] : 1.0f;
+  }
+  const int id = lane < 16 * RT ? adapter_of(p, row0 + lane) : -1;
+  uint64_t todo = __ballot(lane < 16 * RT && row0 + lane < p.M);
+  bool again = false;
+  for (int pass = 0; todo; pass++) {
+    const int cur = __builtin_amdgcn_readlane(id, __builtin_ctzll(todo));
+    const uint64_t mine = __ballot(id == cur) & todo;   // (rows without an adapter are a pass too)
+    todo &= ~mine;
+    if (pass % p.groups != group) continue;
+    const uint16_t *B = p.B + (int64_t)max(cur, 0) * p.N * p.R;
+    const float s = cur >= 0 && p.s ? p.s[cur] : 1.0f;
+    // The result's rows 4 g + v of a row tile lie in other lanes than t's row l15: their factors
+    float sv[RT][4];
+#pragma unroll
+    for (int i = 0; i < RT; i++)
+#pragma unroll
+      for (int v = 0; v < 4; v++) sv[i][v] = F16 ? __shfl(up[i], 4 * g + v, 64) : 1.0f;
+    for (int c = c0 + 16 * HT * wave; c < c1; c += 64 * HT) {
+      s16x8 b[HT][NB];
+#pragma unroll
+      for (int h = 0; h < HT; h++)
+#pragma unroll
+        for (int k = 0; k < NB; k++) {
+          const int r = NS > 1 ? 32 * k + 8 * g : 8 * (g & 1);
+          b[h][k] = *reinterpret_cast<const s16x8 *>(B + ((uint32_t)min(c + HT * l15 + h, c1 - 1) * (uint32_t)p.R + min(r, p.R - 8)));
+        }
+      if (again || c != c0 + 16 * HT * wave) fetch_y(c, 0, y0);
+#pragma unroll
+      for (int h = 0; h < HT; h++)
+#pragma unroll
+        for (int k = 0; k < NB; k++)
+          if ((NS > 1 ? 32 * k + 8 * g : 8 * (g & 1)) >= p.R) b[h][k] = s16x8{0, 0, 0, 0, 0, 0, 0, 0};
+#pragma unroll
+      for (int i = 0; i < RT; i++) {
+        Run(&y)[4] = i & 1 ? y1 : y0;
+        if (i + 1 < RT) fetch_y(c, i + 1, i & 1 ? y0 : y1);
+        f32x4_t acc[HT];
+#pragma unroll
+        for (int h = 0; h < HT; h++) {
+          acc[h] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+          if (cur >= 0) {
+#pragma unroll
+            for (int k = 0; k < NS; k++) acc[h] = mfma16<F16>(tf[i][k], b[h][k % NB], acc[h]);
+          }
+        }
+#pragma unroll
+        for (int v = 0; v < 4; v++) {
+          Run out = y[v];
+          if (cur >= 0) {
+#pragma unroll
+            for (int h = 0; h < HT; h += 2) {
+              const float lo = __builtin_fmaf(F16 ? acc[h][v] * sv[i][v] : acc[h][v], s, low16<F16>(out[h / 2]));
+              const float hi = __builtin_fmaf(F16 ? acc[h + 1][v] * sv[i][v] : acc[h + 1][v], s, high16<F16>(out[h / 2]));
+              out[h / 2] = pack16<F16>(lo, hi);
+            }
+          }
+          if ((mine >> (16 * i + 4 * g + v) & 1) && c + HT * l15 < c1)
+            *reinterpret_cast<Run *>(ot + ((uint32_t)(16 * i + 4 * g + v) * (uint32_t)p.N + (uint32_t)(c + HT * l15))) = out;
+        }
+      }
+    }
+    again = true;
+  }
+}
+
 // ------------------------------------------------------------------------------------------- host side
 
 struct LoraPlan {
   int nt, shrink_rt, rt, splits, groups, cols;
+  bool runs;   // lora_expand_runs_kernel
 };
 static LoraPlan lora_plan(int64_t M, int64_t K, int64_t N, int64_t R, int64_t n) {
   LoraPlan a;
@@ -373,11 +480,13 @@ static LoraPlan lora_plan(int64_t M, int64_t K, int64_t N, int64_t R, int64_t n)
   const bool few = M <= 256;
   a.shrink_rt = M >= 8192 || (a.nt == 8 && M >= 1024) ? 2 : 1;
   a.rt = M < 1024 ? 1 : a.nt == 8 ? 2 : 4;
-  a.groups = few ? (int)std::min<int64_t>(std::min<int64_t>(n + 1, M), 16) : 1;
+  // (more rows: most tiles hold one adapter's, some two)
+  a.groups = few ? (int)std::min<int64_t>(std::min<int64_t>(n + 1, M), 16) : n > 1 && M <= 8192 ? 2 : 1;
   a.splits = few ? (int)std::max<int64_t>(std::min<int64_t>(K / 512, kMaxSplits), 1) : 1;   // (a wave 128 of K at least)
   const int64_t tiles = (M + 16 * a.rt - 1) / (16 * a.rt);
-  a.cols = 128;
-  while (!few && a.cols < 1024 && tiles * ((N + 2 * a.cols - 1) / (2 * a.cols)) >= 256) a.cols *= 2;
+  a.runs = a.rt == 4 && a.nt <= 2;
+  a.cols = a.runs ? 512 : 128;   // (a step of the workgroup's waves)
+  while (!few && a.cols < 1024 && tiles * ((N + 2 * a.cols - 1) / (2 * a.cols)) >= (a.runs ? 512 : 256)) a.cols *= 2;
   return a;
 }
 static size_t lora_t_bytes(const LoraPlan &a, int64_t M, int64_t R) {
@@ -411,9 +520,9 @@ int gpic_fp8_lora_rows(const uint16_t *y, int64_t ldy, const uint16_t *x, int64_
   if (M < 0 || N <= 0 || K <= 0 || R <= 0 || n <= 0 || per <= 0) return GPIC_EINVAL;
   if (M > 0 && (!y || !x || !A || !B || !ids || !out)) return GPIC_EINVAL;
   if (dtype != GPIC_DTYPE_BF16 && dtype != GPIC_DTYPE_F16) return GPIC_EDTYPE;
-  const int64_t most = int64_t(1) << 30;
-  if (N % 8 || K % 8 || R % 8 || R > kMaxRank || per >= most || ldx % 8 || ldx < K || ldy % 8 || ldy < N || M >= most || N >= most || K >= most ||
-      n >= most)
+  const int64_t most = int64_t(1) << 30, wide = int64_t(1) << 24;   // (a tile's offsets in 32 bits)
+  if (N % 8 || K % 8 || R % 8 || R > kMaxRank || per >= most || ldx % 8 || ldx < K || ldy % 8 || ldy < N || M >= most || N >= wide || K >= wide ||
+      ldx >= wide || ldy >= wide || n >= most)
     return GPIC_ESHAPE;
   if (!aligned16(y) || !aligned16(x) || !aligned16(A) || !aligned16(B) || !aligned16(out) || !aligned16(ws)) return GPIC_EALIGN;
   if (M == 0) return GPIC_OK;
@@ -437,6 +546,8 @@ int gpic_fp8_lora_rows(const uint16_t *y, int64_t ldy, const uint16_t *x, int64_
       if (a.splits > 1) lora_shrink_kernel<F, 1, T, true><<<shrink, 64 * kShrinkWaves<T>, 0, st>>>(p);
       else if (a.shrink_rt == 2) lora_shrink_kernel<F, 2, T, false><<<shrink, 64 * kShrinkWaves<T>, 0, st>>>(p);
       else lora_shrink_kernel<F, 1, T, false><<<shrink, 64 * kShrinkWaves<T>, 0, st>>>(p);
+      if constexpr (T <= 2)
+        if (a.runs) return lora_expand_runs_kernel<F, 4, T><<<expand, 256, 0, st>>>(p);
       if (a.splits > 1) lora_expand_kernel<F, 1, T, true><<<expand, 256, 0, st>>>(p);
       else if (a.rt == W) lora_expand_kernel<F, W, T, false><<<expand, 256, 0, st>>>(p);
       else lora_expand_kernel<F, 1, T, false><<<expand, 256, 0, st>>>(p);
