@@ -479,7 +479,7 @@ int gpic_fp8_attention_bwd(const uint16_t *dout, const int64_t *ds, const uint16
  *   y [M, N] (row stride ldy; the shared projection's output), x [M, K] (row stride ldx), A [n, R, K], B [n, N, R], out [M, N], of
  *   dtype (bf16 or fp16); scales [n] fp32 (NULL: ones); ids int32, or int64 with wide_ids: one for every `per` rows.
  *   Sums are fp32, x A_i^T is kept to 2^-16 and better, out is rounded once; what an adapter holds reaches no row but its own.
- *   N, K, R % 8 == 0, R <= 128; M, N, K, n < 2^30. out may not overlap the inputs. Deterministic.
+ *   N, K, R % 8 == 0, R <= 128; M, n < 2^30; N, K, ldx, ldy < 2^24. out may not overlap the inputs. Deterministic.
  *   ws: gpic_fp8_lora_rows_workspace_bytes(M, N, K, R, n) bytes, scratch of this call.
  */
 size_t gpic_fp8_lora_rows_workspace_bytes(int64_t M, int64_t N, int64_t K, int64_t R, int64_t n);

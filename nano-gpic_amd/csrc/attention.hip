@@ -867,6 +867,7 @@ __global__ __launch_bounds__(256) void attn_dkv_join_kernel(AttnArgs p) {
 // ------------------------------------------------------------------------------------------- host side
 
 constexpr int kMaxAttnD = 128;
+constexpr float kLog2e = 1.44269504f;
 constexpr int kFewRows = 16;
 constexpr int kMaxKeySplits = 64;   // (a wave joins them)
 constexpr int64_t kMaxBlocks = int64_t(1) << 23;   // (a launch's threads are counted in 32 bits)
@@ -907,7 +908,7 @@ static int attn_shape(int dtype, int64_t B, int64_t H, int64_t Hk, int64_t N, in
   if (H % Hk || D % 8 || D > kMaxAttnD) return GPIC_ESHAPE;
   const int64_t most = int64_t(1) << 30;
   if (B > most || H > most || N > most || L > most || H / Hk * N > most || B * H > most) return GPIC_ESHAPE;
-  if (B * Hk * ((H / Hk * N + 63) / 64) * 32 >= kMaxBlocks * 32 || B * Hk * ((L + 63) / 64) >= kMaxBlocks) return GPIC_ESHAPE;
+  if (B * Hk * ((H / Hk * N + 63) / 64) >= kMaxBlocks || B * Hk * ((L + 63) / 64) >= kMaxBlocks) return GPIC_ESHAPE;
   return GPIC_OK;
 }
 static int strides_ok(const void *p, const int64_t *s, int64_t (&out)[3]) {
@@ -949,7 +950,7 @@ int gpic_fp8_attention(const uint16_t *q, const int64_t *qs, const uint16_t *k, 
   status_scope();
   int e = attn_shape(dtype, B, H, Hk, N, L, D);
   if (e != GPIC_OK) return e;
-  if (!(scale > 0.0f) || scale == kInf) return GPIC_EINVAL;
+  if (!(scale > 0.0f) || scale * kLog2e == kInf) return GPIC_EINVAL;
   if (B * N == 0) return GPIC_OK;
   if (!q || !o || (L > 0 && (!k || !v)) || (mask && ldm < 0)) return GPIC_EINVAL;
   AttnArgs p{};
@@ -963,7 +964,7 @@ int gpic_fp8_attention(const uint16_t *q, const int64_t *qs, const uint16_t *k, 
   p.q = q, p.k = k, p.v = v, p.out = o, p.lens = lens, p.mask = mask, p.ldm = ldm, p.lse = lse;
   p.part = static_cast<float *>(ws);
   p.B = (int)B, p.H = (int)H, p.Hk = (int)Hk, p.N = (int)N, p.L = (int)L, p.D = (int)D, p.G = (int)(H / Hk);
-  p.rows = p.G * p.N, p.tiles = a.tiles, p.splits = a.splits, p.scale = scale, p.c = scale * 1.44269504f;
+  p.rows = p.G * p.N, p.tiles = a.tiles, p.splits = a.splits, p.scale = scale, p.c = scale * kLog2e;
   const hipStream_t st = (hipStream_t)stream;
   const unsigned grid = (unsigned)(B * Hk * a.tiles * a.splits);
   with_attn(dtype, D, [&](auto f, auto dp) {
@@ -1004,7 +1005,7 @@ int gpic_fp8_attention_bwd(const uint16_t *dout, const int64_t *ds, const uint16
   status_scope();
   int e = attn_shape(dtype, B, H, Hk, N, L, D);
   if (e != GPIC_OK) return e;
-  if (!(scale > 0.0f) || scale == kInf) return GPIC_EINVAL;
+  if (!(scale > 0.0f) || scale * kLog2e == kInf) return GPIC_EINVAL;
   if (!dk != !dv) return GPIC_EINVAL;
   const bool rows = B * N > 0, keys = B * L > 0;
   if (!rows && !keys) return GPIC_OK;
@@ -1024,7 +1025,7 @@ int gpic_fp8_attention_bwd(const uint16_t *dout, const int64_t *ds, const uint16
   p.delta = reinterpret_cast<float *>(w), p.rowmax = reinterpret_cast<float *>(w + space.rowmax);
   p.part = reinterpret_cast<float *>(w + space.part);
   p.B = (int)B, p.H = (int)H, p.Hk = (int)Hk, p.N = (int)N, p.L = (int)L, p.D = (int)D, p.G = (int)(H / Hk);
-  p.rows = p.G * p.N, p.scale = scale, p.c = scale * 1.44269504f, p.rtiles = a.btiles;
+  p.rows = p.G * p.N, p.scale = scale, p.c = scale * kLog2e, p.rtiles = a.btiles;
   const hipStream_t st = (hipStream_t)stream;
   with_attn(dtype, D, [&](auto f, auto dp) {
     constexpr bool F = decltype(f)::value;

@@ -485,7 +485,7 @@ static LoraPlan lora_plan(int64_t M, int64_t K, int64_t N, int64_t R, int64_t n)
   a.splits = few ? (int)std::max<int64_t>(std::min<int64_t>(K / 512, kMaxSplits), 1) : 1;   // (a wave 128 of K at least)
   const int64_t tiles = (M + 16 * a.rt - 1) / (16 * a.rt);
   a.runs = a.rt == 4 && a.nt <= 2;
-  a.cols = a.runs ? 512 : 128;   // (a step of the workgroup's waves)
+  a.cols = a.runs ? 512 : few ? 256 : 128;   // (a step of the workgroup's waves, few rows two)
   while (!few && a.cols < 1024 && tiles * ((N + 2 * a.cols - 1) / (2 * a.cols)) >= (a.runs ? 512 : 256)) a.cols *= 2;
   return a;
 }

@@ -18,6 +18,13 @@ from .rows import _run, _same_device
 
 DTYPES = {torch.bfloat16: 0, torch.float16: 2}
 MAX_RANK = 128
+MAX_WIDTH = 1 << 24
+
+
+def _near_rows(t):
+    """_rows, and a copy where the rows lie further apart than the kernels' offsets reach."""
+    t, ld = _rows(t)
+    return (t, ld) if ld < 1 << 24 else _rows(t.contiguous())
 
 
 def _check(y, x, A, B, ids, scale):
@@ -30,8 +37,9 @@ def _check(y, x, A, B, ids, scale):
         raise ValueError(f"lora_rows takes bf16 or fp16 y, x, A and B of one type, got {y.dtype}, {x.dtype}, {A.dtype} and {B.dtype}")
     n, R, K = A.shape
     N = y.shape[-1]
-    if N % 8 or K % 8 or R % 8 or not N or not K or not 0 < R <= MAX_RANK:
-        raise ValueError(f"lora_rows needs N, K and R multiples of 8 and R <= {MAX_RANK}, got N = {N}, K = {K}, R = {R}")
+    if N % 8 or K % 8 or R % 8 or not 0 < N < MAX_WIDTH or not 0 < K < MAX_WIDTH or not 0 < R <= MAX_RANK:
+        raise ValueError(f"lora_rows needs N, K and R multiples of 8, N and K below 2^24 and R <= {MAX_RANK}, got N = {N}, K = {K}, "
+                         f"R = {R}")
     if ids.dtype not in (torch.int32, torch.int64) or (ids.shape != x.shape[:-1] and ids.shape != x.shape[:1]):
         raise ValueError(f"ids must be int32 or int64 {tuple(x.shape[:-1])}, or [{x.shape[0]}] for the batch, got {ids.dtype} "
                          f"{tuple(ids.shape)}")
@@ -54,7 +62,7 @@ def lora_rows_op(y: torch.Tensor, x: torch.Tensor, A: torch.Tensor, B: torch.Ten
     M = out.numel() // N
     if M == 0:
         return out
-    (y2, ldy), (x2, ldx) = _rows(y.reshape(M, N)), _rows(x.reshape(M, K))
+    (y2, ldy), (x2, ldx) = _near_rows(y.reshape(M, N)), _near_rows(x.reshape(M, K))
     A, B, ids = L.aligned(A.contiguous()), L.aligned(B.contiguous()), ids.contiguous()
     scale = scale.contiguous() if scale is not None else None
     with L.on_device(y.device):
@@ -76,6 +84,6 @@ def lora_rows(y, x, A, B, ids, scale=None):
     """y + scale_i (x A_i^T) B_i^T, a new tensor like y: y [..., N] a shared projection's output of x [..., K]; A [n, R, K] and
     B [n, N, R] the adapters' factors (a smaller rank than R: zeros), bf16 or fp16 all four; ids int32 or int64, one a row
     (x.shape[:-1]) or one a batch entry ([x.shape[0]]): i = ids of the row, and a row whose id is none of 0 .. n - 1 (-1) keeps y;
-    scale [n] fp32, or None for ones. N, K and R are multiples of 8, R <= 128. Sums are fp32 and the result is rounded once. What
+    scale [n] fp32, or None for ones. N, K and R are multiples of 8, N and K below 2^24, R <= 128. Sums are fp32 and the result is rounded once. What
     an adapter holds (an infinity, a NaN) reaches no row but its own. Forward only."""
     return _run(lora_rows_op, "lora_rows", y, y, x, A, B, ids, scale)

@@ -69,7 +69,7 @@ def test_forward_codes(p):
     need = L.lib().gpic_fp8_attention_workspace_bytes
     assert call(N=0) == 0 and call(B=0, q=None, o=None) == 0
     for bad in (dict(B=-1), dict(H=0), dict(Hk=0), dict(N=-1), dict(L=-1), dict(D=0), dict(q=None), dict(k=None), dict(v=None),
-                dict(o=None), dict(scale=0.0), dict(scale=-1.0), dict(scale=float("nan")), dict(scale=float("inf")), dict(qs=None),
+                dict(o=None), dict(scale=0.0), dict(scale=-1.0), dict(scale=float("nan")), dict(scale=float("inf")), dict(scale=3e38), dict(qs=None),
                 dict(mask=p, ldm=-1), dict(ks=S(0, -8, 8))):
         assert call(**bad) == -1, bad
     assert call(dt=1) == call(dt=3) == -2

@@ -36,9 +36,11 @@ def test_the_c_entry_checks():
         assert call(**bad) == -1, bad
     assert call(dt=1) == call(dt=3) == -2
     for bad in (dict(N=20), dict(K=20), dict(R=12), dict(R=136), dict(ldx=24), dict(ldx=36), dict(ldy=8), dict(ldy=20),
-                dict(M=1 << 30), dict(n=1 << 30), dict(N=1 << 29, ldy=1 << 29)):
+                dict(M=1 << 30), dict(n=1 << 30), dict(N=1 << 24, ldy=1 << 24), dict(ldx=1 << 24), dict(ldy=1 << 24),
+                dict(K=1 << 24, ldx=1 << 24)):
         assert call(**bad) == -3, bad
     for bad in (dict(y=p + 8), dict(x=p + 2), dict(A=p + 8), dict(B=p + 8), dict(out=p + 8), dict(ws=p + 8)):
         assert call(**bad) == -4, bad
-    assert need(0, 16, 32, 8, 2) == need(4, 16, 32, 136, 2) == 0 and need(4, 16, 32, 8, 2) == 4 * 8 * 4
-    assert call(nws=127) == call(ws=None) == -5
+    assert need(0, 16, 32, 8, 2) == need(4, 16, 32, 136, 2) == 0
+    n = need(4, 16, 32, 8, 2)
+    assert n >= 4 * 8 * 4 and call(nws=n - 1) == call(ws=None) == -5
