@@ -39,6 +39,8 @@ struct LayerNormArgs {
   float eps;
 };
 
+// Bound by memory: x_new and the bytes of [32768 x 1024] with residual, 7 bytes an element, 46 us, 5.1 TB/s; [8191 x 4096] fp32 52
+// us, 5.1 TB/s; one row 3.9 us (the sum, the deviations' and the maximum one after another).
 // A team takes `chunk` rows one after another; the row after the current one is requested before the current one's sums, and w
 // and b are kept in registers. kQ: h goes to q, s (and to h only if it is asked for).
 template <int T, int kV, int E, bool kRes, bool kQ>
@@ -148,6 +150,7 @@ struct LayerNormBwdArgs {
   int C, wt;
 };
 
+// Bound by memory: [8191 x 4096] fp32 79 us, 5.3 TB/s, and 7 us for the column sums; [6528 x 1024] bf16 with dx_new 15.6 and 3.8.
 // The rows of a workgroup in their order, each thread's columns' dw and db in registers; a workgroup's teams are added in their
 // order, then the workgroups in theirs (column_sums_kernel): the same sums in every run.
 template <int T, int kV, int E>

@@ -266,15 +266,16 @@ def test_other_stream(dev):
 
 @pytest.mark.parametrize("shape", [(2, 4, 2, 1, 2000, 64), (2, 4, 2, 70, 2000, 64), (3, 4, 4, 128, 90, 128)])
 def test_captured_and_replayed(dev, shape):
-    """Forward and backward in a graph, replayed with other inputs, lengths and masks and eager work between."""
+    """Forward and backward in a graph, replayed with other inputs, lengths and masks and eager work between. (The leaves are made
+    inside the capture: torch's engine waits for the stream of a leaf's older graph.)"""
     B, H, Hk, N, L, D = shape
     q, k, v, do = make(*shape, BF, 15)
     lens, mask = keys(B, L, "lens+mask")
-    q, k, v = leaves = [t.detach().requires_grad_() for t in (q, k, v)]
 
     def step():
-        o = G.cross_attention(q, k, v, lens, mask)
-        return [o, *torch.autograd.grad(o, leaves, do), G.cross_attention(q.detach(), k.detach(), v.detach(), lens)]
+        leaves = [t.detach().requires_grad_() for t in (q, k, v)]
+        o = G.cross_attention(*leaves, lens, mask)
+        return [o.detach(), *torch.autograd.grad(o, leaves, do), G.cross_attention(q, k, v, lens)]
     st = torch.cuda.Stream()
     st.wait_stream(torch.cuda.current_stream())
     with torch.cuda.stream(st):
@@ -284,12 +285,11 @@ def test_captured_and_replayed(dev, shape):
     with torch.cuda.graph(g):
         out = step()
     for i in range(4):
-        with torch.no_grad():
-            for t, n in zip((q, k, v, do), make(*shape, BF, 20 + i)):
-                t.copy_(n)
-            for t, n in zip((lens, mask), keys(B, L, "lens+mask", 20 + i)):
-                t.copy_(n)
-        ref = [t.detach().clone() for t in step()]
+        for t, n in zip((q, k, v, do), make(*shape, BF, 20 + i)):
+            t.copy_(n)
+        for t, n in zip((lens, mask), keys(B, L, "lens+mask", 20 + i)):
+            t.copy_(n)
+        ref = [t.clone() for t in step()]
         torch.cuda.synchronize()
         g.replay()
         assert all(torch.equal(a, b) for a, b in zip(out, ref)), i

@@ -266,13 +266,14 @@ def test_other_stream_and_threads_of_work(dev):
 
 
 def test_captured_and_replayed(dev):
-    """Forward and backward in a graph, replayed with other inputs and eager work between, against the eager calls."""
+    """Forward and backward in a graph, replayed with other inputs and eager work between, against the eager calls. (The leaves are
+    made inside the capture: torch's engine waits for the stream of a leaf's older graph.)"""
     x, a, w, b, dh, dxn = make((300, 520), BF, 13)
-    leaves = [t.requires_grad_() for t in (x, a, w, b)]
 
     def step():
-        xn, h = G.layer_norm(x, w, b, EPS, a)
-        return [xn, h, *torch.autograd.grad((xn, h), leaves, (dxn, dh))]
+        leaves = [t.detach().requires_grad_() for t in (x, a, w, b)]
+        xn, h = G.layer_norm(leaves[0], leaves[2], leaves[3], EPS, leaves[1])
+        return [xn.detach(), h.detach(), *torch.autograd.grad((xn, h), leaves, (dxn, dh))]
     st = torch.cuda.Stream()
     st.wait_stream(torch.cuda.current_stream())
     with torch.cuda.stream(st):
@@ -282,9 +283,8 @@ def test_captured_and_replayed(dev):
     with torch.cuda.graph(g):
         out = step()
     for i in range(4):
-        with torch.no_grad():
-            for t, n in zip((x, a, w, b, dh, dxn), make((300, 520), BF, 20 + i)):
-                t.copy_(n)
+        for t, n in zip((x, a, w, b, dh, dxn), make((300, 520), BF, 20 + i)):
+            t.copy_(n)
         ref = [t.clone() for t in step()]
         torch.cuda.synchronize()
         g.replay()
