@@ -534,7 +534,7 @@ __global__ __launch_bounds__(256, 2) void attn_dq_kernel(AttnArgs p) {
   __shared__ float norms[4];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l15 = lane & 15, g = lane >> 4;
   const uint32_t id = xcd_order(blockIdx.x, gridDim.x);
-  const int rt = id % p.tiles, pair = id / p.tiles;
+  const int rt = id % p.tiles, split = id / p.tiles % p.splits, pair = id / p.tiles / p.splits;
   const int b = pair / p.Hk, hk = pair - b * p.Hk;
   const Keys keys(p, b);
   const Places<DP> at(lane);
@@ -576,7 +576,7 @@ __global__ __launch_bounds__(256, 2) void attn_dq_kernel(AttnArgs p) {
     for (int o = 8; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor(most, o, 64));
     if (lane == 0) norms[wave] = most;
     __syncthreads();
-    if (threadIdx.x == 0) p.rowmax[id] = fmaxf(fmaxf(norms[0], norms[1]), fmaxf(norms[2], norms[3]));
+    if (threadIdx.x == 0 && split == 0) p.rowmax[pair * (int64_t)p.tiles + rt] = fmaxf(fmaxf(norms[0], norms[1]), fmaxf(norms[2], norms[3]));
   }
   f32x4_t dQ[QT][DT];
 #pragma unroll
@@ -584,9 +584,10 @@ __global__ __launch_bounds__(256, 2) void attn_dq_kernel(AttnArgs p) {
 #pragma unroll
     for (int d = 0; d < DT; d++) dQ[i][d] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
   const uint16_t *kb = p.k + b * p.ks[0] + hk * p.ks[1], *vb = p.v + b * p.vs[0] + hk * p.vs[1];
-  const int end = (keys.len + kTile - 1) / kTile;
+  const int n = (keys.len + kTile - 1) / kTile, per = (n + p.splits - 1) / p.splits;
+  const int end = min(n, (split + 1) * per);
   uint64_t bits = 0, nbits = 0;
-  int i = keys.next(0, end, bits);
+  int i = keys.next(split * per, end, bits);
   const RowStage<DP> sk(p.ks[2]), sv(p.vs[2]);
   if (i < end) {
     sk.load(kt[0], kb + (int64_t)i * kTile * p.ks[2], bits, p.D);
@@ -629,7 +630,7 @@ __global__ __launch_bounds__(256, 2) void attn_dq_kernel(AttnArgs p) {
         for (int v = 0; v < 4; v++) S[q][t][v] = __builtin_amdgcn_exp2f(__builtin_fmaf(S[q][t][v], p.c, -lse[q]));
   };
   int j = i < end ? keys.next(i + 1, end, nbits) : end;
-  if (i < end && j == end) {
+  if ((p.splits == 1 || n == 1) && i < end && j == end) {
     // One tile alone: delta as the sum of P dP. The few keys' dP are as large as delta, which the rounding of o would move by
     // as much as dS's own rounding does.
 #pragma unroll
@@ -648,7 +649,7 @@ __global__ __launch_bounds__(256, 2) void attn_dq_kernel(AttnArgs p) {
   }
 #pragma unroll
   for (int q = 0; q < QT; q++)
-    if (g == 0 && row0 + 16 * q + l15 < p.rows) p.delta[(int64_t)pair * p.rows + row0 + 16 * q + l15] = delta[q];
+    if (g == 0 && split == 0 && row0 + 16 * q + l15 < p.rows) p.delta[(int64_t)pair * p.rows + row0 + 16 * q + l15] = delta[q];
   for (int cur = 0; i < end; cur ^= 1) {
     if (j < end) {
       sk.load(kt[cur ^ 1], kb + (int64_t)j * kTile * p.ks[2], nbits, p.D);
@@ -686,6 +687,15 @@ __global__ __launch_bounds__(256, 2) void attn_dq_kernel(AttnArgs p) {
     const int r = row0 + 16 * q + l15;
     if (r >= p.rows) continue;
     const float f = F16 ? p.scale / up[q] : p.scale;
+    if (p.splits > 1) {   // (added by attn_dq_join_kernel)
+      float *part = p.part + (((int64_t)split * p.B * p.Hk + pair) * p.rows + r) * p.D;
+#pragma unroll
+      for (int d = 0; d < DT; d++)
+        if (16 * d + 4 * g < p.D)
+          *reinterpret_cast<f32x4_t *>(part + 16 * d + 4 * g) =
+              f32x4_t{dQ[q][d][0] * f, dQ[q][d][1] * f, dQ[q][d][2] * f, dQ[q][d][3] * f};
+      continue;
+    }
     uint16_t *o = p.dq + row_at(p, p.dqs, b, hk, r);
 #pragma unroll
     for (int d = 0; d < DT; d++)
@@ -853,6 +863,20 @@ __global__ __launch_bounds__(256, 2) void attn_dkv_kernel(AttnArgs p) {
   }
 }
 
+// The splits' dq added in their order: a thread four columns of one row.
+template <bool F16>
+__global__ __launch_bounds__(256) void attn_dq_join_kernel(AttnArgs p) {
+  const int q = p.D / 4;
+  const int64_t n4 = (int64_t)p.B * p.Hk * p.rows * q, x = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (x >= n4) return;
+  f32x4_t a{0.0f, 0.0f, 0.0f, 0.0f};
+  for (int s = 0; s < p.splits; s++) a += *reinterpret_cast<const f32x4_t *>(p.part + 4 * (s * n4 + x));
+  const int64_t row = x / q;
+  const int c = (int)(x - row * q), pair = (int)(row / p.rows), r = (int)(row - (int64_t)pair * p.rows), b = pair / p.Hk;
+  *reinterpret_cast<u32x2 *>(p.dq + row_at(p, p.dqs, b, pair - b * p.Hk, r) + 4 * c) =
+      u32x2{pack16<F16>(a[0], a[1]), pack16<F16>(a[2], a[3])};
+}
+
 // The splits' dk and dv added in their order: a thread four columns of one key's dk or dv.
 template <bool F16>
 __global__ __launch_bounds__(256) void attn_dkv_join_kernel(AttnArgs p) {
@@ -875,34 +899,40 @@ __global__ __launch_bounds__(256) void attn_dkv_join_kernel(AttnArgs p) {
 constexpr int kMaxAttnD = 128;
 constexpr float kLog2e = 1.44269504f;
 constexpr int kFewRows = 16;
-constexpr int kMaxKeySplits = 64;   // (a wave joins them)
+constexpr int kMaxSplits = 64;   // (a wave joins the forward's)
 constexpr int64_t kMaxBlocks = int64_t(1) << 23;   // (a launch's threads are counted in 32 bits)
 
 struct AttnPlan {
   bool few;
   int qt, tiles, splits;        // forward: 16-row tiles a wave, row tiles, key splits
-  int bqt, btiles, kt, ktiles, ksplits;
+  int bqt, btiles, bsplits;      // dq: the same
+  int kt, ktiles, ksplits;       // dkv: 16-key tiles a wave, key tiles, splits of the rows
 };
+// Two 16-row tiles a wave where the workgroups still fill the device twice (us, one / two: 128 x 16 heads of 256 over up to 320
+// 83 / 73 and dq 101 / 98; 2 x 4 pairs of 8188 rows over 4097, dimension 128, 215 / 155 and 244 / 193); two 16-key tiles for long states of
+// dimension 64 (4 x 16 heads of 1024 over 1024 48 / 44; over states of up to 320, whose masked part it doubles, 135 / 161, and for 128 the
+// registers do not hold them).
+// Keys (dkv: rows) are split while there would be fewer workgroups than CUs: 100 rows of 4 pairs over 4000 keys 51 -> 9.4 + 4.2 for the
+// join, 320 of one pair over 8000 of dimension 128 170 -> 15 + 4; up to two a CU (32 pairs of 512 over 512, 128: dkv 22 -> 20.5 + 9.3) it
+// costs what it gains. Few rows likewise (us, 256 / 512 / 1024 workgroups wanted: 64 pairs over up to 8191 keys of dimension 128
+// 43 / 46 / 45, 256 over 4096 of 64 51 / 65 / 63 with the join).
 static AttnPlan attn_plan(int64_t B, int64_t H, int64_t Hk, int64_t N, int64_t L, int64_t D) {
   AttnPlan a;
   const int64_t pairs = std::max<int64_t>(B * Hk, 1), rows = H / Hk * N;
+  auto splits = [](int64_t blocks, int64_t most) {
+    const int64_t want = 256 / std::max<int64_t>(blocks, 1);
+    return (int)std::max<int64_t>(std::min<int64_t>(std::min(want, most), kMaxSplits), 1);
+  };
   a.few = rows <= kFewRows;
-  if (a.few) {
-    a.qt = 1, a.tiles = 1;
-    const int64_t want = (256 + pairs - 1) / pairs, most = (L + 255) / 256;
-    a.splits = (int)std::max<int64_t>(std::min<int64_t>(std::min(want, most), kMaxKeySplits), 1);
-  } else {
-    a.qt = pairs * ((rows + 127) / 128) >= 512 ? 2 : 1;
-    a.tiles = (int)((rows + 64 * a.qt - 1) / (64 * a.qt));
-    const int64_t want = 512 / (pairs * a.tiles), most = (L + 511) / 512;
-    a.splits = (int)std::max<int64_t>(std::min<int64_t>(std::min(want, most), kMaxKeySplits), 1);
-  }
   a.bqt = pairs * ((rows + 127) / 128) >= 512 ? 2 : 1;
   a.btiles = (int)((rows + 64 * a.bqt - 1) / (64 * a.bqt));
+  a.bsplits = splits(pairs * a.btiles, (L + 511) / 512);
+  a.qt = a.few ? 1 : a.bqt;
+  a.tiles = a.few ? 1 : a.btiles;
+  a.splits = a.few ? splits(pairs, (L + 255) / 256) : a.bsplits;
   a.kt = D <= 64 && L >= 1024 && pairs * ((L + 127) / 128) >= 512 ? 2 : 1;
   a.ktiles = (int)((L + 64 * a.kt - 1) / (64 * a.kt));
-  const int64_t want = 512 / std::max<int64_t>(pairs * a.ktiles, 1), most = (H / Hk * ((N + 63) / 64) + 3) / 4;
-  a.ksplits = (int)std::max<int64_t>(std::min(want, most), 1);
+  a.ksplits = splits(pairs * a.ktiles, (H / Hk * ((N + 63) / 64) + 3) / 4);
   return a;
 }
 static int attn_dp(int64_t D) { return D <= 64 ? 64 : 128; }
@@ -984,7 +1014,7 @@ int gpic_fp8_attention(const uint16_t *q, const int64_t *qs, const uint16_t *k, 
   return (int)hipGetLastError();
 }
 
-// delta, the row tiles' largest norms, the splits' parts of dk and dv: bytes before each, and of all
+// delta, the row tiles' largest norms, the splits' parts of dq, then of dk and dv: bytes before each, and of all
 struct AttnBwdSpace {
   size_t rowmax, part, all;
 };
@@ -993,7 +1023,9 @@ static AttnBwdSpace attn_bwd_space(const AttnPlan &a, int64_t B, int64_t H, int6
   AttnBwdSpace s;
   s.rowmax = up((size_t)B * H * N * sizeof(float));
   s.part = s.rowmax + up((size_t)B * Hk * a.btiles * sizeof(float));
-  s.all = s.part + (a.ksplits > 1 ? (size_t)a.ksplits * B * Hk * L * 2 * D * sizeof(float) : 0);
+  // (dq's parts are joined before dk's and dv's are written: one place)
+  s.all = s.part + std::max(a.bsplits > 1 ? (size_t)a.bsplits * B * H * N * D * sizeof(float) : 0,
+                            a.ksplits > 1 ? (size_t)a.ksplits * B * Hk * L * 2 * D * sizeof(float) : 0);
   return s;
 }
 
@@ -1037,10 +1069,11 @@ int gpic_fp8_attention_bwd(const uint16_t *dout, const int64_t *ds, const uint16
     constexpr bool F = decltype(f)::value;
     constexpr int DP = decltype(dp)::value;
     if (rows) {
-      p.tiles = a.btiles, p.splits = 1;
-      const unsigned grid = (unsigned)(B * Hk * a.btiles);
+      p.tiles = a.btiles, p.splits = a.bsplits;
+      const unsigned grid = (unsigned)(B * Hk * a.btiles * a.bsplits);
       if (a.bqt == 2) attn_dq_kernel<F, DP, 2><<<grid, 256, 0, st>>>(p);
       else attn_dq_kernel<F, DP, 1><<<grid, 256, 0, st>>>(p);
+      if (a.bsplits > 1) attn_dq_join_kernel<F><<<(unsigned)((B * H * N * (D / 4) + 255) / 256), 256, 0, st>>>(p);
     }
     if (keys && dk) {
       p.tiles = a.ktiles, p.splits = a.ksplits;

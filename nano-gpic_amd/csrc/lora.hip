@@ -337,6 +337,7 @@ __global__ __launch_bounds__(256) void lora_expand_kernel(LoraArgs p) {
           if ((NS > 1 ? 32 * k + 8 * g : 8 * (g & 1)) >= p.R) f.b[h][k] = s16x8{0, 0, 0, 0, 0, 0, 0, 0};
 #pragma unroll
       for (int i = 0; i < RT; i++) {
+        if (!(mine >> (16 * i) & 0xffff)) continue;   // (a row tile without rows of the pass)
         u32x4 out = f.y[i];
         if (cur >= 0) {
           f32x4_t acc[2] = {f32x4_t{0.0f, 0.0f, 0.0f, 0.0f}, f32x4_t{0.0f, 0.0f, 0.0f, 0.0f}};
@@ -414,6 +415,7 @@ __global__ __launch_bounds__(256) void lora_expand_runs_kernel(LoraArgs p) {
     const uint64_t mine = __ballot(id == cur) & todo;   // (rows without an adapter are a pass too)
     todo &= ~mine;
     if (pass % p.groups != group) continue;
+    auto part = [&](int i) { return (mine >> (16 * i) & 0xffff) != 0; };   // whether row tile i has rows of the pass
     const uint16_t *B = p.B + (int64_t)max(cur, 0) * p.N * p.R;
     const float s = cur >= 0 && p.s ? p.s[cur] : 1.0f;
     // The result's rows 4 g + v of a row tile lie in other lanes than t's row l15: their factors
@@ -431,7 +433,7 @@ __global__ __launch_bounds__(256) void lora_expand_runs_kernel(LoraArgs p) {
           const int r = NS > 1 ? 32 * k + 8 * g : 8 * (g & 1);
           b[h][k] = *reinterpret_cast<const s16x8 *>(B + ((uint32_t)min(c + HT * l15 + h, c1 - 1) * (uint32_t)p.R + min(r, p.R - 8)));
         }
-      if (again || c != c0 + 16 * HT * wave) fetch_y(c, 0, y0);
+      if (part(0) && (again || c != c0 + 16 * HT * wave)) fetch_y(c, 0, y0);
 #pragma unroll
       for (int h = 0; h < HT; h++)
 #pragma unroll
@@ -440,7 +442,8 @@ __global__ __launch_bounds__(256) void lora_expand_runs_kernel(LoraArgs p) {
 #pragma unroll
       for (int i = 0; i < RT; i++) {
         Run(&y)[4] = i & 1 ? y1 : y0;
-        if (i + 1 < RT) fetch_y(c, i + 1, i & 1 ? y0 : y1);
+        if (i + 1 < RT && part(i + 1)) fetch_y(c, i + 1, i & 1 ? y0 : y1);
+        if (!part(i)) continue;
         f32x4_t acc[HT];
 #pragma unroll
         for (int h = 0; h < HT; h++) {
@@ -476,14 +479,18 @@ struct LoraPlan {
   int nt, shrink_rt, rt, splits, groups, cols;
   bool runs;   // lora_expand_runs_kernel
 };
+// us, first + second product. Up to 256 rows the parts, few rows' columns and up to 16 workgroups for a tile's passes: 200 rows of rank
+// 64, 2048 to 2048, 5.0 + 7.0, as many rows 11.6 + 4.2; 100 of rank 16, 1024 to 4096, 4.1 + 3.5 against 6.8 + 4.8; 500 of rank 16
+// the other way, 4.3 + 7.4 against 4.9 + 4.4. Two workgroups for a tile's passes while one would not fill the device: 500 rows of
+// rank 64, 4096 to 4096, 20.7 + 7.9 against 38.8 + 8.8, 4000 rows 24 + 22 against 25 + 19. Two row tiles share A's reads where x
+// is large: 4000 rows x 4096 17.3 against 23.9, 1500 x 1024 9.0 against 7.8.
 static LoraPlan lora_plan(int64_t M, int64_t K, int64_t N, int64_t R, int64_t n) {
   LoraPlan a;
   a.nt = R <= 16 ? 1 : R <= 32 ? 2 : R <= 64 ? 4 : 8;
   const bool few = M <= 256;
-  a.shrink_rt = M >= 8192 || (a.nt == 8 && M >= 1024) ? 2 : 1;
+  a.shrink_rt = !few && M * K >= (int64_t(1) << 23) ? 2 : 1;
   a.rt = M < 1024 ? 1 : a.nt == 8 ? 2 : 4;
-  // (more rows: most tiles hold one adapter's, some two)
-  a.groups = few ? (int)std::min<int64_t>(std::min<int64_t>(n + 1, M), 16) : n > 1 && M <= 8192 ? 2 : 1;
+  a.groups = few ? (int)std::min<int64_t>(std::min<int64_t>(n + 1, M), 16) : M < 4096 ? 2 : 1;
   a.splits = few ? (int)std::max<int64_t>(std::min<int64_t>(K / 512, kMaxSplits), 1) : 1;   // (a wave 128 of K at least)
   const int64_t tiles = (M + 16 * a.rt - 1) / (16 * a.rt);
   a.runs = a.rt == 4 && a.nt <= 2;
