@@ -10,7 +10,8 @@
 // independent: few rows spread them over workgroups of their own.
 // t stays exact to 2^-16 and better: the second product reads it as the sum of two 16-bit numbers, its rounding and what the
 // rounding left, beside each other on the reduction, which costs little for a rank this small. Many rows: the first launch leaves
-// them so, [M, 2 RP] (RP: the rank in tiles of 16). Few rows: it leaves fp32 parts of K by different workgroups, [splits, M, R].
+// them so, [M, 2 RP] (RP: the rank in tiles of 16). Few rows: it leaves fp32 parts of K by different workgroups, [splits, M, R];
+// in between, where K is long, parts that a small launch adds and leaves as many rows'.
 #include <algorithm>
 #include <type_traits>
 
@@ -28,6 +29,7 @@ struct LoraArgs {
   const void *ids;
   uint16_t *out;
   void *t;
+  const float *parts;   // what lora_pack_kernel adds
   float *up;   // fp16: the factors of t's rows
   int64_t ldx, ldy;
   int M, per, N, K, R, n, wide_ids;   // wide_ids: 64-bit ids
@@ -214,6 +216,36 @@ __global__ __launch_bounds__(64 * kShrinkWaves<NT>) void lora_shrink_kernel(Lora
     }
     __syncthreads();
   }
+}
+
+// The parts of t added in their order and left in halves: 16 threads a row, 8 of the rank each. (Rows without an adapter have no
+// parts: what is made of them is not used.)
+template <bool F16, int NT>
+__global__ __launch_bounds__(256) void lora_pack_kernel(LoraArgs p) {
+  const int row = blockIdx.x * 16 + (threadIdx.x >> 4), c = threadIdx.x & 15;
+  const bool on = row < p.M && 8 * c < p.R;
+  float t[8], most = 0.0f, down = 1.0f, up = 1.0f;
+#pragma unroll
+  for (int e = 0; e < 8; e++) t[e] = 0.0f;
+  for (int s = 0; on && s < p.splits; s++) {
+    const float4 *src = reinterpret_cast<const float4 *>(p.parts + ((int64_t)s * p.M + row) * p.R + 8 * c);
+    const float4 a = src[0], b = src[1];
+    t[0] += a.x, t[1] += a.y, t[2] += a.z, t[3] += a.w, t[4] += b.x, t[5] += b.y, t[6] += b.z, t[7] += b.w;
+  }
+  if (F16) {
+#pragma unroll
+    for (int e = 0; e < 8; e++) most = fmaxf(most, fabsf(t[e]));
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor(most, o, 64));
+    row_factor(most, down, up);
+#pragma unroll
+    for (int e = 0; e < 8; e++) t[e] *= down;
+  }
+  if (row >= p.M || c >= 2 * NT) return;
+  uint16_t *o = static_cast<uint16_t *>(p.t) + (int64_t)row * 32 * NT + 8 * c;
+  *reinterpret_cast<s16x8 *>(o) = half_of<F16>(t, false);
+  *reinterpret_cast<s16x8 *>(o + 16 * NT) = half_of<F16>(t, true);
+  if (F16 && c == 0) p.up[row] = up;
 }
 
 // 2648 rows of rank 64 to 4096 columns 19 us, 64 rows of rank 16 on 32 adapters 6.5, one row 3.1.
@@ -477,29 +509,43 @@ __global__ __launch_bounds__(256) void lora_expand_runs_kernel(LoraArgs p) {
 
 struct LoraPlan {
   int nt, shrink_rt, rt, splits, groups, cols;
-  bool runs;   // lora_expand_runs_kernel
+  bool few, runs;   // few rows: their parts go into the second product; runs: lora_expand_runs_kernel
 };
 // us, first + second product. Up to 256 rows the parts, few rows' columns and up to 16 workgroups for a tile's passes: 200 rows of rank
 // 64, 2048 to 2048, 5.0 + 7.0, as many rows 11.6 + 4.2; 100 of rank 16, 1024 to 4096, 4.1 + 3.5 against 6.8 + 4.8; 500 of rank 16
 // the other way, 4.3 + 7.4 against 4.9 + 4.4. Two workgroups for a tile's passes while one would not fill the device: 500 rows of
 // rank 64, 4096 to 4096, 20.7 + 7.9 against 38.8 + 8.8, 4000 rows 24 + 22 against 25 + 19. Two row tiles share A's reads where x
-// is large: 4000 rows x 4096 17.3 against 23.9, 1500 x 1024 9.0 against 7.8.
+// is large, or the rank: 4000 rows x 4096 17.3 against 23.9, 3000 x 2048 to rank 128 22.3 against 34.8, 1500 x 1024 9.0 against
+// 7.8. Long K is split and packed while there are few tiles: 500 rows of rank 64, 4096 to 4096, 7.6 + 4.3 + 7.8 against
+// 20.7 + 7.9; 2256 of rank 32, 7056 to 224, 20 + 4 + 7 against 29 + 7; 2000 of rank 16, 8192 to 1024, 17 + 4 + 7 against 24 + 7;
+// 4000 rows x 4096 lose by it (20 + 4 against 17).
 static LoraPlan lora_plan(int64_t M, int64_t K, int64_t N, int64_t R, int64_t n) {
   LoraPlan a;
   a.nt = R <= 16 ? 1 : R <= 32 ? 2 : R <= 64 ? 4 : 8;
-  const bool few = M <= 256;
-  a.shrink_rt = !few && M * K >= (int64_t(1) << 23) ? 2 : 1;
+  const bool few = a.few = M <= 256;
+  a.shrink_rt = !few && (M * K >= (int64_t(1) << 23) || (a.nt == 8 && M >= 1024)) ? 2 : 1;
   a.rt = M < 1024 ? 1 : a.nt == 8 ? 2 : 4;
   a.groups = few ? (int)std::min<int64_t>(std::min<int64_t>(n + 1, M), 16) : M < 4096 ? 2 : 1;
-  a.splits = few ? (int)std::max<int64_t>(std::min<int64_t>(K / 512, kMaxSplits), 1) : 1;   // (a wave 128 of K at least)
+  const int64_t blocks = (M + 16 * a.shrink_rt - 1) / (16 * a.shrink_rt) * a.groups;
+  a.splits = (int)std::max<int64_t>(std::min<int64_t>(few ? K / 512 : K >= 4096 ? std::min(K / 1024, 448 / blocks) : 1, kMaxSplits), 1);
+  if (a.splits > 1) a.shrink_rt = 1;
   const int64_t tiles = (M + 16 * a.rt - 1) / (16 * a.rt);
   a.runs = a.rt == 4 && a.nt <= 2;
   a.cols = a.runs ? 512 : few ? 256 : 128;   // (a step of the workgroup's waves, few rows two)
   while (!few && a.cols < 1024 && tiles * ((N + 2 * a.cols - 1) / (2 * a.cols)) >= (a.runs ? 512 : 256)) a.cols *= 2;
   return a;
 }
-static size_t lora_t_bytes(const LoraPlan &a, int64_t M, int64_t R) {
-  return a.splits > 1 ? (size_t)a.splits * M * R * sizeof(float) : (size_t)M * 32 * a.nt * sizeof(uint16_t);
+// t's halves (few rows: its parts), its rows' factors, and the parts that are packed: bytes before each, and of all
+struct LoraSpace {
+  size_t up, parts, all;
+};
+static LoraSpace lora_space(const LoraPlan &a, int64_t M, int64_t R) {
+  const size_t parts = a.splits > 1 ? (size_t)a.splits * M * R * sizeof(float) : 0, halves = (size_t)M * 32 * a.nt * sizeof(uint16_t);
+  LoraSpace s;
+  s.up = a.few && parts ? parts : halves;
+  s.parts = (s.up + M * sizeof(float) + 15) & ~size_t(15);
+  s.all = s.parts + (a.few ? 0 : parts);
+  return s;
 }
 
 template <class F>
@@ -518,8 +564,7 @@ extern "C" {
 
 size_t gpic_fp8_lora_rows_workspace_bytes(int64_t M, int64_t N, int64_t K, int64_t R, int64_t n) {
   if (M <= 0 || N <= 0 || K <= 0 || R <= 0 || n <= 0 || R > kMaxRank) return 0;
-  const LoraPlan a = lora_plan(M, K, N, R, n);
-  return lora_t_bytes(a, M, R) + (size_t)M * sizeof(float);
+  return lora_space(lora_plan(M, K, N, R, n), M, R).all;
 }
 
 int gpic_fp8_lora_rows(const uint16_t *y, int64_t ldy, const uint16_t *x, int64_t ldx, const uint16_t *A, const uint16_t *B,
@@ -543,8 +588,9 @@ int gpic_fp8_lora_rows(const uint16_t *y, int64_t ldy, const uint16_t *x, int64_
   if (tiles * blocks * a.groups >= (int64_t(1) << 24) || stiles * a.splits * a.groups >= (int64_t(1) << 24))
     return GPIC_ESHAPE;
   char *w = static_cast<char *>(ws);
-  const LoraArgs p{y, x, A, B, scales, ids, out, w, reinterpret_cast<float *>(w + lora_t_bytes(a, M, R)), ldx, ldy, (int)M, (int)per,
-                   (int)N, (int)K, (int)R, (int)n, wide_ids, a.splits, a.groups, (int)blocks, a.cols};
+  const LoraSpace space = lora_space(a, M, R);
+  LoraArgs p{y, x, A, B, scales, ids, out, w, reinterpret_cast<const float *>(w + space.parts), reinterpret_cast<float *>(w + space.up),
+             ldx, ldy, (int)M, (int)per, (int)N, (int)K, (int)R, (int)n, wide_ids, a.splits, a.groups, (int)blocks, a.cols};
   const hipStream_t st = (hipStream_t)stream;
   const dim3 shrink((unsigned)stiles, (unsigned)a.splits, (unsigned)a.groups),
       expand((unsigned)(tiles * blocks), (unsigned)a.groups);
@@ -552,12 +598,17 @@ int gpic_fp8_lora_rows(const uint16_t *y, int64_t ldy, const uint16_t *x, int64_
     constexpr bool F = decltype(f16)::value;
     with_rank(a.nt, [&](auto nt) {
       constexpr int T = decltype(nt)::value, W = T == 8 ? 2 : 4;
-      if (a.splits > 1) lora_shrink_kernel<F, 1, T, true><<<shrink, 64 * kShrinkWaves<T>, 0, st>>>(p);
+      if (a.splits > 1) {
+        LoraArgs q = p;
+        if (!a.few) q.t = w + space.parts;
+        lora_shrink_kernel<F, 1, T, true><<<shrink, 64 * kShrinkWaves<T>, 0, st>>>(q);
+        if (!a.few) lora_pack_kernel<F, T><<<(unsigned)((M + 15) / 16), 256, 0, st>>>(p);
+      }
       else if (a.shrink_rt == 2) lora_shrink_kernel<F, 2, T, false><<<shrink, 64 * kShrinkWaves<T>, 0, st>>>(p);
       else lora_shrink_kernel<F, 1, T, false><<<shrink, 64 * kShrinkWaves<T>, 0, st>>>(p);
       if constexpr (T <= 2)
         if (a.runs) return lora_expand_runs_kernel<F, 4, T><<<expand, 256, 0, st>>>(p);
-      if (a.splits > 1) lora_expand_kernel<F, 1, T, true><<<expand, 256, 0, st>>>(p);
+      if (a.few && a.splits > 1) lora_expand_kernel<F, 1, T, true><<<expand, 256, 0, st>>>(p);
       else if (a.rt == W) lora_expand_kernel<F, W, T, false><<<expand, 256, 0, st>>>(p);
       else lora_expand_kernel<F, 1, T, false><<<expand, 256, 0, st>>>(p);
     });

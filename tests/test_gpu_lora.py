@@ -58,6 +58,15 @@ def test_against_64_bits(dev, dt, R, M, K, N, n):
         check(G.lora_rows(y, x, A, B, ids), y, x, A, B, ids, None)
 
 
+@pytest.mark.parametrize("dt", [BF, FP])
+@pytest.mark.parametrize("M,K,N,n,R", [(300, 4104, 264, 3, 24), (700, 8192, 136, 40, 64), (1500, 4160, 72, 2, 128), (260, 20000, 8, 1, 8)])
+def test_long_reductions_in_parts(dev, dt, M, K, N, n, R):
+    y, x, A, B, ids, s = make(M, K, N, n, R, dt, 9)
+    check(G.lora_rows(y, x, A, B, ids, s), y, x, A, B, ids, s)
+    out = G.lora_rows(y, x, A, B, ids, s)
+    assert torch.equal(G.lora_rows(y, x, A, B, ids, s), out)
+
+
 @pytest.mark.parametrize("order", ["runs", "same", "none", "mixed", "outside"])
 @pytest.mark.parametrize("M", [40, 2500])
 def test_orders_of_ids(dev, order, M):
