@@ -41,6 +41,7 @@ struct AttnArgs {
   float *lse, *delta, *rowmax, *part;
   int B, H, Hk, N, L, D, G, rows, tiles, splits;   // rows: G N; tiles: row (or key) tiles of a (batch entry, key head) pair
   int rtiles;                                      // row tiles of the dq kernel
+  int budget, least;   // Runs: workgroups of a key head (0: no runs, `splits` for every pair), a run's least tiles
   float c, scale;                                  // c: scale log2 e
 };
 
@@ -325,19 +326,40 @@ __global__ __launch_bounds__(256, 2) void attn_fwd_kernel(AttnArgs p) {
   }
 }
 
+// Requests of unlike lengths: a key head's tiles of 32 keys, entry after entry, dealt out in equal runs to `budget` workgroups
+// (of `least` tiles at least; an entry without keys counts as a tile). A run that goes past an entry's end goes on in the next entry, and
+// an entry's splits are the runs that meet it. Lane b of a wave holds where entry b begins and ends.
+struct Runs {
+  uint32_t run, begin, end, all;
+  __device__ __forceinline__ explicit Runs(const AttnArgs &p) {
+    const int lane = threadIdx.x & 63;
+    const uint32_t n = lane < p.B ? max(((uint32_t)min(max(p.lens[lane], 0), p.L) + 31) / 32, 1u) : 0;
+    end = n;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      const uint32_t below = __shfl_up(end, o, 64);
+      if (lane >= o) end += below;
+    }
+    begin = end - n;
+    all = __builtin_amdgcn_readlane(end, 63);
+    run = max((all + p.budget - 1) / p.budget, (uint32_t)p.least);
+  }
+  // Of this lane's entry: the first run, and how many.
+  __device__ __forceinline__ uint32_t first() const { return begin / run; }
+  __device__ __forceinline__ uint32_t count() const { return end > begin ? (end - 1) / run - first() + 1 : 0; }
+};
+
 // Up to 16 rows a pair (a token's heads): memory bounds it, k and v once: 8 x 8 pairs over 8191 keys of dimension 128 54 us, 4.95
 // TB/s; 256 pairs over 4096 of 64 51 us, 5.2 TB/s. Each wave walks keys of its own, 32 a step: k goes from
 // memory to the lanes as they multiply it, v through the wave's own staged tile, both requested a step ahead; no barrier until the
 // waves' results are joined.
+// attn_few: keys of tiles `from` to `to` of a pair, its split-th part.
 template <bool F16, int DP>
-__global__ __launch_bounds__(256, 2) void attn_few_kernel(AttnArgs p) {
+__device__ __forceinline__ void attn_few(const AttnArgs &p, uint16_t (&vt)[4][32 * DP], float (&joined)[4][16][DP + 4], int b,
+                                         int hk, int split, int from, int to) {
   constexpr int KS = DP / 32, DT = DP / 16, kC = DP / 8, kU = 32 * kC / 64;
-  __shared__ __attribute__((aligned(16))) uint16_t vt[4][32 * DP];
-  __shared__ __attribute__((aligned(16))) float joined[4][16][DP + 4];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l15 = lane & 15, g = lane >> 4;
-  const uint32_t id = xcd_order(blockIdx.x, gridDim.x);
-  const int split = id % p.splits, pair = id / p.splits;
-  const int b = pair / p.Hk, hk = pair - b * p.Hk;
+  const int pair = b * p.Hk + hk;
   const Keys keys(p, b);
   const Places<DP> at(lane);
   s16x8 qf[KS];
@@ -349,8 +371,7 @@ __global__ __launch_bounds__(256, 2) void attn_few_kernel(AttnArgs p) {
   for (int d = 0; d < DT; d++) O[d] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
   Softmax sm;
   const uint16_t *kb = p.k + b * p.ks[0] + hk * p.ks[1], *vb = p.v + b * p.vs[0] + hk * p.vs[1];
-  const int n = (keys.len + 31) / 32, per = (n + 4 * p.splits - 1) / (4 * p.splits);
-  const int first = (split * 4 + wave) * per, end = min(n, first + per);
+  const int per = (to - from + 3) / 4, first = from + wave * per, end = min(to, first + per);
   s16x8 K[2][KS], Kn[2][KS];
   u32x4 V[kU];
   const uint16_t *kl = kb + l15 * p.ks[2] + 8 * g, *vl = vb + (lane / kC) * p.vs[2] + 8 * (lane % kC);
@@ -468,6 +489,30 @@ __global__ __launch_bounds__(256, 2) void attn_few_kernel(AttnArgs p) {
   }
 }
 
+template <bool F16, int DP, bool kRuns>
+__global__ __launch_bounds__(256, 2) void attn_few_kernel(AttnArgs p) {
+  __shared__ __attribute__((aligned(16))) uint16_t vt[4][32 * DP];
+  __shared__ __attribute__((aligned(16))) float joined[4][16][DP + 4];
+  const uint32_t id = xcd_order(blockIdx.x, gridDim.x);
+  if constexpr (kRuns) {
+    const int hk = id / p.budget;
+    const Runs runs(p);
+    const uint32_t r = id - hk * p.budget, stop = min((r + 1) * runs.run, runs.all);
+    for (uint32_t at = r * runs.run; at < stop;) {
+      const int b = __builtin_ctzll(__ballot(at < runs.end));
+      const uint32_t begin = __builtin_amdgcn_readlane(runs.begin, b),
+                     upto = min(stop, (uint32_t)__builtin_amdgcn_readlane(runs.end, b));
+      attn_few<F16, DP>(p, vt, joined, b, hk, r - begin / runs.run, at - begin, upto - begin);
+      at = upto;
+      __syncthreads();
+    }
+  } else {
+    const int pair = id / p.splits, split = id - pair * p.splits, b = pair / p.Hk;
+    const int n = (Keys(p, b).len + 31) / 32, per = (n + p.splits - 1) / p.splits;
+    attn_few<F16, DP>(p, vt, joined, b, pair - b * p.Hk, split, min(n, split * per), min(n, (split + 1) * per));
+  }
+}
+
 // The splits' parts of a row, joined in their order, by one wave: lane s holds split s's maximum and factor; the parts' columns are
 // read two a lane, eight splits at a time.
 template <bool F16, int DP>
@@ -476,8 +521,13 @@ __global__ __launch_bounds__(64) void attn_join_kernel(AttnArgs p) {
   const int lane = threadIdx.x;
   const float *x = p.part + row * (DP + 2);
   const int64_t step = all * (DP + 2);
-  const bool on = lane < p.splits;
-  const float2 ml = on ? *reinterpret_cast<const float2 *>(x + lane * step + DP) : float2{-kInf, 0.0f};
+  float2 ml = lane < p.splits ? *reinterpret_cast<const float2 *>(x + lane * step + DP) : float2{-kInf, 0.0f};
+  const int pair = (int)(row / p.rows), r = (int)(row - (int64_t)pair * p.rows), b = pair / p.Hk;
+  int splits = p.splits;
+  if (p.budget) {
+    splits = __builtin_amdgcn_readlane(Runs(p).count(), b);
+    if (lane >= splits) ml = float2{-kInf, 0.0f};
+  }
   float m = ml.x;
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
@@ -489,22 +539,21 @@ __global__ __launch_bounds__(64) void attn_join_kernel(AttnArgs p) {
   float o[kV];
 #pragma unroll
   for (int v = 0; v < kV; v++) o[v] = 0.0f;
-  for (int s0 = 0; s0 < p.splits; s0 += 8) {
+  for (int s0 = 0; s0 < splits; s0 += 8) {
     float part[8][kV];
 #pragma unroll
     for (int i = 0; i < 8; i++)
 #pragma unroll
-      for (int v = 0; v < kV; v++) part[i][v] = x[min(s0 + i, p.splits - 1) * step + lane + 64 * v];
+      for (int v = 0; v < kV; v++) part[i][v] = x[min(s0 + i, splits - 1) * step + lane + 64 * v];
 #pragma unroll
     for (int i = 0; i < 8; i++) {
       const float fs = __shfl(f, min(s0 + i, 63), 64);
-      if (s0 + i < p.splits && fs != 0.0f) {
+      if (s0 + i < splits && fs != 0.0f) {
 #pragma unroll
         for (int v = 0; v < kV; v++) o[v] = __builtin_fmaf(fs, part[i][v], o[v]);
       }
     }
   }
-  const int pair = (int)(row / p.rows), r = (int)(row - (int64_t)pair * p.rows), b = pair / p.Hk;
   const float inv = sum == 0.0f ? 0.0f : __fdiv_rn(1.0f, sum);
   uint16_t *out = p.out + row_at(p, p.os, b, pair - b * p.Hk, r);
 #pragma unroll
@@ -576,7 +625,8 @@ __global__ __launch_bounds__(256, 2) void attn_dq_kernel(AttnArgs p) {
     for (int o = 8; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor(most, o, 64));
     if (lane == 0) norms[wave] = most;
     __syncthreads();
-    if (threadIdx.x == 0 && split == 0) p.rowmax[pair * (int64_t)p.tiles + rt] = fmaxf(fmaxf(norms[0], norms[1]), fmaxf(norms[2], norms[3]));
+    if (threadIdx.x == 0 && split == 0)
+      p.rowmax[pair * (int64_t)p.tiles + rt] = fmaxf(fmaxf(norms[0], norms[1]), fmaxf(norms[2], norms[3]));
   }
   f32x4_t dQ[QT][DT];
 #pragma unroll
@@ -705,8 +755,8 @@ __global__ __launch_bounds__(256, 2) void attn_dq_kernel(AttnArgs p) {
   }
 }
 
-// 128 x 16 heads of 256 over up to 320 136 us; 4 x 16 of 1024 over 2048, dimension 128, 163 us, 0.84 PFLOP/s of its four products: there LDS
-// is read four times for 16 keys a wave, and 32 do not fit the registers.
+// 128 x 16 heads of 256 over up to 320 136 us; 4 x 16 of 1024 over 2048, dimension 128, 163 us, 0.84 PFLOP/s of its four
+// products: there LDS is read four times for 16 keys a wave, and 32 do not fit the registers.
 // dk and dv of 64 KT keys: the waves' k and v stay in registers, the pair's rows (or the split's part of them) pass by in staged
 // tiles of q and do. A shared key's gradient sums over its heads here, in a fixed order.
 template <bool F16, int DP, int KT>
@@ -905,18 +955,23 @@ constexpr int64_t kMaxBlocks = int64_t(1) << 23;   // (a launch's threads are co
 struct AttnPlan {
   bool few;
   int qt, tiles, splits;        // forward: 16-row tiles a wave, row tiles, key splits
+  int budget, least;             // few rows of requests of unlike lengths: for Runs; splits is then a pair's most
   int bqt, btiles, bsplits;      // dq: the same
   int kt, ktiles, ksplits;       // dkv: 16-key tiles a wave, key tiles, splits of the rows
 };
 // Two 16-row tiles a wave where the workgroups still fill the device twice (us, one / two: 128 x 16 heads of 256 over up to 320
-// 83 / 73 and dq 101 / 98; 2 x 4 pairs of 8188 rows over 4097, dimension 128, 215 / 155 and 244 / 193); two 16-key tiles for long states of
-// dimension 64 (4 x 16 heads of 1024 over 1024 48 / 44; over states of up to 320, whose masked part it doubles, 135 / 161, and for 128 the
-// registers do not hold them).
-// Keys (dkv: rows) are split while there would be fewer workgroups than CUs: 100 rows of 4 pairs over 4000 keys 51 -> 9.4 + 4.2 for the
-// join, 320 of one pair over 8000 of dimension 128 170 -> 15 + 4; up to two a CU (32 pairs of 512 over 512, 128: dkv 22 -> 20.5 + 9.3) it
-// costs what it gains. Few rows likewise (us, 256 / 512 / 1024 workgroups wanted: 64 pairs over up to 8191 keys of dimension 128
-// 43 / 46 / 45, 256 over 4096 of 64 51 / 65 / 63 with the join).
-static AttnPlan attn_plan(int64_t B, int64_t H, int64_t Hk, int64_t N, int64_t L, int64_t D) {
+// 83 / 73 and dq 101 / 98; 2 x 4 pairs of 8188 rows over 4097, dimension 128, 215 / 155 and 244 / 193); two 16-key tiles for long
+// states of dimension 64 (4 x 16 heads of 1024 over 1024 48 / 44; over states of up to 320, whose masked part it doubles,
+// 135 / 161, and for 128 the registers do not hold them).
+// Keys (dkv: rows) are split while there would be fewer workgroups than CUs: 100 rows of 4 pairs over 4000 keys 51 -> 9.4 + 4.2
+// for the join, 320 of one pair over 8000 of dimension 128 170 -> 15 + 4; up to two a CU (32 pairs of 512 over 512, 128: dkv
+// 22 -> 20.5 + 9.3) it costs what it gains. Few rows likewise (us, 256 / 512 / 1024 workgroups wanted: 64 pairs over up to 8191
+// keys of dimension 128 43 / 46 / 45, 256 over 4096 of 64 51 / 65 / 63 with the join).
+// Entries with lengths of their own are dealt out in runs (us with the join, splits or a workgroup for each pair / runs; lengths
+// drawn evenly, then all full): 64 pairs over up to 8191 keys of dimension 128 46 / 38, 59 / 59; 256 146 / 128, 196 / 193; 480
+// over 4096 136 / 107, 189 / 189; 256 over 4096 of 64 39 / 34, 51 / 55. Not where k and v are small, as going on in the next entry
+// takes 4 and the join as much: 256 over 2048 of 64 20 / 21, 128 over 4096 23.8 / 22.2, 27 / 30, 16 of 128 14 / 18.
+static AttnPlan attn_plan(bool lens, int64_t B, int64_t H, int64_t Hk, int64_t N, int64_t L, int64_t D) {
   AttnPlan a;
   const int64_t pairs = std::max<int64_t>(B * Hk, 1), rows = H / Hk * N;
   auto splits = [](int64_t blocks, int64_t most) {
@@ -930,6 +985,13 @@ static AttnPlan attn_plan(int64_t B, int64_t H, int64_t Hk, int64_t N, int64_t L
   a.qt = a.few ? 1 : a.bqt;
   a.tiles = a.few ? 1 : a.btiles;
   a.splits = a.few ? splits(pairs, (L + 255) / 256) : a.bsplits;
+  a.budget = a.least = 0;
+  if (a.few && lens && B > 1 && B <= 64 && Hk <= 64 && pairs < 512 && pairs * L * D >= (int64_t(3) << 24)) {
+    a.budget = (int)(256 / Hk);
+    const int64_t n = (L + 31) / 32;
+    a.least = (int)std::max<int64_t>((n + kMaxSplits - 3) / (kMaxSplits - 2), 8);
+    a.splits = (int)std::min<int64_t>(a.budget, (n - 2) / a.least + 2);   // (an entry may begin and end inside runs)
+  }
   a.kt = D <= 64 && L >= 1024 && pairs * ((L + 127) / 128) >= 512 ? 2 : 1;
   a.ktiles = (int)((L + 64 * a.kt - 1) / (64 * a.kt));
   a.ksplits = splits(pairs * a.ktiles, (H / Hk * ((N + 63) / 64) + 3) / 4);
@@ -975,8 +1037,8 @@ extern "C" {
 
 size_t gpic_fp8_attention_workspace_bytes(int64_t B, int64_t H, int64_t Hk, int64_t N, int64_t L, int64_t D) {
   if (attn_shape(GPIC_DTYPE_BF16, B, H, Hk, N, L, D) != GPIC_OK || B * N == 0) return 0;
-  const AttnPlan a = attn_plan(B, H, Hk, N, L, D);
-  return a.splits > 1 ? (size_t)a.splits * B * H * N * (attn_dp(D) + 2) * sizeof(float) : 0;
+  const int splits = std::max(attn_plan(false, B, H, Hk, N, L, D).splits, attn_plan(true, B, H, Hk, N, L, D).splits);
+  return splits > 1 ? (size_t)splits * B * H * N * (attn_dp(D) + 2) * sizeof(float) : 0;
 }
 
 int gpic_fp8_attention(const uint16_t *q, const int64_t *qs, const uint16_t *k, const int64_t *ks, const uint16_t *v,
@@ -995,18 +1057,20 @@ int gpic_fp8_attention(const uint16_t *q, const int64_t *qs, const uint16_t *k, 
     return e;
   if (!aligned16(ws)) return GPIC_EALIGN;
   if (ws_bytes < gpic_fp8_attention_workspace_bytes(B, H, Hk, N, L, D)) return GPIC_EWORKSPACE;
-  const AttnPlan a = attn_plan(B, H, Hk, N, L, D);
+  const AttnPlan a = attn_plan(lens != nullptr, B, H, Hk, N, L, D);
   if (a.splits > 1 && !ws) return GPIC_EWORKSPACE;
   p.q = q, p.k = k, p.v = v, p.out = o, p.lens = lens, p.mask = mask, p.ldm = ldm, p.lse = lse;
   p.part = static_cast<float *>(ws);
   p.B = (int)B, p.H = (int)H, p.Hk = (int)Hk, p.N = (int)N, p.L = (int)L, p.D = (int)D, p.G = (int)(H / Hk);
   p.rows = p.G * p.N, p.tiles = a.tiles, p.splits = a.splits, p.scale = scale, p.c = scale * kLog2e;
   const hipStream_t st = (hipStream_t)stream;
-  const unsigned grid = (unsigned)(B * Hk * a.tiles * a.splits);
+  p.budget = a.budget, p.least = a.least;
+  const unsigned grid = (unsigned)(a.budget ? Hk * a.budget : B * Hk * a.tiles * a.splits);
   with_attn(dtype, D, [&](auto f, auto dp) {
     constexpr bool F = decltype(f)::value;
     constexpr int DP = decltype(dp)::value;
-    if (a.few) attn_few_kernel<F, DP><<<grid, 256, 0, st>>>(p);
+    if (a.few && a.budget) attn_few_kernel<F, DP, true><<<grid, 256, 0, st>>>(p);
+    else if (a.few) attn_few_kernel<F, DP, false><<<grid, 256, 0, st>>>(p);
     else if (a.qt == 2) attn_fwd_kernel<F, DP, 2><<<grid, 256, 0, st>>>(p);
     else attn_fwd_kernel<F, DP, 1><<<grid, 256, 0, st>>>(p);
     if (a.splits > 1) attn_join_kernel<F, DP><<<(unsigned)(B * Hk * p.rows), 64, 0, st>>>(p);
@@ -1031,7 +1095,7 @@ static AttnBwdSpace attn_bwd_space(const AttnPlan &a, int64_t B, int64_t H, int6
 
 size_t gpic_fp8_attention_bwd_workspace_bytes(int64_t B, int64_t H, int64_t Hk, int64_t N, int64_t L, int64_t D) {
   if (attn_shape(GPIC_DTYPE_BF16, B, H, Hk, N, L, D) != GPIC_OK) return 0;
-  return attn_bwd_space(attn_plan(B, H, Hk, N, L, D), B, H, Hk, N, L, D).all;
+  return attn_bwd_space(attn_plan(false, B, H, Hk, N, L, D), B, H, Hk, N, L, D).all;
 }
 
 int gpic_fp8_attention_bwd(const uint16_t *dout, const int64_t *ds, const uint16_t *q, const int64_t *qs, const uint16_t *k,
@@ -1054,7 +1118,7 @@ int gpic_fp8_attention_bwd(const uint16_t *dout, const int64_t *ds, const uint16
       (dk && ((e = strides_ok(dk, dks, p.dks)) || (e = strides_ok(dv, dvs, p.dvs)))))
     return e;
   if (!aligned16(ws)) return GPIC_EALIGN;
-  const AttnPlan a = attn_plan(B, H, Hk, N, L, D);
+  const AttnPlan a = attn_plan(false, B, H, Hk, N, L, D);
   const AttnBwdSpace space = attn_bwd_space(a, B, H, Hk, N, L, D);
   if (ws_bytes < space.all || (space.all && !ws)) return GPIC_EWORKSPACE;
   p.q = q, p.k = k, p.v = v, p.o = o, p.dout = dout, p.dq = dq, p.dk = dk, p.dv = dv, p.lens = lens, p.mask = mask, p.ldm = ldm;

@@ -511,8 +511,8 @@ struct LoraPlan {
   int nt, shrink_rt, rt, splits, groups, cols;
   bool few, runs;   // few rows: their parts go into the second product; runs: lora_expand_runs_kernel
 };
-// us, first + second product. Up to 256 rows the parts, few rows' columns and up to 16 workgroups for a tile's passes: 200 rows of rank
-// 64, 2048 to 2048, 5.0 + 7.0, as many rows 11.6 + 4.2; 100 of rank 16, 1024 to 4096, 4.1 + 3.5 against 6.8 + 4.8; 500 of rank 16
+// us, first + second product. Up to 256 rows the parts, few rows' columns and up to 16 workgroups for a tile's passes: 200 rows of
+// rank 64, 2048 to 2048, 5.0 + 7.0, as many rows 11.6 + 4.2; 100 of rank 16, 1024 to 4096, 4.1 + 3.5 against 6.8 + 4.8; 500 of rank 16
 // the other way, 4.3 + 7.4 against 4.9 + 4.4. Two workgroups for a tile's passes while one would not fill the device: 500 rows of
 // rank 64, 4096 to 4096, 20.7 + 7.9 against 38.8 + 8.8, 4000 rows 24 + 22 against 25 + 19. Two row tiles share A's reads where x
 // is large, or the rank: 4000 rows x 4096 17.3 against 23.9, 3000 x 2048 to rank 128 22.3 against 34.8, 1500 x 1024 9.0 against
@@ -575,8 +575,8 @@ int gpic_fp8_lora_rows(const uint16_t *y, int64_t ldy, const uint16_t *x, int64_
   if (M > 0 && (!y || !x || !A || !B || !ids || !out)) return GPIC_EINVAL;
   if (dtype != GPIC_DTYPE_BF16 && dtype != GPIC_DTYPE_F16) return GPIC_EDTYPE;
   const int64_t most = int64_t(1) << 30, wide = int64_t(1) << 24;   // (a tile's offsets in 32 bits)
-  if (N % 8 || K % 8 || R % 8 || R > kMaxRank || per >= most || ldx % 8 || ldx < K || ldy % 8 || ldy < N || M >= most || N >= wide || K >= wide ||
-      ldx >= wide || ldy >= wide || n >= most)
+  if (N % 8 || K % 8 || R % 8 || R > kMaxRank || per >= most || ldx % 8 || ldx < K || ldy % 8 || ldy < N || M >= most || N >= wide ||
+      K >= wide || ldx >= wide || ldy >= wide || n >= most)
     return GPIC_ESHAPE;
   if (!aligned16(y) || !aligned16(x) || !aligned16(A) || !aligned16(B) || !aligned16(out) || !aligned16(ws)) return GPIC_EALIGN;
   if (M == 0) return GPIC_OK;
@@ -597,20 +597,21 @@ int gpic_fp8_lora_rows(const uint16_t *y, int64_t ldy, const uint16_t *x, int64_
   auto launch = [&](auto f16) {
     constexpr bool F = decltype(f16)::value;
     with_rank(a.nt, [&](auto nt) {
-      constexpr int T = decltype(nt)::value, W = T == 8 ? 2 : 4;
+      constexpr int T = decltype(nt)::value;
       if (a.splits > 1) {
         LoraArgs q = p;
         if (!a.few) q.t = w + space.parts;
         lora_shrink_kernel<F, 1, T, true><<<shrink, 64 * kShrinkWaves<T>, 0, st>>>(q);
         if (!a.few) lora_pack_kernel<F, T><<<(unsigned)((M + 15) / 16), 256, 0, st>>>(p);
+      } else if (a.shrink_rt == 2) {
+        lora_shrink_kernel<F, 2, T, false><<<shrink, 64 * kShrinkWaves<T>, 0, st>>>(p);
+      } else {
+        lora_shrink_kernel<F, 1, T, false><<<shrink, 64 * kShrinkWaves<T>, 0, st>>>(p);
       }
-      else if (a.shrink_rt == 2) lora_shrink_kernel<F, 2, T, false><<<shrink, 64 * kShrinkWaves<T>, 0, st>>>(p);
-      else lora_shrink_kernel<F, 1, T, false><<<shrink, 64 * kShrinkWaves<T>, 0, st>>>(p);
-      if constexpr (T <= 2)
-        if (a.runs) return lora_expand_runs_kernel<F, 4, T><<<expand, 256, 0, st>>>(p);
       if (a.few && a.splits > 1) lora_expand_kernel<F, 1, T, true><<<expand, 256, 0, st>>>(p);
-      else if (a.rt == W) lora_expand_kernel<F, W, T, false><<<expand, 256, 0, st>>>(p);
-      else lora_expand_kernel<F, 1, T, false><<<expand, 256, 0, st>>>(p);
+      else if (a.rt == 1) lora_expand_kernel<F, 1, T, false><<<expand, 256, 0, st>>>(p);
+      else if constexpr (T <= 2) lora_expand_runs_kernel<F, 4, T><<<expand, 256, 0, st>>>(p);
+      else lora_expand_kernel<F, T == 8 ? 2 : 4, T, false><<<expand, 256, 0, st>>>(p);
     });
   };
   if (dtype == GPIC_DTYPE_F16) launch(std::true_type());

@@ -84,6 +84,6 @@ def lora_rows(y, x, A, B, ids, scale=None):
     """y + scale_i (x A_i^T) B_i^T, a new tensor like y: y [..., N] a shared projection's output of x [..., K]; A [n, R, K] and
     B [n, N, R] the adapters' factors (a smaller rank than R: zeros), bf16 or fp16 all four; ids int32 or int64, one a row
     (x.shape[:-1]) or one a batch entry ([x.shape[0]]): i = ids of the row, and a row whose id is none of 0 .. n - 1 (-1) keeps y;
-    scale [n] fp32, or None for ones. N, K and R are multiples of 8, N and K below 2^24, R <= 128. Sums are fp32 and the result is rounded once. What
-    an adapter holds (an infinity, a NaN) reaches no row but its own. Forward only."""
+    scale [n] fp32, or None for ones. N, K and R are multiples of 8, N and K below 2^24, R <= 128. Sums are fp32 and the result is
+    rounded once. What an adapter holds (an infinity, a NaN) reaches no row but its own. Forward only."""
     return _run(lora_rows_op, "lora_rows", y, y, x, A, B, ids, scale)

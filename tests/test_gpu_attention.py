@@ -75,6 +75,48 @@ def test_larger_and_split(dev, shape, kind):
     both(q, k, v, do, *keys(B, L, kind, 1))
 
 
+@pytest.mark.parametrize("B,H,Hk,N,L,D", [(9, 16, 8, 1, 6200, 128), (64, 16, 4, 4, 3100, 64), (2, 8, 1, 2, 262144, 96), (3, 64, 64, 1, 4100, 72)])
+@pytest.mark.parametrize("kind", ["none", "ones", "one long", "tiles", "full", "drawn", "mask"])
+def test_one_token_of_unlike_lengths(dev, B, H, Hk, N, L, D, kind):
+    """Lengths that put an entry's ends inside, at and outside the runs that workgroups take; o and lse, with 64-bit lengths too."""
+    g = torch.Generator(device="cuda").manual_seed(B)
+    r = lambda h, n: torch.randn(B, n, h, D, generator=g, device="cuda").to(BF).transpose(1, 2)  # noqa: E731
+    q, k, v = r(H, N), r(Hk, L), r(Hk, L)
+    few = torch.arange(B, dtype=torch.int32, device="cuda")
+    drawn = torch.randint(0, L + 1, (B,), generator=g, device="cuda", dtype=torch.int32)
+    lens = {"none": 0 * few, "ones": 0 * few + 1, "one long": torch.where(few == B // 2, L, few % 3), "tiles": 32 * (few % 5) + 256,
+            "full": 0 * few + L, "drawn": drawn, "mask": drawn}[kind].to(torch.int32)
+    mask = torch.rand(B, L, generator=g, device="cuda") < 0.02 if kind == "mask" else None
+    o, lse = G.cross_attention_fwd(q, k, v, lens, mask)
+    assert torch.equal(G.cross_attention(q, k, v, lens.long(), mask), o)
+    ok = valid_keys(B, L, lens, mask, "cuda")
+    for b in range(B):   # (an entry at a time: 64 bits of all would not fit beside each other)
+        check(q[b:b + 1], k[b:b + 1], v[b:b + 1], ok[b:b + 1], D ** -0.5, o[b:b + 1])
+        _, alone = G.cross_attention_fwd(q[b:b + 1], k[b:b + 1], v[b:b + 1], lens[b:b + 1], None if mask is None else mask[b:b + 1])
+        assert torch.equal(torch.isinf(alone), torch.isinf(lse[b:b + 1]))
+        # (p's sums in another order: fp32 steps of the sum, as many as its longest chain of additions, and of the maximum's exponent)
+        assert ((alone - lse[b:b + 1]).nan_to_num(0).abs() <= 2.0 ** -24 * (L / 8 + 64)).all()
+
+
+def test_captured_lengths_change(dev):
+    B, H, Hk, L, D = 9, 16, 8, 6200, 128
+    g = torch.Generator(device="cuda").manual_seed(4)
+    r = lambda h, n: torch.randn(B, n, h, D, generator=g, device="cuda").to(FP).transpose(1, 2)  # noqa: E731
+    q, k, v = r(H, 1), r(Hk, L), r(Hk, L)
+    lens = torch.full((B,), L, dtype=torch.int32, device="cuda")
+    G.cross_attention(q, k, v, lens)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        o = G.cross_attention(q, k, v, lens)
+    for i in range(5):
+        lens.copy_(torch.randint(0, L + 1, (B,), generator=g, device="cuda") * (i != 2))
+        ref = G.cross_attention(q, k, v, lens)
+        graph.replay()
+        assert torch.equal(o, ref), i
+    assert not torch.equal(o, torch.zeros_like(o))
+
+
 @pytest.mark.parametrize("dt", [BF, FP])
 @pytest.mark.parametrize("N", [1, 100])
 def test_padding_may_hold_anything(dev, dt, N):
