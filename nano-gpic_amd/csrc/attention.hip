@@ -66,15 +66,6 @@ __device__ __forceinline__ float groups_max(float v) {
   return over_groups(v, [](float a, float b) { return fmaxf(a, b); });
 }
 
-// A read by rows takes 16 lanes at a time, those of one group with rows 0-3 and 12-15 and those of the next with rows 4-11: the
-// values for the former are pairs (x, x ^ 1), so that the latter's, one chunk on, are the other pairs. A read by columns takes 8
-// rows: the values of each half are of different pairs.
-template <int DP>
-__device__ __forceinline__ int swz(int r) {
-  const int u = DP == 64 ? r >> 1 & 7 : r & 15, half = DP == 64 ? 4 : 8, high = u / half;
-  return ((u + high * half / 2) & (half - 1)) << 1 | high;
-}
-
 // A lane's places in a staged tile (element offsets): for the read by rows of 16-row tile t and step ks, add t 16 DP to row[ks];
 // for the read by columns of tile t and columns 16 dt.., add t 16 DP to col[dt].
 template <int DP>
@@ -100,9 +91,6 @@ __device__ __forceinline__ s16x8 by_columns(uint16_t *tile, int t, int place) {
   const s16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)(tile + (t + 1) * 16 * DP + place));
   return s16x8{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
 }
-
-// Sixteen zero bytes, for the lanes of a staged tile that have none of their own.
-__device__ const u32x4 kZeros = {0u, 0u, 0u, 0u};
 
 // How 256 threads stage a tile of kTile rows: kU loads each, load u of wave w to places 64 (4 u + w) + lane, of which place i is
 // place i % kC of row i / kC and takes that row's chunk (i % kC) ^ swz(row).

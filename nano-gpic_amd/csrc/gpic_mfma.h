@@ -65,6 +65,24 @@ __device__ __forceinline__ uint32_t lds_at(const void *p) {
 __device__ __forceinline__ void to_lds(const void *src, uint32_t lds) {
   asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" : : "v"(src), "s"(lds) : "memory", "m0");
 }
+// (with loads of later tiles behind them that may stay in flight)
+template <int kInFlight>
+__device__ __forceinline__ void staged_but() {
+  asm volatile("s_waitcnt vmcnt(%0)" : : "n"(kInFlight) : "memory");
+}
 __device__ __forceinline__ void staged() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+
+// Rows of a staged tile: 16-byte chunk c of row r lies in place c ^ swz(r).
+// A read by rows takes 16 lanes at a time, those of one group with rows 0-3 and 12-15 and those of the next with rows 4-11: the
+// values for the former are pairs (x, x ^ 1), so that the latter's, one chunk on, are the other pairs. A read by columns takes 8
+// rows: the values of each half are of different pairs.
+template <int DP>
+__device__ __forceinline__ int swz(int r) {
+  const int u = DP == 64 ? r >> 1 & 7 : r & 15, half = DP == 64 ? 4 : 8, high = u / half;
+  return ((u + high * half / 2) & (half - 1)) << 1 | high;
+}
+
+// Sixteen zero bytes, for the lanes of a staged tile that have none of their own.
+__device__ const u32x4 kZeros = {0u, 0u, 0u, 0u};
 
 }  // namespace gpic

@@ -35,7 +35,7 @@ struct LoraArgs {
   int M, per, N, K, R, n, wide_ids;   // wide_ids: 64-bit ids
   int splits, groups, blocks, cols;   // parts of K; workgroups that share a tile's passes; column blocks, of cols columns each
 };
-constexpr int kMaxSplits = 4;
+constexpr int kMaxSplits = 4, kMaxPacked = 8;   // parts that the second product adds, that are packed
 
 // The adapter of row m, or -1.
 __device__ __forceinline__ int adapter_of(const LoraArgs &p, int m) {
@@ -74,39 +74,55 @@ __device__ __forceinline__ void row_factor(float most, float &down, float &up) {
   }
 }
 
-// [16384 x 4096] to rank 32 44 us (3.3 TB/s of reads), [2648 x 1024] to rank 64 12, one row 2.6.
-// t of 16 RT rows (NT tiles of 16 of the rank): the workgroups' parts of K (kParts), and in them the waves', added in their
-// order.
+// A row's t in halves: 16 threads a row, 8 of the rank each (zeros past R); kept where `on`.
+template <bool F16, int NT>
+__device__ __forceinline__ void leave_halves(const LoraArgs &p, int row, bool on, float (&t)[8]) {
+  const int c = threadIdx.x & 15;
+  float most = 0.0f, down = 1.0f, up = 1.0f;
+  if (F16) {
+#pragma unroll
+    for (int e = 0; e < 8; e++) most = fmaxf(most, fabsf(t[e]));
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor(most, o, 64));
+    row_factor(most, down, up);
+#pragma unroll
+    for (int e = 0; e < 8; e++) t[e] *= down;
+  }
+  if (!on || c >= 2 * NT) return;
+  uint16_t *o = static_cast<uint16_t *>(p.t) + (int64_t)row * 32 * NT + 8 * c;
+  *reinterpret_cast<s16x8 *>(o) = half_of<F16>(t, false);
+  *reinterpret_cast<s16x8 *>(o + 16 * NT) = half_of<F16>(t, true);
+  if (F16 && c == 0) p.up[row] = up;
+}
+
+// One row 2.6 us, [1500 x 1024] to rank 32 5.6.
+// t of 16 rows (NT tiles of 16 of the rank): the workgroups' parts of K (kParts), and in them the waves', added in their order.
 template <int NT>
 constexpr int kShrinkWaves = NT == 8 ? 4 : 8;
 
-template <bool F16, int RT, int NT, bool kParts>
+template <bool F16, int NT, bool kParts>
 __global__ __launch_bounds__(64 * kShrinkWaves<NT>) void lora_shrink_kernel(LoraArgs p) {
   constexpr int W = kShrinkWaves<NT>;
-  __shared__ float red[W][16 * RT][16 * NT + 1];
+  __shared__ float red[W][16][16 * NT + 1];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l15 = lane & 15, g = lane >> 4;
-  const int row0 = blockIdx.x * 16 * RT;
+  const int row0 = blockIdx.x * 16;
   const int split = blockIdx.y, group = blockIdx.z;
   const int steps = (p.K + 63) / 64, per = (steps + W * p.splits - 1) / (W * p.splits);
   const int first = (split * W + wave) * per, end = min(steps, first + per), whole = min(end, p.K / 64);
   // 64 of K a step, 16 from 16 g for group g: whole lines of x and A at a time. Loads have no conditions, so that they stay in
   // flight behind the products of the step before: rows past the last and of other passes, and the rank's past R, are read from
   // rows that are there, and what they give is not kept. K's last step, where it is none of 64, loads zeros past K.
-  const uint16_t *xr[RT];
-#pragma unroll
-  for (int i = 0; i < RT; i++) xr[i] = p.x + (int64_t)min(row0 + 16 * i + l15, p.M - 1) * p.ldx;
+  const uint16_t *xr = p.x + (int64_t)min(row0 + l15, p.M - 1) * p.ldx;
   struct Step {
-    s16x8 a[RT][2], b[NT][2];
+    s16x8 a[2], b[NT][2];
   };
   auto fetch_x = [&](int s, Step &f) {
 #pragma unroll
-    for (int h = 0; h < 2; h++)
-#pragma unroll
-      for (int i = 0; i < RT; i++) f.a[i][h] = chunk16(xr[i], 8 * s + 2 * g + h);
+    for (int h = 0; h < 2; h++) f.a[h] = chunk16(xr, 8 * s + 2 * g + h);
   };
   Step f0, f1;
   if (first < whole) fetch_x(first, f0);   // (before the ids are known, which A waits for)
-  const int id = lane < 16 * RT ? adapter_of(p, row0 + lane) : -1;
+  const int id = lane < 16 ? adapter_of(p, row0 + lane) : -1;
   uint64_t todo = __ballot(id >= 0);
   bool again = false;
   for (int pass = 0; todo; pass++) {
@@ -114,11 +130,9 @@ __global__ __launch_bounds__(64 * kShrinkWaves<NT>) void lora_shrink_kernel(Lora
     const uint64_t mine = __ballot(id == cur);
     todo &= ~mine;
     if (pass % p.groups != group) continue;
-    f32x4_t acc[RT][NT];
+    f32x4_t acc[NT];
 #pragma unroll
-    for (int i = 0; i < RT; i++)
-#pragma unroll
-      for (int j = 0; j < NT; j++) acc[i][j] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+    for (int j = 0; j < NT; j++) acc[j] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
     const uint16_t *Ar[NT];
 #pragma unroll
     for (int j = 0; j < NT; j++) Ar[j] = p.A + ((int64_t)cur * p.R + min(16 * j + l15, p.R - 1)) * p.K;
@@ -136,9 +150,7 @@ __global__ __launch_bounds__(64 * kShrinkWaves<NT>) void lora_shrink_kernel(Lora
 #pragma unroll
       for (int h = 0; h < 2; h++)
 #pragma unroll
-        for (int i = 0; i < RT; i++)
-#pragma unroll
-          for (int j = 0; j < NT; j++) acc[i][j] = mfma16<F16>(f.a[i][h], f.b[j][h], acc[i][j]);
+        for (int j = 0; j < NT; j++) acc[j] = mfma16<F16>(f.a[h], f.b[j][h], acc[j]);
     };
     int s = first;
     if (s < whole) {
@@ -165,19 +177,16 @@ __global__ __launch_bounds__(64 * kShrinkWaves<NT>) void lora_shrink_kernel(Lora
 #pragma unroll
       for (int h = 0; h < 2; h++) {
         const int c = 8 * s + 2 * g + h;
-#pragma unroll
-        for (int i = 0; i < RT; i++) f0.a[i][h] = chunk16(xr[i], c, 8 * c < p.K);
+        f0.a[h] = chunk16(xr, c, 8 * c < p.K);
 #pragma unroll
         for (int j = 0; j < NT; j++) f0.b[j][h] = chunk16(Ar[j], c, 8 * c < p.K);
       }
       multiply(f0);
     }
 #pragma unroll
-    for (int i = 0; i < RT; i++)
+    for (int j = 0; j < NT; j++)
 #pragma unroll
-      for (int j = 0; j < NT; j++)
-#pragma unroll
-        for (int v = 0; v < 4; v++) red[wave][16 * i + 4 * g + v][16 * j + l15] = acc[i][j][v];
+      for (int v = 0; v < 4; v++) red[wave][4 * g + v][16 * j + l15] = acc[j][v];
     __syncthreads();
     auto sum = [&](int m, int r) {
       float x = red[0][m][r];
@@ -186,45 +195,129 @@ __global__ __launch_bounds__(64 * kShrinkWaves<NT>) void lora_shrink_kernel(Lora
       return x;
     };
     if constexpr (kParts) {
-      for (int e = threadIdx.x; e < 16 * RT * p.R; e += 64 * W) {
+      for (int e = threadIdx.x; e < 16 * p.R; e += 64 * W) {
         const int m = e / p.R, r = e - m * p.R;
         if (mine >> m & 1) static_cast<float *>(p.t)[((int64_t)split * p.M + row0 + m) * p.R + r] = sum(m, r);
       }
     } else {
-      const int c = threadIdx.x & 15;   // (16 threads a row, 8 of the rank each)
-      for (int m = threadIdx.x >> 4; m < 16 * RT; m += 4 * W) {
-        float t[8], most = 0.0f, down = 1.0f, up = 1.0f;
+      const int c = threadIdx.x & 15;
+      for (int m = threadIdx.x >> 4; m < 16; m += 4 * W) {
+        float t[8];
 #pragma unroll
         for (int e = 0; e < 8; e++) t[e] = 8 * c < p.R ? sum(m, 8 * c + e) : 0.0f;
-        if (F16) {
-#pragma unroll
-          for (int e = 0; e < 8; e++) most = fmaxf(most, fabsf(t[e]));
-#pragma unroll
-          for (int o = 8; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor(most, o, 64));
-          row_factor(most, down, up);
-#pragma unroll
-          for (int e = 0; e < 8; e++) t[e] *= down;
-        }
-        if (!(mine >> m & 1)) continue;
-        uint16_t *o = static_cast<uint16_t *>(p.t) + (int64_t)(row0 + m) * 32 * NT + 8 * c;
-        if (c < 2 * NT) {
-          *reinterpret_cast<s16x8 *>(o) = half_of<F16>(t, false);
-          *reinterpret_cast<s16x8 *>(o + 16 * NT) = half_of<F16>(t, true);
-        }
-        if (F16 && c == 0) p.up[row0 + m] = up;
+        leave_halves<F16, NT>(p, row0 + m, mine >> m & 1, t);
       }
     }
     __syncthreads();
   }
 }
 
-// The parts of t added in their order and left in halves: 16 threads a row, 8 of the rank each. (Rows without an adapter have no
-// parts: what is made of them is not used.)
+// [16384 x 4096] to rank 32 41 us (beside the writing out of the second product's results), [2648 x 1024] to rank 64 9.9.
+// The same for many rows, 64 a workgroup: x and A come past the registers into LDS, whole lines at a time and stages ahead, each
+// wave multiplies 16 rows. (Rows across the lanes, as above, take the memory pipeline four times as long.)
+template <int NT>
+constexpr int kStages = NT <= 4 ? 5 : 4;
+
+template <bool F16, int NT, bool kParts>
+__global__ __launch_bounds__(256) void lora_shrink_staged_kernel(LoraArgs p) {
+  constexpr int KC = 64, C = KC / 8;   // columns of a stage, and 16-byte chunks
+  constexpr int S = kStages<NT>, AR = NT == 1 ? 32 : 16 * NT, kX = C / 4, kA = AR * C / 256, kLoads = kX + kA;   // loads a lane
+  __shared__ __attribute__((aligned(16))) uint16_t xt[S][64 * KC], at[S][AR * KC];
+  __shared__ float red[4][16][16 * NT + 1];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l15 = lane & 15, g = lane >> 4;
+  const int row0 = blockIdx.x * 64, split = blockIdx.y, group = blockIdx.z;
+  const int steps = (p.K + KC - 1) / KC, per = (steps + p.splits - 1) / p.splits, first = split * per, end = min(steps, first + per);
+  const int whole = min(end, p.K / KC);
+  // load u of a wave: 1 KiB of a tile, a lane one chunk
+  auto row_of = [&](int u) { return (64 * (4 * u + wave) + lane) / C; };
+  auto chunk_of = [&](int u) { return lane % C ^ swz<KC>(row_of(u)); };
+  const uint16_t *xr[kX], *Ar[kA], *xs[kX];
+#pragma unroll
+  for (int u = 0; u < kX; u++)
+    xs[u] = p.x + (int64_t)min(row0 + row_of(u), p.M - 1) * p.ldx + KC * first + 8 * chunk_of(u);
+  // The next step's loads into a buffer, and on; in the last ones (past K or the last step) zeros, so that as many loads are
+  // always in flight.
+  auto request = [&](int s, int buf, auto whole) {
+    auto load = [&](uint16_t *tile, int u, const uint16_t *&from) {
+      const void *src = from;
+      if constexpr (!decltype(whole)::value) src = s < end && KC * s + 8 * chunk_of(u) < p.K ? src : (const void *)&kZeros;
+      to_lds(src, lds_at(tile) + 1024 * (4 * u + wave));
+      from += KC;
+    };
+#pragma unroll
+    for (int u = 0; u < kX; u++) load(xt[buf], u, xr[u]);
+#pragma unroll
+    for (int u = 0; u < kA; u++) load(at[buf], u, Ar[u]);
+  };
+  int place[KC / 32];
+#pragma unroll
+  for (int k = 0; k < KC / 32; k++) place[k] = l15 * KC + ((4 * k + g) ^ swz<KC>(l15)) * 8;
+  const int id = adapter_of(p, row0 + lane);
+  uint64_t todo = __ballot(id >= 0);
+  for (int pass = 0; todo; pass++) {
+    const int cur = __builtin_amdgcn_readlane(id, __builtin_ctzll(todo));
+    const uint64_t mine = __ballot(id == cur);
+    todo &= ~mine;
+    if (pass % p.groups != group) continue;
+#pragma unroll
+    for (int u = 0; u < kX; u++) xr[u] = xs[u];
+#pragma unroll
+    for (int u = 0; u < kA; u++) Ar[u] = p.A + ((int64_t)cur * p.R + min(row_of(u), p.R - 1)) * p.K + KC * first + 8 * chunk_of(u);
+    f32x4_t acc[NT];
+#pragma unroll
+    for (int j = 0; j < NT; j++) acc[j] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int i = 0; i < S - 1; i++) request(first + i, i, std::false_type());
+    int s = first, buf = 0;
+    auto step = [&](auto whole) {
+      staged_but<(S - 2) * kLoads>();
+      __syncthreads();   // (stage s is there, and stage s - 1 read)
+      request(s + S - 1, buf == 0 ? S - 1 : buf - 1, whole);
+#pragma unroll
+      for (int k = 0; k < KC / 32; k++) {
+        const s16x8 a = *reinterpret_cast<const s16x8 *>(xt[buf] + wave * 16 * KC + place[k]);
+#pragma unroll
+        for (int j = 0; j < NT; j++)
+          acc[j] = mfma16<F16>(a, *reinterpret_cast<const s16x8 *>(at[buf] + j * 16 * KC + place[k]), acc[j]);
+      }
+      buf = buf + 1 == S ? 0 : buf + 1;
+    };
+    for (; s + S - 1 < whole; s++) step(std::true_type());
+    for (; s < end; s++) step(std::false_type());
+    staged();
+#pragma unroll
+    for (int j = 0; j < NT; j++)
+#pragma unroll
+      for (int v = 0; v < 4; v++) red[wave][4 * g + v][16 * j + l15] = acc[j][v];
+    __syncthreads();
+    const int c = threadIdx.x & 15;
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      const int m = 16 * i + (threadIdx.x >> 4);
+      const bool on = mine >> m & 1;
+      float t[8];
+#pragma unroll
+      for (int e = 0; e < 8; e++) t[e] = 8 * c < p.R ? red[i][threadIdx.x >> 4][8 * c + e] : 0.0f;
+      if constexpr (kParts) {
+        float *o = static_cast<float *>(p.t) + ((int64_t)split * p.M + row0 + m) * p.R + 8 * c;
+        if (on && 8 * c < p.R) {
+          *reinterpret_cast<f32x4_t *>(o) = f32x4_t{t[0], t[1], t[2], t[3]};
+          *reinterpret_cast<f32x4_t *>(o + 4) = f32x4_t{t[4], t[5], t[6], t[7]};
+        }
+      } else {
+        leave_halves<F16, NT>(p, row0 + m, on, t);
+      }
+    }
+    __syncthreads();
+  }
+}
+
+// The parts of t added in their order and left in halves. (Rows without an adapter have no parts: what is made of them is not used.)
 template <bool F16, int NT>
 __global__ __launch_bounds__(256) void lora_pack_kernel(LoraArgs p) {
   const int row = blockIdx.x * 16 + (threadIdx.x >> 4), c = threadIdx.x & 15;
   const bool on = row < p.M && 8 * c < p.R;
-  float t[8], most = 0.0f, down = 1.0f, up = 1.0f;
+  float t[8];
 #pragma unroll
   for (int e = 0; e < 8; e++) t[e] = 0.0f;
   for (int s = 0; on && s < p.splits; s++) {
@@ -232,20 +325,7 @@ __global__ __launch_bounds__(256) void lora_pack_kernel(LoraArgs p) {
     const float4 a = src[0], b = src[1];
     t[0] += a.x, t[1] += a.y, t[2] += a.z, t[3] += a.w, t[4] += b.x, t[5] += b.y, t[6] += b.z, t[7] += b.w;
   }
-  if (F16) {
-#pragma unroll
-    for (int e = 0; e < 8; e++) most = fmaxf(most, fabsf(t[e]));
-#pragma unroll
-    for (int o = 8; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor(most, o, 64));
-    row_factor(most, down, up);
-#pragma unroll
-    for (int e = 0; e < 8; e++) t[e] *= down;
-  }
-  if (row >= p.M || c >= 2 * NT) return;
-  uint16_t *o = static_cast<uint16_t *>(p.t) + (int64_t)row * 32 * NT + 8 * c;
-  *reinterpret_cast<s16x8 *>(o) = half_of<F16>(t, false);
-  *reinterpret_cast<s16x8 *>(o + 16 * NT) = half_of<F16>(t, true);
-  if (F16 && c == 0) p.up[row] = up;
+  leave_halves<F16, NT>(p, row, row < p.M, t);
 }
 
 // 2648 rows of rank 64 to 4096 columns 19 us, 64 rows of rank 16 on 32 adapters 6.5, one row 3.1.
@@ -508,27 +588,27 @@ __global__ __launch_bounds__(256) void lora_expand_runs_kernel(LoraArgs p) {
 // ------------------------------------------------------------------------------------------- host side
 
 struct LoraPlan {
-  int nt, shrink_rt, rt, splits, groups, cols;
-  bool few, runs;   // few rows: their parts go into the second product; runs: lora_expand_runs_kernel
+  int nt, rt, splits, groups, cols;
+  bool few, staged, runs;   // few rows: their parts go into the second product; staged, runs: the kernels of those names
 };
 // us, first + second product. Up to 256 rows the parts, few rows' columns and up to 16 workgroups for a tile's passes: 200 rows of
-// rank 64, 2048 to 2048, 5.0 + 7.0, as many rows 11.6 + 4.2; 100 of rank 16, 1024 to 4096, 4.1 + 3.5 against 6.8 + 4.8; 500 of rank 16
-// the other way, 4.3 + 7.4 against 4.9 + 4.4. Two workgroups for a tile's passes while one would not fill the device: 500 rows of
-// rank 64, 4096 to 4096, 20.7 + 7.9 against 38.8 + 8.8, 4000 rows 24 + 22 against 25 + 19. Two row tiles share A's reads where x
-// is large, or the rank: 4000 rows x 4096 17.3 against 23.9, 3000 x 2048 to rank 128 22.3 against 34.8, 1500 x 1024 9.0 against
-// 7.8. Long K is split and packed while there are few tiles: 500 rows of rank 64, 4096 to 4096, 7.6 + 4.3 + 7.8 against
-// 20.7 + 7.9; 2256 of rank 32, 7056 to 224, 20 + 4 + 7 against 29 + 7; 2000 of rank 16, 8192 to 1024, 17 + 4 + 7 against 24 + 7;
-// 4000 rows x 4096 lose by it (20 + 4 against 17).
+// rank 64, 2048 to 2048, 5.0 + 7.0, as many rows 11.6 + 4.2; 100 of rank 16, 1024 to 4096, 4.1 + 3.5 against 6.8 + 4.8; 500 of
+// rank 16 the other way, 4.3 + 7.4 against 4.9 + 4.4. Two workgroups for a tile's passes while one would not fill the device: 500
+// rows of rank 64, 4096 to 4096, 20.7 + 7.9 against 38.8 + 8.8, 4000 rows 24 + 22 against 25 + 19.
+// First product, tiles from the registers / staged: 2648 rows x 1024 to rank 64 12.3 / 9.9, 5000 x 2048 to 32 18 / 16, 16384 x 256
+// to 128 12.9 / 8.6, 16384 x 4096 to 32 45 / 41.5; but 1500 x 1024 to 32 5.6 / 6.7, 4096 x 512 to 16 4.2 / 5.3. Long K in parts
+// while there are few tiles, and 4.3 to pack them: 4096 rows x 4096 to 32 18.4 / 9.4, 1000 x 8192 17.4 / 6.8, 4096 x 2048 to 128
+// 20.5 / 12.7; 2500 x 2048 to 32 loses by it.
 static LoraPlan lora_plan(int64_t M, int64_t K, int64_t N, int64_t R, int64_t n) {
   LoraPlan a;
   a.nt = R <= 16 ? 1 : R <= 32 ? 2 : R <= 64 ? 4 : 8;
   const bool few = a.few = M <= 256;
-  a.shrink_rt = !few && (M * K >= (int64_t(1) << 23) || (a.nt == 8 && M >= 1024)) ? 2 : 1;
   a.rt = M < 1024 ? 1 : a.nt == 8 ? 2 : 4;
   a.groups = few ? (int)std::min<int64_t>(std::min<int64_t>(n + 1, M), 16) : M < 4096 ? 2 : 1;
-  const int64_t blocks = (M + 16 * a.shrink_rt - 1) / (16 * a.shrink_rt) * a.groups;
-  a.splits = (int)std::max<int64_t>(std::min<int64_t>(few ? K / 512 : K >= 4096 ? std::min(K / 1024, 448 / blocks) : 1, kMaxSplits), 1);
-  if (a.splits > 1) a.shrink_rt = 1;
+  a.staged = !few && (a.nt >= 4 || K >= 4096 || M * K >= (int64_t(1) << 23));
+  int64_t splits = few ? std::min<int64_t>(K / 512, kMaxSplits) : 1;
+  if (a.staged && K >= (a.nt == 8 ? 2048 : 4096)) splits = std::min<int64_t>({K / 512, 256 / ((M + 63) / 64), kMaxPacked});
+  a.splits = (int)std::max<int64_t>(splits, 1);
   const int64_t tiles = (M + 16 * a.rt - 1) / (16 * a.rt);
   a.runs = a.rt == 4 && a.nt <= 2;
   a.cols = a.runs ? 512 : few ? 256 : 128;   // (a step of the workgroup's waves, few rows two)
@@ -583,7 +663,7 @@ int gpic_fp8_lora_rows(const uint16_t *y, int64_t ldy, const uint16_t *x, int64_
   if (ws_bytes < gpic_fp8_lora_rows_workspace_bytes(M, N, K, R, n) || !ws) return GPIC_EWORKSPACE;
   const LoraPlan a = lora_plan(M, K, N, R, n);
   const int64_t tiles = (M + 16 * a.rt - 1) / (16 * a.rt), blocks = (N + a.cols - 1) / a.cols;
-  const int64_t stiles = (M + 16 * a.shrink_rt - 1) / (16 * a.shrink_rt);
+  const int64_t stiles = a.staged ? (M + 63) / 64 : (M + 15) / 16;
   // (a launch's threads are counted in 32 bits)
   if (tiles * blocks * a.groups >= (int64_t(1) << 24) || stiles * a.splits * a.groups >= (int64_t(1) << 24))
     return GPIC_ESHAPE;
@@ -598,15 +678,17 @@ int gpic_fp8_lora_rows(const uint16_t *y, int64_t ldy, const uint16_t *x, int64_
     constexpr bool F = decltype(f16)::value;
     with_rank(a.nt, [&](auto nt) {
       constexpr int T = decltype(nt)::value;
-      if (a.splits > 1) {
+      if (a.staged && a.splits > 1) {
         LoraArgs q = p;
-        if (!a.few) q.t = w + space.parts;
-        lora_shrink_kernel<F, 1, T, true><<<shrink, 64 * kShrinkWaves<T>, 0, st>>>(q);
-        if (!a.few) lora_pack_kernel<F, T><<<(unsigned)((M + 15) / 16), 256, 0, st>>>(p);
-      } else if (a.shrink_rt == 2) {
-        lora_shrink_kernel<F, 2, T, false><<<shrink, 64 * kShrinkWaves<T>, 0, st>>>(p);
+        q.t = w + space.parts;
+        lora_shrink_staged_kernel<F, T, true><<<shrink, 256, 0, st>>>(q);
+        lora_pack_kernel<F, T><<<(unsigned)((M + 15) / 16), 256, 0, st>>>(p);
+      } else if (a.staged) {
+        lora_shrink_staged_kernel<F, T, false><<<shrink, 256, 0, st>>>(p);
+      } else if (a.splits > 1) {
+        lora_shrink_kernel<F, T, true><<<shrink, 64 * kShrinkWaves<T>, 0, st>>>(p);
       } else {
-        lora_shrink_kernel<F, 1, T, false><<<shrink, 64 * kShrinkWaves<T>, 0, st>>>(p);
+        lora_shrink_kernel<F, T, false><<<shrink, 64 * kShrinkWaves<T>, 0, st>>>(p);
       }
       if (a.few && a.splits > 1) lora_expand_kernel<F, 1, T, true><<<expand, 256, 0, st>>>(p);
       else if (a.rt == 1) lora_expand_kernel<F, 1, T, false><<<expand, 256, 0, st>>>(p);

@@ -59,7 +59,8 @@ def test_against_64_bits(dev, dt, R, M, K, N, n):
 
 
 @pytest.mark.parametrize("dt", [BF, FP])
-@pytest.mark.parametrize("M,K,N,n,R", [(300, 4104, 264, 3, 24), (700, 8192, 136, 40, 64), (1500, 4160, 72, 2, 128), (260, 20000, 8, 1, 8)])
+@pytest.mark.parametrize("M,K,N,n,R", [(300, 4104, 264, 3, 24), (700, 8192, 136, 40, 64), (1500, 4160, 72, 2, 128), (260, 20000, 8, 1, 8),
+                                         (8200, 4104, 72, 3, 40), (5000, 2056, 40, 5, 72), (16390, 520, 24, 2, 16)])
 def test_long_reductions_in_parts(dev, dt, M, K, N, n, R):
     y, x, A, B, ids, s = make(M, K, N, n, R, dt, 9)
     check(G.lora_rows(y, x, A, B, ids, s), y, x, A, B, ids, s)
