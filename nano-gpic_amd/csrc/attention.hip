@@ -315,8 +315,8 @@ __global__ __launch_bounds__(256, 2) void attn_fwd_kernel(AttnArgs p) {
 }
 
 // Requests of unlike lengths: a key head's tiles of 32 keys, entry after entry, dealt out in equal runs to `budget` workgroups
-// (of `least` tiles at least; an entry without keys counts as a tile). A run that goes past an entry's end goes on in the next entry, and
-// an entry's splits are the runs that meet it. Lane b of a wave holds where entry b begins and ends.
+// (of `least` tiles at least; an entry without keys counts as a tile). A run that goes past an entry's end goes on in the next
+// entry, and an entry's splits are the runs that meet it. Lane b of a wave holds where entry b begins and ends.
 struct Runs {
   uint32_t run, begin, end, all;
   __device__ __forceinline__ explicit Runs(const AttnArgs &p) {
