@@ -51,6 +51,21 @@ __device__ __forceinline__ s16x8 operand(f32x4_t a, f32x4_t b) {
   return __builtin_bit_cast(s16x8, u32x4{pack16<F16>(a[0], a[1]), pack16<F16>(a[2], a[3]), pack16<F16>(b[0], b[1]),
                                          pack16<F16>(b[2], b[3])});
 }
+// A result row, f times x, to 16 bits in memory (zeros unless `valid`), where `on`: the groups of 16 lanes hold 4 columns of a tile
+// each; two tiles' exchanged between neighbouring groups are 8 beside each other, 16 bytes a store.
+template <bool F16, int DT>
+__device__ __forceinline__ void put_row(uint16_t *row, int D, const f32x4_t (&x)[DT], float f, bool on, bool valid = true) {
+  const int g = (threadIdx.x & 63) >> 4;
+#pragma unroll
+  for (int d = 0; d < DT; d += 2) {
+    const auto lo = __builtin_amdgcn_permlane16_swap(pack16<F16>(x[d][0] * f, x[d][1] * f),
+                                                     pack16<F16>(x[d + 1][0] * f, x[d + 1][1] * f), false, false);
+    const auto hi = __builtin_amdgcn_permlane16_swap(pack16<F16>(x[d][2] * f, x[d][3] * f),
+                                                     pack16<F16>(x[d + 1][2] * f, x[d + 1][3] * f), false, false);
+    const int col = 16 * (d + (g & 1)) + 8 * (g >> 1);
+    if (on && col < D) *reinterpret_cast<u32x4 *>(row + col) = valid ? u32x4{lo[0], hi[0], lo[1], hi[1]} : u32x4{0u, 0u, 0u, 0u};
+  }
+}
 // Sum, or maximum, of a value over the four groups of 16 lanes, in every lane: two exchanges of half the lanes, in registers.
 template <class F>
 __device__ __forceinline__ float over_groups(float v, F f) {
@@ -290,9 +305,10 @@ __global__ __launch_bounds__(256, 2) void attn_fwd_kernel(AttnArgs p) {
   for (int q = 0; q < QT; q++) {
     const int r = row0 + 16 * q + l15;
     const float l = groups_sum((l4[q][0] + l4[q][1]) + (l4[q][2] + l4[q][3]));
-    if (r >= p.rows) continue;
+    const bool on = r < p.rows;
     if (p.splits > 1) {
       // (partial o, its maximum and sum: joined by attn_join_kernel)
+      if (!on) continue;
       const int64_t at_row = ((int64_t)split * p.B * p.Hk + pair) * p.rows + r;
       float *o = p.part + at_row * (DP + 2);
 #pragma unroll
@@ -303,13 +319,8 @@ __global__ __launch_bounds__(256, 2) void attn_fwd_kernel(AttnArgs p) {
       continue;
     }
     const float inv = l == 0.0f ? 0.0f : __fdiv_rn(1.0f, l);
-    uint16_t *o = p.out + row_at(p, p.os, b, hk, r);
-#pragma unroll
-    for (int d = 0; d < DT; d++)
-      if (16 * d + 4 * g < p.D)
-        *reinterpret_cast<u32x2 *>(o + 16 * d + 4 * g) = u32x2{pack16<F16>(O[q][d][0] * inv, O[q][d][1] * inv),
-                                                               pack16<F16>(O[q][d][2] * inv, O[q][d][3] * inv)};
-    if (p.lse && g == 0)
+    put_row<F16, DT>(p.out + row_at(p, p.os, b, hk, min(r, p.rows - 1)), p.D, O[q], inv, on);
+    if (p.lse && g == 0 && on)
       p.lse[(int64_t)pair * p.rows + r] = l == 0.0f ? kInf : sm[q].base() + __builtin_amdgcn_logf(l);
   }
 }
@@ -723,9 +734,9 @@ __global__ __launch_bounds__(256, 2) void attn_dq_kernel(AttnArgs p) {
 #pragma unroll
   for (int q = 0; q < QT; q++) {
     const int r = row0 + 16 * q + l15;
-    if (r >= p.rows) continue;
     const float f = F16 ? p.scale / up[q] : p.scale;
     if (p.splits > 1) {   // (added by attn_dq_join_kernel)
+      if (r >= p.rows) continue;
       float *part = p.part + (((int64_t)split * p.B * p.Hk + pair) * p.rows + r) * p.D;
 #pragma unroll
       for (int d = 0; d < DT; d++)
@@ -734,12 +745,7 @@ __global__ __launch_bounds__(256, 2) void attn_dq_kernel(AttnArgs p) {
               f32x4_t{dQ[q][d][0] * f, dQ[q][d][1] * f, dQ[q][d][2] * f, dQ[q][d][3] * f};
       continue;
     }
-    uint16_t *o = p.dq + row_at(p, p.dqs, b, hk, r);
-#pragma unroll
-    for (int d = 0; d < DT; d++)
-      if (16 * d + 4 * g < p.D)
-        *reinterpret_cast<u32x2 *>(o + 16 * d + 4 * g) = u32x2{pack16<F16>(dQ[q][d][0] * f, dQ[q][d][1] * f),
-                                                               pack16<F16>(dQ[q][d][2] * f, dQ[q][d][3] * f)};
+    put_row<F16, DT>(p.dq + row_at(p, p.dqs, b, hk, min(r, p.rows - 1)), p.D, dQ[q], f, r < p.rows);
   }
 }
 
@@ -872,8 +878,8 @@ __global__ __launch_bounds__(256, 2) void attn_dkv_kernel(AttnArgs p) {
 #pragma unroll
   for (int x = 0; x < KT; x++) {
     const int j = key0 + 16 * x + l15;
-    if (j >= p.L) continue;
     if (p.splits > 1) {
+      if (j >= p.L) continue;
       float *o = p.part + (((int64_t)split * p.B * p.Hk + pair) * p.L + j) * 2 * p.D;
 #pragma unroll
       for (int d = 0; d < DT; d++)
@@ -886,18 +892,9 @@ __global__ __launch_bounds__(256, 2) void attn_dkv_kernel(AttnArgs p) {
         }
       continue;
     }
-    uint16_t *ok = p.dk + b * p.dks[0] + hk * p.dks[1] + j * p.dks[2], *ov = p.dv + b * p.dvs[0] + hk * p.dvs[1] + j * p.dvs[2];
-#pragma unroll
-    for (int d = 0; d < DT; d++)
-      if (16 * d + 4 * g < p.D) {
-        u32x2 a{0u, 0u}, c{0u, 0u};
-        if (on[x]) {
-          a = u32x2{pack16<F16>(dK[x][d][0] * fk, dK[x][d][1] * fk), pack16<F16>(dK[x][d][2] * fk, dK[x][d][3] * fk)};
-          c = u32x2{pack16<F16>(dV[x][d][0] * fv, dV[x][d][1] * fv), pack16<F16>(dV[x][d][2] * fv, dV[x][d][3] * fv)};
-        }
-        *reinterpret_cast<u32x2 *>(ok + 16 * d + 4 * g) = a;
-        *reinterpret_cast<u32x2 *>(ov + 16 * d + 4 * g) = c;
-      }
+    const int64_t jc = min(j, p.L - 1);
+    put_row<F16, DT>(p.dk + b * p.dks[0] + hk * p.dks[1] + jc * p.dks[2], p.D, dK[x], fk, j < p.L, on[x]);
+    put_row<F16, DT>(p.dv + b * p.dvs[0] + hk * p.dvs[1] + jc * p.dvs[2], p.D, dV[x], fv, j < p.L, on[x]);
   }
 }
 
