@@ -52,7 +52,8 @@ __device__ __forceinline__ s16x8 operand(f32x4_t a, f32x4_t b) {
                                          pack16<F16>(b[2], b[3])});
 }
 // A result row, f times x, to 16 bits in memory (zeros unless `valid`), where `on`: the groups of 16 lanes hold 4 columns of a tile
-// each; two tiles' exchanged between neighbouring groups are 8 beside each other, 16 bytes a store.
+// each; two tiles' exchanged between neighbouring groups are 8 beside each other, 16 bytes a store (8: the kernels take 4 to 12%
+// longer, dk and dv most).
 template <bool F16, int DT>
 __device__ __forceinline__ void put_row(uint16_t *row, int D, const f32x4_t (&x)[DT], float f, bool on, bool valid = true) {
   const int g = (threadIdx.x & 63) >> 4;
@@ -189,7 +190,7 @@ struct Softmax {
 // ------------------------------------------------------------------------------------------- forward
 
 // Between memory, VALU and MFMA: 2 x 256 rows over up to 77 keys 5.0 us (latency); 128 x 16 heads of 256 over up to 320, dimension
-// 64, 73 us (VALU two thirds busy, 3 TB/s); 4 x 16 of 1024 over 2048, dimension 128, 81 us, 0.85 PFLOP/s.
+// 64, 69 us (VALU two thirds busy, 3 TB/s); 4 x 16 of 1024 over 2048, dimension 128, 81 us, 0.85 PFLOP/s.
 // A workgroup's four waves take 16 QT rows each and walk the pair's keys (or its split's part of them) by tiles of 64, k and v
 // staged through two buffers: the next tile's loads are under way during the current one's products.
 template <bool F16, int DP, int QT>
@@ -349,9 +350,9 @@ struct Runs {
 };
 
 // Up to 16 rows a pair (a token's heads): memory bounds it, k and v once: 8 x 8 pairs over 8191 keys of dimension 128 54 us, 4.95
-// TB/s; 256 pairs over 4096 of 64 51 us, 5.2 TB/s. Each wave walks keys of its own, 32 a step: k goes from
-// memory to the lanes as they multiply it, v through the wave's own staged tile, both requested a step ahead; no barrier until the
-// waves' results are joined.
+// TB/s, over up to as many, dealt out in runs, 28 us, 5.1 TB/s; 256 pairs over 4096 of 64 51 us, 5.2 TB/s. Each wave walks keys of
+// its own, 32 a step: k goes from memory to the lanes as they multiply it, v through the wave's own staged tile, both requested a
+// step ahead; no barrier until the waves' results are joined.
 // attn_few: keys of tiles `from` to `to` of a pair, its split-th part.
 template <bool F16, int DP>
 __device__ __forceinline__ void attn_few(const AttnArgs &p, uint16_t (&vt)[4][32 * DP], float (&joined)[4][16][DP + 4], int b,
@@ -573,7 +574,7 @@ __device__ __forceinline__ float norm_factor(float norm2) {
   return __builtin_ldexpf(1.0f, min(max(4 - e, -60), 60));
 }
 
-// 128 x 16 heads of 256 over up to 320 98 us; 4 x 16 of 1024 over 2048, dimension 128, 100 us, 1.03 PFLOP/s of its three products.
+// 128 x 16 heads of 256 over up to 320 96 us; 4 x 16 of 1024 over 2048, dimension 128, 100 us, 1.03 PFLOP/s of its three products.
 // dq, delta and (fp16) the largest row norm of the workgroup's do; the forward's walk over the keys.
 template <bool F16, int DP, int QT>
 __global__ __launch_bounds__(256, 2) void attn_dq_kernel(AttnArgs p) {
@@ -749,7 +750,7 @@ __global__ __launch_bounds__(256, 2) void attn_dq_kernel(AttnArgs p) {
   }
 }
 
-// 128 x 16 heads of 256 over up to 320 136 us; 4 x 16 of 1024 over 2048, dimension 128, 163 us, 0.84 PFLOP/s of its four
+// 128 x 16 heads of 256 over up to 320 124 us; 4 x 16 of 1024 over 2048, dimension 128, 163 us, 0.84 PFLOP/s of its four
 // products: there LDS is read four times for 16 keys a wave, and 32 do not fit the registers.
 // dk and dv of 64 KT keys: the waves' k and v stay in registers, the pair's rows (or the split's part of them) pass by in staged
 // tiles of q and do. A shared key's gradient sums over its heads here, in a fixed order.
